@@ -95,6 +95,35 @@ class DecodeArgs(ctypes.Structure):
         ("status", ctypes.c_void_p)]
 
 
+class DecodeWeightedArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("dtype", "B", "Hq", "Hkv", "L", "D", "bs", "T", "kk")] + [
+        ("scale", ctypes.c_float)] + [(n, View) for n in ("q", "k", "v", "o")] + [
+        ("sel", ctypes.c_void_p), ("sel_sb", ctypes.c_int64), ("sel_sh", ctypes.c_int64),
+        ("gate", ctypes.c_void_p), ("gate_sb", ctypes.c_int64), ("gate_sh", ctypes.c_int64),
+        ("weight", ctypes.c_void_p), ("weight_sb", ctypes.c_int64), ("weight_sh", ctypes.c_int64),
+        ("status", ctypes.c_void_p)]
+
+
+class EvictArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("dtype", "B", "Hkv", "L", "D", "bs", "budget", "recent", "sink", "seen")] + [
+        ("k", View), ("v", View),
+        ("weight", ctypes.c_void_p), ("w_sb", ctypes.c_int64), ("w_sh", ctypes.c_int64),
+        ("pos", ctypes.c_void_p), ("p_sb", ctypes.c_int64), ("p_sh", ctypes.c_int64),
+        ("weight_out", ctypes.c_void_p), ("wo_sb", ctypes.c_int64), ("wo_sh", ctypes.c_int64),
+        ("pos_out", ctypes.c_void_p), ("po_sb", ctypes.c_int64), ("po_sh", ctypes.c_int64),
+        ("kmin", ctypes.c_void_p), ("kmax", ctypes.c_void_p), ("km_sb", ctypes.c_int64),
+        ("km_sh", ctypes.c_int64), ("km_sn", ctypes.c_int64)]
+
+
+class DecodePrefixArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in
+                ("dtype", "B", "Hq", "Hkv", "D", "P", "S", "T")] + [
+        ("scale", ctypes.c_float)] + [(n, View) for n in ("q", "pk", "pv", "k", "v", "o")] + [
+        ("lens", ctypes.c_void_p), ("status", ctypes.c_void_p)]
+
+
 class ScoresArgs(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("G", "nblk", "topk", "sink")] + [
         ("score", ctypes.c_void_p), ("score_sg", ctypes.c_int64), ("score_si", ctypes.c_int64),
@@ -153,6 +182,15 @@ SYMBOLS = {
     "bsa_decode_workspace": (ctypes.c_size_t, [ctypes.POINTER(DecodeArgs)]),
     "bsa_decode": (ctypes.c_int, [ctypes.POINTER(DecodeArgs), ctypes.c_void_p, ctypes.c_size_t,
                                   ctypes.c_void_p]),
+    "bsa_decode_weighted_workspace": (ctypes.c_size_t, [ctypes.POINTER(DecodeWeightedArgs)]),
+    "bsa_decode_weighted": (ctypes.c_int, [ctypes.POINTER(DecodeWeightedArgs), ctypes.c_void_p,
+                                           ctypes.c_size_t, ctypes.c_void_p]),
+    "bsa_evict_workspace": (ctypes.c_size_t, [ctypes.POINTER(EvictArgs)]),
+    "bsa_evict": (ctypes.c_int, [ctypes.POINTER(EvictArgs), ctypes.c_void_p, ctypes.c_size_t,
+                                 ctypes.c_void_p]),
+    "bsa_decode_prefix_workspace": (ctypes.c_size_t, [ctypes.POINTER(DecodePrefixArgs)]),
+    "bsa_decode_prefix": (ctypes.c_int, [ctypes.POINTER(DecodePrefixArgs), ctypes.c_void_p,
+                                         ctypes.c_size_t, ctypes.c_void_p]),
     "bsa_status_decode": (ctypes.c_int, [ctypes.c_int32]),
     "bsa_last_error": (ctypes.c_char_p, []),
     "bsa_version": (ctypes.c_int32, []),
@@ -523,6 +561,195 @@ def decode(q, k, v, sel, gate=None, *, bs, L=None, mask_mode=MASK_TOKEN, scale=N
         _check(L_.bsa_decode(ctypes.byref(a), None, 0, _stream()))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     _check(L_.bsa_decode(ctypes.byref(a), ctypes.c_void_p(ws.data_ptr()), nbytes, _stream()))
+    return o
+
+
+def _same_device(first, **ts):
+    """Every tensor given lives on first's CUDA device."""
+    _need_cuda(first)
+    for name, t in ts.items():
+        if t is not None and t.device != first.device:
+            _need_cuda(t)
+            raise BsaShapeError(ERR_ARG, "%s is on %s, q / k on %s" % (name, t.device, first.device))
+
+
+def _cache_operand(t, name, B, Hkv, D, dtype):
+    """A K/V operand that is read or changed in place: never copied."""
+    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != Hkv or t.shape[3] != D:
+        raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, *, %d); got %s" % (name, B, Hkv, D, tuple(t.shape)))
+    if t.dtype != dtype:
+        raise BsaError(ERR_DTYPE, "%s must be %s; got %s" % (name, dtype, t.dtype))
+    if t.stride(3) != 1:
+        raise BsaError(ERR_STRIDE, "%s must have unit stride along D" % name)
+
+
+def _row_operand(t, name, B, Hkv, n, dtype):
+    """A (B, Hkv, >= n) per-slot tensor with unit stride along the slots."""
+    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != Hkv or t.shape[2] < n:
+        raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, >= %d); got %s" % (name, B, Hkv, n, tuple(t.shape)))
+    if t.dtype != dtype:
+        raise BsaError(ERR_DTYPE, "%s must be %s; got %s" % (name, dtype, t.dtype))
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise BsaError(ERR_STRIDE, "%s must have unit stride along the slots" % name)
+
+
+def _query_out(q, out):
+    """(q with unit stride along D, o) of a decode step."""
+    if q.dim() != 4:
+        raise BsaShapeError(ERR_SHAPE, "q must be (B, Hq, T, D)")
+    if q.stride(3) != 1:
+        q = q.contiguous()
+    if out is None:
+        return q, torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+        raise BsaShapeError(ERR_SHAPE, "out must have q's shape and dtype and unit stride along D")
+    return q, out
+
+
+def _launch(name, a, t):
+    """Workspace and launch of entry point `name` on t's device and its current stream."""
+    if t.device.index != torch.cuda.current_device():
+        with torch.cuda.device(t.device):
+            return _launch(name, a, t)
+    L, ref = lib(), ctypes.byref(a)
+    nbytes = getattr(L, name + "_workspace")(ref)
+    if nbytes == 0:   # validation failed: the call reports why
+        _check(getattr(L, name)(ref, None, 0, _stream()))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
+    _check(getattr(L, name)(ref, ws.data_ptr(), nbytes, _stream()))
+
+
+def _v4(t):
+    return (t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+
+
+def decode_weighted(q, k, v, weight, sel=None, gate=None, *, bs=None, L=None, scale=None, out=None):
+    """Decode step that adds every slot's attention weight to a running sum
+    (bsa_decode_weighted).  q (B, Hq, T, D): the tokens at positions L-T .. L-1; k, v
+    (B, Hkv, >= L, D): the cache; weight fp32 (B, Hkv, >= L): weight[b, hk, j] +=
+    sum over hk's query heads and the T rows of their softmax weight on slot j.
+    sel: int32 (B, kk) or (B, 1 or Hkv, kk) ids of blocks of bs slots (None: every
+    slot), TOKEN masks; gate: optional fp32 like sel.  Returns o (B, Hq, T, D)."""
+    _same_device(q, k=k, v=v, weight=weight, sel=sel, gate=gate, out=out)
+    q, o = _query_out(q, out)
+    B, Hq, T, D = q.shape
+    if k.dim() != 4:
+        raise BsaShapeError(ERR_SHAPE, "k must be (B, Hkv, >= L, D)")
+    Hkv = k.shape[1]
+    _cache_operand(k, "k", B, Hkv, D, q.dtype)
+    _cache_operand(v, "v", B, Hkv, D, q.dtype)
+    L = min(k.shape[2], v.shape[2]) if L is None else int(L)
+    if L > min(k.shape[2], v.shape[2]):
+        raise BsaShapeError(ERR_SHAPE, "decode_weighted: L = %d is more than k and v hold" % L)
+    _row_operand(weight, "weight", B, Hkv, L, torch.float32)
+    kk = s_sb = s_sh = g_sb = g_sh = 0
+    if sel is not None:
+        if bs is None or not 0 < bs < 2 ** 30:
+            raise BsaShapeError(ERR_ARG, "decode_weighted: a selection needs its block size bs")
+        if sel.dtype != torch.int32 or sel.stride(-1) != 1:
+            sel = sel.to(torch.int32).contiguous()
+        if not ((sel.dim() == 2 and sel.shape[0] == B) or
+                (sel.dim() == 3 and sel.shape[0] == B and sel.shape[1] in (1, Hkv))):
+            raise BsaShapeError(ERR_SHAPE, "decode_weighted: sel must be (B, kk) or (B, Hkv, kk)")
+        kk, s_sb = sel.shape[-1], sel.stride(0)
+        s_sh = sel.stride(1) if sel.dim() == 3 and sel.shape[1] > 1 else 0
+        if gate is not None:
+            if gate.shape != sel.shape:
+                raise BsaShapeError(ERR_SHAPE, "decode_weighted: gate must have the shape of sel")
+            if gate.dtype != torch.float32 or gate.stride(-1) != 1:
+                gate = gate.to(torch.float32).contiguous()
+            g_sb = gate.stride(0)
+            g_sh = gate.stride(1) if gate.dim() == 3 and gate.shape[1] > 1 else 0
+    elif gate is not None:
+        raise BsaShapeError(ERR_ARG, "decode_weighted: a gate needs a selection")
+    a = DecodeWeightedArgs(
+        _dtype(q), B, Hq, Hkv, L, D, bs if sel is not None else 0, T, kk, D ** -0.5 if scale is None else scale,
+        _v4(q), _v4(k), _v4(v), _v4(o), sel.data_ptr() if sel is not None else None, s_sb, s_sh,
+        gate.data_ptr() if gate is not None else None, g_sb, g_sh,
+        weight.data_ptr(), weight.stride(0), weight.stride(1),
+        status_tensor(q.device).data_ptr() if sel is not None else None)
+    _launch("bsa_decode_weighted", a, q)
+    return o
+
+
+def evict(k, v, weight, pos, *, budget, L=None, seen=None, recent=0, sink=0, kmin=None, kmax=None,
+          bs=None, weight_out=None, pos_out=None):
+    """Cuts a cache from L slots to `budget` in place (bsa_evict).  k, v (B, Hkv, >= L, D);
+    weight fp32 and pos int32 (B, Hkv, >= L): every slot's accumulated attention weight
+    and token position.  Per (b, hk) the slots with pos < sink or pos >= seen - recent
+    survive first (seen: tokens appended so far, default L), then those of most weight,
+    ties to the lower slot; survivors beyond the budget fill the freed slots in order.
+    weight / pos follow (into weight_out / pos_out when given), and kmin / kmax (fp32
+    (B, Hkv, >= ceil(budget / bs), D), both or none) of the changed blocks of bs slots
+    are pooled anew."""
+    _same_device(k, v=v, weight=weight, pos=pos, kmin=kmin, kmax=kmax, weight_out=weight_out,
+                 pos_out=pos_out)
+    if k.dim() != 4:
+        raise BsaShapeError(ERR_SHAPE, "k must be (B, Hkv, >= L, D)")
+    B, Hkv, cap, D = k.shape
+    _cache_operand(k, "k", B, Hkv, D, k.dtype)
+    _cache_operand(v, "v", B, Hkv, D, k.dtype)
+    L = min(cap, v.shape[2]) if L is None else int(L)
+    if L > min(cap, v.shape[2]):
+        raise BsaShapeError(ERR_SHAPE, "evict: L = %d is more than k and v hold" % L)
+    seen = L if seen is None else int(seen)
+    if not (0 < budget <= L and 0 <= recent <= budget and 0 <= sink <= budget and L <= seen < 2 ** 31):
+        raise BsaShapeError(ERR_SHAPE, "evict: needs 1 <= budget <= L <= seen < 2^31 and recent, sink "
+                                       "within the budget")
+    if bs is not None and not 0 < bs <= 1024:
+        raise BsaShapeError(ERR_SHAPE, "evict: bs must lie in 1 .. 1024")
+    wo = weight if weight_out is None else weight_out
+    po = pos if pos_out is None else pos_out
+    _row_operand(weight, "weight", B, Hkv, L, torch.float32)
+    _row_operand(pos, "pos", B, Hkv, L, torch.int32)
+    _row_operand(wo, "weight_out", B, Hkv, budget, torch.float32)
+    _row_operand(po, "pos_out", B, Hkv, budget, torch.int32)
+    if (kmin is None) != (kmax is None):
+        raise BsaShapeError(ERR_ARG, "evict: kmin and kmax go together")
+    km, kx, km_st = None, None, (0, 0, 0)
+    if kmin is not None:
+        if bs is None:
+            raise BsaShapeError(ERR_ARG, "evict: kmin and kmax need bs")
+        nb = (budget + bs - 1) // bs
+        for name, t in (("kmin", kmin), ("kmax", kmax)):
+            _cache_operand(t, name, B, Hkv, D, torch.float32)
+            if t.shape[2] < nb or t.stride() != kmin.stride():
+                raise BsaShapeError(ERR_SHAPE, "evict: kmin and kmax need one layout and %d blocks" % nb)
+        km, kx, km_st = kmin.data_ptr(), kmax.data_ptr(), kmin.stride()[:3]
+    a = EvictArgs(
+        _dtype(k), B, Hkv, L, D, 64 if bs is None else bs, budget, recent, sink, seen,
+        _v4(k), _v4(v), weight.data_ptr(), weight.stride(0), weight.stride(1),
+        pos.data_ptr(), pos.stride(0), pos.stride(1), wo.data_ptr(), wo.stride(0), wo.stride(1),
+        po.data_ptr(), po.stride(0), po.stride(1), km, kx, *km_st)
+    _launch("bsa_evict", a, k)
+
+
+def decode_prefix(q, pk, pv, k, v, lens, *, scale=None, out=None):
+    """Decode step of a batch that shares a prefix (bsa_decode_prefix).  q (B, Hq, T, D);
+    pk, pv (Hkv, P, D): the prefix, read once for the batch; k, v (B, Hkv, S, D): each
+    sequence's own slots, lens int32 (B,) of them in use, the T new tokens last.  Row t
+    sees the prefix and the own slots j <= lens[b] - T + t.  Returns o (B, Hq, T, D)."""
+    _same_device(q, pk=pk, pv=pv, k=k, v=v, lens=lens, out=out)
+    q, o = _query_out(q, out)
+    B, Hq, T, D = q.shape
+    if k.dim() != 4 or pk.dim() != 3 or pv.shape != pk.shape:
+        raise BsaShapeError(ERR_SHAPE, "decode_prefix: k, v must be (B, Hkv, S, D) and pk, pv (Hkv, P, D)")
+    Hkv, S = k.shape[1], k.shape[2]
+    _cache_operand(k, "k", B, Hkv, D, q.dtype)
+    _cache_operand(v, "v", B, Hkv, D, q.dtype)
+    if v.shape[2] != S:
+        raise BsaShapeError(ERR_SHAPE, "decode_prefix: k and v hold different numbers of slots")
+    pk, pv = pk.unsqueeze(0), pv.unsqueeze(0)
+    _cache_operand(pk, "pk", 1, Hkv, D, q.dtype)
+    _cache_operand(pv, "pv", 1, Hkv, D, q.dtype)
+    if lens.dim() != 1 or lens.shape[0] != B or lens.is_floating_point():
+        raise BsaShapeError(ERR_SHAPE, "decode_prefix: lens must be (B,) whole numbers")
+    if lens.dtype != torch.int32 or not lens.is_contiguous():
+        lens = lens.to(torch.int32).contiguous()
+    a = DecodePrefixArgs(
+        _dtype(q), B, Hq, Hkv, D, pk.shape[2], S, T, D ** -0.5 if scale is None else scale,
+        _v4(q), _v4(pk), _v4(pv), _v4(k), _v4(v), _v4(o), lens.data_ptr(), status_tensor(q.device).data_ptr())
+    _launch("bsa_decode_prefix", a, q)
     return o
 
 

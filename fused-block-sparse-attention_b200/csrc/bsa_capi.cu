@@ -26,6 +26,12 @@ bsa_status run_scores_topk(const bsa_scores_args *a, cudaStream_t st);
 bsa_status run_qmax(const bsa_qmax_args *a, cudaStream_t st);
 size_t decode_workspace(const bsa_decode_args *a);
 bsa_status run_decode(const bsa_decode_args *a, void *ws, size_t ws_bytes, cudaStream_t st);
+size_t weighted_workspace(const bsa_decode_weighted_args *a);
+bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_bytes, cudaStream_t st);
+size_t evict_workspace(const bsa_evict_args *a);
+bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStream_t st);
+size_t prefix_workspace(const bsa_decode_prefix_args *a);
+bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes, cudaStream_t st);
 
 static bsa_status check_view(const bsa_view &v, int dtype, const char *name, bool vec16) {
   if (!v.ptr) return fail(BSA_ERR_ARG, std::string(name) + " is NULL");
@@ -236,6 +242,30 @@ bsa_status bsa_decode(const bsa_decode_args *a, void *workspace, size_t workspac
                       bsa_stream_t stream) {
   if (!a) return fail(BSA_ERR_ARG, "decode: args is NULL");
   return run_decode(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t bsa_decode_weighted_workspace(const bsa_decode_weighted_args *a) { return a ? weighted_workspace(a) : 0; }
+
+bsa_status bsa_decode_weighted(const bsa_decode_weighted_args *a, void *workspace, size_t workspace_bytes,
+                  bsa_stream_t stream) {
+  if (!a) return fail(BSA_ERR_ARG, "decode_weighted: args is NULL");
+  return run_weighted(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t bsa_evict_workspace(const bsa_evict_args *a) { return a ? evict_workspace(a) : 0; }
+
+bsa_status bsa_evict(const bsa_evict_args *a, void *workspace, size_t workspace_bytes,
+                  bsa_stream_t stream) {
+  if (!a) return fail(BSA_ERR_ARG, "evict: args is NULL");
+  return run_evict(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t bsa_decode_prefix_workspace(const bsa_decode_prefix_args *a) { return a ? prefix_workspace(a) : 0; }
+
+bsa_status bsa_decode_prefix(const bsa_decode_prefix_args *a, void *workspace, size_t workspace_bytes,
+                  bsa_stream_t stream) {
+  if (!a) return fail(BSA_ERR_ARG, "decode_prefix: args is NULL");
+  return run_prefix(a, workspace, workspace_bytes, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int32_t bsa_select_scores_width(const bsa_scores_args *a) {

@@ -1,0 +1,351 @@
+// Reduction of a K/V cache to a budget of slots by accumulated attention weight.
+//
+// Of the L slots of each (batch, K/V head) the `budget` best survive: protected
+// slots first (the first `sink` and the last `recent` token positions), then by
+// weight, ties to the lower slot.  Survivors below the budget keep their slot; the
+// others fill the freed slots, both in ascending order.  That moves the fewest
+// rows, and since every source is >= budget and every destination below it, the
+// moves run in place in any order.
+//
+//   evict_pick_kernel  a cluster of CTAs per (b, head), each with its share of the
+//                      slots: the key of the budget-th best slot by a radix search
+//                      (11 + 11 + 10 bits, histograms summed over the cluster), then
+//                      the lists of freed slots and of sources by prefix counts
+//   evict_move_kernel  CTA per (b, head, block of slots): moves rows, weights and
+//                      positions, and pools the min / max of a changed block while
+//                      its rows pass through registers
+// Bound by HBM for a large cut (rows moved) and by latency for a single slot.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
+#include "bsa_common.cuh"
+#include "bsa_host.h"
+
+namespace cg = cooperative_groups;
+
+namespace bsa {
+
+namespace {
+constexpr int kPickThreads = 1024;
+constexpr int kBins = 2048;
+
+struct EvictWork {
+  int *hole, *tail;  // [B*Hkv][m_cap]
+  int *off;          // [B*Hkv][nblk + 1]: freed slots before each block
+  int m_cap, nblk;
+};
+
+// Monotone 32-bit key: protected slots above everything, NaN with -infinity below.
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, int sink, int first_recent) {
+  if (pos < sink || pos >= first_recent) return 0xffffffffu;
+  if (isnan(w)) w = -INFINITY;
+  const uint32_t u = __float_as_uint(w + 0.f);  // -0 becomes +0
+  return (u >> 31) ? ~u : (u | 0x80000000u);
+}
+
+// Inclusive-to-exclusive block scan of one int per thread (1024 threads); total
+// in *total.  s: 33 ints.
+__device__ __forceinline__ int block_scan(int v, int *s, int *total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  __syncthreads();
+  if (lane == 31) s[warp] = x;
+  __syncthreads();
+  if (warp == 0) {
+    int y = s[lane];
+    const int y0 = y;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int z = __shfl_up_sync(0xffffffffu, y, o);
+      if (lane >= o) y += z;
+    }
+    s[lane] = y - y0;
+    if (lane == 31) s[32] = y;
+  }
+  __syncthreads();
+  *total = s[32];
+  return s[warp] + x - v;
+}
+}  // namespace
+
+__global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const bsa_evict_args a, const EvictWork w) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int nc = cl.num_blocks(), rank = cl.block_rank();
+  const int bh = blockIdx.x / nc, b = bh / a.Hkv, h = bh % a.Hkv;
+  const int tid = threadIdx.x;
+  __shared__ int hist[kBins];
+  __shared__ int s_scan[33];
+  __shared__ int s_bin, s_need, s_cnt[3];
+  const float *wt = a.weight + b * a.w_sb + h * a.w_sh;
+  const int32_t *ps = a.pos + b * a.p_sb + h * a.p_sh;
+  const int first_recent = a.seen - a.recent;
+  // this CTA's slots, a multiple of the block size of the scans
+  const int per = ((a.L + nc - 1) / nc + kPickThreads - 1) / kPickThreads * kPickThreads;
+  const int lo = min(a.L, rank * per), hi = min(a.L, lo + per);
+  auto key = [&](int i) { return evict_key(__ldg(wt + i), __ldg(ps + i), a.sink, first_recent); };
+
+  // ---- key of the budget-th best slot, 11 + 11 + 10 bits from the top
+  uint32_t prefix = 0;
+  int need = a.budget;  // slots still wanted among those that share the prefix
+  const int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+#pragma unroll
+  for (int ps_ = 0; ps_ < 3; ++ps_) {
+    const int sh = shift[ps_], nb = 1 << bits[ps_];
+    for (int i = tid; i < kBins; i += kPickThreads) hist[i] = 0;
+    __syncthreads();
+    for (int i = lo + tid; i < hi; i += kPickThreads) {
+      const uint32_t k = key(i);
+      if (ps_ == 0 || (k >> (sh + bits[ps_])) == prefix) atomicAdd(&hist[(k >> sh) & (nb - 1)], 1);
+    }
+    cl.sync();
+    // bins from the top, two per thread; sums over the cluster
+    int c0 = 0, c1 = 0;
+    const int b0 = nb - 1 - 2 * tid, b1 = b0 - 1;
+    if (b1 >= 0)
+      for (int r = 0; r < nc; ++r) {
+        const int *hr = cl.map_shared_rank(hist, r);
+        c0 += hr[b0];
+        c1 += hr[b1];
+      }
+    int total;
+    const int before = block_scan(c0 + c1, s_scan, &total);
+    if (before < need && before + c0 >= need) {
+      s_bin = b0;
+      s_need = need - before;
+    } else if (before + c0 < need && before + c0 + c1 >= need) {
+      s_bin = b1;
+      s_need = need - before - c0;
+    }
+    cl.sync();  // also: nobody reads a histogram any more
+    prefix = (prefix << bits[ps_]) | (uint32_t)s_bin;
+    need = s_need;
+    __syncthreads();
+  }
+  const uint32_t kth = prefix;  // better keys survive, and the first `need` equal ones
+
+  // ---- equal keys before this CTA's slots
+  int eq = 0;
+  for (int i = lo + tid; i < hi; i += kPickThreads) eq += key(i) == kth;
+  int eq_total;
+  block_scan(eq, s_scan, &eq_total);
+  if (tid == 0) s_cnt[0] = eq_total;
+  cl.sync();
+  int eq_before = 0;
+  for (int r = 0; r < rank; ++r) eq_before += cl.map_shared_rank(s_cnt, r)[0];
+  // ---- freed slots below the budget and survivors beyond it, in this CTA
+  int holes = 0, tails = 0, e0 = eq_before;
+  for (int i0 = lo; i0 < hi; i0 += kPickThreads) {
+    const int i = i0 + tid;
+    const uint32_t k = i < hi ? key(i) : 0u;
+    const bool same = i < hi && k == kth;
+    int t;
+    const int er = block_scan(same, s_scan, &t) + e0;
+    e0 += t;
+    const bool keep = i < hi && (k > kth || (same && er < need));
+    holes += i < hi && i < a.budget && !keep;
+    tails += i < hi && i >= a.budget && keep;
+  }
+  int ht, tt;
+  block_scan(holes, s_scan, &ht);
+  block_scan(tails, s_scan, &tt);
+  if (tid == 0) s_cnt[1] = ht, s_cnt[2] = tt;
+  cl.sync();
+  int hb = 0, tb = 0;
+  for (int r = 0; r < rank; ++r) {
+    hb += cl.map_shared_rank(s_cnt, r)[1];
+    tb += cl.map_shared_rank(s_cnt, r)[2];
+  }
+  int hall = hb;
+  for (int r = rank; r < nc; ++r) hall += cl.map_shared_rank(s_cnt, r)[1];
+  cl.sync();  // nobody leaves while its counts may be read
+  // ---- the lists
+  int *hole = w.hole + (long long)bh * w.m_cap, *tail = w.tail + (long long)bh * w.m_cap;
+  int *off = w.off + (long long)bh * (w.nblk + 1);
+  if (rank == 0 && tid == 0) off[w.nblk] = hall;
+  e0 = eq_before;
+  for (int i0 = lo; i0 < hi; i0 += kPickThreads) {
+    const int i = i0 + tid;
+    const uint32_t k = i < hi ? key(i) : 0u;
+    const bool same = i < hi && k == kth;
+    int t;
+    const int er = block_scan(same, s_scan, &t) + e0;
+    e0 += t;
+    const bool keep = i < hi && (k > kth || (same && er < need));
+    const bool fr = i < hi && i < a.budget && !keep, sv = i < hi && i >= a.budget && keep;
+    const int hr = block_scan(fr, s_scan, &t) + hb;
+    hb += t;
+    const int tr = block_scan(sv, s_scan, &t) + tb;
+    tb += t;
+    if (i < hi && i < a.budget && i % a.bs == 0) off[i / a.bs] = hr;
+    if (fr && hr < w.m_cap) hole[hr] = i;
+    if (sv && tr < w.m_cap) tail[tr] = i;
+  }
+}
+
+// One CTA of 256 threads per block of slots.  A row of D elements is D*es/16
+// 16-byte pieces; a thread owns one piece column and every (256 / pieces)-th row.
+template <typename T>
+__global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a, const EvictWork w) {
+  constexpr int E = 16 / sizeof(T);
+  extern __shared__ int s_src[];  // [bs] source slot, then the min / max of each thread row
+  const int blk = blockIdx.x % w.nblk, bh = blockIdx.x / w.nblk;
+  const int b = bh / a.Hkv, h = bh % a.Hkv, tid = threadIdx.x;
+  const int s0 = blk * a.bs, rows = min(a.bs, a.budget - s0);
+  const int *off = w.off + (long long)bh * (w.nblk + 1);
+  const int m0 = off[blk], m1 = off[blk + 1];
+  const bool moves = m1 > m0;
+  const float *wt = a.weight + b * a.w_sb + h * a.w_sh;
+  const int32_t *ps = a.pos + b * a.p_sb + h * a.p_sh;
+  float *wo = a.weight_out + b * a.wo_sb + h * a.wo_sh;
+  int32_t *po = a.pos_out + b * a.po_sb + h * a.po_sh;
+  const bool same = a.weight_out == a.weight && a.pos_out == a.pos;
+  const bool pool = a.kmin && (moves || rows < a.bs);
+  if (!moves && !pool && same) return;
+  for (int i = tid; i < rows; i += 256) s_src[i] = s0 + i;
+  __syncthreads();
+  for (int m = m0 + tid; m < m1; m += 256)
+    s_src[w.hole[(long long)bh * w.m_cap + m] - s0] = w.tail[(long long)bh * w.m_cap + m];
+  __syncthreads();
+  for (int i = tid; i < rows; i += 256) {
+    const int s = s_src[i];
+    if (s != s0 + i || !same) {
+      wo[s0 + i] = wt[s];
+      po[s0 + i] = ps[s];
+    }
+  }
+  if (!moves && !pool) return;
+  const int pc = a.D / E, rg = 256 / pc;   // pieces per row, rows side by side
+  const int c = tid % pc, r0 = tid / pc;
+  T *kp = reinterpret_cast<T *>(a.k.ptr) + b * a.k.sb + h * a.k.sh + c * E;
+  T *vp = reinterpret_cast<T *>(a.v.ptr) + b * a.v.sb + h * a.v.sh + c * E;
+  float mn[E], mx[E];
+  const bool pad = rows < a.bs;  // rows past the budget count as zeros
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    mn[e] = pad ? 0.f : INFINITY;
+    mx[e] = pad ? 0.f : -INFINITY;
+  }
+  for (int r = r0; r < rows; r += rg) {
+    const int s = s_src[r];
+    const bool mv = s != s0 + r;
+    if (mv || pool) {
+      const uint4 kv = *reinterpret_cast<const uint4 *>(kp + (long long)s * a.k.sl);
+      if (mv) {
+        const uint4 vv = *reinterpret_cast<const uint4 *>(vp + (long long)s * a.v.sl);
+        *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv;
+        *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv;
+      }
+      const T *ke = reinterpret_cast<const T *>(&kv);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float x;
+        if constexpr (sizeof(T) == 2)
+          x = Mma<T>::to_f(ke[e]);
+        else
+          x = ke[e];
+        mn[e] = fminf(mn[e], x);
+        mx[e] = fmaxf(mx[e], x);
+      }
+    }
+  }
+  if (!pool) return;
+  float *sp = reinterpret_cast<float *>(s_src + a.bs);  // [2][rg][D]
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    sp[r0 * a.D + c * E + e] = mn[e];
+    sp[(rg + r0) * a.D + c * E + e] = mx[e];
+  }
+  __syncthreads();
+  for (int d = tid; d < a.D; d += 256) {
+    float x = sp[d], y = sp[rg * a.D + d];
+    for (int r = 1; r < rg; ++r) {
+      x = fminf(x, sp[r * a.D + d]);
+      y = fmaxf(y, sp[(rg + r) * a.D + d]);
+    }
+    const long long at = b * a.km_sb + h * a.km_sh + (long long)blk * a.km_sn + d;
+    a.kmin[at] = x;
+    a.kmax[at] = y;
+  }
+}
+
+// ------------------------------------------------------------------ host
+static bsa_status evict_check(const bsa_evict_args *a) {
+  if (a->dtype != BSA_BF16 && a->dtype != BSA_F16 && a->dtype != BSA_F32)
+    return fail(BSA_ERR_DTYPE, "evict: dtype must be bf16, f16 or f32");
+  if (a->B <= 0 || a->Hkv <= 0 || a->L <= 0 || a->bs <= 0)
+    return fail(BSA_ERR_SHAPE, "evict: sizes must be positive");
+  if (a->D != 32 && a->D != 64 && a->D != 128 && a->D != 256)
+    return fail(BSA_ERR_UNSUPPORTED, "evict: D must be 32, 64, 128 or 256");
+  if (a->bs > 1024) return fail(BSA_ERR_UNSUPPORTED, "evict: bs must be <= 1024");
+  if (a->budget <= 0 || a->budget > a->L) return fail(BSA_ERR_SHAPE, "evict: needs 1 <= budget <= L");
+  if (a->recent < 0 || a->sink < 0 || (long long)a->recent + a->sink > a->budget)
+    return fail(BSA_ERR_SHAPE, "evict: recent + sink must lie in [0, budget]");
+  if (a->seen < a->L) return fail(BSA_ERR_SHAPE, "evict: seen must be at least L");
+  if (a->L > (1 << 29) || (long long)a->B * a->Hkv >= (1 << 24))
+    return fail(BSA_ERR_SHAPE, "evict: L or B*Hkv too large");
+  if (!a->k.ptr || !a->v.ptr || !a->weight || !a->pos || !a->weight_out || !a->pos_out)
+    return fail(BSA_ERR_ARG, "evict: NULL tensor");
+  if (!a->kmin != !a->kmax) return fail(BSA_ERR_ARG, "evict: kmin and kmax go together");
+  const int64_t es = (int64_t)elem_size(a->dtype);
+  for (const bsa_view *v : {&a->k, &a->v})
+    if (reinterpret_cast<uintptr_t>(v->ptr) % 16 || (v->sb * es) % 16 || (v->sh * es) % 16 || (v->sl * es) % 16)
+      return fail(BSA_ERR_STRIDE, "evict: k and v need 16-byte aligned bases and strides");
+  const long long nblk = (a->budget + a->bs - 1) / a->bs;
+  if (nblk * a->B * a->Hkv >= (1LL << 31)) return fail(BSA_ERR_SHAPE, "evict: too many blocks");
+  return BSA_OK;
+}
+
+static size_t evict_plan(const bsa_evict_args *a, EvictWork *w, uint8_t *base) {
+  w->m_cap = std::max(1, std::min(a->budget, a->L - a->budget));
+  w->nblk = (a->budget + a->bs - 1) / a->bs;
+  const size_t bh = (size_t)a->B * a->Hkv, list = align_up(bh * w->m_cap * 4, 256);
+  w->hole = reinterpret_cast<int *>(base);
+  w->tail = reinterpret_cast<int *>(base + list);
+  w->off = reinterpret_cast<int *>(base + 2 * list);
+  return 2 * list + align_up(bh * (w->nblk + 1) * 4, 256);
+}
+
+size_t evict_workspace(const bsa_evict_args *a) {
+  EvictWork w;
+  return evict_check(a) == BSA_OK ? evict_plan(a, &w, nullptr) : 0;
+}
+
+bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStream_t st) {
+  if (bsa_status s = evict_check(a)) return s;
+  EvictWork w;
+  const size_t need = evict_plan(a, &w, static_cast<uint8_t *>(ws));
+  if (!ws || ws_bytes < need) return fail(BSA_ERR_WORKSPACE, "evict: workspace too small");
+  const int bh = a->B * a->Hkv;
+  // CTAs per (b, head): one per 8192 slots, at most 8 (the portable cluster size)
+  int nc = 1;
+  while (nc < 8 && (long long)nc * 8192 < a->L) nc *= 2;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)bh * nc);
+  cfg.blockDim = dim3(kPickThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = nc, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, evict_pick_kernel, *a, w);
+  if (bsa_status s = check_launch("evict_pick")) return s;
+  const unsigned grid = (unsigned)bh * w.nblk;
+  const int es = (int)elem_size(a->dtype), rg = 256 / (a->D * es / 16);
+  const size_t smem = (size_t)a->bs * 4 + 2ull * rg * a->D * 4;
+  if (a->dtype == BSA_BF16)
+    evict_move_kernel<__nv_bfloat16><<<grid, 256, smem, st>>>(*a, w);
+  else if (a->dtype == BSA_F16)
+    evict_move_kernel<__half><<<grid, 256, smem, st>>>(*a, w);
+  else
+    evict_move_kernel<float><<<grid, 256, smem, st>>>(*a, w);
+  return check_launch("evict_move");
+}
+
+}  // namespace bsa

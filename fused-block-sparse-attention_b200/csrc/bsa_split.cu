@@ -1,0 +1,1141 @@
+// Split-key attention of few query rows (decode steps) in bf16 / f16 / fp32, the
+// join of the splits, and the running sum of every slot's attention weight.
+//
+//   split_mma_kernel   bf16, f16: mma.sync; one warp streams its own keys
+//   split_f32_kernel   fp32 FMA; warps share the key tile, split rows and keys
+//   split_join_kernel  joins the splits of every row; with weights, also adds
+//                      sum over the rows of p = 2^(x - lse) to each slot's sum
+// The kernels are bound by reading K and V once (HBM).
+#include <algorithm>
+#include <cmath>
+
+#include "bsa_host.h"
+#include "bsa_split.cuh"
+
+namespace bsa {
+
+namespace {
+constexpr int kSplitWarps = 4;
+constexpr int kMaxLive = 512;  // block ids of one selection row
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
+  const int n = live ? 16 : 0;  // the rest of the 16 bytes is filled with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+// Maximum that keeps a NaN: a row with a NaN logit ends as NaN, not as an empty row.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Live block ids (and gates) of one selection row: the first occurrence of each id
+// that holds slots before L, unless its gate is -inf; in slot order; by one warp.  Returns their count.
+__device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_blk, float *s_gate,
+                          int *s_raw) {
+  const int lane = threadIdx.x & 31;
+  const int32_t *row = p.sel + b * p.sel_sb + hk * p.sel_sh;
+  const float *gr = p.gate ? p.gate + b * p.gate_sb + hk * p.gate_sh : nullptr;
+  const int nblk = (len + p.bs - 1) / p.bs;
+  for (int j = lane; j < p.kk; j += 32) s_raw[j] = __ldg(row + j);
+  __syncwarp();
+  int n = 0;
+  for (int j0 = 0; j0 < p.kk; j0 += 32) {
+    const int j = j0 + lane;
+    bool ok = false;
+    int kb = 0;
+    float gv = 0.f;
+    if (j < p.kk) {
+      kb = s_raw[j];
+      if (kb < 0 || kb >= nblk) {
+        report(p.status, BSA_DEVERR_INDEX);
+      } else {
+        ok = true;
+        for (int i = 0; i < j && ok; ++i) ok = s_raw[i] != kb;
+        if (gr) gv = __ldg(gr + j) * kLog2e;
+        if (gv == -INFINITY) ok = false;  // masked as a whole: its rows are not read
+      }
+    }
+    const unsigned live = __ballot_sync(0xffffffffu, ok);
+    const int at = n + __popc(live & ((1u << lane) - 1u));
+    if (ok) {
+      s_blk[at] = kb;
+      s_gate[at] = gv;
+    }
+    n += __popc(live);
+  }
+  return n;
+}
+}  // namespace
+
+// ------------------------------------------------------------------ bf16 / f16
+// CTA = (K/V head group, 16*MT query rows, split); each of its 4 warps takes every
+// fourth chunk of KC keys and keeps its own m, l and O, so the warps meet only at
+// the end.  A chunk's K and V rows arrive by 16-byte cp.async in a ring of NST
+// stages per warp, rows past the end zero-filled (never read).  S = Q K^T and
+// O += P V are m16n8k16 products with the query rows as M; 16 rows are mostly
+// padding in a decode step (grp = 8: half), which costs nothing while HBM is the
+// bound: 8 KB of keys take 350 cycles of the SM's share of HBM, their products 64.
+// P is split in two 16-bit terms (p = hi + lo, hi = round(p), lo = round(p - hi)),
+// so its rounding does not add to the output's; the extra products are free here.
+// Keys that some rows of the tile must not see (the newest T - 1) are multiplied
+// one by one in fp32 and skipped where p = 0: an infinity or NaN in a masked V row
+// never reaches a row that does not see it.
+template <int D>
+struct SplitCfg {
+  static constexpr int KC = D >= 128 ? 16 : 32;
+  static constexpr int STAGE = KC * D * 2 * 2;        // K and V of a chunk, bytes
+  static constexpr int NST = D == 32 ? 5 : 3;
+  static constexpr int MINB = D == 256 ? 1 : 2;       // CTAs per SM
+  static constexpr int RING = kSplitWarps * NST * STAGE;
+};
+
+template <int D>
+__device__ __forceinline__ uint32_t sw_off(int row, int chunk) {  // 16-byte chunk of a D-wide row
+  if constexpr (D == 32)
+    return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+  else
+    return row * (D * 2) + (((chunk & ~7) | ((chunk ^ row) & 7)) << 4);
+}
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
+    split_mma_kernel(const SplitParams p, int rtiles, int min_chunks) {
+  using C = SplitCfg<D>;
+  constexpr int KC = C::KC, NST = C::NST, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int s_blk[kMaxLive], s_raw[kMaxLive];
+  __shared__ float s_gate[kMaxLive];
+  __shared__ int s_n;
+  __shared__ float s_m[kSplitWarps][ROWS], s_l[kSplitWarps][ROWS];
+  uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
+  uint8_t *ring = sm + ROWS * D * 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, tq = lane & 3;
+  const int rt = blockIdx.x % rtiles, grpid = blockIdx.x / rtiles;
+  const int b = p.fold ? 0 : grpid / p.Hkv, hk = grpid % p.Hkv;
+  const int r0 = rt * ROWS;
+
+  int len = p.nkeys;
+  if (p.lens) {
+    len = __ldg(p.lens + b);
+    if (len < 0 || len > p.nkeys) {
+      if (tid == 0) report(p.status, BSA_DEVERR_INDEX);
+      len = len < 0 ? 0 : p.nkeys;
+    }
+  }
+  int nv = len;  // virtual keys: the slots, or those of the live blocks one after another
+  if (p.sel) {
+    if (warp == 0) {
+      const int n = build_live(p, b, hk, len, s_blk, s_gate, s_raw);
+      if (lane == 0) s_n = n;
+      if (p.live && blockIdx.y == 0 && rt == 0) {
+        __syncwarp();
+        int *lv = p.live + (long long)grpid * (1 + p.kk);
+        for (int i = lane; i < n; i += 32) lv[1 + i] = s_blk[i];
+        if (lane == 0) lv[0] = n;
+      }
+    }
+    __syncthreads();
+    nv = s_n * p.bs;
+  }
+  const int nch = (nv + KC - 1) / KC;
+  const int cps = max(min_chunks, (nch + p.nsplit - 1) / p.nsplit);
+  const int c_lo = min(nch, (int)blockIdx.y * cps), c_hi = min(nch, c_lo + cps);
+  const int split = p.split0 + blockIdx.y;
+  if (c_lo >= c_hi) {  // nothing to see here: the join skips this split
+    for (int r = tid; r < ROWS && r0 + r < p.R; r += blockDim.x) {
+      int rb, rh, rtt;
+      const long long gr = split_row(p, b, hk, r0 + r, rb, rh, rtt);
+      p.pml[(long long)split * p.rows + gr] = make_float2(-INFINITY, 0.f);
+    }
+    return;
+  }
+
+  const T *kb_ = reinterpret_cast<const T *>(p.k) + (p.fold ? 0 : b * p.k_sb) + hk * p.k_sh;
+  const T *vb_ = reinterpret_cast<const T *>(p.v) + (p.fold ? 0 : b * p.v_sb) + hk * p.v_sh;
+  uint8_t *wring = ring + warp * NST * C::STAGE;
+  // first key of chunk c, and its gate
+  auto key_of = [&](int c, float &gate) -> int {
+    const int j = c * KC;
+    if (!p.sel) {
+      gate = 0.f;
+      return j;
+    }
+    const int i = j / p.bs;
+    gate = s_gate[i];
+    return s_blk[i] * p.bs + (j - i * p.bs);
+  };
+  auto load = [&](int c, int st) {
+    if (c < c_hi) {
+      float gt;
+      const int key0 = key_of(c, gt);
+      const uint32_t dk = smem_u32(wring + st * C::STAGE), dv = dk + KC * D * 2;
+#pragma unroll
+      for (int it = 0; it < KC * D / 8 / 32; ++it) {
+        const int i = it * 32 + lane, row = i / (D / 8), ch = i % (D / 8);
+        const bool ok = key0 + row < len;
+        const long long key = ok ? key0 + row : 0;
+        const uint32_t off = sw_off<D>(row, ch);
+        cp16(dk + off, kb_ + key * p.k_sl + ch * 8, ok);
+        cp16(dv + off, vb_ + key * p.v_sl + ch * 8, ok);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) load(c_lo + warp + s * kSplitWarps, s);
+
+  // query rows, zeros past R
+  for (int i = tid; i < ROWS * (D / 8); i += blockDim.x) {
+    const int r = i / (D / 8), ch = i % (D / 8);
+    alignas(16) T e[8];
+#pragma unroll
+    for (int x = 0; x < 8; ++x) e[x] = Mma<T>::from_f(0.f);
+    if (r0 + r < p.R) {
+      int rb, rh, rtt;
+      split_row(p, b, hk, r0 + r, rb, rh, rtt);
+      const T *qp = reinterpret_cast<const T *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + ch * 8;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) e[x] = qp[x];
+    }
+    *reinterpret_cast<uint4 *>(sQ + sw_off<D>(r, ch)) = *reinterpret_cast<uint4 *>(e);
+  }
+  __syncthreads();
+
+  constexpr bool QREG = D <= 128 && MT == 1;
+  const uint32_t qa = smem_u32(sQ);
+  uint32_t qf[QREG ? KS : 1][4];
+  auto ldq = [&](int mt, int ks, uint32_t *a) {
+    const int row = mt * 16 + (lane & 15), ch = ks * 2 + (lane >> 4);
+    ldsm_x4(qa + sw_off<D>(row, ch), a[0], a[1], a[2], a[3]);
+  };
+  if constexpr (QREG)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) ldq(0, ks, qf[ks]);
+
+  float acc[MT][NT][4], m[MT][2], l[MT][2];
+  int qlast[MT][2];  // newest key that the row sees
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[mt][n][e] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[mt][h] = -INFINITY;
+      l[mt][h] = 0.f;
+      const int r = r0 + mt * 16 + g + 8 * h;
+      qlast[mt][h] = p.causal ? len - p.T + r % p.T : len - 1;
+    }
+  }
+  const int all_see = p.causal ? len - p.T : len - 1;  // newest key that every row sees
+
+  int st = 0;
+  for (int c = c_lo + warp; c < c_hi; c += kSplitWarps) {
+    cp_wait<NST - 2>();
+    __syncwarp();
+    {
+      int nst = st + NST - 1;
+      if (nst >= NST) nst -= NST;
+      load(c + (NST - 1) * kSplitWarps, nst);
+    }
+    const uint32_t ka = smem_u32(wring + st * C::STAGE), va = ka + KC * D * 2;
+    float gate;
+    const int key0 = key_of(c, gate);
+    // ---- S = Q K^T
+    float s[MT][KC / 8][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < KC / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if constexpr (QREG) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) a[mt][e] = qf[ks][e];
+        } else {
+          ldq(mt, ks, a[mt]);
+        }
+      }
+#pragma unroll
+      for (int n2 = 0; n2 < KC / 16; ++n2) {
+        uint32_t b0, b1, b2, b3;
+        const int row = n2 * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
+        ldsm_x4(ka + sw_off<D>(row, ch), b0, b1, b2, b3);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          Mma<T>::run(s[mt][2 * n2], a[mt], b0, b1);
+          Mma<T>::run(s[mt][2 * n2 + 1], a[mt], b2, b3);
+        }
+      }
+    }
+    // ---- online softmax (log2 domain); masked and missing keys are -inf
+    const bool masked = key0 + KC - 1 > all_see;
+    const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < KC / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = fmaf(s[mt][n][e], p.scale2, gate);
+          if (masked && key0 + n * 8 + tq * 2 + (e & 1) > qlast[mt][e >> 1]) x = -INFINITY;
+          s[mt][n][e] = x;
+          mx[e >> 1] = fmax_nan(mx[e >> 1], x);
+        }
+      if (p.logits) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = r0 + mt * 16 + g + 8 * h;
+          if (r < p.R) {
+            float *lp = p.logits + ((long long)grpid * p.R + r) * p.ncap + (long long)c * KC + tq * 2;
+#pragma unroll
+            for (int n = 0; n < KC / 8; ++n)
+              *reinterpret_cast<float2 *>(lp + n * 8) = make_float2(s[mt][n][2 * h], s[mt][n][2 * h + 1]);
+          }
+        }
+      }
+      float al[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+        mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+        const float mn = fmax_nan(m[mt][h], mx[h]);
+        al[h] = mn == -INFINITY ? 1.f : ex2(m[mt][h] - mn);
+        m[mt][h] = mn;
+      }
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) l[mt][h] *= al[h];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[mt][n][e] *= al[e >> 1];
+      }
+      const float off[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0], m[mt][1] == -INFINITY ? 0.f : m[mt][1]};
+#pragma unroll
+      for (int n = 0; n < KC / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[mt][n][e] = ex2(s[mt][n][e] - off[e >> 1]);
+          l[mt][e >> 1] += s[mt][n][e];
+        }
+    }
+    // ---- O += P V
+    if (!mixed) {
+#pragma unroll
+      for (int k2 = 0; k2 < KC / 16; ++k2) {
+        uint32_t hi[MT][4], lo[MT][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float x = s[mt][2 * k2 + (e >> 1)][2 * (e & 1)], y = s[mt][2 * k2 + (e >> 1)][2 * (e & 1) + 1];
+            hi[mt][e] = Mma<T>::pack(x, y);
+            const T *ht = reinterpret_cast<const T *>(&hi[mt][e]);
+            lo[mt][e] = Mma<T>::pack(x - Mma<T>::to_f(ht[0]), y - Mma<T>::to_f(ht[1]));
+          }
+#pragma unroll
+        for (int n2 = 0; n2 < NT / 2; ++n2) {
+          uint32_t b0, b1, b2, b3;
+          const int row = k2 * 16 + (lane & 15), ch = n2 * 2 + (lane >> 4);
+          ldsm_x4_t(va + sw_off<D>(row, ch), b0, b1, b2, b3);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            Mma<T>::run(acc[mt][2 * n2], hi[mt], b0, b1);
+            Mma<T>::run(acc[mt][2 * n2 + 1], hi[mt], b2, b3);
+            Mma<T>::run(acc[mt][2 * n2], lo[mt], b0, b1);
+            Mma<T>::run(acc[mt][2 * n2 + 1], lo[mt], b2, b3);
+          }
+        }
+      }
+    } else {
+      // P through the chunk's K buffer (its reads are done), then key by key
+      __syncwarp();
+      float *sp = reinterpret_cast<float *>(wring + st * C::STAGE);  // [ROWS][KC]
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int n = 0; n < KC / 8; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sp[(mt * 16 + g + 8 * (e >> 1)) * KC + n * 8 + tq * 2 + (e & 1)] = s[mt][n][e];
+      __syncwarp();
+      const uint8_t *sv = wring + st * C::STAGE + KC * D * 2;
+#pragma unroll 1
+      for (int k = 0; k < KC && key0 + k < len; ++k) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const float pa = sp[(mt * 16 + g) * KC + k], pb = sp[(mt * 16 + g + 8) * KC + k];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const T *vp = reinterpret_cast<const T *>(sv + sw_off<D>(k, n) + tq * 4);
+            const float v0 = Mma<T>::to_f(vp[0]), v1 = Mma<T>::to_f(vp[1]);
+            if (pa != 0.f) {
+              acc[mt][n][0] = fmaf(pa, v0, acc[mt][n][0]);
+              acc[mt][n][1] = fmaf(pa, v1, acc[mt][n][1]);
+            }
+            if (pb != 0.f) {
+              acc[mt][n][2] = fmaf(pb, v0, acc[mt][n][2]);
+              acc[mt][n][3] = fmaf(pb, v1, acc[mt][n][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    if (++st == NST) st = 0;
+  }
+
+  // ---- join the four warps
+  cp_wait<0>();
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
+      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
+      if (tq == 0) {
+        s_m[warp][mt * 16 + g + 8 * h] = m[mt][h];
+        s_l[warp][mt * 16 + g + 8 * h] = l[mt][h];
+      }
+    }
+  __syncthreads();
+  float *so = reinterpret_cast<float *>(ring);  // [warp][ROWS][D]
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = mt * 16 + g + 8 * h;
+      float M = s_m[0][r];
+#pragma unroll
+      for (int w = 1; w < kSplitWarps; ++w) M = fmax_nan(M, s_m[w][r]);
+      const float f = m[mt][h] == -INFINITY ? 0.f : ex2(m[mt][h] - M);
+      if (r0 + r < p.R) {
+        float *op = so + (warp * ROWS + r) * D + tq * 2;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          *reinterpret_cast<float2 *>(op + n * 8) = make_float2(acc[mt][n][2 * h] * f, acc[mt][n][2 * h + 1] * f);
+      }
+    }
+  __syncthreads();
+  const int nr = min(ROWS, p.R - r0);
+  for (int i = tid; i < nr * (D / 4); i += blockDim.x) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    float4 o = *reinterpret_cast<const float4 *>(so + r * D + d);
+#pragma unroll
+    for (int w = 1; w < kSplitWarps; ++w) {
+      const float4 x = *reinterpret_cast<const float4 *>(so + (w * ROWS + r) * D + d);
+      o.x += x.x;
+      o.y += x.y;
+      o.z += x.z;
+      o.w += x.w;
+    }
+    int rb, rh, rtt;
+    const long long at = (long long)split * p.rows + split_row(p, b, hk, r0 + r, rb, rh, rtt);
+    *reinterpret_cast<float4 *>(p.po + at * D + d) = o;
+    if (d == 0) {
+      float M = s_m[0][r], L = 0.f;
+#pragma unroll
+      for (int w = 1; w < kSplitWarps; ++w) M = fmax_nan(M, s_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < kSplitWarps; ++w)
+        L += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2(s_m[w][r] - M);
+      p.pml[at] = make_float2(M, L);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ fp32
+// CTA = 8 warps over (K/V head group, 8*WR query rows, split).  Key tiles of KT
+// rows (K and V) are staged by cp.async for the whole CTA; warp w takes rows
+// 8*(w % WR).. and every (8/WR)-th group of the tile's keys, so few rows split the
+// keys and many rows share them.  A key's dot products with the 8 rows: each lane
+// multiplies its 16-byte slice of K with the rows' slices (kept in registers) and
+// a butterfly that halves the number of values at every step leaves row r's sum in
+// the lanes whose index bits spell r.  P V runs on the same slices.
+template <int D>
+struct SplitF32 {
+  static constexpr int LPK = D >= 128 ? 32 : D / 4;  // lanes per key
+  static constexpr int KP = 32 / LPK;                // keys side by side in a warp
+  static constexpr int V4 = D / 4 / LPK;             // 16-byte slices per lane
+  static constexpr int KT = D == 256 ? 16 : 32;      // keys per tile
+  static constexpr int NST = 3;
+  static constexpr int STAGE = KT * D * 4 * 2;
+  static constexpr int MINB = D == 256 ? 1 : 2;      // 128 registers hold q and O at D 256
+};
+
+template <int D, int WR>
+__global__ void __launch_bounds__(256, SplitF32<D>::MINB)
+    split_f32_kernel(const SplitParams p, int rtiles, int min_tiles) {
+  using C = SplitF32<D>;
+  constexpr int LPK = C::LPK, KP = C::KP, V4 = C::V4, KT = C::KT, NST = C::NST, WK = 8 / WR;
+  constexpr int ROWS = 8 * WR;
+  constexpr int KW = KT / WK;      // keys of a tile for one warp
+  constexpr int IT = KW / KP > 0 ? KW / KP : 1;
+  static_assert(KW % KP == 0, "a warp's share of the tile is whole steps");
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int s_blk[kMaxLive], s_raw[kMaxLive];
+  __shared__ float s_gate[kMaxLive];
+  __shared__ int s_n;
+  __shared__ float s_m[8][8], s_l[8][8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp % WR, wk = warp / WR;
+  const int rt = blockIdx.x % rtiles, grpid = blockIdx.x / rtiles;
+  const int b = p.fold ? 0 : grpid / p.Hkv, hk = grpid % p.Hkv;
+  const int r0 = rt * ROWS + wr * 8;
+
+  int len = p.nkeys;
+  if (p.lens) {
+    len = __ldg(p.lens + b);
+    if (len < 0 || len > p.nkeys) {
+      if (tid == 0) report(p.status, BSA_DEVERR_INDEX);
+      len = len < 0 ? 0 : p.nkeys;
+    }
+  }
+  int nv = len;
+  if (p.sel) {
+    if (warp == 0) {
+      const int n = build_live(p, b, hk, len, s_blk, s_gate, s_raw);
+      if (lane == 0) s_n = n;
+      if (p.live && blockIdx.y == 0 && rt == 0) {
+        __syncwarp();
+        int *lv = p.live + (long long)grpid * (1 + p.kk);
+        for (int i = lane; i < n; i += 32) lv[1 + i] = s_blk[i];
+        if (lane == 0) lv[0] = n;
+      }
+    }
+    __syncthreads();
+    nv = s_n * p.bs;
+  }
+  const int nt = (nv + KT - 1) / KT;
+  const int tps = max(min_tiles, (nt + p.nsplit - 1) / p.nsplit);
+  const int t_lo = min(nt, (int)blockIdx.y * tps), t_hi = min(nt, t_lo + tps);
+  const int split = p.split0 + blockIdx.y;
+  if (t_lo >= t_hi) {
+    for (int r = tid; r < ROWS; r += blockDim.x)
+      if (rt * ROWS + r < p.R) {
+        int rb, rh, rtt;
+        const long long gr = split_row(p, b, hk, rt * ROWS + r, rb, rh, rtt);
+        p.pml[(long long)split * p.rows + gr] = make_float2(-INFINITY, 0.f);
+      }
+    return;
+  }
+  const float *kb_ = reinterpret_cast<const float *>(p.k) + (p.fold ? 0 : b * p.k_sb) + hk * p.k_sh;
+  const float *vb_ = reinterpret_cast<const float *>(p.v) + (p.fold ? 0 : b * p.v_sb) + hk * p.v_sh;
+  auto key_of = [&](int t, float &gate) -> int {
+    const int j = t * KT;
+    if (!p.sel) {
+      gate = 0.f;
+      return j;
+    }
+    const int i = j / p.bs;
+    gate = s_gate[i];
+    return s_blk[i] * p.bs + (j - i * p.bs);
+  };
+  auto load = [&](int t, int st) {
+    if (t < t_hi) {
+      float gt;
+      const int key0 = key_of(t, gt);
+      const uint32_t dk = smem_u32(sm + st * C::STAGE), dv = dk + KT * D * 4;
+#pragma unroll
+      for (int it = 0; it < KT * D / 4 / 256; ++it) {
+        const int i = it * 256 + tid, row = i / (D / 4), ch = i % (D / 4);
+        const bool ok = key0 + row < len;
+        const long long key = ok ? key0 + row : 0;
+        cp16(dk + i * 16, kb_ + key * p.k_sl + ch * 4, ok);
+        cp16(dv + i * 16, vb_ + key * p.v_sl + ch * 4, ok);
+      }
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) load(t_lo + s, s);
+
+  const int kl = lane / LPK, dl = lane % LPK;  // this lane's key among KP, and slice
+  float q[8][V4 * 4], acc[8][V4 * 4];
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    const float *qp = nullptr;
+    if (r0 + r < p.R) {
+      int rb, rh, rtt;
+      split_row(p, b, hk, r0 + r, rb, rh, rtt);
+      qp = reinterpret_cast<const float *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl;
+    }
+#pragma unroll
+    for (int x = 0; x < V4 * 4; ++x) {
+      q[r][x] = qp ? qp[(x / 4) * LPK * 4 + dl * 4 + (x & 3)] : 0.f;
+      acc[r][x] = 0.f;
+    }
+  }
+  // the row whose sums end in this lane
+  const int myrow = LPK == 32 ? lane >> 2 : LPK == 16 ? (lane >> 1) & 7 : lane & 7;
+  constexpr int RSH = LPK == 32 ? 2 : LPK == 16 ? 1 : 0;  // lane of row r: (kl * LPK) + (r << RSH)
+  const int qlast = p.causal ? len - p.T + (r0 + myrow) % p.T : len - 1;
+  const int all_see = p.causal ? len - p.T : len - 1;
+  float m = -INFINITY, l = 0.f;
+  float *lrow = p.logits && r0 + myrow < p.R && (LPK != 32 || (lane & 3) == 0) &&
+                        (LPK != 16 || (lane & 1) == 0)
+                    ? p.logits + ((long long)grpid * p.R + r0 + myrow) * p.ncap
+                    : nullptr;
+
+  int st = 0;
+  for (int t = t_lo; t < t_hi; ++t) {
+    cp_wait<NST - 2>();
+    __syncthreads();
+    {
+      int nst = st + NST - 1;
+      if (nst >= NST) nst -= NST;
+      load(t + NST - 1, nst);
+    }
+    if (r0 < p.R) {
+      float gate;
+      const int key0 = key_of(t, gate);
+      const float *sk = reinterpret_cast<const float *>(sm + st * C::STAGE), *sv = sk + KT * D;
+      const bool masked = key0 + KT - 1 > all_see;
+      constexpr int BT = IT < 4 ? IT : 4;  // steps whose maximum is taken together
+#pragma unroll 1
+      for (int i0 = 0; i0 < IT; i0 += BT) {
+        float x[BT];
+#pragma unroll
+        for (int i = 0; i < BT; ++i) {
+          const int kr = wk * KW + (i0 + i) * KP + kl;
+          float d[8];
+#pragma unroll
+          for (int r = 0; r < 8; ++r) d[r] = 0.f;
+#pragma unroll
+          for (int v = 0; v < V4; ++v) {
+            const float4 k4 = *reinterpret_cast<const float4 *>(sk + kr * D + v * LPK * 4 + dl * 4);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+              d[r] = fmaf(q[r][v * 4], k4.x, d[r]);
+              d[r] = fmaf(q[r][v * 4 + 1], k4.y, d[r]);
+              d[r] = fmaf(q[r][v * 4 + 2], k4.z, d[r]);
+              d[r] = fmaf(q[r][v * 4 + 3], k4.w, d[r]);
+            }
+          }
+#pragma unroll
+          for (int h = 4, sh = LPK / 2; h >= 1; h >>= 1, sh >>= 1) {
+            const bool up = lane & sh;
+#pragma unroll
+            for (int r = 0; r < h; ++r) {
+              const float keep = up ? d[r + h] : d[r], give = up ? d[r] : d[r + h];
+              d[r] = keep + __shfl_xor_sync(0xffffffffu, give, sh);
+            }
+          }
+          if (LPK == 32) d[0] += __shfl_xor_sync(0xffffffffu, d[0], 2);
+          if (LPK >= 16) d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
+          x[i] = fmaf(d[0], p.scale2, gate);
+          if (masked && key0 + kr > qlast) x[i] = -INFINITY;
+          if (lrow) lrow[(long long)t * KT + kr] = x[i];
+        }
+        float mx = x[0];
+#pragma unroll
+        for (int i = 1; i < BT; ++i) mx = fmax_nan(mx, x[i]);
+        if (KP >= 2) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        if (KP >= 4) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        const float mn = fmax_nan(m, mx);
+        const float al = mn == -INFINITY ? 1.f : ex2(m - mn);
+        m = mn;
+        if (__any_sync(0xffffffffu, al != 1.f)) {
+          l *= al;
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const float ar = __shfl_sync(0xffffffffu, al, kl * LPK + (r << RSH));
+#pragma unroll
+            for (int e = 0; e < V4 * 4; ++e) acc[r][e] *= ar;
+          }
+        }
+        const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < BT; ++i) {
+          const float pr = ex2(x[i] - off);
+          l += pr;
+          const int kr = wk * KW + (i0 + i) * KP + kl;
+          float v[V4 * 4];
+#pragma unroll
+          for (int w = 0; w < V4; ++w) {
+            const float4 v4 = *reinterpret_cast<const float4 *>(sv + kr * D + w * LPK * 4 + dl * 4);
+            v[w * 4] = v4.x;
+            v[w * 4 + 1] = v4.y;
+            v[w * 4 + 2] = v4.z;
+            v[w * 4 + 3] = v4.w;
+          }
+#pragma unroll
+          for (int r = 0; r < 8; ++r) {
+            const float pv = __shfl_sync(0xffffffffu, pr, kl * LPK + (r << RSH));
+            if (!masked || pv != 0.f) {
+#pragma unroll
+              for (int e = 0; e < V4 * 4; ++e) acc[r][e] = fmaf(pv, v[e], acc[r][e]);
+            }
+          }
+        }
+      }
+    }
+    if (++st == NST) st = 0;
+  }
+  // ---- join the warps of a row group (and the KP keys side by side)
+  cp_wait<0>();
+  if (KP >= 2) l += __shfl_xor_sync(0xffffffffu, l, 16);
+  if (KP >= 4) l += __shfl_xor_sync(0xffffffffu, l, 8);
+  s_m[warp][myrow] = m;
+  s_l[warp][myrow] = l;
+  __syncthreads();
+  float *so = reinterpret_cast<float *>(sm);  // [wk][ROWS][D]
+#pragma unroll
+  for (int r = 0; r < 8; ++r) {
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) M = fmax_nan(M, s_m[w * WR + wr][r]);
+    const float mm = s_m[warp][r];
+    const float f = mm == -INFINITY ? 0.f : ex2(mm - M);
+#pragma unroll
+    for (int x = 0; x < V4 * 4; ++x) {
+      float a = acc[r][x] * f;
+      if (KP >= 2) a += __shfl_xor_sync(0xffffffffu, a, 16);
+      if (KP >= 4) a += __shfl_xor_sync(0xffffffffu, a, 8);
+      if (kl == 0) so[(wk * ROWS + wr * 8 + r) * D + (x / 4) * LPK * 4 + dl * 4 + (x & 3)] = a;
+    }
+  }
+  __syncthreads();
+  const int nr = min(ROWS, p.R - rt * ROWS);
+  for (int i = tid; i < nr * D; i += 256) {
+    const int r = i / D, d = i % D;
+    float o = so[r * D + d];
+#pragma unroll
+    for (int w = 1; w < WK; ++w) o += so[(w * ROWS + r) * D + d];
+    int rb, rh, rtt;
+    const long long at = (long long)split * p.rows + split_row(p, b, hk, rt * ROWS + r, rb, rh, rtt);
+    p.po[at * D + d] = o;
+    if (d == 0) {
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; ++w) M = fmax_nan(M, s_m[w * WR + r / 8][r % 8]);
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float mw = s_m[w * WR + r / 8][r % 8];
+        L += mw == -INFINITY ? 0.f : s_l[w * WR + r / 8][r % 8] * ex2(mw - M);
+      }
+      p.pml[at] = make_float2(M, L);
+    }
+  }
+}
+
+// ------------------------------------------------------------------ join
+struct JoinParams {
+  void *o;
+  int64_t o_sb, o_sh, o_sl;
+  int B, Hq, Hkv, grp, T, D, nsplit, R;
+  long long rows;
+  const float *po;
+  const float2 *pml;
+  const float *logits;  // with weights
+  long long ncap;
+  const int *live;
+  int kk, bs, L;
+  float *weight;
+  int64_t w_sb, w_sh;
+  int wtiles;           // weight blocks per (b, hk); they follow the row blocks
+};
+
+constexpr int kJoinThreads = 256;
+
+// Row blocks: one query row each; the warps take every eighth split, lanes the
+// columns.  Weight blocks: 1024 slots of one (b, hk): lse of its R rows from the
+// splits' (m, l), then the sum over the rows, in row order, of 2^(x - lse).
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinParams p) {
+  extern __shared__ float sj[];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (blockIdx.x < p.rows) {
+    const long long gr = blockIdx.x;
+    __shared__ float s_f[8];
+    float m = -INFINITY;
+    for (int s = tid; s < p.nsplit; s += kJoinThreads) m = fmax_nan(m, p.pml[s * p.rows + gr].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if (lane == 0) s_f[warp] = m;
+    __syncthreads();
+    float M = s_f[0];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) M = fmax_nan(M, s_f[w]);
+    // this warp's splits: columns lane*4 + 128*c
+    float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+    float l = 0.f;
+    if (M != -INFINITY)
+      for (int s = warp; s < p.nsplit; s += 8) {
+        const float2 ml = p.pml[s * p.rows + gr];
+        if (ml.x == -INFINITY) continue;
+        const float f = ex2(ml.x - M);
+        l = fmaf(ml.y, f, l);
+        const float *op = p.po + (s * p.rows + gr) * p.D;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int d = lane * 4 + 128 * c;
+          if (d < p.D) {
+            const float4 x = *reinterpret_cast<const float4 *>(op + d);
+            acc[c].x = fmaf(x.x, f, acc[c].x);
+            acc[c].y = fmaf(x.y, f, acc[c].y);
+            acc[c].z = fmaf(x.z, f, acc[c].z);
+            acc[c].w = fmaf(x.w, f, acc[c].w);
+          }
+        }
+      }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int d = lane * 4 + 128 * c;
+      if (d < p.D) *reinterpret_cast<float4 *>(sj + warp * p.D + d) = acc[c];
+    }
+    __shared__ float s_l[8];
+    if (lane == 0) s_l[warp] = l;
+    __syncthreads();
+    if (tid < p.D) {
+      float o = 0.f, lt = 0.f;
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        o += sj[w * p.D + tid];
+        lt += s_l[w];
+      }
+      const float y = lt == 0.f ? 0.f : o / lt;
+      const int t = (int)(gr % p.T);
+      const long long bh = gr / p.T;
+      T *op = reinterpret_cast<T *>(p.o) + (bh / p.Hq) * p.o_sb + (bh % p.Hq) * p.o_sh + t * p.o_sl + tid;
+      if constexpr (sizeof(T) == 2)
+        *op = Mma<T>::from_f(y);
+      else
+        *op = y;
+    }
+    return;
+  }
+  const long long wb = blockIdx.x - p.rows;
+  const int bh = (int)(wb / p.wtiles), tile = (int)(wb % p.wtiles);
+  const int b = bh / p.Hkv, hk = bh % p.Hkv;
+  for (int r = warp; r < p.R; r += 8) {
+    const long long gr = ((long long)b * p.Hq + hk * p.grp) * p.T + r;
+    float m = -INFINITY;
+    for (int s = lane; s < p.nsplit; s += 32) m = fmax_nan(m, p.pml[s * p.rows + gr].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f;
+    for (int s = lane; s < p.nsplit; s += 32) {
+      const float2 ml = p.pml[s * p.rows + gr];
+      if (ml.x != -INFINITY) l = fmaf(ml.y, ex2(ml.x - m), l);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lane == 0) {  // offset and factor: p = 2^(x - m) / l
+      sj[2 * r] = l == 0.f ? INFINITY : m;
+      sj[2 * r + 1] = l == 0.f ? 0.f : 1.f / l;
+    }
+  }
+  __syncthreads();
+  const int *lv = p.live ? p.live + (long long)bh * (1 + p.kk) : nullptr;
+  const long long nv = lv ? (long long)lv[0] * p.bs : p.L;
+  const float *lg = p.logits + (long long)bh * p.R * p.ncap;
+  float *wp = p.weight + b * p.w_sb + hk * p.w_sh;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const long long j = tile * 1024LL + i * kJoinThreads + tid;
+    if (j >= nv) break;
+    long long key = j;
+    if (lv) {
+      const long long blk = j / p.bs;
+      key = (long long)lv[1 + blk] * p.bs + (j - blk * p.bs);
+    }
+    if (key >= p.L) continue;
+    float w = 0.f;
+    for (int r = 0; r < p.R; ++r) w = fmaf(ex2(lg[(long long)r * p.ncap + j] - sj[2 * r]), sj[2 * r + 1], w);
+    wp[key] += w;
+  }
+}
+
+// ------------------------------------------------------------------ launchers
+// Number of key splits: the one with the least (waves of CTAs) x (key steps of a
+// CTA + its fixed cost in steps), for `groups` CTAs per split and `slots` resident.
+static int choose_split(long long groups, long long steps, int slots, int fixed, int cap) {
+  long long best = -1;
+  int ns = 1;
+  for (int s = 1; s <= cap && s <= std::max<long long>(1, steps); ++s) {
+    const long long cost = ((groups * s + slots - 1) / slots) * ((steps + s - 1) / s + fixed);
+    if (best < 0 || cost < best) {
+      best = cost;
+      ns = s;
+    }
+  }
+  return ns;
+}
+
+constexpr int kMaxSplit = 296;
+
+// Splits of the mma / f32 kernels for n keys, `groups` K/V head groups and R rows each.
+int split_count(int dtype, int D, long long groups, int R, long long n) {
+  if (dtype == BSA_F32) {
+    const int kt = D == 256 ? 16 : 32;
+    const int wr = R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8;
+    const long long g = groups * ((R + 8 * wr - 1) / (8 * wr));
+    return choose_split(g, (n + kt - 1) / kt, 296, 4, kMaxSplit);
+  }
+  const int kc = D >= 128 ? 16 : 32, mt = R > 16 && D >= 64 && D <= 128 ? 2 : 1;
+  const long long g = groups * ((R + 16 * mt - 1) / (16 * mt));
+  const long long steps = (n + kc * kSplitWarps - 1) / (kc * kSplitWarps);
+  return choose_split(g, steps, D == 256 ? 148 : 296, 4, kMaxSplit);
+}
+
+template <typename T, int D, int MT>
+static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_t st) {
+  using C = SplitCfg<D>;
+  const int rtiles = (p.R + 16 * MT - 1) / (16 * MT);
+  const int smem = 16 * MT * D * 2 + C::RING;
+  auto kern = split_mma_kernel<T, D, MT>;
+  static_assert(C::RING >= kSplitWarps * 16 * MT * D * 4, "the ring holds the warps' O for the join");
+  static_assert(C::KC * D * 2 >= 16 * MT * C::KC * 4, "a chunk's K buffer holds its P");
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  kern<<<dim3((unsigned)(groups * rtiles), p.nsplit), kSplitWarps * 32, smem, st>>>(p, rtiles, kSplitWarps);
+  return check_launch("split_mma");
+}
+
+template <int D, int WR>
+static bsa_status launch_f32(const SplitParams &p, long long groups, cudaStream_t st) {
+  using C = SplitF32<D>;
+  const int rtiles = (p.R + 8 * WR - 1) / (8 * WR);
+  const int smem = C::NST * C::STAGE;
+  auto kern = split_f32_kernel<D, WR>;
+  static_assert(C::NST * C::STAGE >= 8 * 8 * D * 4, "the ring holds the warps' O for the join");
+  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  kern<<<dim3((unsigned)(groups * rtiles), p.nsplit), 256, smem, st>>>(p, rtiles, 1);
+  return check_launch("split_f32");
+}
+
+template <typename T, int D>
+static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStream_t st) {
+  if constexpr (D >= 64 && D <= 128)
+    if (p.R > 16) return launch_mma<T, D, 2>(p, groups, st);
+  return launch_mma<T, D, 1>(p, groups, st);
+}
+
+template <int D>
+static bsa_status launch_split_d(int dtype, const SplitParams &p, long long groups, cudaStream_t st) {
+  if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D>(p, groups, st);
+  if (dtype == BSA_F16) return launch_mma_d<__half, D>(p, groups, st);
+  if (p.R <= 8) return launch_f32<D, 1>(p, groups, st);
+  if (p.R <= 16) return launch_f32<D, 2>(p, groups, st);
+  if (p.R <= 32) return launch_f32<D, 4>(p, groups, st);
+  return launch_f32<D, 8>(p, groups, st);
+}
+
+bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStream_t st) {
+  const long long groups = p.fold ? p.Hkv : (long long)p.B * p.Hkv;
+  switch (D) {
+    case 32: return launch_split_d<32>(dtype, p, groups, st);
+    case 64: return launch_split_d<64>(dtype, p, groups, st);
+    case 128: return launch_split_d<128>(dtype, p, groups, st);
+    default: return launch_split_d<256>(dtype, p, groups, st);
+  }
+}
+
+static bsa_status launch_join(int dtype, const JoinParams &p, cudaStream_t st) {
+  const size_t smem = std::max<size_t>(8 * p.D * 4, p.weight ? (size_t)p.R * 8 : 0);
+  const unsigned grid = (unsigned)(p.rows + (p.weight ? (long long)p.B * p.Hkv * p.wtiles : 0));
+  if (dtype == BSA_BF16)
+    split_join_kernel<__nv_bfloat16><<<grid, kJoinThreads, smem, st>>>(p);
+  else if (dtype == BSA_F16)
+    split_join_kernel<__half><<<grid, kJoinThreads, smem, st>>>(p);
+  else
+    split_join_kernel<float><<<grid, kJoinThreads, smem, st>>>(p);
+  return check_launch("split_join");
+}
+
+static bsa_status check_rows(const char *who, int dtype, int B, int Hq, int Hkv, int D, int T, float scale) {
+  const std::string w(who);
+  if (dtype != BSA_BF16 && dtype != BSA_F16 && dtype != BSA_F32)
+    return fail(BSA_ERR_DTYPE, w + ": dtype must be bf16, f16 or f32");
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || T <= 0 || Hq % Hkv)
+    return fail(BSA_ERR_SHAPE, w + ": sizes must be positive and Hq a multiple of Hkv");
+  if (D != 32 && D != 64 && D != 128 && D != 256)
+    return fail(BSA_ERR_UNSUPPORTED, w + ": D must be 32, 64, 128 or 256");
+  if ((long long)B * Hq * T >= (1LL << 30)) return fail(BSA_ERR_SHAPE, w + ": B*Hq*T too large");
+  if (!(scale > 0.f) || !std::isfinite(scale)) return fail(BSA_ERR_ARG, w + ": bad scale");
+  return BSA_OK;
+}
+
+// A K/V operand: 16-byte aligned base and strides.
+static bsa_status check_kv(const bsa_view &v, int dtype, const char *who, const char *name, bool batch) {
+  const int64_t es = (int64_t)elem_size(dtype);
+  if (!v.ptr) return fail(BSA_ERR_ARG, std::string(who) + ": " + name + " is NULL");
+  if (reinterpret_cast<uintptr_t>(v.ptr) % 16 || (v.sl * es) % 16 || (v.sh * es) % 16 ||
+      (batch && (v.sb * es) % 16))
+    return fail(BSA_ERR_STRIDE, std::string(who) + ": " + name + " needs a 16-byte aligned base and strides");
+  return BSA_OK;
+}
+
+// ------------------------------------------------------------------ decode_weighted
+namespace {
+constexpr int kMaxWeightRows = 4096;
+struct WeightedPlan {
+  int nsplit;
+  long long ncap, rows;
+  size_t o_po, o_ml, o_lg, o_lv, bytes;
+};
+WeightedPlan weighted_plan(const bsa_decode_weighted_args *a) {
+  WeightedPlan w;
+  const int R = (a->Hq / a->Hkv) * a->T;
+  const long long n = a->sel ? (long long)a->kk * a->bs : a->L;
+  w.nsplit = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, n);
+  w.ncap = (n + 31) / 32 * 32;
+  w.rows = (long long)a->B * a->Hq * a->T;
+  w.o_po = 0;
+  w.o_ml = align_up((size_t)w.nsplit * w.rows * a->D * 4, 256);
+  w.o_lg = align_up(w.o_ml + (size_t)w.nsplit * w.rows * 8, 256);
+  w.o_lv = align_up(w.o_lg + (size_t)w.rows * w.ncap * 4, 256);
+  w.bytes = align_up(w.o_lv + (a->sel ? (size_t)a->B * a->Hkv * (1 + a->kk) * 4 : 0), 256);
+  return w;
+}
+}  // namespace
+
+static bsa_status weighted_check(const bsa_decode_weighted_args *a) {
+  if (bsa_status s = check_rows("decode_weighted", a->dtype, a->B, a->Hq, a->Hkv, a->D, a->T, a->scale)) return s;
+  if (a->L <= 0 || a->T > a->L) return fail(BSA_ERR_SHAPE, "decode_weighted: needs 1 <= T <= L");
+  if ((a->Hq / a->Hkv) * (long long)a->T > kMaxWeightRows)
+    return fail(BSA_ERR_UNSUPPORTED, "decode_weighted: (Hq/Hkv) * T must be <= 4096");
+  if (a->sel) {
+    if (a->kk <= 0) return fail(BSA_ERR_SHAPE, "decode_weighted: kk must be positive");
+    if (a->kk > kMaxLive) return fail(BSA_ERR_UNSUPPORTED, "decode_weighted: kk must be <= 512");
+    if (a->bs <= 0 || a->bs % 32) return fail(BSA_ERR_UNSUPPORTED, "decode_weighted: bs must be a multiple of 32");
+    if ((long long)a->kk * a->bs >= (1LL << 30)) return fail(BSA_ERR_SHAPE, "decode_weighted: kk*bs too large");
+  } else if (a->gate) {
+    return fail(BSA_ERR_ARG, "decode_weighted: a gate needs a selection");
+  }
+  if (a->L >= (1 << 30)) return fail(BSA_ERR_SHAPE, "decode_weighted: L too large");
+  if (!a->q.ptr || !a->o.ptr || !a->weight) return fail(BSA_ERR_ARG, "decode_weighted: NULL tensor");
+  if (bsa_status s = check_kv(a->k, a->dtype, "decode_weighted", "k", true)) return s;
+  return check_kv(a->v, a->dtype, "decode_weighted", "v", true);
+}
+
+size_t weighted_workspace(const bsa_decode_weighted_args *a) {
+  return weighted_check(a) == BSA_OK ? weighted_plan(a).bytes : 0;
+}
+
+bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_bytes, cudaStream_t st) {
+  if (bsa_status s = weighted_check(a)) return s;
+  const WeightedPlan w = weighted_plan(a);
+  if (!ws || ws_bytes < w.bytes) return fail(BSA_ERR_WORKSPACE, "decode_weighted: workspace too small");
+  uint8_t *base = static_cast<uint8_t *>(ws);
+  SplitParams p{};
+  p.q = a->q.ptr, p.q_sb = a->q.sb, p.q_sh = a->q.sh, p.q_sl = a->q.sl;
+  p.k = a->k.ptr, p.k_sb = a->k.sb, p.k_sh = a->k.sh, p.k_sl = a->k.sl;
+  p.v = a->v.ptr, p.v_sb = a->v.sb, p.v_sh = a->v.sh, p.v_sl = a->v.sl;
+  p.B = a->B, p.Hq = a->Hq, p.Hkv = a->Hkv, p.grp = a->Hq / a->Hkv, p.T = a->T;
+  p.R = p.grp * a->T;
+  p.nkeys = a->L;
+  p.causal = 1;
+  p.scale2 = a->scale * kLog2e;
+  p.sel = a->sel, p.sel_sb = a->sel_sb, p.sel_sh = a->sel_sh;
+  p.kk = a->sel ? a->kk : 0, p.bs = a->bs;
+  p.gate = a->gate, p.gate_sb = a->gate_sb, p.gate_sh = a->gate_sh;
+  p.nsplit = w.nsplit;
+  p.rows = w.rows;
+  p.po = reinterpret_cast<float *>(base + w.o_po);
+  p.pml = reinterpret_cast<float2 *>(base + w.o_ml);
+  p.logits = reinterpret_cast<float *>(base + w.o_lg);
+  p.ncap = w.ncap;
+  p.live = a->sel ? reinterpret_cast<int *>(base + w.o_lv) : nullptr;
+  p.status = a->status;
+  if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
+  JoinParams j{};
+  j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
+  j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;
+  j.nsplit = w.nsplit, j.R = p.R, j.rows = w.rows, j.po = p.po, j.pml = p.pml;
+  j.logits = p.logits, j.ncap = w.ncap, j.live = p.live, j.kk = p.kk, j.bs = a->bs, j.L = a->L;
+  j.weight = a->weight, j.w_sb = a->weight_sb, j.w_sh = a->weight_sh;
+  j.wtiles = (int)((w.ncap + 1023) / 1024);
+  return launch_join(a->dtype, j, st);
+}
+
+// ------------------------------------------------------------------ decode_prefix
+namespace {
+struct PrefixPlan {
+  int np, ns;  // splits of the prefix and of the own slots
+  long long rows;
+  size_t o_ml, bytes;
+};
+PrefixPlan prefix_plan(const bsa_decode_prefix_args *a) {
+  PrefixPlan w;
+  const int R = (a->Hq / a->Hkv) * a->T;
+  w.np = a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P) : 0;
+  w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S);
+  w.rows = (long long)a->B * a->Hq * a->T;
+  w.o_ml = align_up((size_t)(w.np + w.ns) * w.rows * a->D * 4, 256);
+  w.bytes = align_up(w.o_ml + (size_t)(w.np + w.ns) * w.rows * 8, 256);
+  return w;
+}
+}  // namespace
+
+static bsa_status prefix_check(const bsa_decode_prefix_args *a) {
+  if (bsa_status s = check_rows("decode_prefix", a->dtype, a->B, a->Hq, a->Hkv, a->D, a->T, a->scale)) return s;
+  if (a->P < 0 || a->S <= 0) return fail(BSA_ERR_SHAPE, "decode_prefix: needs P >= 0 and S >= 1");
+  if (a->P >= (1 << 30) || a->S >= (1 << 30)) return fail(BSA_ERR_SHAPE, "decode_prefix: P or S too large");
+  if (!a->q.ptr || !a->o.ptr || !a->lens) return fail(BSA_ERR_ARG, "decode_prefix: NULL tensor");
+  if (a->P > 0) {
+    if (bsa_status s = check_kv(a->pk, a->dtype, "decode_prefix", "pk", false)) return s;
+    if (bsa_status s = check_kv(a->pv, a->dtype, "decode_prefix", "pv", false)) return s;
+  }
+  if (bsa_status s = check_kv(a->k, a->dtype, "decode_prefix", "k", true)) return s;
+  return check_kv(a->v, a->dtype, "decode_prefix", "v", true);
+}
+
+size_t prefix_workspace(const bsa_decode_prefix_args *a) {
+  return prefix_check(a) == BSA_OK ? prefix_plan(a).bytes : 0;
+}
+
+bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes, cudaStream_t st) {
+  if (bsa_status s = prefix_check(a)) return s;
+  const PrefixPlan w = prefix_plan(a);
+  if (!ws || ws_bytes < w.bytes) return fail(BSA_ERR_WORKSPACE, "decode_prefix: workspace too small");
+  uint8_t *base = static_cast<uint8_t *>(ws);
+  SplitParams p{};
+  p.q = a->q.ptr, p.q_sb = a->q.sb, p.q_sh = a->q.sh, p.q_sl = a->q.sl;
+  p.B = a->B, p.Hq = a->Hq, p.Hkv = a->Hkv, p.grp = a->Hq / a->Hkv, p.T = a->T;
+  p.scale2 = a->scale * kLog2e;
+  p.rows = w.rows;
+  p.po = reinterpret_cast<float *>(base);
+  p.pml = reinterpret_cast<float2 *>(base + w.o_ml);
+  p.status = a->status;
+  if (a->P > 0) {
+    p.k = a->pk.ptr, p.k_sb = 0, p.k_sh = a->pk.sh, p.k_sl = a->pk.sl;
+    p.v = a->pv.ptr, p.v_sb = 0, p.v_sh = a->pv.sh, p.v_sl = a->pv.sl;
+    p.fold = 1;
+    p.R = a->B * p.grp * a->T;
+    p.nkeys = a->P;
+    p.split0 = 0, p.nsplit = w.np;
+    if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
+  }
+  p.k = a->k.ptr, p.k_sb = a->k.sb, p.k_sh = a->k.sh, p.k_sl = a->k.sl;
+  p.v = a->v.ptr, p.v_sb = a->v.sb, p.v_sh = a->v.sh, p.v_sl = a->v.sl;
+  p.fold = 0;
+  p.R = p.grp * a->T;
+  p.nkeys = a->S;
+  p.lens = a->lens;
+  p.causal = 1;
+  p.split0 = w.np, p.nsplit = w.ns;
+  if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
+  JoinParams j{};
+  j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
+  j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;
+  j.nsplit = w.np + w.ns, j.R = p.R, j.rows = w.rows, j.po = p.po, j.pml = p.pml;
+  return launch_join(a->dtype, j, st);
+}
+
+}  // namespace bsa

@@ -1,0 +1,57 @@
+// Split attention of a few query rows over a long K/V: parameters shared by the
+// partial kernels (mma.sync, fp32 and tcgen05) and by the kernel that joins them.
+//
+// Every partial kernel leaves, for each query row and each split of the keys,
+//   m = max_j x_j,   l = sum_j 2^(x_j - m),   O = sum_j 2^(x_j - m) v_j
+// in fp32, with x_j = (scale * q.k_j + gate) * log2(e).  The join is
+//   M = max_s m_s,   o = (sum_s 2^(m_s - M) O_s) / (sum_s 2^(m_s - M) l_s),
+// so splits of one cache and splits of two different K/V (a shared prefix and a
+// sequence's own slots) are joined alike.
+#pragma once
+#include "bsa_common.cuh"
+
+namespace bsa {
+
+struct SplitParams {
+  const void *q;
+  int64_t q_sb, q_sh, q_sl;
+  const void *k, *v;
+  int64_t k_sb, k_sh, k_sl, v_sb, v_sh, v_sl;
+  int B, Hq, Hkv, grp, T;
+  int fold;             // 1: the rows of all sequences read one K/V (a shared prefix)
+  int R;                // query rows per K/V head: grp*T, or B*grp*T when folded
+  int nkeys;            // rows of k, v in use (the capacity when lens is given)
+  const int32_t *lens;  // optional (B): each sequence's own count, clamped to [0, nkeys]
+  int causal;           // row t sees key j <= len - T + t (else every key)
+  float scale2;         // scale * log2(e)
+  const int32_t *sel;   // optional block ids per (b, hk)
+  int64_t sel_sb, sel_sh;
+  int kk, bs;
+  const float *gate;
+  int64_t gate_sb, gate_sh;
+  int split0, nsplit;   // this kernel's splits are split0 .. split0 + nsplit - 1
+  long long rows;       // B*Hq*T
+  float *po;            // [split][rows][D]
+  float2 *pml;          // [split][rows] (m, l); m = -inf: nothing visible, O not written
+  float *logits;        // optional [b*Hkv + hk][R][ncap]: x_j of each row
+  long long ncap;
+  int *live;            // with sel and logits: [b*Hkv + hk][1 + kk] count and live block ids
+  int32_t *status;
+};
+
+// Global row (b*Hq + h)*T + t of local row r of K/V head hk.
+__device__ __forceinline__ long long split_row(const SplitParams &p, int b, int hk, int r, int &rb,
+                                               int &rh, int &rt) {
+  const int per = p.grp * p.T;
+  if (p.fold) {
+    rb = r / per;
+    r -= rb * per;
+  } else {
+    rb = b;
+  }
+  rh = hk * p.grp + r / p.T;
+  rt = r % p.T;
+  return ((long long)rb * p.Hq + rh) * p.T + rt;
+}
+
+}  // namespace bsa

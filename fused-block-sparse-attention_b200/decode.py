@@ -15,25 +15,53 @@ cache (kept incrementally: an append re-pools only the blocks it touches),
 then causal top-k + own block (+ sink) sorted ascending (:87-99).  Attention
 masks are the TOKEN rules (key position <= query position, repeated ids
 once), as in blocksparse_forward.
+
+A cache within a budget.  With track=True the cache also keeps, per slot, the sum of
+the attention weight it has received and its token position; a decode step through
+decode_attention_weighted adds to the sums, and evict keeps the slots of most weight
+beside the first `sink` and the last `recent` tokens:
+
+    cache = DecodeCache(B, Hkv, 4096 + 64, D, bs=128, track=True)
+    o = decode_attention_weighted(q_new, cache)     # every slot; or sel, as above
+    cache.evict(4096, recent=256, sink=4)
+
+A survivor may move to a freed slot (cache.pos tells its token position), so keys are
+cached with their rotary embedding already applied, as the attention expects them.
+
+A batch behind one prefix.  PrefixCache holds the prefix's K/V once and every
+sequence's own continuation, of any length; prefix_attention reads the prefix once
+for the whole batch:
+
+    cache = PrefixCache(prefix_k, prefix_v, B, max_len)   # (Hkv, P, D) each
+    cache.append(k_new, v_new)                      # (B, Hkv, T, D) each
+    o = prefix_attention(q_new, cache)              # (B, Hq, T, D)
 """
 import torch
 
 import _bsa
 
-__all__ = ["DecodeCache", "decode_attention"]
+__all__ = ["DecodeCache", "decode_attention", "decode_attention_weighted", "PrefixCache",
+           "prefix_attention"]
 
 
 class DecodeCache:
-    """K/V cache (B, Hkv, max_len, D) with per-block min / max key summaries."""
+    """K/V cache (B, Hkv, max_len, D) with per-block min / max key summaries; with
+    track=True also each slot's accumulated attention weight (fp32) and token position
+    (int32), both (B, Hkv, max_len)."""
 
-    def __init__(self, B, Hkv, max_len, D, *, bs, dtype=torch.bfloat16, device="cuda"):
+    def __init__(self, B, Hkv, max_len, D, *, bs, dtype=torch.bfloat16, device="cuda", track=False):
         self.bs = bs
         self.k = torch.zeros(B, Hkv, max_len, D, dtype=dtype, device=device)
         self.v = torch.zeros_like(self.k)
         nblk = (max_len + bs - 1) // bs
         self.kmin = torch.zeros(B, Hkv, nblk, D, dtype=torch.float32, device=device)
         self.kmax = torch.zeros_like(self.kmin)
-        self.L = 0
+        self.L = 0          # slots in use
+        self.seen = 0       # tokens appended so far
+        self.weight = self.pos = None
+        if track:
+            self.weight = torch.zeros(B, Hkv, max_len, dtype=torch.float32, device=device)
+            self.pos = torch.zeros(B, Hkv, max_len, dtype=torch.int32, device=device)
 
     def append(self, k_new, v_new):
         T = k_new.shape[2]
@@ -49,6 +77,24 @@ class DecodeCache:
                            vmin=True, vmax=True)
         self.kmin[:, :, b0:b1] = mn
         self.kmax[:, :, b0:b1] = mx
+        if self.weight is not None:
+            self.weight[:, :, L0:L1] = 0
+            self.pos[:, :, L0:L1] = torch.arange(self.seen, self.seen + T, dtype=torch.int32,
+                                                 device=self.pos.device)
+        self.seen += T
+
+    def evict(self, budget, *, recent=0, sink=0):
+        """Keeps `budget` slots per (b, hk): the first `sink` and last `recent` tokens,
+        then the slots of most accumulated weight.  Returns how many slots went."""
+        if self.weight is None:
+            raise ValueError("evict needs a cache with track=True")
+        gone = self.L - budget
+        if gone <= 0:
+            return 0
+        _bsa.evict(self.k, self.v, self.weight, self.pos, budget=budget, L=self.L, seen=self.seen,
+                   recent=recent, sink=sink, kmin=self.kmin, kmax=self.kmax, bs=self.bs)
+        self.L = budget
+        return gone
 
     def select_quest(self, q_new, *, topk, sink=True):
         """(B, Hkv, W) block ids for the current block: Quest bound of the new tokens'
@@ -71,3 +117,56 @@ def decode_attention(q_new, cache, sel, gate=None, *, scale=None, mask_mode=_bsa
     """o (B, Hq, T, D) of the T newest tokens attending to their selected cache blocks."""
     return _bsa.decode(q_new, cache.k, cache.v, sel, gate, bs=cache.bs, L=cache.L,
                        mask_mode=mask_mode, scale=scale)
+
+
+def decode_attention_weighted(q_new, cache, sel=None, gate=None, *, scale=None):
+    """decode_attention under TOKEN masks that also adds every slot's attention weight to
+    cache.weight (a cache with track=True).  sel=None attends to every slot."""
+    if cache.weight is None:
+        raise ValueError("decode_attention_weighted needs a cache with track=True")
+    return _bsa.decode_weighted(q_new, cache.k, cache.v, cache.weight, sel, gate, bs=cache.bs,
+                                L=cache.L, scale=scale)
+
+
+class PrefixCache:
+    """The K/V of one prefix, (Hkv, P, D) each and not copied, and the continuations of B
+    sequences behind it: k, v (B, Hkv, max_len, D), lens int32 (B,) on the device."""
+
+    def __init__(self, prefix_k, prefix_v, B, max_len):
+        if prefix_k.dim() != 3 or prefix_v.shape != prefix_k.shape:
+            raise ValueError("prefix_k and prefix_v must be (Hkv, P, D)")
+        Hkv, _, D = prefix_k.shape
+        self.prefix_k, self.prefix_v = prefix_k, prefix_v
+        self.k = torch.zeros(B, Hkv, max_len, D, dtype=prefix_k.dtype, device=prefix_k.device)
+        self.v = torch.zeros_like(self.k)
+        self.lens = torch.zeros(B, dtype=torch.int32, device=prefix_k.device)
+        self.used = [0] * B     # the same lengths on the host
+
+    def append(self, k_new, v_new, active=None):
+        """Appends T tokens (B, Hkv, T, D) to every sequence, or to those whose entry of
+        `active` (B truth values) is true."""
+        T = k_new.shape[2]
+        who = [b for b in range(len(self.used)) if active is None or active[b]]
+        if any(self.used[b] + T > self.k.shape[2] for b in who):
+            raise ValueError("cache full")
+        dev = self.k.device
+        b = torch.tensor(who, device=dev, dtype=torch.long)
+        at = torch.tensor([self.used[i] for i in who], device=dev, dtype=torch.long).view(-1, 1) + \
+            torch.arange(T, device=dev)
+        self.k[b.view(-1, 1), :, at] = k_new[b].transpose(1, 2).to(self.k.dtype)
+        self.v[b.view(-1, 1), :, at] = v_new[b].transpose(1, 2).to(self.v.dtype)
+        self.lens[b] += T
+        for i in who:
+            self.used[i] += T
+
+    def reset(self, b):
+        """Empties the continuation of sequence b (a new question about the same prefix)."""
+        self.used[b] = 0
+        self.lens[b] = 0
+
+
+def prefix_attention(q_new, cache, *, scale=None):
+    """o (B, Hq, T, D) of every sequence's T newest tokens attending to the shared prefix
+    and to their own continuation (a PrefixCache)."""
+    return _bsa.decode_prefix(q_new, cache.prefix_k, cache.prefix_v, cache.k, cache.v, cache.lens,
+                              scale=scale)

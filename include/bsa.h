@@ -258,6 +258,83 @@ size_t bsa_decode_workspace(const bsa_decode_args *a);
 bsa_status bsa_decode(const bsa_decode_args *a, void *workspace, size_t workspace_bytes,
                       bsa_stream_t stream);
 
+/* Decode with a running sum of attention weight: bsa_decode's step for the T
+ * newest tokens (positions L-T .. L-1, no block boundary implied), which also adds
+ * every slot's attention weight to weight[b, hk, slot]: the sum over the query
+ * heads of the group and the T rows of softmax(scale * q.k + gate).  sel == NULL
+ * reads every slot; otherwise int32 block ids (B, Hs, kk) under TOKEN masks (key
+ * position <= query position, a repeated id counts once, an id outside the cache is
+ * skipped and reported, a block whose gate is -inf is skipped), and the other slots'
+ * sums stay as they are.  A row that sees no key gives o = 0 and no weight.  Masked and unused K/V rows
+ * may hold anything, infinities and NaN included.  No counterpart in the reference.
+ * Limits: D 32, 64, 128 or 256; (Hq/Hkv) * T <= 4096; bs a multiple of 32 and
+ * kk <= 512 with a selection; k, v bases and strides multiples of 16 bytes.  Device
+ * workspace: the splits' partial sums and the fp32 logits (4 bytes per query row
+ * and slot). */
+typedef struct {
+  int32_t dtype, B, Hq, Hkv, L, D, bs, T, kk;
+  float scale;
+  bsa_view q, k, v, o;
+  const int32_t *sel;
+  int64_t sel_sb, sel_sh;
+  const float *gate; /* optional, addressed like sel */
+  int64_t gate_sb, gate_sh;
+  float *weight; /* fp32 (B, Hkv, >= L), unit stride along the slots */
+  int64_t weight_sb, weight_sh;
+  int32_t *status;
+} bsa_decode_weighted_args;
+size_t bsa_decode_weighted_workspace(const bsa_decode_weighted_args *a);
+bsa_status bsa_decode_weighted(const bsa_decode_weighted_args *a, void *workspace,
+                               size_t workspace_bytes, bsa_stream_t stream);
+
+/* Reduction of a cache from L slots to `budget`, per (b, hk).  Best first: slots
+ * whose token position pos is < sink or >= seen - recent, then by weight (NaN with
+ * -infinity last), ties to the lower slot; the first `budget` survive.  Survivors in
+ * slots < budget stay; the others fill the freed slots, both in ascending order:
+ * the fewest rows move, and slots >= budget keep their contents.  k, v: (B, Hkv,
+ * >= L, D), changed in place.  weight_out, pos_out: (B, Hkv, >= budget), the
+ * survivors' sums and positions; they may be weight and pos themselves.  kmin, kmax
+ * (optional, both or none): fp32 per-block min / max of the keys (block stride
+ * km_sn, unit D stride) as bsa_pool computes them; blocks whose rows changed are
+ * pooled anew, and a last block that ends at the budget counts zeros past it.
+ * No counterpart in the reference.  D 32, 64, 128 or 256; bs <= 1024. */
+typedef struct {
+  int32_t dtype, B, Hkv, L, D, bs, budget, recent, sink, seen;
+  bsa_view k, v;
+  const float *weight;
+  int64_t w_sb, w_sh;
+  const int32_t *pos;
+  int64_t p_sb, p_sh;
+  float *weight_out;
+  int64_t wo_sb, wo_sh;
+  int32_t *pos_out;
+  int64_t po_sb, po_sh;
+  float *kmin, *kmax;
+  int64_t km_sb, km_sh, km_sn;
+} bsa_evict_args;
+size_t bsa_evict_workspace(const bsa_evict_args *a);
+bsa_status bsa_evict(const bsa_evict_args *a, void *workspace, size_t workspace_bytes,
+                     bsa_stream_t stream);
+
+/* Decode of a batch whose sequences share a prefix: pk, pv (Hkv, P, D; the sb of
+ * their views is unused) are read once for the whole batch, k, v (B, Hkv, S, D) are
+ * each sequence's own continuation, of which lens[b] slots are in use (the T new
+ * tokens the last of them; clamped to [0, S], reported when outside).  Row t sees
+ * the whole prefix and the own slots j <= lens[b] - T + t; o = softmax over both.
+ * A row that sees no key gives 0.  P may be 0.  Unused and masked slots may hold
+ * anything.  No counterpart in the reference.  D 32, 64, 128 or 256; k, v, pk, pv
+ * bases and strides multiples of 16 bytes.  Workspace: the splits' partial sums. */
+typedef struct {
+  int32_t dtype, B, Hq, Hkv, D, P, S, T;
+  float scale;
+  bsa_view q, pk, pv, k, v, o;
+  const int32_t *lens;
+  int32_t *status;
+} bsa_decode_prefix_args;
+size_t bsa_decode_prefix_workspace(const bsa_decode_prefix_args *a);
+bsa_status bsa_decode_prefix(const bsa_decode_prefix_args *a, void *workspace,
+                             size_t workspace_bytes, bsa_stream_t stream);
+
 /* Top-k of a caller-supplied score matrix with _finish semantics (reference
  * src/qwen_blocksparse.py:87-99): per row i of score (G, nblk, nblk) (element
  * strides score_sg, score_si, unit column stride) the top min(topk, nblk) over
