@@ -1065,6 +1065,10 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
 }
 
 // ------------------------------------------------------------------ decode_prefix
+bool prefix_sm100_applicable(const bsa_decode_prefix_args *a);
+int prefix_sm100_splits(const bsa_decode_prefix_args *a);
+bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParams &p, cudaStream_t st);
+
 namespace {
 struct PrefixPlan {
   int np, ns;  // splits of the prefix and of the own slots
@@ -1074,7 +1078,9 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(const bsa_decode_prefix_args *a) {
   PrefixPlan w;
   const int R = (a->Hq / a->Hkv) * a->T;
-  w.np = a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P) : 0;
+  w.np = a->P <= 0                    ? 0
+         : prefix_sm100_applicable(a) ? prefix_sm100_splits(a)
+                                      : split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P);
   w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S);
   w.rows = (long long)a->B * a->Hq * a->T;
   w.o_ml = align_up((size_t)(w.np + w.ns) * w.rows * a->D * 4, 256);
@@ -1120,7 +1126,8 @@ bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes
     p.R = a->B * p.grp * a->T;
     p.nkeys = a->P;
     p.split0 = 0, p.nsplit = w.np;
-    if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
+    if (bsa_status s = prefix_sm100_applicable(a) ? launch_prefix_sm100(a, p, st) : launch_split(a->dtype, a->D, p, st))
+      return s;
   }
   p.k = a->k.ptr, p.k_sb = a->k.sb, p.k_sh = a->k.sh, p.k_sl = a->k.sl;
   p.v = a->v.ptr, p.v_sb = a->v.sb, p.v_sh = a->v.sh, p.v_sl = a->v.sl;
