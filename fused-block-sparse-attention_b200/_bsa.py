@@ -6,6 +6,7 @@ the library is missing, or a tensor is not on a CUDA device, it raises.
 """
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -266,8 +267,11 @@ _status = {}
 
 def status_tensor(device):
     """The persistent device status word of `device` (int32, cleared by check_status)."""
-    dev = torch.device(device)
-    key = dev.index if dev.index is not None else torch.cuda.current_device()
+    if isinstance(device, int):
+        key = device
+    else:
+        dev = torch.device(device)
+        key = dev.index if dev.index is not None else torch.cuda.current_device()
     if key not in _status:
         _status[key] = torch.zeros(1, dtype=torch.int32, device="cuda:%d" % key)
     return _status[key]
@@ -564,33 +568,39 @@ def decode(q, k, v, sel, gate=None, *, bs, L=None, mask_mode=MASK_TOKEN, scale=N
     return o
 
 
-def _same_device(first, **ts):
-    """Every tensor given lives on first's CUDA device."""
-    _need_cuda(first)
-    for name, t in ts.items():
-        if t is not None and t.device != first.device:
+def _same_device(names, first, *ts):
+    """Every tensor given (None: absent) lives on first's CUDA device.  Returns its index."""
+    dev = first.get_device()
+    if dev < 0:
+        _need_cuda(first)
+    for i, t in enumerate(ts):
+        if t is not None and t.get_device() != dev:
             _need_cuda(t)
-            raise BsaShapeError(ERR_ARG, "%s is on %s, q / k on %s" % (name, t.device, first.device))
+            raise BsaShapeError(ERR_ARG, "%s is on %s, the first operand on %s" %
+                                (names[i], t.device, first.device))
+    return dev
 
 
-def _cache_operand(t, name, B, Hkv, D, dtype):
-    """A K/V operand that is read or changed in place: never copied."""
-    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != Hkv or t.shape[3] != D:
-        raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, *, %d); got %s" % (name, B, Hkv, D, tuple(t.shape)))
+def _cache_operand(t, name, shape, st, B, Hkv, D, dtype):
+    """A K/V operand (its shape and strides) that is read or changed in place: never copied."""
+    if len(shape) != 4 or shape[0] != B or shape[1] != Hkv or shape[3] != D:
+        raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, *, %d); got %s" % (name, B, Hkv, D, tuple(shape)))
     if t.dtype != dtype:
         raise BsaError(ERR_DTYPE, "%s must be %s; got %s" % (name, dtype, t.dtype))
-    if t.stride(3) != 1:
+    if st[3] != 1:
         raise BsaError(ERR_STRIDE, "%s must have unit stride along D" % name)
 
 
 def _row_operand(t, name, B, Hkv, n, dtype):
-    """A (B, Hkv, >= n) per-slot tensor with unit stride along the slots."""
-    if t.dim() != 3 or t.shape[0] != B or t.shape[1] != Hkv or t.shape[2] < n:
-        raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, >= %d); got %s" % (name, B, Hkv, n, tuple(t.shape)))
+    """Strides of a (B, Hkv, >= n) per-slot tensor with unit stride along the slots."""
+    shape, st = t.shape, t.stride()
+    if len(shape) != 3 or shape[0] != B or shape[1] != Hkv or shape[2] < n:
+        raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, >= %d); got %s" % (name, B, Hkv, n, tuple(shape)))
     if t.dtype != dtype:
         raise BsaError(ERR_DTYPE, "%s must be %s; got %s" % (name, dtype, t.dtype))
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    if shape[2] > 1 and st[2] != 1:
         raise BsaError(ERR_STRIDE, "%s must have unit stride along the slots" % name)
+    return st
 
 
 def _query_out(q, out):
@@ -600,27 +610,44 @@ def _query_out(q, out):
     if q.stride(3) != 1:
         q = q.contiguous()
     if out is None:
-        return q, torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        return q, torch.empty_like(q, memory_format=torch.contiguous_format)
     if out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise BsaShapeError(ERR_SHAPE, "out must have q's shape and dtype and unit stride along D")
     return q, out
 
 
-def _launch(name, a, t):
-    """Workspace and launch of entry point `name` on t's device and its current stream."""
-    if t.device.index != torch.cuda.current_device():
-        with torch.cuda.device(t.device):
-            return _launch(name, a, t)
-    L, ref = lib(), ctypes.byref(a)
-    nbytes = getattr(L, name + "_workspace")(ref)
+def _format(cls):
+    """struct format of a ctypes structure: packing a flat tuple costs a fifth of filling
+    the structure, and a decode step is short enough to notice."""
+    code = {ctypes.c_int32: "i", ctypes.c_float: "f", ctypes.c_void_p: "P", ctypes.c_int64: "q", View: "Pqqq"}
+    return struct.Struct("@" + "".join(code[f] for _, f in cls._fields_) + "0P")
+
+
+_PACK = {"bsa_decode_weighted": _format(DecodeWeightedArgs), "bsa_evict": _format(EvictArgs),
+         "bsa_decode_prefix": _format(DecodePrefixArgs)}
+_packed_fn = {}
+
+
+def _launch(name, packed, dev):
+    """Workspace and launch of entry point `name` (its argument struct as bytes) on CUDA
+    device `dev` and its current stream."""
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _launch(name, packed, dev)
+    if name not in _packed_fn:
+        run, size = lib()[name], lib()[name + "_workspace"]
+        run.restype, size.restype = ctypes.c_int, ctypes.c_size_t
+        run.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
+        size.argtypes = [ctypes.c_char_p]
+        _packed_fn[name] = run, size
+    run, size = _packed_fn[name]
+    nbytes = size(packed)
     if nbytes == 0:   # validation failed: the call reports why
-        _check(getattr(L, name)(ref, None, 0, _stream()))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=t.device)
-    _check(getattr(L, name)(ref, ws.data_ptr(), nbytes, _stream()))
-
-
-def _v4(t):
-    return (t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))
+        _check(run(packed, None, 0, None))
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    st = run(packed, ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+    if st:
+        _check(st)
 
 
 def decode_weighted(q, k, v, weight, sel=None, gate=None, *, bs=None, L=None, scale=None, out=None):
@@ -630,45 +657,43 @@ def decode_weighted(q, k, v, weight, sel=None, gate=None, *, bs=None, L=None, sc
     sum over hk's query heads and the T rows of their softmax weight on slot j.
     sel: int32 (B, kk) or (B, 1 or Hkv, kk) ids of blocks of bs slots (None: every
     slot), TOKEN masks; gate: optional fp32 like sel.  Returns o (B, Hq, T, D)."""
-    _same_device(q, k=k, v=v, weight=weight, sel=sel, gate=gate, out=out)
+    dev = _same_device(("k", "v", "weight", "sel", "gate", "out"), q, k, v, weight, sel, gate, out)
     q, o = _query_out(q, out)
     B, Hq, T, D = q.shape
-    if k.dim() != 4:
-        raise BsaShapeError(ERR_SHAPE, "k must be (B, Hkv, >= L, D)")
-    Hkv = k.shape[1]
-    _cache_operand(k, "k", B, Hkv, D, q.dtype)
-    _cache_operand(v, "v", B, Hkv, D, q.dtype)
-    L = min(k.shape[2], v.shape[2]) if L is None else int(L)
-    if L > min(k.shape[2], v.shape[2]):
+    ks, vs, kst, vst = k.shape, v.shape, k.stride(), v.stride()
+    Hkv, dt = ks[1] if len(ks) == 4 else -1, q.dtype
+    _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
+    _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
+    cap = min(ks[2], vs[2])
+    L = cap if L is None else int(L)
+    if L > cap:
         raise BsaShapeError(ERR_SHAPE, "decode_weighted: L = %d is more than k and v hold" % L)
-    _row_operand(weight, "weight", B, Hkv, L, torch.float32)
-    kk = s_sb = s_sh = g_sb = g_sh = 0
+    wst = _row_operand(weight, "weight", B, Hkv, L, torch.float32)
+    kk = s_ptr = s_sb = s_sh = g_ptr = g_sb = g_sh = status = 0
     if sel is not None:
         if bs is None or not 0 < bs < 2 ** 30:
             raise BsaShapeError(ERR_ARG, "decode_weighted: a selection needs its block size bs")
         if sel.dtype != torch.int32 or sel.stride(-1) != 1:
             sel = sel.to(torch.int32).contiguous()
-        if not ((sel.dim() == 2 and sel.shape[0] == B) or
-                (sel.dim() == 3 and sel.shape[0] == B and sel.shape[1] in (1, Hkv))):
+        ss, sst = sel.shape, sel.stride()
+        if not (ss[0] == B and (len(ss) == 2 or (len(ss) == 3 and ss[1] in (1, Hkv)))):
             raise BsaShapeError(ERR_SHAPE, "decode_weighted: sel must be (B, kk) or (B, Hkv, kk)")
-        kk, s_sb = sel.shape[-1], sel.stride(0)
-        s_sh = sel.stride(1) if sel.dim() == 3 and sel.shape[1] > 1 else 0
+        kk, s_ptr, s_sb = ss[-1], sel.data_ptr(), sst[0]
+        s_sh = sst[1] if len(ss) == 3 and ss[1] > 1 else 0
+        status = status_tensor(dev).data_ptr()
         if gate is not None:
-            if gate.shape != sel.shape:
+            if gate.shape != ss:
                 raise BsaShapeError(ERR_SHAPE, "decode_weighted: gate must have the shape of sel")
             if gate.dtype != torch.float32 or gate.stride(-1) != 1:
                 gate = gate.to(torch.float32).contiguous()
-            g_sb = gate.stride(0)
-            g_sh = gate.stride(1) if gate.dim() == 3 and gate.shape[1] > 1 else 0
+            gst = gate.stride()
+            g_ptr, g_sb, g_sh = gate.data_ptr(), gst[0], gst[1] if s_sh or (len(ss) == 3 and ss[1] > 1) else 0
     elif gate is not None:
         raise BsaShapeError(ERR_ARG, "decode_weighted: a gate needs a selection")
-    a = DecodeWeightedArgs(
+    _launch("bsa_decode_weighted", _PACK["bsa_decode_weighted"].pack(
         _dtype(q), B, Hq, Hkv, L, D, bs if sel is not None else 0, T, kk, D ** -0.5 if scale is None else scale,
-        _v4(q), _v4(k), _v4(v), _v4(o), sel.data_ptr() if sel is not None else None, s_sb, s_sh,
-        gate.data_ptr() if gate is not None else None, g_sb, g_sh,
-        weight.data_ptr(), weight.stride(0), weight.stride(1),
-        status_tensor(q.device).data_ptr() if sel is not None else None)
-    _launch("bsa_decode_weighted", a, q)
+        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *kst[:3], v.data_ptr(), *vst[:3], o.data_ptr(),
+        *o.stride()[:3], s_ptr, s_sb, s_sh, g_ptr, g_sb, g_sh, weight.data_ptr(), wst[0], wst[1], status), dev)
     return o
 
 
@@ -682,46 +707,50 @@ def evict(k, v, weight, pos, *, budget, L=None, seen=None, recent=0, sink=0, kmi
     weight / pos follow (into weight_out / pos_out when given), and kmin / kmax (fp32
     (B, Hkv, >= ceil(budget / bs), D), both or none) of the changed blocks of bs slots
     are pooled anew."""
-    _same_device(k, v=v, weight=weight, pos=pos, kmin=kmin, kmax=kmax, weight_out=weight_out,
-                 pos_out=pos_out)
-    if k.dim() != 4:
+    dev = _same_device(("v", "weight", "pos", "kmin", "kmax", "weight_out", "pos_out"), k, v, weight, pos,
+                       kmin, kmax, weight_out, pos_out)
+    ks, vs, kst, vst = k.shape, v.shape, k.stride(), v.stride()
+    if len(ks) != 4:
         raise BsaShapeError(ERR_SHAPE, "k must be (B, Hkv, >= L, D)")
-    B, Hkv, cap, D = k.shape
-    _cache_operand(k, "k", B, Hkv, D, k.dtype)
-    _cache_operand(v, "v", B, Hkv, D, k.dtype)
-    L = min(cap, v.shape[2]) if L is None else int(L)
-    if L > min(cap, v.shape[2]):
+    B, Hkv, cap, D = ks
+    _cache_operand(k, "k", ks, kst, B, Hkv, D, k.dtype)
+    _cache_operand(v, "v", vs, vst, B, Hkv, D, k.dtype)
+    cap = min(cap, vs[2])
+    L = cap if L is None else int(L)
+    if L > cap:
         raise BsaShapeError(ERR_SHAPE, "evict: L = %d is more than k and v hold" % L)
     seen = L if seen is None else int(seen)
-    if not (0 < budget <= L and 0 <= recent <= budget and 0 <= sink <= budget and L <= seen < 2 ** 31):
+    if not (0 < budget <= L <= seen < 2 ** 31 and 0 <= recent <= budget and 0 <= sink <= budget):
         raise BsaShapeError(ERR_SHAPE, "evict: needs 1 <= budget <= L <= seen < 2^31 and recent, sink "
                                        "within the budget")
     if bs is not None and not 0 < bs <= 1024:
         raise BsaShapeError(ERR_SHAPE, "evict: bs must lie in 1 .. 1024")
-    wo = weight if weight_out is None else weight_out
-    po = pos if pos_out is None else pos_out
-    _row_operand(weight, "weight", B, Hkv, L, torch.float32)
-    _row_operand(pos, "pos", B, Hkv, L, torch.int32)
-    _row_operand(wo, "weight_out", B, Hkv, budget, torch.float32)
-    _row_operand(po, "pos_out", B, Hkv, budget, torch.int32)
-    if (kmin is None) != (kmax is None):
-        raise BsaShapeError(ERR_ARG, "evict: kmin and kmax go together")
-    km, kx, km_st = None, None, (0, 0, 0)
-    if kmin is not None:
+    wst = _row_operand(weight, "weight", B, Hkv, L, torch.float32)
+    pst = _row_operand(pos, "pos", B, Hkv, L, torch.int32)
+    wo, wost, po, post = weight, wst, pos, pst
+    if weight_out is not None:
+        wo, wost = weight_out, _row_operand(weight_out, "weight_out", B, Hkv, budget, torch.float32)
+    if pos_out is not None:
+        po, post = pos_out, _row_operand(pos_out, "pos_out", B, Hkv, budget, torch.int32)
+    km = kx = 0
+    kmst = (0, 0, 0, 1)
+    if kmin is not None and kmax is not None:
         if bs is None:
             raise BsaShapeError(ERR_ARG, "evict: kmin and kmax need bs")
-        nb = (budget + bs - 1) // bs
+        kmst = kmin.stride()
         for name, t in (("kmin", kmin), ("kmax", kmax)):
-            _cache_operand(t, name, B, Hkv, D, torch.float32)
-            if t.shape[2] < nb or t.stride() != kmin.stride():
-                raise BsaShapeError(ERR_SHAPE, "evict: kmin and kmax need one layout and %d blocks" % nb)
-        km, kx, km_st = kmin.data_ptr(), kmax.data_ptr(), kmin.stride()[:3]
-    a = EvictArgs(
+            s, st = t.shape, t.stride()
+            _cache_operand(t, name, s, st, B, Hkv, D, torch.float32)
+            if s[2] * bs < budget or st != kmst:
+                raise BsaShapeError(ERR_SHAPE, "evict: kmin and kmax need one layout and ceil(budget / bs) blocks")
+        km, kx = kmin.data_ptr(), kmax.data_ptr()
+    elif kmin is not None or kmax is not None:
+        raise BsaShapeError(ERR_ARG, "evict: kmin and kmax go together")
+    _launch("bsa_evict", _PACK["bsa_evict"].pack(
         _dtype(k), B, Hkv, L, D, 64 if bs is None else bs, budget, recent, sink, seen,
-        _v4(k), _v4(v), weight.data_ptr(), weight.stride(0), weight.stride(1),
-        pos.data_ptr(), pos.stride(0), pos.stride(1), wo.data_ptr(), wo.stride(0), wo.stride(1),
-        po.data_ptr(), po.stride(0), po.stride(1), km, kx, *km_st)
-    _launch("bsa_evict", a, k)
+        k.data_ptr(), *kst[:3], v.data_ptr(), *vst[:3], weight.data_ptr(), wst[0], wst[1],
+        pos.data_ptr(), pst[0], pst[1], wo.data_ptr(), wost[0], wost[1], po.data_ptr(), post[0], post[1],
+        km, kx, *kmst[:3]), dev)
 
 
 def decode_prefix(q, pk, pv, k, v, lens, *, scale=None, out=None):
@@ -729,27 +758,28 @@ def decode_prefix(q, pk, pv, k, v, lens, *, scale=None, out=None):
     pk, pv (Hkv, P, D): the prefix, read once for the batch; k, v (B, Hkv, S, D): each
     sequence's own slots, lens int32 (B,) of them in use, the T new tokens last.  Row t
     sees the prefix and the own slots j <= lens[b] - T + t.  Returns o (B, Hq, T, D)."""
-    _same_device(q, pk=pk, pv=pv, k=k, v=v, lens=lens, out=out)
+    dev = _same_device(("pk", "pv", "k", "v", "lens", "out"), q, pk, pv, k, v, lens, out)
     q, o = _query_out(q, out)
     B, Hq, T, D = q.shape
-    if k.dim() != 4 or pk.dim() != 3 or pv.shape != pk.shape:
+    ks, vs, ps, kst, vst, pkst, pvst = k.shape, v.shape, pk.shape, k.stride(), v.stride(), pk.stride(), pv.stride()
+    if len(ks) != 4 or len(ps) != 3 or pv.shape != ps:
         raise BsaShapeError(ERR_SHAPE, "decode_prefix: k, v must be (B, Hkv, S, D) and pk, pv (Hkv, P, D)")
-    Hkv, S = k.shape[1], k.shape[2]
-    _cache_operand(k, "k", B, Hkv, D, q.dtype)
-    _cache_operand(v, "v", B, Hkv, D, q.dtype)
-    if v.shape[2] != S:
+    Hkv, S, dt = ks[1], ks[2], q.dtype
+    _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
+    _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
+    if vs[2] != S:
         raise BsaShapeError(ERR_SHAPE, "decode_prefix: k and v hold different numbers of slots")
-    pk, pv = pk.unsqueeze(0), pv.unsqueeze(0)
-    _cache_operand(pk, "pk", 1, Hkv, D, q.dtype)
-    _cache_operand(pv, "pv", 1, Hkv, D, q.dtype)
+    _cache_operand(pk, "pk", (1, *ps), (0, *pkst), 1, Hkv, D, dt)
+    _cache_operand(pv, "pv", (1, *ps), (0, *pvst), 1, Hkv, D, dt)
     if lens.dim() != 1 or lens.shape[0] != B or lens.is_floating_point():
         raise BsaShapeError(ERR_SHAPE, "decode_prefix: lens must be (B,) whole numbers")
     if lens.dtype != torch.int32 or not lens.is_contiguous():
         lens = lens.to(torch.int32).contiguous()
-    a = DecodePrefixArgs(
-        _dtype(q), B, Hq, Hkv, D, pk.shape[2], S, T, D ** -0.5 if scale is None else scale,
-        _v4(q), _v4(pk), _v4(pv), _v4(k), _v4(v), _v4(o), lens.data_ptr(), status_tensor(q.device).data_ptr())
-    _launch("bsa_decode_prefix", a, q)
+    _launch("bsa_decode_prefix", _PACK["bsa_decode_prefix"].pack(
+        _dtype(q), B, Hq, Hkv, D, ps[1], S, T, D ** -0.5 if scale is None else scale,
+        q.data_ptr(), *q.stride()[:3], pk.data_ptr(), 0, pkst[0], pkst[1], pv.data_ptr(), 0, pvst[0], pvst[1],
+        k.data_ptr(), *kst[:3], v.data_ptr(), *vst[:3], o.data_ptr(), *o.stride()[:3], lens.data_ptr(),
+        status_tensor(dev).data_ptr()), dev)
     return o
 
 

@@ -137,6 +137,15 @@ __device__ __forceinline__ void prefetch_tmap(const CUtensorMap *map) {
   asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
 }
 
+// Programmatic dependent launch: the first lets the next kernel of the stream (when
+// launched by launch_after) start once every CTA of this one has called it or left;
+// the second waits until every kernel before this one has finished and its writes are
+// visible.
+__device__ __forceinline__ void pdl_trigger() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- swizzle
 // A tile of R rows x D cols (16-bit elements) is stored as D/64 regions of
 // R x 128 bytes, each written by one TMA box with CU_TENSOR_MAP_SWIZZLE_128B:

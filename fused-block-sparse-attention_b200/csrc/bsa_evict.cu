@@ -44,147 +44,171 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sink, int fi
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// Inclusive-to-exclusive block scan of one int per thread (1024 threads); total
-// in *total.  s: 33 ints.
-__device__ __forceinline__ int block_scan(int v, int *s, int *total) {
+// Exclusive prefix over the 32 warps of one count per warp (the same in all its
+// lanes) and the total over the CTA; s: 32 ints of its own, one barrier.
+__device__ __forceinline__ int warp_prefix(int v, int *s, int *total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
+  if (lane == 0) s[warp] = v;
+  __syncthreads();
+  const int mine = s[lane];
+  int x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
     if (lane >= o) x += y;
   }
-  __syncthreads();
-  if (lane == 31) s[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    int y = s[lane];
-    const int y0 = y;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
-    }
-    s[lane] = y - y0;
-    if (lane == 31) s[32] = y;
-  }
-  __syncthreads();
-  *total = s[32];
-  return s[warp] + x - v;
+  *total = __shfl_sync(0xffffffffu, x, 31);
+  return __shfl_sync(0xffffffffu, x - mine, warp);
 }
 }  // namespace
 
-__global__ void __launch_bounds__(kPickThreads) evict_pick_kernel(const bsa_evict_args a, const EvictWork w) {
+// IPT > 0: a thread's IPT keys stay in registers (up to 8 * 1024 * 16 slots per
+// head); IPT = 0: they are read again in every pass, for any length.  Warp w of a CTA
+// owns 32 * ipt consecutive slots, lane l of it slots l, l + 32, ..., so a rank among
+// them is a ballot, and one prefix over the warps per list.
+template <int IPT>
+__global__ void __launch_bounds__(kPickThreads)
+    evict_pick_kernel(const bsa_evict_args a, const EvictWork w, const int ipt_) {
   cg::cluster_group cl = cg::this_cluster();
   const int nc = cl.num_blocks(), rank = cl.block_rank();
   const int bh = blockIdx.x / nc, b = bh / a.Hkv, h = bh % a.Hkv;
-  const int tid = threadIdx.x;
-  __shared__ int hist[kBins];
-  __shared__ int s_scan[33];
-  __shared__ int s_bin, s_need, s_cnt[3];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const unsigned below = (1u << lane) - 1u;
+  pdl_trigger();
+  __shared__ int hist[3][kBins];
+  __shared__ int s_scan[6][32];
+  __shared__ int s_bin[3], s_need[3], s_cnt[3];
   const float *wt = a.weight + b * a.w_sb + h * a.w_sh;
   const int32_t *ps = a.pos + b * a.p_sb + h * a.p_sh;
   const int first_recent = a.seen - a.recent;
-  // this CTA's slots, a multiple of the block size of the scans
-  const int per = ((a.L + nc - 1) / nc + kPickThreads - 1) / kPickThreads * kPickThreads;
-  const int lo = min(a.L, rank * per), hi = min(a.L, lo + per);
-  auto key = [&](int i) { return evict_key(__ldg(wt + i), __ldg(ps + i), a.sink, first_recent); };
+  const int ipt = IPT > 0 ? IPT : ipt_;
+  const int base = (rank * 32 + warp) * 32 * ipt + lane;  // this lane's first slot
+  auto read = [&](int s) -> uint32_t {
+    return s < a.L ? evict_key(__ldg(wt + s), __ldg(ps + s), a.sink, first_recent) : 0u;
+  };
+  uint32_t kr[IPT > 0 ? IPT : 1];
+  if constexpr (IPT > 0)
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) kr[i] = read(base + 32 * i);
+  auto key = [&](int i) -> uint32_t {
+    if constexpr (IPT > 0)
+      return kr[i];
+    else
+      return read(base + 32 * i);
+  };
+  auto sync_all = [&] {
+    if (nc > 1)
+      cl.sync();
+    else
+      __syncthreads();
+  };
+  for (int i = tid; i < 3 * kBins; i += kPickThreads) (&hist[0][0])[i] = 0;
+  __syncthreads();
 
   // ---- key of the budget-th best slot, 11 + 11 + 10 bits from the top
   uint32_t prefix = 0;
   int need = a.budget;  // slots still wanted among those that share the prefix
-  const int shift[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
 #pragma unroll
-  for (int ps_ = 0; ps_ < 3; ++ps_) {
-    const int sh = shift[ps_], nb = 1 << bits[ps_];
-    for (int i = tid; i < kBins; i += kPickThreads) hist[i] = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += kPickThreads) {
+  for (int r3 = 0; r3 < 3; ++r3) {
+    const int sh = r3 == 0 ? 21 : r3 == 1 ? 10 : 0, nb = r3 == 2 ? 1024 : 2048;
+    int *hs = hist[r3];
+#pragma unroll
+    for (int i = 0; i < ipt; ++i) {
       const uint32_t k = key(i);
-      if (ps_ == 0 || (k >> (sh + bits[ps_])) == prefix) atomicAdd(&hist[(k >> sh) & (nb - 1)], 1);
+      if (base + 32 * i < a.L && (r3 == 0 || (k >> (sh + (r3 == 2 ? 10 : 11))) == prefix))
+        atomicAdd(&hs[(k >> sh) & (nb - 1)], 1);
     }
-    cl.sync();
+    sync_all();
     // bins from the top, two per thread; sums over the cluster
     int c0 = 0, c1 = 0;
     const int b0 = nb - 1 - 2 * tid, b1 = b0 - 1;
     if (b1 >= 0)
       for (int r = 0; r < nc; ++r) {
-        const int *hr = cl.map_shared_rank(hist, r);
+        const int *hr = cl.map_shared_rank(hs, r);
         c0 += hr[b0];
         c1 += hr[b1];
       }
-    int total;
-    const int before = block_scan(c0 + c1, s_scan, &total);
-    if (before < need && before + c0 >= need) {
-      s_bin = b0;
-      s_need = need - before;
-    } else if (before + c0 < need && before + c0 + c1 >= need) {
-      s_bin = b1;
-      s_need = need - before - c0;
+    int x = c0 + c1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
     }
-    cl.sync();  // also: nobody reads a histogram any more
-    prefix = (prefix << bits[ps_]) | (uint32_t)s_bin;
-    need = s_need;
+    int total;
+    const int before = warp_prefix(__shfl_sync(0xffffffffu, x, 31), s_scan[r3], &total) + x - c0 - c1;
+    if (before < need && before + c0 >= need) {
+      s_bin[r3] = b0;
+      s_need[r3] = need - before;
+    } else if (before + c0 < need && before + c0 + c1 >= need) {
+      s_bin[r3] = b1;
+      s_need[r3] = need - before - c0;
+    }
     __syncthreads();
+    prefix = (prefix << (r3 == 2 ? 10 : 11)) | (uint32_t)s_bin[r3];
+    need = s_need[r3];
   }
   const uint32_t kth = prefix;  // better keys survive, and the first `need` equal ones
 
-  // ---- equal keys before this CTA's slots
+  // ---- equal keys before this warp's slots
   int eq = 0;
-  for (int i = lo + tid; i < hi; i += kPickThreads) eq += key(i) == kth;
+#pragma unroll
+  for (int i = 0; i < ipt; ++i)
+    eq += __popc(__ballot_sync(0xffffffffu, base + 32 * i < a.L && key(i) == kth));
   int eq_total;
-  block_scan(eq, s_scan, &eq_total);
-  if (tid == 0) s_cnt[0] = eq_total;
-  cl.sync();
-  int eq_before = 0;
-  for (int r = 0; r < rank; ++r) eq_before += cl.map_shared_rank(s_cnt, r)[0];
-  // ---- freed slots below the budget and survivors beyond it, in this CTA
-  int holes = 0, tails = 0, e0 = eq_before;
-  for (int i0 = lo; i0 < hi; i0 += kPickThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < hi ? key(i) : 0u;
-    const bool same = i < hi && k == kth;
-    int t;
-    const int er = block_scan(same, s_scan, &t) + e0;
-    e0 += t;
-    const bool keep = i < hi && (k > kth || (same && er < need));
-    holes += i < hi && i < a.budget && !keep;
-    tails += i < hi && i >= a.budget && keep;
+  int eq0 = warp_prefix(eq, s_scan[3], &eq_total);
+  if (nc > 1) {
+    if (tid == 0) s_cnt[0] = eq_total;
+    cl.sync();
+    for (int r = 0; r < rank; ++r) eq0 += cl.map_shared_rank(s_cnt, r)[0];
   }
-  int ht, tt;
-  block_scan(holes, s_scan, &ht);
-  block_scan(tails, s_scan, &tt);
-  if (tid == 0) s_cnt[1] = ht, s_cnt[2] = tt;
-  cl.sync();
-  int hb = 0, tb = 0;
-  for (int r = 0; r < rank; ++r) {
-    hb += cl.map_shared_rank(s_cnt, r)[1];
-    tb += cl.map_shared_rank(s_cnt, r)[2];
+  // ---- freed slots below the budget and survivors beyond it, in this warp
+  int holes = 0, tails = 0, e = eq0;
+#pragma unroll
+  for (int i = 0; i < ipt; ++i) {
+    const int s = base + 32 * i;
+    const uint32_t k = key(i);
+    const unsigned same = __ballot_sync(0xffffffffu, s < a.L && k == kth);
+    const bool keep = k > kth || (k == kth && e + __popc(same & below) < need);
+    e += __popc(same);
+    holes += __popc(__ballot_sync(0xffffffffu, s < a.budget && !keep));
+    tails += __popc(__ballot_sync(0xffffffffu, s >= a.budget && s < a.L && keep));
   }
-  int hall = hb;
-  for (int r = rank; r < nc; ++r) hall += cl.map_shared_rank(s_cnt, r)[1];
-  cl.sync();  // nobody leaves while its counts may be read
+  int hall, tall;
+  int hb = warp_prefix(holes, s_scan[4], &hall), tb = warp_prefix(tails, s_scan[5], &tall);
+  if (nc > 1) {
+    if (tid == 0) s_cnt[1] = hall, s_cnt[2] = tall;
+    cl.sync();
+    hall = 0;
+    for (int r = 0; r < nc; ++r) {
+      const int *c = cl.map_shared_rank(s_cnt, r);
+      hall += c[1];
+      if (r < rank) {
+        hb += c[1];
+        tb += c[2];
+      }
+    }
+    cl.sync();  // nobody leaves while its counts may be read
+  }
   // ---- the lists
   int *hole = w.hole + (long long)bh * w.m_cap, *tail = w.tail + (long long)bh * w.m_cap;
   int *off = w.off + (long long)bh * (w.nblk + 1);
   if (rank == 0 && tid == 0) off[w.nblk] = hall;
-  e0 = eq_before;
-  for (int i0 = lo; i0 < hi; i0 += kPickThreads) {
-    const int i = i0 + tid;
-    const uint32_t k = i < hi ? key(i) : 0u;
-    const bool same = i < hi && k == kth;
-    int t;
-    const int er = block_scan(same, s_scan, &t) + e0;
-    e0 += t;
-    const bool keep = i < hi && (k > kth || (same && er < need));
-    const bool fr = i < hi && i < a.budget && !keep, sv = i < hi && i >= a.budget && keep;
-    const int hr = block_scan(fr, s_scan, &t) + hb;
-    hb += t;
-    const int tr = block_scan(sv, s_scan, &t) + tb;
-    tb += t;
-    if (i < hi && i < a.budget && i % a.bs == 0) off[i / a.bs] = hr;
-    if (fr && hr < w.m_cap) hole[hr] = i;
-    if (sv && tr < w.m_cap) tail[tr] = i;
+  e = eq0;
+#pragma unroll
+  for (int i = 0; i < ipt; ++i) {
+    const int s = base + 32 * i;
+    const uint32_t k = key(i);
+    const unsigned same = __ballot_sync(0xffffffffu, s < a.L && k == kth);
+    const bool keep = k > kth || (k == kth && e + __popc(same & below) < need);
+    e += __popc(same);
+    const bool fr = s < a.budget && !keep, sv = s >= a.budget && s < a.L && keep;
+    const unsigned fm = __ballot_sync(0xffffffffu, fr), sm = __ballot_sync(0xffffffffu, sv);
+    const int hr = hb + __popc(fm & below), tr = tb + __popc(sm & below);
+    hb += __popc(fm);
+    tb += __popc(sm);
+    if (s < a.budget && s % a.bs == 0) off[s / a.bs] = hr;
+    if (fr && hr < w.m_cap) hole[hr] = s;
+    if (sv && tr < w.m_cap) tail[tr] = s;
   }
 }
 
@@ -197,6 +221,7 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a,
   const int blk = blockIdx.x % w.nblk, bh = blockIdx.x / w.nblk;
   const int b = bh / a.Hkv, h = bh % a.Hkv, tid = threadIdx.x;
   const int s0 = blk * a.bs, rows = min(a.bs, a.budget - s0);
+  pdl_wait();
   const int *off = w.off + (long long)bh * (w.nblk + 1);
   const int m0 = off[blk], m1 = off[blk + 1];
   const bool moves = m1 > m0;
@@ -231,26 +256,38 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a,
     mn[e] = pad ? 0.f : INFINITY;
     mx[e] = pad ? 0.f : -INFINITY;
   }
-  for (int r = r0; r < rows; r += rg) {
-    const int s = s_src[r];
-    const bool mv = s != s0 + r;
-    if (mv || pool) {
-      const uint4 kv = *reinterpret_cast<const uint4 *>(kp + (long long)s * a.k.sl);
-      if (mv) {
-        const uint4 vv = *reinterpret_cast<const uint4 *>(vp + (long long)s * a.v.sl);
-        *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv;
-        *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv;
-      }
-      const T *ke = reinterpret_cast<const T *>(&kv);
+  constexpr int U = 4;  // rows in flight per thread
+  for (int rb = r0; rb < rows; rb += U * rg) {
+    uint4 kv[U], vv[U];
+    int src[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        float x;
-        if constexpr (sizeof(T) == 2)
-          x = Mma<T>::to_f(ke[e]);
-        else
-          x = ke[e];
-        mn[e] = fminf(mn[e], x);
-        mx[e] = fmaxf(mx[e], x);
+    for (int u = 0; u < U; ++u) {
+      const int r = rb + u * rg;
+      src[u] = r < rows ? s_src[r] : -1;
+      if (src[u] >= 0 && (pool || src[u] != s0 + r))
+        kv[u] = *reinterpret_cast<const uint4 *>(kp + (long long)src[u] * a.k.sl);
+      if (src[u] >= 0 && src[u] != s0 + r)
+        vv[u] = *reinterpret_cast<const uint4 *>(vp + (long long)src[u] * a.v.sl);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = rb + u * rg;
+      if (src[u] >= 0 && src[u] != s0 + r) {
+        *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv[u];
+        *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv[u];
+      }
+      if (src[u] >= 0 && pool) {
+        const T *ke = reinterpret_cast<const T *>(&kv[u]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          float x;
+          if constexpr (sizeof(T) == 2)
+            x = Mma<T>::to_f(ke[e]);
+          else
+            x = ke[e];
+          mn[e] = fminf(mn[e], x);
+          mx[e] = fmaxf(mx[e], x);
+        }
       }
     }
   }
@@ -322,9 +359,12 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
   const size_t need = evict_plan(a, &w, static_cast<uint8_t *>(ws));
   if (!ws || ws_bytes < need) return fail(BSA_ERR_WORKSPACE, "evict: workspace too small");
   const int bh = a->B * a->Hkv;
-  // CTAs per (b, head): one per 8192 slots, at most 8 (the portable cluster size)
+  // CTAs per (b, head): enough that a thread's slots fit its registers (16), up to one
+  // per 4096 slots while all fit the SMs at once; at most 8, the portable cluster size
   int nc = 1;
-  while (nc < 8 && (long long)nc * 8192 < a->L) nc *= 2;
+  while (nc < 8 && ((long long)nc * 16384 < a->L || ((long long)nc * 4096 < a->L && (long long)bh * nc * 2 <= 148)))
+    nc *= 2;
+  const int ipt = (int)((a->L + (long long)nc * kPickThreads - 1) / ((long long)nc * kPickThreads));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)bh * nc);
   cfg.blockDim = dim3(kPickThreads);
@@ -334,17 +374,24 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
   at.val.clusterDim.x = nc, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  cudaLaunchKernelEx(&cfg, evict_pick_kernel, *a, w);
+  if (ipt <= 1)
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<1>, *a, w, ipt);
+  else if (ipt <= 4)
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<4>, *a, w, ipt);
+  else if (ipt <= 16)
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<16>, *a, w, ipt);
+  else
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<0>, *a, w, ipt);
   if (bsa_status s = check_launch("evict_pick")) return s;
   const unsigned grid = (unsigned)bh * w.nblk;
   const int es = (int)elem_size(a->dtype), rg = 256 / (a->D * es / 16);
   const size_t smem = (size_t)a->bs * 4 + 2ull * rg * a->D * 4;
   if (a->dtype == BSA_BF16)
-    evict_move_kernel<__nv_bfloat16><<<grid, 256, smem, st>>>(*a, w);
+    launch_after(evict_move_kernel<__nv_bfloat16>, grid, 256, smem, st, *a, w);
   else if (a->dtype == BSA_F16)
-    evict_move_kernel<__half><<<grid, 256, smem, st>>>(*a, w);
+    launch_after(evict_move_kernel<__half>, grid, 256, smem, st, *a, w);
   else
-    evict_move_kernel<float><<<grid, 256, smem, st>>>(*a, w);
+    launch_after(evict_move_kernel<float>, grid, 256, smem, st, *a, w);
   return check_launch("evict_move");
 }
 

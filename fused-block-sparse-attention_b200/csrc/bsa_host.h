@@ -5,6 +5,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <string>
 
 #include "../../include/bsa.h"
@@ -16,6 +17,35 @@ bsa_status fail(bsa_status st, const std::string &msg);
 
 // Maps the last CUDA runtime error (if any) to BSA_ERR_LAUNCH.
 bsa_status check_launch(const char *what);
+
+// Launches `kern` so that it may start before the kernel in front of it on the stream
+// has finished (programmatic dependent launch): it must call pdl_wait() before it
+// touches anything that kernel writes or reads.
+template <typename K, typename... A>
+inline void launch_after(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, const A &...args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// Raises a kernel's dynamic shared-memory limit once per device (`done`: one bit each,
+// a static of the call site).
+inline void allow_smem(const void *kern, int bytes, std::atomic<uint64_t> &done) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess)
+    done.fetch_or(bit, std::memory_order_relaxed);
+}
 
 inline size_t elem_size(int dtype) { return dtype == BSA_F32 ? 4 : 2; }
 

@@ -399,7 +399,8 @@ bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParam
   {                                                                                                     \
     auto kern = prefix_sm100_kernel<T_, D_, N_>;                                                        \
     static_assert(PX<D_, N_>::SMEM <= 231000, "shared memory of one CTA");                              \
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PX<D_, N_>::SMEM);          \
+    static std::atomic<uint64_t> done{0};                                                               \
+    allow_smem(reinterpret_cast<const void *>(kern), PX<D_, N_>::SMEM, done);                           \
     kern<<<grid, PX_THREADS, PX<D_, N_>::SMEM, st>>>(mk.map, mv.map, pk(mk), pk(mv), p, a->D, rtiles,   \
                                                      cps, qvec);                                        \
   }

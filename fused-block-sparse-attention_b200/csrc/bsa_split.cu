@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
   uint8_t *ring = sm + ROWS * D * 2;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, tq = lane & 3;
+  pdl_trigger();  // the join may take its place on the SMs; it waits for this grid
   const int rt = blockIdx.x % rtiles, grpid = blockIdx.x / rtiles;
   const int b = p.fold ? 0 : grpid / p.Hkv, hk = grpid % p.Hkv;
   const int r0 = rt * ROWS;
@@ -494,6 +495,7 @@ __global__ void __launch_bounds__(256, SplitF32<D>::MINB)
   __shared__ float s_m[8][8], s_l[8][8];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % WR, wk = warp / WR;
+  pdl_trigger();
   const int rt = blockIdx.x % rtiles, grpid = blockIdx.x / rtiles;
   const int b = p.fold ? 0 : grpid / p.Hkv, hk = grpid % p.Hkv;
   const int r0 = rt * ROWS + wr * 8;
@@ -753,74 +755,99 @@ struct JoinParams {
 
 constexpr int kJoinThreads = 256;
 
-// Row blocks: one query row each; the warps take every eighth split, lanes the
-// columns.  Weight blocks: 1024 slots of one (b, hk): lse of its R rows from the
-// splits' (m, l), then the sum over the rows, in row order, of 2^(x - lse).
-template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinParams p) {
+// Row blocks: 8 / wpr query rows each.  A row's columns take D/4 lanes; the remaining
+// lanes of its warps, and its wpr warps, take splits side by side.  Weight blocks:
+// 1024 slots of one (b, hk), four per thread: lse of its R rows from the splits'
+// (m, l), then the sum over the rows, in row order, of 2^(x - m) / l.
+template <typename T, int D>
+__global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinParams p, const int wpr) {
   extern __shared__ float sj[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (blockIdx.x < p.rows) {
-    const long long gr = blockIdx.x;
-    __shared__ float s_f[8];
+  const int rpb = 8 / wpr;
+  const long long rblocks = (p.rows + rpb - 1) / rpb;
+  pdl_wait();
+  if (blockIdx.x < rblocks) {
+    constexpr int LPR = D / 4 < 32 ? D / 4 : 32, G = 32 / LPR, V = D / 4 / LPR;
+    const int sub = warp % wpr, col = (lane % LPR) * 4;
+    const long long gr = blockIdx.x * (long long)rpb + warp / wpr;
+    const bool live = gr < p.rows;
     float m = -INFINITY;
-    for (int s = tid; s < p.nsplit; s += kJoinThreads) m = fmax_nan(m, p.pml[s * p.rows + gr].x);
+    if (live)
+      for (int s = lane; s < p.nsplit; s += 32) m = fmax_nan(m, p.pml[s * p.rows + gr].x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) m = fmax_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (lane == 0) s_f[warp] = m;
-    __syncthreads();
-    float M = s_f[0];
+    float4 acc[V];
 #pragma unroll
-    for (int w = 1; w < 8; ++w) M = fmax_nan(M, s_f[w]);
-    // this warp's splits: columns lane*4 + 128*c
-    float4 acc[2] = {make_float4(0, 0, 0, 0), make_float4(0, 0, 0, 0)};
+    for (int c = 0; c < V; ++c) acc[c] = make_float4(0, 0, 0, 0);
     float l = 0.f;
-    if (M != -INFINITY)
-      for (int s = warp; s < p.nsplit; s += 8) {
+    if (live && m != -INFINITY) {
+#pragma unroll 4
+      for (int s = sub * G + lane / LPR; s < p.nsplit; s += wpr * G) {
         const float2 ml = p.pml[s * p.rows + gr];
-        if (ml.x == -INFINITY) continue;
-        const float f = ex2(ml.x - M);
+        if (ml.x == -INFINITY) continue;  // its O was not written
+        const float f = ex2(ml.x - m);
         l = fmaf(ml.y, f, l);
-        const float *op = p.po + (s * p.rows + gr) * p.D;
+        const float *op = p.po + (s * p.rows + gr) * D + col;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int d = lane * 4 + 128 * c;
-          if (d < p.D) {
-            const float4 x = *reinterpret_cast<const float4 *>(op + d);
-            acc[c].x = fmaf(x.x, f, acc[c].x);
-            acc[c].y = fmaf(x.y, f, acc[c].y);
-            acc[c].z = fmaf(x.z, f, acc[c].z);
-            acc[c].w = fmaf(x.w, f, acc[c].w);
-          }
+        for (int c = 0; c < V; ++c) {
+          const float4 x = *reinterpret_cast<const float4 *>(op + 128 * c);
+          acc[c].x = fmaf(x.x, f, acc[c].x);
+          acc[c].y = fmaf(x.y, f, acc[c].y);
+          acc[c].z = fmaf(x.z, f, acc[c].z);
+          acc[c].w = fmaf(x.w, f, acc[c].w);
         }
       }
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int d = lane * 4 + 128 * c;
-      if (d < p.D) *reinterpret_cast<float4 *>(sj + warp * p.D + d) = acc[c];
     }
-    __shared__ float s_l[8];
-    if (lane == 0) s_l[warp] = l;
-    __syncthreads();
-    if (tid < p.D) {
-      float o = 0.f, lt = 0.f;
 #pragma unroll
-      for (int w = 0; w < 8; ++w) {
-        o += sj[w * p.D + tid];
-        lt += s_l[w];
+    for (int o = LPR; o < 32; o <<= 1) {
+      l += __shfl_xor_sync(0xffffffffu, l, o);
+#pragma unroll
+      for (int c = 0; c < V; ++c) {
+        acc[c].x += __shfl_xor_sync(0xffffffffu, acc[c].x, o);
+        acc[c].y += __shfl_xor_sync(0xffffffffu, acc[c].y, o);
+        acc[c].z += __shfl_xor_sync(0xffffffffu, acc[c].z, o);
+        acc[c].w += __shfl_xor_sync(0xffffffffu, acc[c].w, o);
       }
-      const float y = lt == 0.f ? 0.f : o / lt;
-      const int t = (int)(gr % p.T);
-      const long long bh = gr / p.T;
-      T *op = reinterpret_cast<T *>(p.o) + (bh / p.Hq) * p.o_sb + (bh % p.Hq) * p.o_sh + t * p.o_sl + tid;
-      if constexpr (sizeof(T) == 2)
-        *op = Mma<T>::from_f(y);
-      else
-        *op = y;
+    }
+    if (wpr > 1) {  // the row's other warps, through shared memory: [warp][D] and [warp]
+      float *sl = sj + 8 * D;
+      if (lane < LPR)
+#pragma unroll
+        for (int c = 0; c < V; ++c) *reinterpret_cast<float4 *>(sj + warp * D + col + 128 * c) = acc[c];
+      if (lane == 0) sl[warp] = l;
+      __syncthreads();
+      if (sub != 0) return;
+      for (int w = 1; w < wpr; ++w) {
+        l += sl[warp + w];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+          const float4 x = *reinterpret_cast<const float4 *>(sj + (warp + w) * D + col + 128 * c);
+          acc[c].x += x.x;
+          acc[c].y += x.y;
+          acc[c].z += x.z;
+          acc[c].w += x.w;
+        }
+      }
+    }
+    if (!live || lane >= LPR) return;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int t = (int)(gr % p.T);
+    const long long bh = gr / p.T;
+    T *op = reinterpret_cast<T *>(p.o) + (bh / p.Hq) * p.o_sb + (bh % p.Hq) * p.o_sh + t * p.o_sl + col;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+      const float y[4] = {acc[c].x * inv, acc[c].y * inv, acc[c].z * inv, acc[c].w * inv};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if constexpr (sizeof(T) == 2)
+          op[128 * c + e] = Mma<T>::from_f(y[e]);
+        else
+          op[128 * c + e] = y[e];
+      }
     }
     return;
   }
-  const long long wb = blockIdx.x - p.rows;
+  const long long wb = blockIdx.x - rblocks;
   const int bh = (int)(wb / p.wtiles), tile = (int)(wb % p.wtiles);
   const int b = bh / p.Hkv, hk = bh % p.Hkv;
   for (int r = warp; r < p.R; r += 8) {
@@ -836,7 +863,7 @@ __global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinPara
     }
 #pragma unroll
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lane == 0) {  // offset and factor: p = 2^(x - m) / l
+    if (lane == 0) {  // offset and factor of the row
       sj[2 * r] = l == 0.f ? INFINITY : m;
       sj[2 * r + 1] = l == 0.f ? 0.f : 1.f / l;
     }
@@ -844,22 +871,32 @@ __global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinPara
   __syncthreads();
   const int *lv = p.live ? p.live + (long long)bh * (1 + p.kk) : nullptr;
   const long long nv = lv ? (long long)lv[0] * p.bs : p.L;
-  const float *lg = p.logits + (long long)bh * p.R * p.ncap;
-  float *wp = p.weight + b * p.w_sb + hk * p.w_sh;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const long long j = tile * 1024LL + i * kJoinThreads + tid;
-    if (j >= nv) break;
-    long long key = j;
-    if (lv) {
-      const long long blk = j / p.bs;
-      key = (long long)lv[1 + blk] * p.bs + (j - blk * p.bs);
-    }
-    if (key >= p.L) continue;
-    float w = 0.f;
-    for (int r = 0; r < p.R; ++r) w = fmaf(ex2(lg[(long long)r * p.ncap + j] - sj[2 * r]), sj[2 * r + 1], w);
-    wp[key] += w;
+  const long long j = tile * 1024LL + tid * 4;  // the row length ncap is a multiple of 4
+  if (j >= nv) return;
+  const float *lg = p.logits + (long long)bh * p.R * p.ncap + j;
+  long long key = j;
+  if (lv) {  // four slots of one block: bs is a multiple of 4
+    const long long blk = j / p.bs;
+    key = (long long)lv[1 + blk] * p.bs + (j - blk * p.bs);
   }
+  float *wp = p.weight + b * p.w_sb + hk * p.w_sh + key;
+  float w0[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) w0[e] = key + e < p.L ? wp[e] : 0.f;
+  float4 w = make_float4(0, 0, 0, 0);
+#pragma unroll 8
+  for (int r = 0; r < p.R; ++r) {
+    const float4 x = *reinterpret_cast<const float4 *>(lg + (long long)r * p.ncap);
+    const float m = sj[2 * r], f = sj[2 * r + 1];
+    w.x = fmaf(ex2(x.x - m), f, w.x);
+    w.y = fmaf(ex2(x.y - m), f, w.y);
+    w.z = fmaf(ex2(x.z - m), f, w.z);
+    w.w = fmaf(ex2(x.w - m), f, w.w);
+  }
+  if (key < p.L) wp[0] = w0[0] + w.x;
+  if (key + 1 < p.L) wp[1] = w0[1] + w.y;
+  if (key + 2 < p.L) wp[2] = w0[2] + w.z;
+  if (key + 3 < p.L) wp[3] = w0[3] + w.w;
 }
 
 // ------------------------------------------------------------------ launchers
@@ -902,7 +939,8 @@ static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_
   auto kern = split_mma_kernel<T, D, MT>;
   static_assert(C::RING >= kSplitWarps * 16 * MT * D * 4, "the ring holds the warps' O for the join");
   static_assert(C::KC * D * 2 >= 16 * MT * C::KC * 4, "a chunk's K buffer holds its P");
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  allow_smem(reinterpret_cast<const void *>(kern), smem, done);
   kern<<<dim3((unsigned)(groups * rtiles), p.nsplit), kSplitWarps * 32, smem, st>>>(p, rtiles, kSplitWarps);
   return check_launch("split_mma");
 }
@@ -914,7 +952,8 @@ static bsa_status launch_f32(const SplitParams &p, long long groups, cudaStream_
   const int smem = C::NST * C::STAGE;
   auto kern = split_f32_kernel<D, WR>;
   static_assert(C::NST * C::STAGE >= 8 * 8 * D * 4, "the ring holds the warps' O for the join");
-  cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  static std::atomic<uint64_t> done{0};
+  allow_smem(reinterpret_cast<const void *>(kern), smem, done);
   kern<<<dim3((unsigned)(groups * rtiles), p.nsplit), 256, smem, st>>>(p, rtiles, 1);
   return check_launch("split_f32");
 }
@@ -946,15 +985,28 @@ bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStream_t st)
   }
 }
 
+template <typename T>
+static void launch_join_t(const JoinParams &p, cudaStream_t st) {
+  // warps per row: enough that a warp walks a few splits at most (8 loads in flight)
+  const int wpr = p.nsplit <= 8 ? 1 : p.nsplit <= 16 ? 2 : p.nsplit <= 32 ? 4 : 8;
+  const long long rblocks = (p.rows * wpr + 7) / 8;
+  const dim3 grid((unsigned)(rblocks + (p.weight ? (long long)p.B * p.Hkv * p.wtiles : 0)));
+  const size_t smem = std::max<size_t>((8 * p.D + 8) * 4, p.weight ? (size_t)p.R * 8 : 0);
+  switch (p.D) {
+    case 32: return launch_after(split_join_kernel<T, 32>, grid, kJoinThreads, smem, st, p, wpr);
+    case 64: return launch_after(split_join_kernel<T, 64>, grid, kJoinThreads, smem, st, p, wpr);
+    case 128: return launch_after(split_join_kernel<T, 128>, grid, kJoinThreads, smem, st, p, wpr);
+    default: return launch_after(split_join_kernel<T, 256>, grid, kJoinThreads, smem, st, p, wpr);
+  }
+}
+
 static bsa_status launch_join(int dtype, const JoinParams &p, cudaStream_t st) {
-  const size_t smem = std::max<size_t>(8 * p.D * 4, p.weight ? (size_t)p.R * 8 : 0);
-  const unsigned grid = (unsigned)(p.rows + (p.weight ? (long long)p.B * p.Hkv * p.wtiles : 0));
   if (dtype == BSA_BF16)
-    split_join_kernel<__nv_bfloat16><<<grid, kJoinThreads, smem, st>>>(p);
+    launch_join_t<__nv_bfloat16>(p, st);
   else if (dtype == BSA_F16)
-    split_join_kernel<__half><<<grid, kJoinThreads, smem, st>>>(p);
+    launch_join_t<__half>(p, st);
   else
-    split_join_kernel<float><<<grid, kJoinThreads, smem, st>>>(p);
+    launch_join_t<float>(p, st);
   return check_launch("split_join");
 }
 

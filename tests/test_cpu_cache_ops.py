@@ -26,7 +26,7 @@ def test_struct_layouts(tmp_path):
     got = dict(x.split() for x in subprocess.run([str(exe)], capture_output=True, text=True,
                                                   check=True).stdout.splitlines())
     for cname, cls in structs.items():
-        assert int(got[cname]) == ctypes.sizeof(cls), cname
+        assert int(got[cname]) == ctypes.sizeof(cls) == _bsa._PACK[cname[:-5]].size, cname
         for f, _ in cls._fields_:
             assert int(got[cname + "." + f]) == getattr(cls, f).offset, (cname, f)
 
@@ -126,7 +126,10 @@ def bsa(monkeypatch):
     calls = []
     monkeypatch.setattr(_bsa, "_need_cuda", lambda *ts: None)
     monkeypatch.setattr(_bsa, "status_tensor", lambda device: torch.zeros(1, dtype=torch.int32))
-    monkeypatch.setattr(_bsa, "_launch", lambda name, a, t: calls.append((name, a)))
+    structs = {"bsa_decode_weighted": _bsa.DecodeWeightedArgs, "bsa_evict": _bsa.EvictArgs,
+               "bsa_decode_prefix": _bsa.DecodePrefixArgs}
+    monkeypatch.setattr(_bsa, "_launch",
+                        lambda name, a, dev: calls.append((name, structs[name].from_buffer_copy(a))))
     _bsa.test_calls = calls
     return _bsa
 
