@@ -8,17 +8,20 @@
 // the keys are split so that all SMs work on few rows.
 //
 // NT = 2 (D 64, 128; more than 128 rows): one CTA owns two row tiles that share every
-// K/V tile: half the shared-memory fill per product, which at one tile per CTA is the
-// bound (64 KB of K/V per 128 x 128 step at D 128: the SMs drain L2).  Four softmax
-// warps per tile, one row per thread; P overlays its tile's S, so S of the next step
-// is issued once PV of this one is complete, while the other tile's softmax runs.
-// NT = 1 (up to 128 rows, or D 256, whose O fills TMEM): eight softmax warps, half a
-// row per thread; S, P and O in separate columns, S of the next step under the
-// exponentials of this one.
+// K/V tile: half the shared-memory fill per product.  NT = 1: up to 128 rows, or D 256,
+// whose O fills TMEM.  Eight softmax warps per tile, half a row per thread (the two
+// halves of a row exchange their maxima through shared memory): a tile's step is a
+// chain S -> softmax -> PV, and with one row per thread its softmax took half of it.
+// With room in TMEM (D 64, or NT = 1) P has columns of its own and S of the next step
+// runs under the exponentials of this one ("early"); at D 128 with two tiles P overlays
+// S, and S of the next step waits for PV of this one while the other tile works.
 //
-// Warps 0-7 softmax, 8 TMA producer, 9 TMEM owner and MMA issuer.  K/V tiles move as
-// 64-column chunks (16 KB) through one ring in the order the products use them.
-// Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the CTA runs on.
+// K and V move as units of min(D, 128) columns x 128 keys in one ring, so that PV is
+// issued with N = 128: a 128x64x16 product costs as much tensor time as three quarters
+// of a 128x128x16 one.  The issuing warp walks both tiles' pending products and issues
+// whichever is ready.  Warps 0 .. 8*NT-1 softmax, then the TMA producer, then the TMEM
+// owner and issuer.  Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the
+// CTA runs on to its end.
 #include <type_traits>
 
 #include "bsa_host.h"
@@ -29,41 +32,49 @@ namespace bsa {
 
 namespace {
 constexpr int PX_KEYS = 128;
-constexpr int PX_TILE = PX_KEYS * 64 * 2;  // 16 KB chunk: 128 rows x 64 columns
-constexpr int PX_WPROD = 8, PX_WMMA = 9, PX_THREADS = 320;
-constexpr float PX_RESCALE = 8.f;          // log2 units
+constexpr int PX_CHUNK = PX_KEYS * 64 * 2;  // 16 KB: 128 rows x 64 columns
+constexpr float PX_RESCALE = 8.f;           // log2 units
 
 template <int DP, int NT>
 struct PX {
   static constexpr int NCH = DP / 64;
-  static constexpr int NSL = DP == 256 ? 9 : DP == 128 ? (NT == 2 ? 9 : 11) : (NT == 2 ? 11 : 12);
-  static constexpr int SMEM = 1024 + NT * NCH * PX_TILE + NSL * PX_TILE;
-  // TMEM columns
-  static constexpr int S(int t) { return NT == 2 ? 128 * t : 0; }
-  static constexpr int P(int t) { return NT == 2 ? 128 * t : 128; }
-  static constexpr int O(int t) { return NT == 2 ? 256 + DP * t : 192; }
-  static constexpr uint32_t COLS = DP == 64 && NT == 1 ? 256 : 512;
+  static constexpr int UC = DP >= 128 ? 2 : 1;     // 64-column chunks per unit
+  static constexpr int NU = NCH / UC;              // units per K or V tile
+  static constexpr int UNIT = UC * PX_CHUNK;
+  static constexpr int U = DP == 64 ? 10 : NT * NCH == 2 ? 6 : 5;  // ring units
+  static constexpr bool EARLY = DP == 64 || NT == 1;
+  static constexpr int WARPS = 8 * NT, THREADS = 32 * (WARPS + 2);
+  static constexpr int XCH = NT * (EARLY ? 2 : 1) * 4 * 2 * 32 * 4;
+  static constexpr int SMEM = NT * NCH * PX_CHUNK + U * UNIT + XCH + 256;
+  // TMEM columns of tile t
+  static constexpr int S(int t) { return 128 * t; }
+  static constexpr int P(int t) { return EARLY ? 128 * NT + 64 * t : 128 * t; }
+  static constexpr int O(int t) { return (EARLY ? 192 * NT : 256) + DP * t; }
+  static constexpr uint32_t COLS = O(NT - 1) + DP <= 256 ? 256 : 512;
+  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 4 * NT) * 8 + 4 <= 256, "fits the SM");
 };
 }  // namespace
 
 template <typename T, int DP, int NT>
-__global__ void __launch_bounds__(PX_THREADS, 1)
+__global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
     prefix_sm100_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                         const int perm_k, const int perm_v, const SplitParams p, const int D,
                         const int rtiles, const int cps, const int qvec) {
   using X = PX<DP, NT>;
-  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value, EARLY = X::EARLY;
   constexpr uint32_t IDESC_S = tc05::idesc_f16(kBF16, 128, 128, false);
-  constexpr uint32_t IDESC_PV = tc05::idesc_f16(kBF16, 128, 64, true);
-  constexpr int NCH = X::NCH, NSL = X::NSL, ROWS = 128 * NT;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem;                            // tile t, chunk c at (t * NCH + c) * TILE
-  uint8_t *sR = sQ + NT * NCH * PX_TILE;
-  __shared__ __align__(8) uint64_t r_full[NSL], r_empty[NSL], s_full[NT], s_empty, p_full[NT], o_done[NT];
-  __shared__ uint32_t tmem_base_sh;
-  __shared__ float s_xch[3][4][2][32];           // NT = 1: half-row maxima (by step parity), row sums
+  constexpr uint32_t IDESC_PV = tc05::idesc_f16(kBF16, 128, 64 * X::UC, true);
+  constexpr int NCH = X::NCH, U = X::U, NU = X::NU, UC = X::UC, ROWS = 128 * NT;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t *sQ = smem;                            // tile t, chunk c at (t * NCH + c) * CHUNK
+  uint8_t *sR = sQ + NT * NCH * PX_CHUNK;        // ring
+  float *s_xch = reinterpret_cast<float *>(sR + U * X::UNIT);  // [parity][tile][quad][half][32]
+  uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(s_xch) + X::XCH);
+  uint64_t *r_full = bars, *r_empty = bars + U, *s_full = bars + 2 * U, *s_empty = s_full + NT,
+           *p_full = s_empty + NT, *o_done = p_full + NT;
+  uint32_t *tmem_sh = reinterpret_cast<uint32_t *>(o_done + NT);
 
+  pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rt = blockIdx.x % rtiles, hk = blockIdx.x / rtiles;
   const int r0 = rt * ROWS;
@@ -71,29 +82,34 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
   const int j0 = blockIdx.y * cps;
   const int nsteps = min(nkt, j0 + cps) - j0;    // >= 1 by the launcher's choice of splits
   const int split = p.split0 + blockIdx.y;
+  // The swizzled layouts count on this alignment of the dynamic shared memory.
+  if (smem_u32(smem) & 1023) {
+    if (tid == 0) report(p.status, BSA_DEVERR_TIMEOUT);
+    return;
+  }
 
   if (tid == 0) {
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
-    for (int s = 0; s < NSL; ++s) {
+    for (int s = 0; s < U; ++s) {
       mbar_init(&r_full[s], 1);
-      mbar_init(&r_empty[s], 1);
+      mbar_init(&r_empty[s], NT);
     }
     for (int t = 0; t < NT; ++t) {
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 8 / NT);
+      mbar_init(&s_empty[t], 8);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_done[t], 1);
     }
-    mbar_init(&s_empty, 8);
     fence_mbar_init();
   }
-  if (warp == PX_WMMA) {
-    tc05::alloc(&tmem_base_sh, X::COLS);
+  if (warp == X::WARPS + 1) {
+    tc05::alloc(tmem_sh, X::COLS);
     tc05::relinquish();
   }
   // query rows of this tile, 16 bytes at a time into the swizzled layout; zeros past
   // the rows and, for D 32, past the columns
-  for (int i = tid; i < ROWS * (DP / 8); i += PX_THREADS) {
+  for (int i = tid; i < ROWS * (DP / 8); i += X::THREADS) {
     const int r = i / (DP / 8), ch = i % (DP / 8);
     uint4 u = make_uint4(0, 0, 0, 0);
     if (r0 + r < p.R && ch * 8 < D) {
@@ -108,159 +124,162 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
         for (int x = 0; x < 8; ++x) e[x] = qp[x];
       }
     }
-    *reinterpret_cast<uint4 *>(sQ + (r >> 7) * NCH * PX_TILE + swz(0, 128, r & 127, ch * 8)) = u;
+    *reinterpret_cast<uint4 *>(sQ + (r >> 7) * NCH * PX_CHUNK + swz(0, 128, r & 127, ch * 8)) = u;
   }
   fence_proxy_async_smem();
   tc05::fence_before();
   __syncthreads();
   tc05::fence_after();
-  const uint32_t tmem = tmem_base_sh;
+  const uint32_t tmem = *tmem_sh;
 
-  // Ring sequence.  NT = 2: K_0, V_0, K_1, V_1, ...; NT = 1: K_0, K_1, V_0, K_2, V_1, ...
-  // (S of the next step goes before PV of this one).
-  if (warp == PX_WPROD) {
+  // Ring sequence, in tiles of NU units.  EARLY: K_0, K_1, V_0, K_2, V_1, ..., else
+  // K_0, V_0, K_1, V_1, ...: the order in which one row tile's products use them.
+  auto k_at = [&](int j) { return (EARLY ? (j == 0 ? 0 : 2 * j - 1) : 2 * j) * NU; };
+  auto v_at = [&](int j) { return (EARLY ? (j + 1 < nsteps ? 2 * j + 2 : 2 * j + 1) : 2 * j + 1) * NU; };
+  if (warp == X::WARPS) {
+    // ================= TMA producer
     int n = 0;
     auto load = [&](bool isv, int j) {
-      for (int c = 0; c < NCH; ++c, ++n) {
-        const int sl = n % NSL;
-        if (n >= NSL && !mbar_wait_warp(&r_empty[sl], ((n / NSL) - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      for (int u = 0; u < NU; ++u, ++n) {
+        const int sl = n % U;
+        if (n >= U && !mbar_wait_warp(&r_empty[sl], ((n / U) - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
         if (tc05::elect_one()) {
-          mbar_expect_tx(&r_full[sl], PX_TILE);
-          tma_load_rhb(sR + sl * PX_TILE, isv ? &tv : &tk, &r_full[sl], isv ? perm_v : perm_k, 64 * c,
-                       (j0 + j) * PX_KEYS, hk, 0);
+          mbar_expect_tx(&r_full[sl], X::UNIT);
+          for (int c = 0; c < UC; ++c)
+            tma_load_rhb(sR + sl * X::UNIT + c * PX_CHUNK, isv ? &tv : &tk, &r_full[sl], isv ? perm_v : perm_k,
+                         64 * (u * UC + c), (j0 + j) * PX_KEYS, hk, 0);
         }
         __syncwarp();
       }
     };
     load(false, 0);
     for (int j = 0; j < nsteps; ++j) {
-      if (NT == 1 && j + 1 < nsteps) load(false, j + 1);
+      if (EARLY && j + 1 < nsteps) load(false, j + 1);
       load(true, j);
-      if (NT == 2 && j + 1 < nsteps) load(false, j + 1);
+      if (!EARLY && j + 1 < nsteps) load(false, j + 1);
     }
-  } else if (warp == PX_WMMA) {
+  } else if (warp == X::WARPS + 1) {
+    // ================= issuer: the warp polls together (voted), one elected lane issues
     const uint64_t dq = tc05::sdesc(smem_u32(sQ), 16, 1024);
-    // S of tile t from the K tile at ring position n0; frees the chunks when `last`
-    auto issue_s = [&](int t, int n0, bool last) {
-      for (int c = 0; c < NCH; ++c) {
-        const int n = n0 + c, sl = n % NSL;
-        if (!mbar_wait_warp(&r_full[sl], (n / NSL) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
-        tc05::fence_after();
-        const uint64_t dk = tc05::sdesc(smem_u32(sR + sl * PX_TILE), 16, 1024);
-        const uint64_t dqc = dq + (t * NCH + c) * (PX_TILE >> 4);
+    auto full = [&](int n) { return __any_sync(0xffffffffu, mbar_test(&r_full[n % U], (n / U) & 1)); };
+    auto wait_full = [&](int n) {
+      if (!mbar_wait_warp(&r_full[n % U], (n / U) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      tc05::fence_after();
+    };
+    auto issue_s = [&](int t, int n0) {
+      for (int u = 0; u < NU; ++u) {
+        const int sl = (n0 + u) % U;
+        wait_full(n0 + u);
+        const uint64_t dk = tc05::sdesc(smem_u32(sR + sl * X::UNIT), 16, 1024);
+        const uint64_t dqu = dq + (t * NCH + u * UC) * (PX_CHUNK >> 4);
         if (tc05::elect_one()) {
 #pragma unroll
-          for (int ks = 0; ks < 4; ++ks)
-            tc05::mma_f16(tc05::taddr(tmem, 0, X::S(t)), dqc + 2 * ks, dk + 2 * ks, IDESC_S,
-                          (c > 0 || ks > 0) ? 1u : 0u);
-          if (last) tc05::commit(&r_empty[sl]);
+          for (int c = 0; c < UC; ++c)
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)
+              tc05::mma_f16(tc05::taddr(tmem, 0, X::S(t)), dqu + c * (PX_CHUNK >> 4) + 2 * ks,
+                            dk + c * (PX_CHUNK >> 4) + 2 * ks, IDESC_S, (u > 0 || c > 0 || ks > 0) ? 1u : 0u);
+          tc05::commit(&r_empty[sl]);
+          if (u == NU - 1) tc05::commit(&s_full[t]);
         }
         __syncwarp();
       }
-      if (tc05::elect_one()) tc05::commit(&s_full[t]);
-      __syncwarp();
     };
-    auto issue_pv = [&](int t, int n0, int j, bool last) {
-      for (int c = 0; c < NCH; ++c) {
-        const int n = n0 + c, sl = n % NSL;
-        if (!mbar_wait_warp(&r_full[sl], (n / NSL) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
-        tc05::fence_after();
-        const uint64_t dv = tc05::sdesc(smem_u32(sR + sl * PX_TILE), PX_TILE, 1024);
+    auto issue_pv = [&](int t, int n0, int j) {
+      for (int u = 0; u < NU; ++u) {
+        const int sl = (n0 + u) % U;
+        wait_full(n0 + u);
+        const uint64_t dv = tc05::sdesc(smem_u32(sR + sl * X::UNIT), PX_CHUNK, 1024);
         if (tc05::elect_one()) {
 #pragma unroll
           for (int ks = 0; ks < PX_KEYS / 16; ++ks)
-            tc05::mma_f16_ts(tc05::taddr(tmem, 0, X::O(t) + 64 * c), tc05::taddr(tmem, 0, X::P(t) + 8 * ks),
+            tc05::mma_f16_ts(tc05::taddr(tmem, 0, X::O(t) + 64 * UC * u), tc05::taddr(tmem, 0, X::P(t) + 8 * ks),
                              dv + 128 * ks, IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-          if (last) tc05::commit(&r_empty[sl]);
+          tc05::commit(&r_empty[sl]);
+          if (u == NU - 1) tc05::commit(&o_done[t]);
         }
         __syncwarp();
       }
-      if (tc05::elect_one()) tc05::commit(&o_done[t]);
-      __syncwarp();
     };
-    if constexpr (NT == 2) {
-      issue_s(0, 0, false);
-      issue_s(1, 0, true);
-      for (int j = 0; j < nsteps; ++j) {
+    int js[NT], jp[NT], left = 2 * NT * nsteps;  // next S and PV of each tile, products to issue
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          if (!mbar_wait_warp(&p_full[t], j & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+    for (int t = 0; t < NT; ++t) js[t] = jp[t] = 0;
+    uint32_t idle = 0;
+    while (left > 0 && idle < kSpinLimit) {
+      ++idle;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        // PV first: it is what the tile's chain waits for
+        if (jp[t] < js[t] && __any_sync(0xffffffffu, mbar_test(&p_full[t], jp[t] & 1)) && full(v_at(jp[t]))) {
           tc05::fence_after();
-          issue_pv(t, (2 * j + 1) * NCH, j, t == 1);
-          if (j + 1 < nsteps) {
-            // P shares its columns with S: its readers must be done
-            if (!mbar_wait_warp(&o_done[t], j & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
-            tc05::fence_after();
-            issue_s(t, (2 * j + 2) * NCH, t == 1);
-          }
+          issue_pv(t, v_at(jp[t]), jp[t]);
+          ++jp[t];
+          --left;
+          idle = 0;
         }
-      }
-    } else {
-      // ring position of K_j: 0 for j = 0, else (2j - 1) * NCH; V_j: (2j + 2) * NCH, and
-      // one tile earlier for the last step (no K follows)
-      issue_s(0, 0, true);
-      for (int j = 0; j < nsteps; ++j) {
-        if (j + 1 < nsteps) {
-          if (!mbar_wait_warp(&s_empty, j & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+        // S_j: its columns are free once S_{j-1} has been read (early) or, where P shares
+        // them, once PV_{j-1} is complete
+        if (js[t] < nsteps && (EARLY || js[t] == jp[t]) &&
+            (js[t] == 0 || __any_sync(0xffffffffu, mbar_test(EARLY ? &s_empty[t] : &o_done[t], (js[t] - 1) & 1))) &&
+            full(k_at(js[t]))) {
           tc05::fence_after();
-          issue_s(0, (2 * j + 1) * NCH, true);
+          issue_s(t, k_at(js[t]));
+          ++js[t];
+          --left;
+          idle = 0;
         }
-        if (!mbar_wait_warp(&p_full[0], j & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
-        tc05::fence_after();
-        issue_pv(0, (j + 1 < nsteps ? 2 * j + 2 : 2 * j + 1) * NCH, j, true);
       }
     }
+    if (left > 0) report(p.status, BSA_DEVERR_TIMEOUT);
   } else {
     // ================= softmax
-    constexpr int W = 128 * NT / 2;              // columns per thread: 128 or 64
-    const int quad = warp & 3, up = warp >> 2;   // up: the tile (NT = 2) or the half row
-    const int t = NT == 2 ? up : 0, hf = NT == 2 ? 0 : up;
+    const int t = warp >> 3, quad = warp & 3, hf = (warp >> 2) & 1;
     const int r = t * 128 + quad * 32 + lane;    // row within the CTA
-    const int cb = W * hf;
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + lane_base + X::S(t) + cb, tp = tmem + lane_base + X::P(t) + cb / 2;
-    const uint32_t to = tmem + lane_base + X::O(t);
-    constexpr int OC = NT == 2 ? DP : DP / 2;    // O columns of this thread
+    const uint32_t ts = tmem + lane_base + X::S(t) + 64 * hf, tp = tmem + lane_base + X::P(t) + 32 * hf;
+    constexpr int OC = DP / 2;                   // O columns of this thread
+    const uint32_t to = tmem + lane_base + X::O(t) + hf * OC;
     const bool rows_here = r0 + t * 128 + quad * 32 < p.R;  // the warp has a row (warp-uniform)
+    const int bar = 1 + t * 4 + quad;
+    // without EARLY one exchange buffer is enough: S_{j+1} follows this row's PV_j, so the
+    // other half cannot be a step ahead
+    auto xch = [&](int par, int half) -> float & {
+      return s_xch[((((EARLY ? par : 0) * NT + t) * 4 + quad) * 2 + half) * 32 + lane];
+    };
     float m_used = -INFINITY, l = 0.f;
     for (int j = 0; j < nsteps; ++j) {
       if (!mbar_wait(&s_full[t], j & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
       tc05::fence_after();
       if (!rows_here) {  // nothing to do but keep step; its P stays what it is
         __syncwarp();
-        if (NT == 1 && j >= 1 && !mbar_wait(&o_done[0], (j - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+        if (EARLY && j >= 1 && !mbar_wait(&o_done[t], (j - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
         tc05::fence_before();
         __syncwarp();
         if (lane == 0) {
-          if (NT == 1) tc05::mbar_arrive(&s_empty);
+          tc05::mbar_arrive(&s_empty[t]);
           tc05::mbar_arrive(&p_full[t]);
         }
         continue;
       }
-      float s[W];
-#pragma unroll
-      for (int c = 0; c < W; c += 32) tc05::ld32(ts + c, s + c);
+      float s[64];
+      tc05::ld32(ts, s);
+      tc05::ld32(ts + 32, s + 32);
       tc05::wait_ld();
-      if (NT == 1) {
+      if (EARLY) {
         tc05::fence_before();
         __syncwarp();
-        if (lane == 0) tc05::mbar_arrive(&s_empty);
+        if (lane == 0) tc05::mbar_arrive(&s_empty[t]);
       }
-      const int left = p.nkeys - (j0 + j) * PX_KEYS - cb;  // keys of this thread's columns
-      if (left < W) {
+      const int left = p.nkeys - (j0 + j) * PX_KEYS - 64 * hf;  // keys of this thread's columns
+      if (left < 64) {
 #pragma unroll
-        for (int c = 0; c < W; ++c)
+        for (int c = 0; c < 64; ++c)
           if (c >= left) s[c] = -INFINITY;
       }
-      float mr = max64(s);
-      if constexpr (NT == 2) {
-        mr = fmaxf(mr, max64(s + W / 2));
-      } else {
-        s_xch[j & 1][quad][hf][lane] = mr;
-        named_bar_sync(1 + quad, 64);
-        mr = fmaxf(mr, s_xch[j & 1][quad][hf ^ 1][lane]);
-      }
-      const float mx = mr * p.scale2;
+      const float mh = max64(s);
+      xch(j & 1, hf) = mh;
+      named_bar_sync(bar, 64);
+      const float mx = fmaxf(mh, xch(j & 1, hf ^ 1)) * p.scale2;
       bool need = false;
       float alpha = 1.f;
       if (mx > -INFINITY && (m_used == -INFINITY || mx > m_used + PX_RESCALE)) {
@@ -271,63 +290,59 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
       }
       const float off = m_used == -INFINITY ? 0.f : -m_used;
       const float2 sc2 = make_float2(p.scale2, p.scale2), of2 = make_float2(off, off);
-      uint32_t w[W / 2];
-      float2 sum[4];
+      uint32_t w[32];
+      float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int c = 0; c < W; c += 2) {
+      for (int c = 0; c < 64; c += 2) {
         const float2 x = fma2(make_float2(s[c], s[c + 1]), sc2, of2);
         const float2 e = make_float2(ex2(x.x), ex2(x.y));
-        sum[(c >> 1) & 3] = add2(sum[(c >> 1) & 3], e);
+        sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], e);
         w[c >> 1] = Mma<T>::pack(e.x, e.y);
       }
-      const float2 st = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+      const float2 st = add2(sum[0], sum[1]);
       l += st.x + st.y;
-      if (NT == 1 && j >= 1) {  // PV of the step before has read its P (and O may be rescaled)
-        if (!mbar_wait(&o_done[0], (j - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      if (EARLY && j >= 1) {  // PV of the step before has read its P (and O may be rescaled)
+        if (!mbar_wait(&o_done[t], (j - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
         tc05::fence_after();
       }
       if (__any_sync(0xffffffffu, need) && j >= 1) {
 #pragma unroll 1
         for (int c = 0; c < OC; c += 32) {
           float o[32];
-          tc05::ld32(to + hf * OC + c, o);
+          tc05::ld32(to + c, o);
           tc05::wait_ld();
 #pragma unroll
           for (int x = 0; x < 32; ++x) o[x] *= alpha;
-          tc05::st32(to + hf * OC + c, o);
+          tc05::st32(to + c, o);
         }
         tc05::wait_st();
       }
-#pragma unroll
-      for (int c = 0; c < W / 2; c += 32) tc05::st32(tp + c, reinterpret_cast<const float *>(w) + c);
+      tc05::st32(tp, reinterpret_cast<const float *>(w));
       tc05::wait_st();
       tc05::fence_before();
       __syncwarp();
       if (lane == 0) tc05::mbar_arrive(&p_full[t]);
     }
     // ---- (m, l) and the unnormalised O of this split
-    if (NT == 1 && rows_here) {
-      s_xch[2][quad][hf][lane] = l;
-      named_bar_sync(1 + quad, 64);
-      l += s_xch[2][quad][hf ^ 1][lane];
-    }
     if (!mbar_wait(&o_done[t], (nsteps - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
     tc05::fence_after();
-    const bool live = r0 + r < p.R;
-    long long at = 0;
-    if (live) {
-      int rb, rh, rtt;
-      at = (long long)split * p.rows + split_row(p, 0, hk, r0 + r, rb, rh, rtt);
-      // a NaN sum with no maximum (every logit NaN) must not read as an empty row
-      if (hf == 0) p.pml[at] = make_float2(m_used == -INFINITY && isnan(l) ? l : m_used, l);
-    }
     if (rows_here) {
+      // past the last PV both halves have read the last maxima
+      xch(nsteps & 1, hf) = l;
+      named_bar_sync(bar, 64);
+      l += xch(nsteps & 1, hf ^ 1);
+      const bool live = r0 + r < p.R;
+      long long at = 0;
+      if (live) {
+        int rb, rh, rtt;
+        at = (long long)split * p.rows + split_row(p, 0, hk, r0 + r, rb, rh, rtt);
+        // a NaN sum with no maximum (every logit NaN) must not read as an empty row
+        if (hf == 0) p.pml[at] = make_float2(m_used == -INFINITY && isnan(l) ? l : m_used, l);
+      }
 #pragma unroll 1
       for (int c = 0; c < OC; c += 32) {
         float o[32];
-        tc05::ld32(to + hf * OC + c, o);
+        tc05::ld32(to + c, o);
         tc05::wait_ld();
         if (live && hf * OC + c < D) {
           float *op = p.po + at * D + hf * OC + c;
@@ -340,7 +355,7 @@ __global__ void __launch_bounds__(PX_THREADS, 1)
   }
   tc05::fence_before();
   __syncthreads();
-  if (warp == PX_WMMA) {
+  if (warp == X::WARPS + 1) {
     tc05::fence_after();
     tc05::dealloc(tmem, X::COLS);
   }
@@ -395,14 +410,13 @@ bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParam
   const int qvec = reinterpret_cast<uintptr_t>(a->q.ptr) % 16 == 0 && a->q.sb % 8 == 0 && a->q.sh % 8 == 0 &&
                    a->q.sl % 8 == 0;
   const dim3 grid((unsigned)(a->Hkv * rtiles), ns);
-#define BSA_PX(T_, D_, N_)                                                                              \
-  {                                                                                                     \
-    auto kern = prefix_sm100_kernel<T_, D_, N_>;                                                        \
-    static_assert(PX<D_, N_>::SMEM <= 231000, "shared memory of one CTA");                              \
-    static std::atomic<uint64_t> done{0};                                                               \
-    allow_smem(reinterpret_cast<const void *>(kern), PX<D_, N_>::SMEM, done);                           \
-    kern<<<grid, PX_THREADS, PX<D_, N_>::SMEM, st>>>(mk.map, mv.map, pk(mk), pk(mv), p, a->D, rtiles,   \
-                                                     cps, qvec);                                        \
+#define BSA_PX(T_, D_, N_)                                                                           \
+  {                                                                                                  \
+    auto kern = prefix_sm100_kernel<T_, D_, N_>;                                                     \
+    static std::atomic<uint64_t> done{0};                                                            \
+    allow_smem(reinterpret_cast<const void *>(kern), PX<D_, N_>::SMEM, done);                        \
+    kern<<<grid, PX<D_, N_>::THREADS, PX<D_, N_>::SMEM, st>>>(mk.map, mv.map, pk(mk), pk(mv), p, a->D, \
+                                                              rtiles, cps, qvec);                    \
   }
 #define BSA_PX_D(T_)                             \
   if (a->D <= 64) {                              \
