@@ -9,19 +9,24 @@
 //
 // NT = 2 (D 64, 128; more than 128 rows): one CTA owns two row tiles that share every
 // K/V tile: half the shared-memory fill per product.  NT = 1: up to 128 rows, or D 256,
-// whose O fills TMEM.  Eight softmax warps per tile, half a row per thread (the two
-// halves of a row exchange their maxima through shared memory): a tile's step is a
-// chain S -> softmax -> PV, and with one row per thread its softmax took half of it.
-// With room in TMEM (D 64, or NT = 1) P has columns of its own and S of the next step
-// runs under the exponentials of this one ("early"); at D 128 with two tiles P overlays
-// S, and S of the next step waits for PV of this one while the other tile works.
+// whose O fills TMEM.  A tile's step is a chain S -> softmax -> PV, so what counts is
+// that the next S is there when a softmax ends:
+//   D 64, or NT = 1: steps of 128 keys; P has columns of its own, so S of the next step
+//     runs under the exponentials of this one.  Eight softmax warps per tile, half a row
+//     per thread; the halves exchange their maxima through shared memory.
+//   D 128 with two tiles ("half steps"): TMEM holds O and 128 columns per tile besides;
+//     steps of 64 keys use them as two S buffers, each overlaid by its own P, so S runs
+//     one step ahead.  (One buffer of 128 keys left S waiting for PV: 6600 cycles per
+//     128 keys and pair of tiles, tensor pipe 33% busy.)  Four warps per tile, a row per
+//     thread.
 //
 // K and V move as units of min(D, 128) columns x 128 keys in one ring, so that PV is
 // issued with N = 128: a 128x64x16 product costs as much tensor time as three quarters
-// of a 128x128x16 one.  The issuing warp walks both tiles' pending products and issues
-// whichever is ready.  Warps 0 .. 8*NT-1 softmax, then the TMA producer, then the TMEM
-// owner and issuer.  Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the
-// CTA runs on to its end.
+// of a 128x128x16 one.  Each tile has its issuing warp, S of the next step before
+// PV of this one: with one for both, the tensor pipe ran dry between the batches.
+// Softmax warps first, then the TMA producer, then the issuers, the first of which owns
+// TMEM.  Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the CTA runs
+// on to its end.
 #include <type_traits>
 
 #include "bsa_host.h"
@@ -42,16 +47,18 @@ struct PX {
   static constexpr int NU = NCH / UC;              // units per K or V tile
   static constexpr int UNIT = UC * PX_CHUNK;
   static constexpr int U = DP == 64 ? 10 : NT * NCH == 2 ? 6 : 5;  // ring units
-  static constexpr bool EARLY = DP == 64 || NT == 1;
-  static constexpr int WARPS = 8 * NT, THREADS = 32 * (WARPS + 2);
-  static constexpr int XCH = NT * (EARLY ? 2 : 1) * 4 * 2 * 32 * 4;
-  static constexpr int SMEM = NT * NCH * PX_CHUNK + U * UNIT + XCH + 256;
-  // TMEM columns of tile t
-  static constexpr int S(int t) { return 128 * t; }
-  static constexpr int P(int t) { return EARLY ? 128 * NT + 64 * t : 128 * t; }
-  static constexpr int O(int t) { return (EARLY ? 192 * NT : 256) + DP * t; }
+  static constexpr bool HALF = DP == 128 && NT == 2;
+  static constexpr int KB = HALF ? 64 : 128;       // keys per step
+  static constexpr int WPT = HALF ? 4 : 8;         // softmax warps per tile
+  static constexpr int WARPS = WPT * NT, THREADS = 32 * (WARPS + 1 + NT);
+  static constexpr int XCH = HALF ? 0 : NT * 2 * 4 * 2 * 32 * 4;
+  static constexpr int SMEM = NT * NCH * PX_CHUNK + U * UNIT + XCH + 320;
+  // TMEM columns of tile t (step parity b)
+  static constexpr int S(int t, int b) { return 128 * t + (HALF ? 64 * b : 0); }
+  static constexpr int P(int t, int b) { return HALF ? S(t, b) : 128 * NT + 64 * t; }
+  static constexpr int O(int t) { return (HALF ? 256 : 192 * NT) + DP * t; }
   static constexpr uint32_t COLS = O(NT - 1) + DP <= 256 ? 256 : 512;
-  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 4 * NT) * 8 + 4 <= 256, "fits the SM");
+  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 7 * NT) * 8 + 4 <= 320, "fits the SM");
 };
 }  // namespace
 
@@ -61,18 +68,20 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
                         const int perm_k, const int perm_v, const SplitParams p, const int D,
                         const int rtiles, const int cps, const int qvec) {
   using X = PX<DP, NT>;
-  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value, EARLY = X::EARLY;
-  constexpr uint32_t IDESC_S = tc05::idesc_f16(kBF16, 128, 128, false);
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value, HALF = X::HALF;
+  constexpr uint32_t IDESC_S = tc05::idesc_f16(kBF16, 128, X::KB, false);
   constexpr uint32_t IDESC_PV = tc05::idesc_f16(kBF16, 128, 64 * X::UC, true);
-  constexpr int NCH = X::NCH, U = X::U, NU = X::NU, UC = X::UC, ROWS = 128 * NT;
+  constexpr int NCH = X::NCH, U = X::U, NU = X::NU, UC = X::UC, KB = X::KB, ROWS = 128 * NT;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint8_t *sQ = smem;                            // tile t, chunk c at (t * NCH + c) * CHUNK
   uint8_t *sR = sQ + NT * NCH * PX_CHUNK;        // ring
   float *s_xch = reinterpret_cast<float *>(sR + U * X::UNIT);  // [parity][tile][quad][half][32]
   uint64_t *bars = reinterpret_cast<uint64_t *>(reinterpret_cast<uint8_t *>(s_xch) + X::XCH);
-  uint64_t *r_full = bars, *r_empty = bars + U, *s_full = bars + 2 * U, *s_empty = s_full + NT,
-           *p_full = s_empty + NT, *o_done = p_full + NT;
-  uint32_t *tmem_sh = reinterpret_cast<uint32_t *>(o_done + NT);
+  // s_full, p_full, o_done: two per tile, by step parity, so that none can complete a
+  // second time before the first was seen
+  uint64_t *r_full = bars, *r_empty = bars + U, *s_full = bars + 2 * U, *p_full = s_full + 2 * NT,
+           *o_done = p_full + 2 * NT, *s_empty = o_done + 2 * NT;
+  uint32_t *tmem_sh = reinterpret_cast<uint32_t *>(s_empty + NT);
 
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -80,7 +89,8 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
   const int r0 = rt * ROWS;
   const int nkt = (p.nkeys + PX_KEYS - 1) / PX_KEYS;
   const int j0 = blockIdx.y * cps;
-  const int nsteps = min(nkt, j0 + cps) - j0;    // >= 1 by the launcher's choice of splits
+  const int ntiles = min(nkt, j0 + cps) - j0;    // >= 1 by the launcher's choice of splits
+  const int nsteps = HALF ? (min(p.nkeys, (j0 + ntiles) * PX_KEYS) - j0 * PX_KEYS + KB - 1) / KB : ntiles;
   const int split = p.split0 + blockIdx.y;
   // The swizzled layouts count on this alignment of the dynamic shared memory.
   if (smem_u32(smem) & 1023) {
@@ -96,10 +106,12 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       mbar_init(&r_empty[s], NT);
     }
     for (int t = 0; t < NT; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&s_empty[t], 8);
-      mbar_init(&p_full[t], 8);
-      mbar_init(&o_done[t], 1);
+      for (int b = 0; b < 2; ++b) {
+        mbar_init(&s_full[2 * t + b], 1);
+        mbar_init(&p_full[2 * t + b], X::WPT);
+        mbar_init(&o_done[2 * t + b], 1);
+      }
+      mbar_init(&s_empty[t], X::WPT);
     }
     fence_mbar_init();
   }
@@ -132,10 +144,11 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
   tc05::fence_after();
   const uint32_t tmem = *tmem_sh;
 
-  // Ring sequence, in tiles of NU units.  EARLY: K_0, K_1, V_0, K_2, V_1, ..., else
-  // K_0, V_0, K_1, V_1, ...: the order in which one row tile's products use them.
-  auto k_at = [&](int j) { return (EARLY ? (j == 0 ? 0 : 2 * j - 1) : 2 * j) * NU; };
-  auto v_at = [&](int j) { return (EARLY ? (j + 1 < nsteps ? 2 * j + 2 : 2 * j + 1) : 2 * j + 1) * NU; };
+  // Ring sequence, in tiles of NU units.  Half steps: K_0, V_0, K_1, V_1, ..., else
+  // K_0, K_1, V_0, K_2, V_1, ...: the order in which one row tile's products use them.
+  // k_at, v_at: position of step j's K and V.
+  auto k_at = [&](int j) { return (HALF ? 2 * (j >> 1) : j == 0 ? 0 : 2 * j - 1) * NU; };
+  auto v_at = [&](int j) { return (HALF ? 2 * (j >> 1) + 1 : j + 1 < nsteps ? 2 * j + 2 : 2 * j + 1) * NU; };
   if (warp == X::WARPS) {
     // ================= TMA producer
     int n = 0;
@@ -153,111 +166,102 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
     };
     load(false, 0);
-    for (int j = 0; j < nsteps; ++j) {
-      if (EARLY && j + 1 < nsteps) load(false, j + 1);
+    for (int j = 0; j < ntiles; ++j) {
+      if (!HALF && j + 1 < ntiles) load(false, j + 1);
       load(true, j);
-      if (!EARLY && j + 1 < nsteps) load(false, j + 1);
+      if (HALF && j + 1 < ntiles) load(false, j + 1);
     }
-  } else if (warp == X::WARPS + 1) {
-    // ================= issuer: the warp polls together (voted), one elected lane issues
+  } else if (warp > X::WARPS) {
+    // ================= issuer of tile t: the whole warp runs the sequence, one elected
+    // lane (always the same) issues the products and commits
+    const int t = warp - X::WARPS - 1;
+    const uint32_t on = tc05::elect_one();
     const uint64_t dq = tc05::sdesc(smem_u32(sQ), 16, 1024);
-    auto full = [&](int n) { return __any_sync(0xffffffffu, mbar_test(&r_full[n % U], (n / U) & 1)); };
-    auto wait_full = [&](int n) {
-      if (!mbar_wait_warp(&r_full[n % U], (n / U) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+    const uint32_t sR0 = smem_u32(sR);
+    auto wait = [&](uint64_t *bar, uint32_t parity) {
+      if (!mbar_wait_warp(bar, parity)) report(p.status, BSA_DEVERR_TIMEOUT);
       tc05::fence_after();
     };
-    auto issue_s = [&](int t, int n0) {
+    // a unit is free once both tiles' last products on it are done
+    auto last_use = [&](int j) { return !HALF || (j & 1) || j == nsteps - 1; };
+    auto issue_s = [&](int j) {
+      const int b = j & 1, n0 = k_at(j);
+      const uint32_t ds = tc05::taddr(tmem, 0, b ? X::S(t, 1) : X::S(t, 0));
       for (int u = 0; u < NU; ++u) {
         const int sl = (n0 + u) % U;
-        wait_full(n0 + u);
-        const uint64_t dk = tc05::sdesc(smem_u32(sR + sl * X::UNIT), 16, 1024);
+        if (!HALF || b == 0) wait(&r_full[sl], ((n0 + u) / U) & 1);  // once per unit
+        // half steps: the tile's upper 64 rows are 8 KB further on
+        const uint64_t dk = tc05::sdesc(sR0 + sl * X::UNIT, 16, 1024) + (HALF ? b * (64 * 128 >> 4) : 0);
         const uint64_t dqu = dq + (t * NCH + u * UC) * (PX_CHUNK >> 4);
-        if (tc05::elect_one()) {
 #pragma unroll
-          for (int c = 0; c < UC; ++c)
+        for (int c = 0; c < UC; ++c)
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              tc05::mma_f16(tc05::taddr(tmem, 0, X::S(t)), dqu + c * (PX_CHUNK >> 4) + 2 * ks,
-                            dk + c * (PX_CHUNK >> 4) + 2 * ks, IDESC_S, (u > 0 || c > 0 || ks > 0) ? 1u : 0u);
-          tc05::commit(&r_empty[sl]);
-          if (u == NU - 1) tc05::commit(&s_full[t]);
-        }
-        __syncwarp();
+          for (int ks = 0; ks < 4; ++ks)
+            tc05::mma_f16_if(on, ds, dqu + c * (PX_CHUNK >> 4) + 2 * ks, dk + c * (PX_CHUNK >> 4) + 2 * ks, IDESC_S,
+                             (u > 0 || c > 0 || ks > 0) ? 1u : 0u);
+        if (last_use(j)) tc05::commit_if(on, &r_empty[sl]);
       }
+      tc05::commit_if(on, &s_full[2 * t + b]);
     };
-    auto issue_pv = [&](int t, int n0, int j) {
+    auto issue_pv = [&](int j) {
+      const int b = j & 1, n0 = v_at(j);
+      const uint32_t ap = tc05::taddr(tmem, 0, b ? X::P(t, 1) : X::P(t, 0));
       for (int u = 0; u < NU; ++u) {
         const int sl = (n0 + u) % U;
-        wait_full(n0 + u);
-        const uint64_t dv = tc05::sdesc(smem_u32(sR + sl * X::UNIT), PX_CHUNK, 1024);
-        if (tc05::elect_one()) {
+        if (!HALF || b == 0) wait(&r_full[sl], ((n0 + u) / U) & 1);  // once per unit
+        const uint64_t dv = tc05::sdesc(sR0 + sl * X::UNIT, PX_CHUNK, 1024) + (HALF ? b * (64 * 128 >> 4) : 0);
 #pragma unroll
-          for (int ks = 0; ks < PX_KEYS / 16; ++ks)
-            tc05::mma_f16_ts(tc05::taddr(tmem, 0, X::O(t) + 64 * UC * u), tc05::taddr(tmem, 0, X::P(t) + 8 * ks),
-                             dv + 128 * ks, IDESC_PV, (j > 0 || ks > 0) ? 1u : 0u);
-          tc05::commit(&r_empty[sl]);
-          if (u == NU - 1) tc05::commit(&o_done[t]);
-        }
-        __syncwarp();
+        for (int ks = 0; ks < KB / 16; ++ks)
+          tc05::mma_f16_ts_if(on, tc05::taddr(tmem, 0, X::O(t) + 64 * UC * u), ap + 8 * ks, dv + 128 * ks, IDESC_PV,
+                              (j > 0 || ks > 0) ? 1u : 0u);
+        if (last_use(j)) tc05::commit_if(on, &r_empty[sl]);
       }
+      tc05::commit_if(on, &o_done[2 * t + b]);
     };
-    int js[NT], jp[NT], left = 2 * NT * nsteps;  // next S and PV of each tile, products to issue
-#pragma unroll
-    for (int t = 0; t < NT; ++t) js[t] = jp[t] = 0;
-    uint32_t idle = 0;
-    while (left > 0 && idle < kSpinLimit) {
-      ++idle;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        // PV first: it is what the tile's chain waits for
-        if (jp[t] < js[t] && __any_sync(0xffffffffu, mbar_test(&p_full[t], jp[t] & 1)) && full(v_at(jp[t]))) {
-          tc05::fence_after();
-          issue_pv(t, v_at(jp[t]), jp[t]);
-          ++jp[t];
-          --left;
-          idle = 0;
-        }
-        // S_j: its columns are free once S_{j-1} has been read (early) or, where P shares
-        // them, once PV_{j-1} is complete
-        if (js[t] < nsteps && (EARLY || js[t] == jp[t]) &&
-            (js[t] == 0 || __any_sync(0xffffffffu, mbar_test(EARLY ? &s_empty[t] : &o_done[t], (js[t] - 1) & 1))) &&
-            full(k_at(js[t]))) {
-          tc05::fence_after();
-          issue_s(t, k_at(js[t]));
-          ++js[t];
-          --left;
-          idle = 0;
-        }
+    issue_s(0);
+    for (int j = 0; j < nsteps; ++j) {
+      if (j + 1 < nsteps) {
+        // the columns of S_{j+1}: free once S_j has been read; with half steps, once
+        // PV_{j-1}, whose P lies in them, is complete
+        if (!HALF)
+          wait(&s_empty[t], j & 1);
+        else if (j >= 1)
+          wait(&o_done[2 * t + ((j - 1) & 1)], ((j - 1) >> 1) & 1);
+        issue_s(j + 1);
       }
+      wait(&p_full[2 * t + (j & 1)], (j >> 1) & 1);
+      issue_pv(j);
     }
-    if (left > 0) report(p.status, BSA_DEVERR_TIMEOUT);
   } else {
     // ================= softmax
-    const int t = warp >> 3, quad = warp & 3, hf = (warp >> 2) & 1;
+    const int t = warp / X::WPT, quad = warp & 3, hf = HALF ? 0 : (warp >> 2) & 1;
     const int r = t * 128 + quad * 32 + lane;    // row within the CTA
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
-    const uint32_t ts = tmem + lane_base + X::S(t) + 64 * hf, tp = tmem + lane_base + X::P(t) + 32 * hf;
-    constexpr int OC = DP / 2;                   // O columns of this thread
+    constexpr int OC = HALF ? DP : DP / 2;       // O columns of this thread
     const uint32_t to = tmem + lane_base + X::O(t) + hf * OC;
     const bool rows_here = r0 + t * 128 + quad * 32 < p.R;  // the warp has a row (warp-uniform)
     const int bar = 1 + t * 4 + quad;
-    // without EARLY one exchange buffer is enough: S_{j+1} follows this row's PV_j, so the
-    // other half cannot be a step ahead
     auto xch = [&](int par, int half) -> float & {
-      return s_xch[((((EARLY ? par : 0) * NT + t) * 4 + quad) * 2 + half) * 32 + lane];
+      return s_xch[(((par * NT + t) * 4 + quad) * 2 + half) * 32 + lane];
+    };
+    auto wait_pv = [&](int j) {
+      if (!mbar_wait(&o_done[2 * t + (j & 1)], (j >> 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      tc05::fence_after();
     };
     float m_used = -INFINITY, l = 0.f;
     for (int j = 0; j < nsteps; ++j) {
-      if (!mbar_wait(&s_full[t], j & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      const uint32_t ts = tmem + lane_base + (j & 1 ? X::S(t, 1) : X::S(t, 0)) + 64 * hf;
+      const uint32_t tp = tmem + lane_base + (j & 1 ? X::P(t, 1) : X::P(t, 0)) + 32 * hf;
+      if (!mbar_wait(&s_full[2 * t + (j & 1)], (j >> 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
       tc05::fence_after();
       if (!rows_here) {  // nothing to do but keep step; its P stays what it is
         __syncwarp();
-        if (EARLY && j >= 1 && !mbar_wait(&o_done[t], (j - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+        if (!HALF && j >= 1) wait_pv(j - 1);
         tc05::fence_before();
         __syncwarp();
         if (lane == 0) {
-          tc05::mbar_arrive(&s_empty[t]);
-          tc05::mbar_arrive(&p_full[t]);
+          if (!HALF) tc05::mbar_arrive(&s_empty[t]);
+          tc05::mbar_arrive(&p_full[2 * t + (j & 1)]);
         }
         continue;
       }
@@ -265,21 +269,24 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       tc05::ld32(ts, s);
       tc05::ld32(ts + 32, s + 32);
       tc05::wait_ld();
-      if (EARLY) {
+      if (!HALF) {
         tc05::fence_before();
         __syncwarp();
         if (lane == 0) tc05::mbar_arrive(&s_empty[t]);
       }
-      const int left = p.nkeys - (j0 + j) * PX_KEYS - 64 * hf;  // keys of this thread's columns
+      const int left = p.nkeys - j0 * PX_KEYS - j * KB - 64 * hf;  // keys of this thread's columns
       if (left < 64) {
 #pragma unroll
         for (int c = 0; c < 64; ++c)
           if (c >= left) s[c] = -INFINITY;
       }
-      const float mh = max64(s);
-      xch(j & 1, hf) = mh;
-      named_bar_sync(bar, 64);
-      const float mx = fmaxf(mh, xch(j & 1, hf ^ 1)) * p.scale2;
+      float mh = max64(s);
+      if constexpr (!HALF) {
+        xch(j & 1, hf) = mh;
+        named_bar_sync(bar, 64);
+        mh = fmaxf(mh, xch(j & 1, hf ^ 1));
+      }
+      const float mx = mh * p.scale2;
       bool need = false;
       float alpha = 1.f;
       if (mx > -INFINITY && (m_used == -INFINITY || mx > m_used + PX_RESCALE)) {
@@ -301,11 +308,10 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
       const float2 st = add2(sum[0], sum[1]);
       l += st.x + st.y;
-      if (EARLY && j >= 1) {  // PV of the step before has read its P (and O may be rescaled)
-        if (!mbar_wait(&o_done[t], (j - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
-        tc05::fence_after();
-      }
-      if (__any_sync(0xffffffffu, need) && j >= 1) {
+      const bool rescale = __any_sync(0xffffffffu, need) && j >= 1;
+      // PV of the step before: has read its P (one P buffer), and O may be rescaled
+      if (j >= 1 && (!HALF || rescale)) wait_pv(j - 1);
+      if (rescale) {
 #pragma unroll 1
         for (int c = 0; c < OC; c += 32) {
           float o[32];
@@ -321,16 +327,16 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       tc05::wait_st();
       tc05::fence_before();
       __syncwarp();
-      if (lane == 0) tc05::mbar_arrive(&p_full[t]);
+      if (lane == 0) tc05::mbar_arrive(&p_full[2 * t + (j & 1)]);
     }
     // ---- (m, l) and the unnormalised O of this split
-    if (!mbar_wait(&o_done[t], (nsteps - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
-    tc05::fence_after();
+    wait_pv(nsteps - 1);
     if (rows_here) {
-      // past the last PV both halves have read the last maxima
-      xch(nsteps & 1, hf) = l;
-      named_bar_sync(bar, 64);
-      l += xch(nsteps & 1, hf ^ 1);
+      if constexpr (!HALF) {  // past the last PV both halves have read the last maxima
+        xch(nsteps & 1, hf) = l;
+        named_bar_sync(bar, 64);
+        l += xch(nsteps & 1, hf ^ 1);
+      }
       const bool live = r0 + r < p.R;
       long long at = 0;
       if (live) {
