@@ -18,6 +18,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "bsa_common.cuh"
 #include "bsa_host.h"
@@ -212,10 +213,59 @@ __global__ void __launch_bounds__(kPickThreads)
   }
 }
 
-// One CTA of 256 threads per block of slots.  A row of D elements is D*es/16
-// 16-byte pieces; a thread owns one piece column and every (256 / pieces)-th row.
+// Running min / max of 16 bytes of a row, kept in the row's own type (both are exact).
 template <typename T>
-__global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a, const EvictWork w) {
+struct MinMax {
+  using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  P mn[4], mx[4];
+  __device__ void init(bool zero) {
+    const T lo = Mma<T>::from_f(zero ? 0.f : -INFINITY), hi = Mma<T>::from_f(zero ? 0.f : INFINITY);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mn[e].x = mn[e].y = hi;
+      mx[e].x = mx[e].y = lo;
+    }
+  }
+  __device__ void add(const uint4 &u) {
+    const P *x = reinterpret_cast<const P *>(&u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mn[e] = __hmin2(mn[e], x[e]);
+      mx[e] = __hmax2(mx[e], x[e]);
+    }
+  }
+  __device__ float min_of(int e) const { return Mma<T>::to_f(e & 1 ? mn[e >> 1].y : mn[e >> 1].x); }
+  __device__ float max_of(int e) const { return Mma<T>::to_f(e & 1 ? mx[e >> 1].y : mx[e >> 1].x); }
+};
+template <>
+struct MinMax<float> {
+  float mn[4], mx[4];
+  __device__ void init(bool zero) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mn[e] = zero ? 0.f : INFINITY;
+      mx[e] = zero ? 0.f : -INFINITY;
+    }
+  }
+  __device__ void add(const uint4 &u) {
+    const float *x = reinterpret_cast<const float *>(&u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      mn[e] = fminf(mn[e], x[e]);
+      mx[e] = fmaxf(mx[e], x[e]);
+    }
+  }
+  __device__ float min_of(int e) const { return mn[e]; }
+  __device__ float max_of(int e) const { return mx[e]; }
+};
+
+// One CTA of 256 threads per block of slots.  A row of D elements is D*es/16
+// 16-byte pieces; a thread owns one piece column and every (256 / pieces)-th row.  A
+// block is a few rows per thread behind a chain of three dependent loads (offsets,
+// lists, rows), so what hides it is CTAs side by side: min and max stay in the row's
+// type and two rows are in flight, which leaves room for five CTAs per SM.
+template <typename T>
+__global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args a, const EvictWork w) {
   constexpr int E = 16 / sizeof(T);
   extern __shared__ int s_src[];  // [bs] source slot, then the min / max of each thread row
   const int blk = blockIdx.x % w.nblk, bh = blockIdx.x / w.nblk;
@@ -225,10 +275,6 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a,
   const int *off = w.off + (long long)bh * (w.nblk + 1);
   const int m0 = off[blk], m1 = off[blk + 1];
   const bool moves = m1 > m0;
-  const float *wt = a.weight + b * a.w_sb + h * a.w_sh;
-  const int32_t *ps = a.pos + b * a.p_sb + h * a.p_sh;
-  float *wo = a.weight_out + b * a.wo_sb + h * a.wo_sh;
-  int32_t *po = a.pos_out + b * a.po_sb + h * a.po_sh;
   const bool same = a.weight_out == a.weight && a.pos_out == a.pos;
   const bool pool = a.kmin && (moves || rows < a.bs);
   if (!moves && !pool && same) return;
@@ -237,6 +283,41 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a,
   for (int m = m0 + tid; m < m1; m += 256)
     s_src[w.hole[(long long)bh * w.m_cap + m] - s0] = w.tail[(long long)bh * w.m_cap + m];
   __syncthreads();
+  MinMax<T> mm;
+  mm.init(rows < a.bs);  // rows past the budget count as zeros
+  const int pc = a.D / E, rg = 256 / pc;   // pieces per row, rows side by side
+  const int c = tid % pc, r0 = tid / pc;
+  if (moves || pool) {
+    T *kp = reinterpret_cast<T *>(a.k.ptr) + b * a.k.sb + h * a.k.sh + c * E;
+    T *vp = reinterpret_cast<T *>(a.v.ptr) + b * a.v.sb + h * a.v.sh + c * E;
+    constexpr int U = 2;  // rows in flight per thread
+    for (int rb = r0; rb < rows; rb += U * rg) {
+      uint4 kv[U], vv[U];
+      int src[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = rb + u * rg;
+        src[u] = r < rows ? s_src[r] : -1;
+        if (src[u] >= 0 && (pool || src[u] != s0 + r))
+          kv[u] = *reinterpret_cast<const uint4 *>(kp + (long long)src[u] * a.k.sl);
+        if (src[u] >= 0 && src[u] != s0 + r)
+          vv[u] = *reinterpret_cast<const uint4 *>(vp + (long long)src[u] * a.v.sl);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int r = rb + u * rg;
+        if (src[u] >= 0 && src[u] != s0 + r) {
+          *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv[u];
+          *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv[u];
+        }
+        if (src[u] >= 0 && pool) mm.add(kv[u]);
+      }
+    }
+  }
+  const float *wt = a.weight + b * a.w_sb + h * a.w_sh;
+  const int32_t *ps = a.pos + b * a.p_sb + h * a.p_sh;
+  float *wo = a.weight_out + b * a.wo_sb + h * a.wo_sh;
+  int32_t *po = a.pos_out + b * a.po_sb + h * a.po_sh;
   for (int i = tid; i < rows; i += 256) {
     const int s = s_src[i];
     if (s != s0 + i || !same) {
@@ -244,70 +325,21 @@ __global__ void __launch_bounds__(256) evict_move_kernel(const bsa_evict_args a,
       po[s0 + i] = ps[s];
     }
   }
-  if (!moves && !pool) return;
-  const int pc = a.D / E, rg = 256 / pc;   // pieces per row, rows side by side
-  const int c = tid % pc, r0 = tid / pc;
-  T *kp = reinterpret_cast<T *>(a.k.ptr) + b * a.k.sb + h * a.k.sh + c * E;
-  T *vp = reinterpret_cast<T *>(a.v.ptr) + b * a.v.sb + h * a.v.sh + c * E;
-  float mn[E], mx[E];
-  const bool pad = rows < a.bs;  // rows past the budget count as zeros
-#pragma unroll
-  for (int e = 0; e < E; ++e) {
-    mn[e] = pad ? 0.f : INFINITY;
-    mx[e] = pad ? 0.f : -INFINITY;
-  }
-  constexpr int U = 4;  // rows in flight per thread
-  for (int rb = r0; rb < rows; rb += U * rg) {
-    uint4 kv[U], vv[U];
-    int src[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = rb + u * rg;
-      src[u] = r < rows ? s_src[r] : -1;
-      if (src[u] >= 0 && (pool || src[u] != s0 + r))
-        kv[u] = *reinterpret_cast<const uint4 *>(kp + (long long)src[u] * a.k.sl);
-      if (src[u] >= 0 && src[u] != s0 + r)
-        vv[u] = *reinterpret_cast<const uint4 *>(vp + (long long)src[u] * a.v.sl);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int r = rb + u * rg;
-      if (src[u] >= 0 && src[u] != s0 + r) {
-        *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv[u];
-        *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv[u];
-      }
-      if (src[u] >= 0 && pool) {
-        const T *ke = reinterpret_cast<const T *>(&kv[u]);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          float x;
-          if constexpr (sizeof(T) == 2)
-            x = Mma<T>::to_f(ke[e]);
-          else
-            x = ke[e];
-          mn[e] = fminf(mn[e], x);
-          mx[e] = fmaxf(mx[e], x);
-        }
-      }
-    }
-  }
   if (!pool) return;
   float *sp = reinterpret_cast<float *>(s_src + a.bs);  // [2][rg][D]
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    sp[r0 * a.D + c * E + e] = mn[e];
-    sp[(rg + r0) * a.D + c * E + e] = mx[e];
+    sp[r0 * a.D + c * E + e] = mm.min_of(e);
+    sp[(rg + r0) * a.D + c * E + e] = mm.max_of(e);
   }
   __syncthreads();
-  for (int d = tid; d < a.D; d += 256) {
-    float x = sp[d], y = sp[rg * a.D + d];
-    for (int r = 1; r < rg; ++r) {
-      x = fminf(x, sp[r * a.D + d]);
-      y = fmaxf(y, sp[(rg + r) * a.D + d]);
-    }
-    const long long at = b * a.km_sb + h * a.km_sh + (long long)blk * a.km_sn + d;
-    a.kmin[at] = x;
-    a.kmax[at] = y;
+  for (int i = tid; i < 2 * a.D; i += 256) {
+    const bool top = i >= a.D;
+    const int d = top ? i - a.D : i;
+    const float *s = sp + (top ? rg * a.D : 0) + d;
+    float x = s[0];
+    for (int r = 1; r < rg; ++r) x = top ? fmaxf(x, s[r * a.D]) : fminf(x, s[r * a.D]);
+    (top ? a.kmax : a.kmin)[b * a.km_sb + h * a.km_sh + (long long)blk * a.km_sn + d] = x;
   }
 }
 

@@ -1,8 +1,7 @@
 // Split-key attention of few query rows (decode steps) in bf16 / f16 / fp32, the
 // join of the splits, and the running sum of every slot's attention weight.
 //
-//   split_mma_kernel   bf16, f16: mma.sync; one warp streams its own keys
-//   split_f32_kernel   fp32 FMA; warps share the key tile, split rows and keys
+//   split_mma_kernel   partial softmax and O of one split; one warp streams its own keys
 //   split_join_kernel  joins the splits of every row; with weights, also adds
 //                      sum over the rows of p = 2^(x - lse) to each slot's sum
 // The kernels are bound by reading K and V once (HBM).
@@ -18,9 +17,34 @@ namespace {
 constexpr int kSplitWarps = 4;
 constexpr int kMaxLive = 512;  // block ids of one selection row
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
+// K and V are read once: they leave L2 first, so that the logits stay there for the join.
+__device__ __forceinline__ uint64_t evict_first_policy() {
+  uint64_t p;
+  asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live, uint64_t policy) {
   const int n = live ? 16 : 0;  // the rest of the 16 bytes is filled with zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(n),
+               "l"(policy)
+               : "memory");
+}
+
+// fp32 products on the tensor cores: x = hi + lo with hi and lo rounded to tf32 (11
+// bits each), x y = hi hi' + hi lo' + lo hi' up to 2^-21 |x y| (lo lo' and lo's own
+// rounding are dropped).  lo of an infinity is 0, so that hi carries it alone.
+__device__ __forceinline__ uint32_t tf32_rn(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
+__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
+  hi = tf32_rn(x);
+  const float d = x - __uint_as_float(hi);
+  lo = isinf(x) ? 0u : tf32_rn(d);
+}
+__device__ __forceinline__ void mma_tf32(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // Maximum that keeps a NaN: a row with a NaN logit ends as NaN, not as an empty row.
 __device__ __forceinline__ float fmax_nan(float a, float b) {
@@ -73,40 +97,54 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 }
 }  // namespace
 
-// ------------------------------------------------------------------ bf16 / f16
+// ------------------------------------------------------------------ partial kernel
 // CTA = (K/V head group, 16*MT query rows, split); each of its 4 warps takes every
 // fourth chunk of KC keys and keeps its own m, l and O, so the warps meet only at
 // the end.  A chunk's K and V rows arrive by 16-byte cp.async in a ring of NST
 // stages per warp, rows past the end zero-filled (never read).  S = Q K^T and
-// O += P V are m16n8k16 products with the query rows as M; 16 rows are mostly
+// O += P V are mma.sync products with the query rows as M; 16 rows are mostly
 // padding in a decode step (grp = 8: half), which costs nothing while HBM is the
-// bound: 8 KB of keys take 350 cycles of the SM's share of HBM, their products 64.
-// P is split in two 16-bit terms (p = hi + lo, hi = round(p), lo = round(p - hi)),
-// so its rounding does not add to the output's; the extra products are free here.
+// bound: 8 KB of keys take 350 cycles of the SM's share of HBM, their products 64
+// (bf16, D 128) or 190 (fp32).
+// 16-bit types (m16n8k16): P is split in two 16-bit terms (p = hi + lo, hi = round(p),
+// lo = round(p - hi)), so its rounding does not add to the output's; the extra products
+// are free here.  fp32 (m16n8k8 on tf32 terms): a contraction may take its index in any
+// order, so a thread's 16-byte piece of a K row feeds two k-steps (its dims 4t .. 4t+3
+// stand for k = t, t + 4 of each), S's accumulator layout is P's operand layout (keys
+// 2t, 2t + 1 stand for k = t, t + 4), and a 16-byte piece of a V row feeds four column
+// tiles (tile e holds columns 4j + e of a group of 32).
 // Keys that some rows of the tile must not see (the newest T - 1) are multiplied
 // one by one in fp32 and skipped where p = 0: an infinity or NaN in a masked V row
 // never reaches a row that does not see it.
-template <int D>
+template <typename T, int D>
 struct SplitCfg {
-  static constexpr int KC = D >= 128 ? 16 : 32;
-  static constexpr int STAGE = KC * D * 2 * 2;        // K and V of a chunk, bytes
-  static constexpr int NST = D == 32 ? 5 : 3;
-  static constexpr int MINB = D == 256 ? 1 : 2;       // CTAs per SM
+  static constexpr int ES = sizeof(T);
+  static constexpr int KC = ES == 2 ? (D >= 128 ? 16 : 32) : (D == 256 ? 8 : 16);
+  static constexpr int STAGE = KC * D * ES * 2;       // K and V of a chunk, bytes
+  static constexpr int NST = STAGE <= 4096 ? 5 : 3;
+  static constexpr int MINB = STAGE >= 16384 ? 1 : 2; // CTAs per SM
   static constexpr int RING = kSplitWarps * NST * STAGE;
 };
 
-template <int D>
-__device__ __forceinline__ uint32_t sw_off(int row, int chunk) {  // 16-byte chunk of a D-wide row
-  if constexpr (D == 32)
+// Byte offset of 16-byte chunk `chunk` of a D-wide row: chunks are permuted within
+// 128 bytes so that the eight rows (16-bit: ldmatrix) or two / four rows (fp32: the
+// pieces of K / V above) read together fall into different banks.
+template <int ES, int D>
+__device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
+  if constexpr (ES == 2 && D == 32)
     return row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
-  else
+  else if constexpr (ES == 2)
     return row * (D * 2) + (((chunk & ~7) | ((chunk ^ row) & 7)) << 4);
+  else
+    return row * (D * 4) + ((chunk ^ ((row & 6) ^ ((row & 1) << 2))) << 4);
 }
 
 template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
+__global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<T, D>::MINB)
     split_mma_kernel(const SplitParams p, int rtiles, int min_chunks) {
-  using C = SplitCfg<D>;
+  using C = SplitCfg<T, D>;
+  constexpr bool F32 = C::ES == 4;
+  constexpr int ES = C::ES, E16 = 16 / ES;            // elements per 16 bytes
   constexpr int KC = C::KC, NST = C::NST, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int s_blk[kMaxLive], s_raw[kMaxLive];
@@ -114,7 +152,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
   __shared__ int s_n;
   __shared__ float s_m[kSplitWarps][ROWS], s_l[kSplitWarps][ROWS];
   uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
-  uint8_t *ring = sm + ROWS * D * 2;
+  uint8_t *ring = sm + ROWS * D * ES;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, tq = lane & 3;
   pdl_trigger();  // the join may take its place on the SMs; it waits for this grid
@@ -161,6 +199,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
   const T *kb_ = reinterpret_cast<const T *>(p.k) + (p.fold ? 0 : b * p.k_sb) + hk * p.k_sh;
   const T *vb_ = reinterpret_cast<const T *>(p.v) + (p.fold ? 0 : b * p.v_sb) + hk * p.v_sh;
   uint8_t *wring = ring + warp * NST * C::STAGE;
+  const uint64_t policy = evict_first_policy();
   // first key of chunk c, and its gate
   auto key_of = [&](int c, float &gate) -> int {
     const int j = c * KC;
@@ -176,15 +215,15 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
     if (c < c_hi) {
       float gt;
       const int key0 = key_of(c, gt);
-      const uint32_t dk = smem_u32(wring + st * C::STAGE), dv = dk + KC * D * 2;
+      const uint32_t dk = smem_u32(wring + st * C::STAGE), dv = dk + KC * D * ES;
 #pragma unroll
-      for (int it = 0; it < KC * D / 8 / 32; ++it) {
-        const int i = it * 32 + lane, row = i / (D / 8), ch = i % (D / 8);
+      for (int it = 0; it < KC * D / E16 / 32; ++it) {
+        const int i = it * 32 + lane, row = i / (D / E16), ch = i % (D / E16);
         const bool ok = key0 + row < len;
         const long long key = ok ? key0 + row : 0;
-        const uint32_t off = sw_off<D>(row, ch);
-        cp16(dk + off, kb_ + key * p.k_sl + ch * 8, ok);
-        cp16(dv + off, vb_ + key * p.v_sl + ch * 8, ok);
+        const uint32_t off = sw_off<ES, D>(row, ch);
+        cp16(dk + off, kb_ + key * p.k_sl + ch * E16, ok, policy);
+        cp16(dv + off, vb_ + key * p.v_sl + ch * E16, ok, policy);
       }
     }
     cp_commit();
@@ -193,28 +232,27 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
   for (int s = 0; s < NST - 1; ++s) load(c_lo + warp + s * kSplitWarps, s);
 
   // query rows, zeros past R
-  for (int i = tid; i < ROWS * (D / 8); i += blockDim.x) {
-    const int r = i / (D / 8), ch = i % (D / 8);
-    alignas(16) T e[8];
-#pragma unroll
-    for (int x = 0; x < 8; ++x) e[x] = Mma<T>::from_f(0.f);
+  for (int i = tid; i < ROWS * (D / E16); i += blockDim.x) {
+    const int r = i / (D / E16), ch = i % (D / E16);
+    alignas(16) T e[E16];
+    *reinterpret_cast<uint4 *>(e) = make_uint4(0, 0, 0, 0);
     if (r0 + r < p.R) {
       int rb, rh, rtt;
       split_row(p, b, hk, r0 + r, rb, rh, rtt);
-      const T *qp = reinterpret_cast<const T *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + ch * 8;
+      const T *qp = reinterpret_cast<const T *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + ch * E16;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) e[x] = qp[x];
+      for (int x = 0; x < E16; ++x) e[x] = qp[x];
     }
-    *reinterpret_cast<uint4 *>(sQ + sw_off<D>(r, ch)) = *reinterpret_cast<uint4 *>(e);
+    *reinterpret_cast<uint4 *>(sQ + sw_off<ES, D>(r, ch)) = *reinterpret_cast<uint4 *>(e);
   }
   __syncthreads();
 
-  constexpr bool QREG = D <= 128 && MT == 1;
+  constexpr bool QREG = !F32 && D <= 128 && MT == 1;
   const uint32_t qa = smem_u32(sQ);
   uint32_t qf[QREG ? KS : 1][4];
   auto ldq = [&](int mt, int ks, uint32_t *a) {
     const int row = mt * 16 + (lane & 15), ch = ks * 2 + (lane >> 4);
-    ldsm_x4(qa + sw_off<D>(row, ch), a[0], a[1], a[2], a[3]);
+    ldsm_x4(qa + sw_off<ES, D>(row, ch), a[0], a[1], a[2], a[3]);
   };
   if constexpr (QREG)
 #pragma unroll
@@ -247,7 +285,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
       if (nst >= NST) nst -= NST;
       load(c + (NST - 1) * kSplitWarps, nst);
     }
-    const uint32_t ka = smem_u32(wring + st * C::STAGE), va = ka + KC * D * 2;
+    const uint32_t ka = smem_u32(wring + st * C::STAGE), va = ka + KC * D * ES;
+    const uint8_t *sk = wring + st * C::STAGE, *sv = sk + KC * D * ES;
     float gate;
     const int key0 = key_of(c, gate);
     // ---- S = Q K^T
@@ -258,27 +297,65 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
       for (int n = 0; n < KC / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+    if constexpr (!F32) {
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      uint32_t a[MT][4];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if constexpr (QREG) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) a[mt][e] = qf[ks][e];
-        } else {
-          ldq(mt, ks, a[mt]);
-        }
-      }
-#pragma unroll
-      for (int n2 = 0; n2 < KC / 16; ++n2) {
-        uint32_t b0, b1, b2, b3;
-        const int row = n2 * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
-        ldsm_x4(ka + sw_off<D>(row, ch), b0, b1, b2, b3);
+      for (int ks = 0; ks < KS; ++ks) {
+        uint32_t a[MT][4];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          Mma<T>::run(s[mt][2 * n2], a[mt], b0, b1);
-          Mma<T>::run(s[mt][2 * n2 + 1], a[mt], b2, b3);
+          if constexpr (QREG) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[mt][e] = qf[ks][e];
+          } else {
+            ldq(mt, ks, a[mt]);
+          }
+        }
+#pragma unroll
+        for (int n2 = 0; n2 < KC / 16; ++n2) {
+          uint32_t b0, b1, b2, b3;
+          const int row = n2 * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
+          ldsm_x4(ka + sw_off<ES, D>(row, ch), b0, b1, b2, b3);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            Mma<T>::run(s[mt][2 * n2], a[mt], b0, b1);
+            Mma<T>::run(s[mt][2 * n2 + 1], a[mt], b2, b3);
+          }
+        }
+      }
+    } else {
+#pragma unroll 4
+      for (int ks = 0; ks < KS; ++ks) {  // 16 dims: two k-steps
+        uint32_t ah[MT][2][4], al[MT][2][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const float4 x = *reinterpret_cast<const float4 *>(sQ + sw_off<ES, D>(mt * 16 + g, ks * 4 + tq));
+          const float4 y = *reinterpret_cast<const float4 *>(sQ + sw_off<ES, D>(mt * 16 + g + 8, ks * 4 + tq));
+          tf32_split(x.x, ah[mt][0][0], al[mt][0][0]);
+          tf32_split(y.x, ah[mt][0][1], al[mt][0][1]);
+          tf32_split(x.y, ah[mt][0][2], al[mt][0][2]);
+          tf32_split(y.y, ah[mt][0][3], al[mt][0][3]);
+          tf32_split(x.z, ah[mt][1][0], al[mt][1][0]);
+          tf32_split(y.z, ah[mt][1][1], al[mt][1][1]);
+          tf32_split(x.w, ah[mt][1][2], al[mt][1][2]);
+          tf32_split(y.w, ah[mt][1][3], al[mt][1][3]);
+        }
+#pragma unroll
+        for (int n = 0; n < KC / 8; ++n) {
+          const float4 k4 = *reinterpret_cast<const float4 *>(sk + sw_off<ES, D>(n * 8 + g, ks * 4 + tq));
+          uint32_t bh[4], bl[4];
+          tf32_split(k4.x, bh[0], bl[0]);
+          tf32_split(k4.y, bh[1], bl[1]);
+          tf32_split(k4.z, bh[2], bl[2]);
+          tf32_split(k4.w, bh[3], bl[3]);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int k2 = 0; k2 < 2; ++k2) {
+              const uint32_t *xh = ah[mt][k2], *xl = al[mt][k2];
+              mma_tf32(s[mt][n], xl[0], xl[1], xl[2], xl[3], bh[2 * k2], bh[2 * k2 + 1]);
+              mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bl[2 * k2], bl[2 * k2 + 1]);
+              mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bh[2 * k2], bh[2 * k2 + 1]);
+            }
         }
       }
     }
@@ -337,29 +414,62 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
     }
     // ---- O += P V
     if (!mixed) {
+      if constexpr (F32) {
 #pragma unroll
-      for (int k2 = 0; k2 < KC / 16; ++k2) {
-        uint32_t hi[MT][4], lo[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float x = s[mt][2 * k2 + (e >> 1)][2 * (e & 1)], y = s[mt][2 * k2 + (e >> 1)][2 * (e & 1) + 1];
-            hi[mt][e] = Mma<T>::pack(x, y);
-            const T *ht = reinterpret_cast<const T *>(&hi[mt][e]);
-            lo[mt][e] = Mma<T>::pack(x - Mma<T>::to_f(ht[0]), y - Mma<T>::to_f(ht[1]));
-          }
-#pragma unroll
-        for (int n2 = 0; n2 < NT / 2; ++n2) {
-          uint32_t b0, b1, b2, b3;
-          const int row = k2 * 16 + (lane & 15), ch = n2 * 2 + (lane >> 4);
-          ldsm_x4_t(va + sw_off<D>(row, ch), b0, b1, b2, b3);
+        for (int k8 = 0; k8 < KC / 8; ++k8) {
+          uint32_t ph[MT][4], pl[MT][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            Mma<T>::run(acc[mt][2 * n2], hi[mt], b0, b1);
-            Mma<T>::run(acc[mt][2 * n2 + 1], hi[mt], b2, b3);
-            Mma<T>::run(acc[mt][2 * n2], lo[mt], b0, b1);
-            Mma<T>::run(acc[mt][2 * n2 + 1], lo[mt], b2, b3);
+            tf32_split(s[mt][k8][0], ph[mt][0], pl[mt][0]);
+            tf32_split(s[mt][k8][2], ph[mt][1], pl[mt][1]);
+            tf32_split(s[mt][k8][1], ph[mt][2], pl[mt][2]);
+            tf32_split(s[mt][k8][3], ph[mt][3], pl[mt][3]);
+          }
+#pragma unroll
+          for (int cg = 0; cg < D / 32; ++cg) {
+            const float4 v0 = *reinterpret_cast<const float4 *>(sv + sw_off<ES, D>(k8 * 8 + 2 * tq, cg * 8 + g));
+            const float4 v1 = *reinterpret_cast<const float4 *>(sv + sw_off<ES, D>(k8 * 8 + 2 * tq + 1, cg * 8 + g));
+            const float x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              uint32_t h0, l0, h1, l1;
+              tf32_split(x0[e], h0, l0);
+              tf32_split(x1[e], h1, l1);
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                float *c = acc[mt][cg * 4 + e];
+                mma_tf32(c, pl[mt][0], pl[mt][1], pl[mt][2], pl[mt][3], h0, h1);
+                mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], l0, l1);
+                mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], h0, h1);
+              }
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int k2 = 0; k2 < KC / 16; ++k2) {
+          uint32_t hi[MT][4], lo[MT][4];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float x = s[mt][2 * k2 + (e >> 1)][2 * (e & 1)], y = s[mt][2 * k2 + (e >> 1)][2 * (e & 1) + 1];
+              hi[mt][e] = Mma<T>::pack(x, y);
+              const T *ht = reinterpret_cast<const T *>(&hi[mt][e]);
+              lo[mt][e] = Mma<T>::pack(x - Mma<T>::to_f(ht[0]), y - Mma<T>::to_f(ht[1]));
+            }
+#pragma unroll
+          for (int n2 = 0; n2 < NT / 2; ++n2) {
+            uint32_t b0, b1, b2, b3;
+            const int row = k2 * 16 + (lane & 15), ch = n2 * 2 + (lane >> 4);
+            ldsm_x4_t(va + sw_off<ES, D>(row, ch), b0, b1, b2, b3);
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+              Mma<T>::run(acc[mt][2 * n2], hi[mt], b0, b1);
+              Mma<T>::run(acc[mt][2 * n2 + 1], hi[mt], b2, b3);
+              Mma<T>::run(acc[mt][2 * n2], lo[mt], b0, b1);
+              Mma<T>::run(acc[mt][2 * n2 + 1], lo[mt], b2, b3);
+            }
           }
         }
       }
@@ -375,7 +485,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
           for (int e = 0; e < 4; ++e)
             sp[(mt * 16 + g + 8 * (e >> 1)) * KC + n * 8 + tq * 2 + (e & 1)] = s[mt][n][e];
       __syncwarp();
-      const uint8_t *sv = wring + st * C::STAGE + KC * D * 2;
 #pragma unroll 1
       for (int k = 0; k < KC && key0 + k < len; ++k) {
 #pragma unroll
@@ -383,8 +492,16 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
           const float pa = sp[(mt * 16 + g) * KC + k], pb = sp[(mt * 16 + g + 8) * KC + k];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const T *vp = reinterpret_cast<const T *>(sv + sw_off<D>(k, n) + tq * 4);
-            const float v0 = Mma<T>::to_f(vp[0]), v1 = Mma<T>::to_f(vp[1]);
+            float v0, v1;  // this thread's two columns of tile n
+            if constexpr (F32) {
+              const int ch = (n >> 2) * 8 + 2 * tq;
+              v0 = *reinterpret_cast<const float *>(sv + sw_off<ES, D>(k, ch) + (n & 3) * 4);
+              v1 = *reinterpret_cast<const float *>(sv + sw_off<ES, D>(k, ch + 1) + (n & 3) * 4);
+            } else {
+              const T *vp = reinterpret_cast<const T *>(sv + sw_off<ES, D>(k, n) + tq * 4);
+              v0 = Mma<T>::to_f(vp[0]);
+              v1 = Mma<T>::to_f(vp[1]);
+            }
             if (pa != 0.f) {
               acc[mt][n][0] = fmaf(pa, v0, acc[mt][n][0]);
               acc[mt][n][1] = fmaf(pa, v1, acc[mt][n][1]);
@@ -426,10 +543,17 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
       for (int w = 1; w < kSplitWarps; ++w) M = fmax_nan(M, s_m[w][r]);
       const float f = m[mt][h] == -INFINITY ? 0.f : ex2(m[mt][h] - M);
       if (r0 + r < p.R) {
-        float *op = so + (warp * ROWS + r) * D + tq * 2;
+        float *op = so + (warp * ROWS + r) * D;
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-          *reinterpret_cast<float2 *>(op + n * 8) = make_float2(acc[mt][n][2 * h] * f, acc[mt][n][2 * h + 1] * f);
+        for (int n = 0; n < NT; ++n) {
+          const float x = acc[mt][n][2 * h] * f, y = acc[mt][n][2 * h + 1] * f;
+          if constexpr (F32) {
+            op[(n >> 2) * 32 + tq * 8 + (n & 3)] = x;
+            op[(n >> 2) * 32 + tq * 8 + 4 + (n & 3)] = y;
+          } else {
+            *reinterpret_cast<float2 *>(op + n * 8 + tq * 2) = make_float2(x, y);
+          }
+        }
       }
     }
   __syncthreads();
@@ -455,282 +579,6 @@ __global__ void __launch_bounds__(kSplitWarps * 32, SplitCfg<D>::MINB)
 #pragma unroll
       for (int w = 0; w < kSplitWarps; ++w)
         L += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2(s_m[w][r] - M);
-      p.pml[at] = make_float2(M, L);
-    }
-  }
-}
-
-// ------------------------------------------------------------------ fp32
-// CTA = 8 warps over (K/V head group, 8*WR query rows, split).  Key tiles of KT
-// rows (K and V) are staged by cp.async for the whole CTA; warp w takes rows
-// 8*(w % WR).. and every (8/WR)-th group of the tile's keys, so few rows split the
-// keys and many rows share them.  A key's dot products with the 8 rows: each lane
-// multiplies its 16-byte slice of K with the rows' slices (kept in registers) and
-// a butterfly that halves the number of values at every step leaves row r's sum in
-// the lanes whose index bits spell r.  P V runs on the same slices.
-template <int D>
-struct SplitF32 {
-  static constexpr int LPK = D >= 128 ? 32 : D / 4;  // lanes per key
-  static constexpr int KP = 32 / LPK;                // keys side by side in a warp
-  static constexpr int V4 = D / 4 / LPK;             // 16-byte slices per lane
-  static constexpr int KT = D == 256 ? 16 : 32;      // keys per tile
-  static constexpr int NST = 3;
-  static constexpr int STAGE = KT * D * 4 * 2;
-  static constexpr int MINB = D == 256 ? 1 : 2;      // 128 registers hold q and O at D 256
-};
-
-template <int D, int WR>
-__global__ void __launch_bounds__(256, SplitF32<D>::MINB)
-    split_f32_kernel(const SplitParams p, int rtiles, int min_tiles) {
-  using C = SplitF32<D>;
-  constexpr int LPK = C::LPK, KP = C::KP, V4 = C::V4, KT = C::KT, NST = C::NST, WK = 8 / WR;
-  constexpr int ROWS = 8 * WR;
-  constexpr int KW = KT / WK;      // keys of a tile for one warp
-  constexpr int IT = KW / KP > 0 ? KW / KP : 1;
-  static_assert(KW % KP == 0, "a warp's share of the tile is whole steps");
-  extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ int s_blk[kMaxLive], s_raw[kMaxLive];
-  __shared__ float s_gate[kMaxLive];
-  __shared__ int s_n;
-  __shared__ float s_m[8][8], s_l[8][8];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wr = warp % WR, wk = warp / WR;
-  pdl_trigger();
-  const int rt = blockIdx.x % rtiles, grpid = blockIdx.x / rtiles;
-  const int b = p.fold ? 0 : grpid / p.Hkv, hk = grpid % p.Hkv;
-  const int r0 = rt * ROWS + wr * 8;
-
-  int len = p.nkeys;
-  if (p.lens) {
-    len = __ldg(p.lens + b);
-    if (len < 0 || len > p.nkeys) {
-      if (tid == 0) report(p.status, BSA_DEVERR_INDEX);
-      len = len < 0 ? 0 : p.nkeys;
-    }
-  }
-  int nv = len;
-  if (p.sel) {
-    if (warp == 0) {
-      const int n = build_live(p, b, hk, len, s_blk, s_gate, s_raw);
-      if (lane == 0) s_n = n;
-      if (p.live && blockIdx.y == 0 && rt == 0) {
-        __syncwarp();
-        int *lv = p.live + (long long)grpid * (1 + p.kk);
-        for (int i = lane; i < n; i += 32) lv[1 + i] = s_blk[i];
-        if (lane == 0) lv[0] = n;
-      }
-    }
-    __syncthreads();
-    nv = s_n * p.bs;
-  }
-  const int nt = (nv + KT - 1) / KT;
-  const int tps = max(min_tiles, (nt + p.nsplit - 1) / p.nsplit);
-  const int t_lo = min(nt, (int)blockIdx.y * tps), t_hi = min(nt, t_lo + tps);
-  const int split = p.split0 + blockIdx.y;
-  if (t_lo >= t_hi) {
-    for (int r = tid; r < ROWS; r += blockDim.x)
-      if (rt * ROWS + r < p.R) {
-        int rb, rh, rtt;
-        const long long gr = split_row(p, b, hk, rt * ROWS + r, rb, rh, rtt);
-        p.pml[(long long)split * p.rows + gr] = make_float2(-INFINITY, 0.f);
-      }
-    return;
-  }
-  const float *kb_ = reinterpret_cast<const float *>(p.k) + (p.fold ? 0 : b * p.k_sb) + hk * p.k_sh;
-  const float *vb_ = reinterpret_cast<const float *>(p.v) + (p.fold ? 0 : b * p.v_sb) + hk * p.v_sh;
-  auto key_of = [&](int t, float &gate) -> int {
-    const int j = t * KT;
-    if (!p.sel) {
-      gate = 0.f;
-      return j;
-    }
-    const int i = j / p.bs;
-    gate = s_gate[i];
-    return s_blk[i] * p.bs + (j - i * p.bs);
-  };
-  auto load = [&](int t, int st) {
-    if (t < t_hi) {
-      float gt;
-      const int key0 = key_of(t, gt);
-      const uint32_t dk = smem_u32(sm + st * C::STAGE), dv = dk + KT * D * 4;
-#pragma unroll
-      for (int it = 0; it < KT * D / 4 / 256; ++it) {
-        const int i = it * 256 + tid, row = i / (D / 4), ch = i % (D / 4);
-        const bool ok = key0 + row < len;
-        const long long key = ok ? key0 + row : 0;
-        cp16(dk + i * 16, kb_ + key * p.k_sl + ch * 4, ok);
-        cp16(dv + i * 16, vb_ + key * p.v_sl + ch * 4, ok);
-      }
-    }
-    cp_commit();
-  };
-#pragma unroll
-  for (int s = 0; s < NST - 1; ++s) load(t_lo + s, s);
-
-  const int kl = lane / LPK, dl = lane % LPK;  // this lane's key among KP, and slice
-  float q[8][V4 * 4], acc[8][V4 * 4];
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    const float *qp = nullptr;
-    if (r0 + r < p.R) {
-      int rb, rh, rtt;
-      split_row(p, b, hk, r0 + r, rb, rh, rtt);
-      qp = reinterpret_cast<const float *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl;
-    }
-#pragma unroll
-    for (int x = 0; x < V4 * 4; ++x) {
-      q[r][x] = qp ? qp[(x / 4) * LPK * 4 + dl * 4 + (x & 3)] : 0.f;
-      acc[r][x] = 0.f;
-    }
-  }
-  // the row whose sums end in this lane
-  const int myrow = LPK == 32 ? lane >> 2 : LPK == 16 ? (lane >> 1) & 7 : lane & 7;
-  constexpr int RSH = LPK == 32 ? 2 : LPK == 16 ? 1 : 0;  // lane of row r: (kl * LPK) + (r << RSH)
-  const int qlast = p.causal ? len - p.T + (r0 + myrow) % p.T : len - 1;
-  const int all_see = p.causal ? len - p.T : len - 1;
-  float m = -INFINITY, l = 0.f;
-  float *lrow = p.logits && r0 + myrow < p.R && (LPK != 32 || (lane & 3) == 0) &&
-                        (LPK != 16 || (lane & 1) == 0)
-                    ? p.logits + ((long long)grpid * p.R + r0 + myrow) * p.ncap
-                    : nullptr;
-
-  int st = 0;
-  for (int t = t_lo; t < t_hi; ++t) {
-    cp_wait<NST - 2>();
-    __syncthreads();
-    {
-      int nst = st + NST - 1;
-      if (nst >= NST) nst -= NST;
-      load(t + NST - 1, nst);
-    }
-    if (r0 < p.R) {
-      float gate;
-      const int key0 = key_of(t, gate);
-      const float *sk = reinterpret_cast<const float *>(sm + st * C::STAGE), *sv = sk + KT * D;
-      const bool masked = key0 + KT - 1 > all_see;
-      constexpr int BT = IT < 4 ? IT : 4;  // steps whose maximum is taken together
-#pragma unroll 1
-      for (int i0 = 0; i0 < IT; i0 += BT) {
-        float x[BT];
-#pragma unroll
-        for (int i = 0; i < BT; ++i) {
-          const int kr = wk * KW + (i0 + i) * KP + kl;
-          float d[8];
-#pragma unroll
-          for (int r = 0; r < 8; ++r) d[r] = 0.f;
-#pragma unroll
-          for (int v = 0; v < V4; ++v) {
-            const float4 k4 = *reinterpret_cast<const float4 *>(sk + kr * D + v * LPK * 4 + dl * 4);
-#pragma unroll
-            for (int r = 0; r < 8; ++r) {
-              d[r] = fmaf(q[r][v * 4], k4.x, d[r]);
-              d[r] = fmaf(q[r][v * 4 + 1], k4.y, d[r]);
-              d[r] = fmaf(q[r][v * 4 + 2], k4.z, d[r]);
-              d[r] = fmaf(q[r][v * 4 + 3], k4.w, d[r]);
-            }
-          }
-#pragma unroll
-          for (int h = 4, sh = LPK / 2; h >= 1; h >>= 1, sh >>= 1) {
-            const bool up = lane & sh;
-#pragma unroll
-            for (int r = 0; r < h; ++r) {
-              const float keep = up ? d[r + h] : d[r], give = up ? d[r] : d[r + h];
-              d[r] = keep + __shfl_xor_sync(0xffffffffu, give, sh);
-            }
-          }
-          if (LPK == 32) d[0] += __shfl_xor_sync(0xffffffffu, d[0], 2);
-          if (LPK >= 16) d[0] += __shfl_xor_sync(0xffffffffu, d[0], 1);
-          x[i] = fmaf(d[0], p.scale2, gate);
-          if (masked && key0 + kr > qlast) x[i] = -INFINITY;
-          if (lrow) lrow[(long long)t * KT + kr] = x[i];
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int i = 1; i < BT; ++i) mx = fmax_nan(mx, x[i]);
-        if (KP >= 2) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        if (KP >= 4) mx = fmax_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        const float mn = fmax_nan(m, mx);
-        const float al = mn == -INFINITY ? 1.f : ex2(m - mn);
-        m = mn;
-        if (__any_sync(0xffffffffu, al != 1.f)) {
-          l *= al;
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const float ar = __shfl_sync(0xffffffffu, al, kl * LPK + (r << RSH));
-#pragma unroll
-            for (int e = 0; e < V4 * 4; ++e) acc[r][e] *= ar;
-          }
-        }
-        const float off = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int i = 0; i < BT; ++i) {
-          const float pr = ex2(x[i] - off);
-          l += pr;
-          const int kr = wk * KW + (i0 + i) * KP + kl;
-          float v[V4 * 4];
-#pragma unroll
-          for (int w = 0; w < V4; ++w) {
-            const float4 v4 = *reinterpret_cast<const float4 *>(sv + kr * D + w * LPK * 4 + dl * 4);
-            v[w * 4] = v4.x;
-            v[w * 4 + 1] = v4.y;
-            v[w * 4 + 2] = v4.z;
-            v[w * 4 + 3] = v4.w;
-          }
-#pragma unroll
-          for (int r = 0; r < 8; ++r) {
-            const float pv = __shfl_sync(0xffffffffu, pr, kl * LPK + (r << RSH));
-            if (!masked || pv != 0.f) {
-#pragma unroll
-              for (int e = 0; e < V4 * 4; ++e) acc[r][e] = fmaf(pv, v[e], acc[r][e]);
-            }
-          }
-        }
-      }
-    }
-    if (++st == NST) st = 0;
-  }
-  // ---- join the warps of a row group (and the KP keys side by side)
-  cp_wait<0>();
-  if (KP >= 2) l += __shfl_xor_sync(0xffffffffu, l, 16);
-  if (KP >= 4) l += __shfl_xor_sync(0xffffffffu, l, 8);
-  s_m[warp][myrow] = m;
-  s_l[warp][myrow] = l;
-  __syncthreads();
-  float *so = reinterpret_cast<float *>(sm);  // [wk][ROWS][D]
-#pragma unroll
-  for (int r = 0; r < 8; ++r) {
-    float M = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WK; ++w) M = fmax_nan(M, s_m[w * WR + wr][r]);
-    const float mm = s_m[warp][r];
-    const float f = mm == -INFINITY ? 0.f : ex2(mm - M);
-#pragma unroll
-    for (int x = 0; x < V4 * 4; ++x) {
-      float a = acc[r][x] * f;
-      if (KP >= 2) a += __shfl_xor_sync(0xffffffffu, a, 16);
-      if (KP >= 4) a += __shfl_xor_sync(0xffffffffu, a, 8);
-      if (kl == 0) so[(wk * ROWS + wr * 8 + r) * D + (x / 4) * LPK * 4 + dl * 4 + (x & 3)] = a;
-    }
-  }
-  __syncthreads();
-  const int nr = min(ROWS, p.R - rt * ROWS);
-  for (int i = tid; i < nr * D; i += 256) {
-    const int r = i / D, d = i % D;
-    float o = so[r * D + d];
-#pragma unroll
-    for (int w = 1; w < WK; ++w) o += so[(w * ROWS + r) * D + d];
-    int rb, rh, rtt;
-    const long long at = (long long)split * p.rows + split_row(p, b, hk, rt * ROWS + r, rb, rh, rtt);
-    p.po[at * D + d] = o;
-    if (d == 0) {
-      float M = -INFINITY, L = 0.f;
-#pragma unroll
-      for (int w = 0; w < WK; ++w) M = fmax_nan(M, s_m[w * WR + r / 8][r % 8]);
-#pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const float mw = s_m[w * WR + r / 8][r % 8];
-        L += mw == -INFINITY ? 0.f : s_l[w * WR + r / 8][r % 8] * ex2(mw - M);
-      }
       p.pml[at] = make_float2(M, L);
     }
   }
@@ -917,51 +765,46 @@ static int choose_split(long long groups, long long steps, int slots, int fixed,
 
 constexpr int kMaxSplit = 296;
 
-// Splits of the mma / f32 kernels for n keys, `groups` K/V head groups and R rows each.
+// Row tiles of 16 or 32: two tiles share a chunk's fragments where O fits the registers.
+constexpr int row_tiles(int D, int R) { return R > 16 && D >= 64 && D <= 128 ? 2 : 1; }
+
+template <typename T, int D>
+static int split_count_t(long long groups, int R, long long n) {
+  using C = SplitCfg<T, D>;
+  const int rows = 16 * row_tiles(D, R);
+  const long long step = C::KC * kSplitWarps;
+  return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, 148 * C::MINB, 4, kMaxSplit);
+}
+
+// Splits of the partial kernel for n keys, `groups` K/V head groups and R rows each.
 int split_count(int dtype, int D, long long groups, int R, long long n) {
-  if (dtype == BSA_F32) {
-    const int kt = D == 256 ? 16 : 32;
-    const int wr = R <= 8 ? 1 : R <= 16 ? 2 : R <= 32 ? 4 : 8;
-    const long long g = groups * ((R + 8 * wr - 1) / (8 * wr));
-    return choose_split(g, (n + kt - 1) / kt, 296, 4, kMaxSplit);
+  const bool f = dtype == BSA_F32;
+  switch (D) {
+    case 32: return f ? split_count_t<float, 32>(groups, R, n) : split_count_t<__half, 32>(groups, R, n);
+    case 64: return f ? split_count_t<float, 64>(groups, R, n) : split_count_t<__half, 64>(groups, R, n);
+    case 128: return f ? split_count_t<float, 128>(groups, R, n) : split_count_t<__half, 128>(groups, R, n);
+    default: return f ? split_count_t<float, 256>(groups, R, n) : split_count_t<__half, 256>(groups, R, n);
   }
-  const int kc = D >= 128 ? 16 : 32, mt = R > 16 && D >= 64 && D <= 128 ? 2 : 1;
-  const long long g = groups * ((R + 16 * mt - 1) / (16 * mt));
-  const long long steps = (n + kc * kSplitWarps - 1) / (kc * kSplitWarps);
-  return choose_split(g, steps, D == 256 ? 148 : 296, 4, kMaxSplit);
 }
 
 template <typename T, int D, int MT>
 static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_t st) {
-  using C = SplitCfg<D>;
+  using C = SplitCfg<T, D>;
   const int rtiles = (p.R + 16 * MT - 1) / (16 * MT);
-  const int smem = 16 * MT * D * 2 + C::RING;
+  const int smem = 16 * MT * D * C::ES + C::RING;
   auto kern = split_mma_kernel<T, D, MT>;
   static_assert(C::RING >= kSplitWarps * 16 * MT * D * 4, "the ring holds the warps' O for the join");
-  static_assert(C::KC * D * 2 >= 16 * MT * C::KC * 4, "a chunk's K buffer holds its P");
+  static_assert(C::KC * D * C::ES >= 16 * MT * C::KC * 4, "a chunk's K buffer holds its P");
   static std::atomic<uint64_t> done{0};
   allow_smem(reinterpret_cast<const void *>(kern), smem, done);
   kern<<<dim3((unsigned)(groups * rtiles), p.nsplit), kSplitWarps * 32, smem, st>>>(p, rtiles, kSplitWarps);
   return check_launch("split_mma");
 }
 
-template <int D, int WR>
-static bsa_status launch_f32(const SplitParams &p, long long groups, cudaStream_t st) {
-  using C = SplitF32<D>;
-  const int rtiles = (p.R + 8 * WR - 1) / (8 * WR);
-  const int smem = C::NST * C::STAGE;
-  auto kern = split_f32_kernel<D, WR>;
-  static_assert(C::NST * C::STAGE >= 8 * 8 * D * 4, "the ring holds the warps' O for the join");
-  static std::atomic<uint64_t> done{0};
-  allow_smem(reinterpret_cast<const void *>(kern), smem, done);
-  kern<<<dim3((unsigned)(groups * rtiles), p.nsplit), 256, smem, st>>>(p, rtiles, 1);
-  return check_launch("split_f32");
-}
-
 template <typename T, int D>
 static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStream_t st) {
-  if constexpr (D >= 64 && D <= 128)
-    if (p.R > 16) return launch_mma<T, D, 2>(p, groups, st);
+  if constexpr (row_tiles(D, 17) == 2)
+    if (row_tiles(D, p.R) == 2) return launch_mma<T, D, 2>(p, groups, st);
   return launch_mma<T, D, 1>(p, groups, st);
 }
 
@@ -969,10 +812,7 @@ template <int D>
 static bsa_status launch_split_d(int dtype, const SplitParams &p, long long groups, cudaStream_t st) {
   if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D>(p, groups, st);
   if (dtype == BSA_F16) return launch_mma_d<__half, D>(p, groups, st);
-  if (p.R <= 8) return launch_f32<D, 1>(p, groups, st);
-  if (p.R <= 16) return launch_f32<D, 2>(p, groups, st);
-  if (p.R <= 32) return launch_f32<D, 4>(p, groups, st);
-  return launch_f32<D, 8>(p, groups, st);
+  return launch_mma_d<float, D>(p, groups, st);
 }
 
 bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStream_t st) {

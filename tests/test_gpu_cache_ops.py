@@ -3,7 +3,8 @@
 
 Tolerances.  A logit of the kernels is a dot product of D exact products in fp32; at
 most n = 8 + D/8 roundings of 2^-23 (the tensor cores truncate) touch a partial sum,
-none of which exceeds |q||k|, so in natural units it is off by at most
+none of which exceeds |q||k| (fp32 operands: three tf32 products for every eight dims,
+3D/8 roundings, and 2^-21 of |q||k| in dropped terms, n = 8 + 3D/8), so in natural units it is off by at most
 d = n 2^-23 |q||k| scale; the offset, the base change and ex2 add at most 2^-18 to the
 exponent's effect for logits up to 2^5.  A softmax weight is then off by a factor within
 1 +- e, e = 2 d + 2^-18, and with sum p = 1 the output by at most 2 e max|v| plus 2^-15
@@ -35,7 +36,7 @@ def _rel(q, k, scale):
     D = q.shape[-1]
     kn = k.double().norm(dim=-1)
     top = q.double().norm(dim=-1).max() * kn[torch.isfinite(kn)].max() * scale
-    return 2 * (8 + D / 8) * 2 ** -23 * float(top) + 2 ** -18
+    return 2 * (8 + (3 * D / 8 if q.dtype == torch.float32 else D / 8)) * 2 ** -23 * float(top) + 2 ** -18
 
 
 def _close_o(o, ref, e, vmax, what, once=0.0):
