@@ -213,64 +213,55 @@ __global__ void __launch_bounds__(kPickThreads)
   }
 }
 
-// Running min / max of 16 bytes of a row, kept in the row's own type (both are exact).
+// Min / max of 16 bytes of a row, element by element, in the row's own type (exact).
 template <typename T>
-struct MinMax {
-  using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-  P mn[4], mx[4];
-  __device__ void init(bool zero) {
-    const T lo = Mma<T>::from_f(zero ? 0.f : -INFINITY), hi = Mma<T>::from_f(zero ? 0.f : INFINITY);
+__device__ __forceinline__ uint4 min16(uint4 a, uint4 b, bool top) {
+  uint32_t *x = reinterpret_cast<uint32_t *>(&a);
+  const uint32_t *y = reinterpret_cast<const uint32_t *>(&b);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mn[e].x = mn[e].y = hi;
-      mx[e].x = mx[e].y = lo;
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 4) {
+      const float u = __uint_as_float(x[e]), v = __uint_as_float(y[e]);
+      x[e] = __float_as_uint(top ? fmaxf(u, v) : fminf(u, v));
+    } else {
+      using P = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+      const P u = *reinterpret_cast<const P *>(&x[e]), v = *reinterpret_cast<const P *>(&y[e]);
+      const P r = top ? __hmax2(u, v) : __hmin2(u, v);
+      x[e] = *reinterpret_cast<const uint32_t *>(&r);
     }
   }
-  __device__ void add(const uint4 &u) {
-    const P *x = reinterpret_cast<const P *>(&u);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mn[e] = __hmin2(mn[e], x[e]);
-      mx[e] = __hmax2(mx[e], x[e]);
-    }
-  }
-  __device__ float min_of(int e) const { return Mma<T>::to_f(e & 1 ? mn[e >> 1].y : mn[e >> 1].x); }
-  __device__ float max_of(int e) const { return Mma<T>::to_f(e & 1 ? mx[e >> 1].y : mx[e >> 1].x); }
-};
-template <>
-struct MinMax<float> {
-  float mn[4], mx[4];
-  __device__ void init(bool zero) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mn[e] = zero ? 0.f : INFINITY;
-      mx[e] = zero ? 0.f : -INFINITY;
-    }
-  }
-  __device__ void add(const uint4 &u) {
-    const float *x = reinterpret_cast<const float *>(&u);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      mn[e] = fminf(mn[e], x[e]);
-      mx[e] = fmaxf(mx[e], x[e]);
-    }
-  }
-  __device__ float min_of(int e) const { return mn[e]; }
-  __device__ float max_of(int e) const { return mx[e]; }
-};
+  return a;
+}
+template <typename T>
+__device__ __forceinline__ uint4 splat16(float x) {
+  uint4 u;
+  if constexpr (sizeof(T) == 4)
+    u.x = __float_as_uint(x);
+  else
+    u.x = Mma<T>::pack(x, x);
+  u.y = u.z = u.w = u.x;
+  return u;
+}
+__device__ __forceinline__ uint4 shfl_xor16(uint4 a, int o) {
+  return make_uint4(__shfl_xor_sync(0xffffffffu, a.x, o), __shfl_xor_sync(0xffffffffu, a.y, o),
+                    __shfl_xor_sync(0xffffffffu, a.z, o), __shfl_xor_sync(0xffffffffu, a.w, o));
+}
 
-// One CTA of 256 threads per block of slots.  A row of D elements is D*es/16
-// 16-byte pieces; a thread owns one piece column and every (256 / pieces)-th row.  A
-// block is a few rows per thread behind a chain of three dependent loads (offsets,
-// lists, rows), so what hides it is CTAs side by side: min and max stay in the row's
-// type and two rows are in flight, which leaves room for five CTAs per SM.
-template <typename T>
+// One CTA of 256 threads per block of slots.  A row is PC 16-byte pieces; a thread
+// owns one piece column (PC <= 32: its warp holds 32 / PC rows side by side) and every
+// RG-th row.  A block is a few rows per thread behind a chain of dependent loads
+// (offsets, lists, rows), so CTAs side by side hide it: min and max stay in the row's
+// type and are joined by shuffles, which leaves room for five CTAs per SM and takes
+// most of the instructions out (an fp32 min / max through shared memory: 42% of the
+// issue slots at half the HBM rate).
+template <typename T, int D>
 __global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args a, const EvictWork w) {
-  constexpr int E = 16 / sizeof(T);
-  extern __shared__ int s_src[];  // [bs] source slot, then the min / max of each thread row
+  constexpr int E = 16 / sizeof(T), PC = D / E, RG = 256 / PC;
+  extern __shared__ int s_src[];  // [bs] source slot, then per warp the min and the max
   const int blk = blockIdx.x % w.nblk, bh = blockIdx.x / w.nblk;
-  const int b = bh / a.Hkv, h = bh % a.Hkv, tid = threadIdx.x;
+  const int b = bh / a.Hkv, h = bh % a.Hkv, tid = threadIdx.x, warp = tid >> 5;
   const int s0 = blk * a.bs, rows = min(a.bs, a.budget - s0);
+  for (int i = tid; i < rows; i += 256) s_src[i] = s0 + i;
   pdl_wait();
   const int *off = w.off + (long long)bh * (w.nblk + 1);
   const int m0 = off[blk], m1 = off[blk + 1];
@@ -278,25 +269,23 @@ __global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args
   const bool same = a.weight_out == a.weight && a.pos_out == a.pos;
   const bool pool = a.kmin && (moves || rows < a.bs);
   if (!moves && !pool && same) return;
-  for (int i = tid; i < rows; i += 256) s_src[i] = s0 + i;
   __syncthreads();
-  for (int m = m0 + tid; m < m1; m += 256)
-    s_src[w.hole[(long long)bh * w.m_cap + m] - s0] = w.tail[(long long)bh * w.m_cap + m];
+  const long long list = (long long)bh * w.m_cap;
+  for (int m = m0 + tid; m < m1; m += 256) s_src[w.hole[list + m] - s0] = w.tail[list + m];
   __syncthreads();
-  MinMax<T> mm;
-  mm.init(rows < a.bs);  // rows past the budget count as zeros
-  const int pc = a.D / E, rg = 256 / pc;   // pieces per row, rows side by side
-  const int c = tid % pc, r0 = tid / pc;
+  const int c = tid % PC, r0 = tid / PC;
+  uint4 mn = splat16<T>(rows < a.bs ? 0.f : INFINITY);  // rows past the budget count as zeros
+  uint4 mx = splat16<T>(rows < a.bs ? 0.f : -INFINITY);
   if (moves || pool) {
     T *kp = reinterpret_cast<T *>(a.k.ptr) + b * a.k.sb + h * a.k.sh + c * E;
     T *vp = reinterpret_cast<T *>(a.v.ptr) + b * a.v.sb + h * a.v.sh + c * E;
     constexpr int U = 2;  // rows in flight per thread
-    for (int rb = r0; rb < rows; rb += U * rg) {
+    for (int rb = r0; rb < rows; rb += U * RG) {
       uint4 kv[U], vv[U];
       int src[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = rb + u * rg;
+        const int r = rb + u * RG;
         src[u] = r < rows ? s_src[r] : -1;
         if (src[u] >= 0 && (pool || src[u] != s0 + r))
           kv[u] = *reinterpret_cast<const uint4 *>(kp + (long long)src[u] * a.k.sl);
@@ -305,12 +294,15 @@ __global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int r = rb + u * rg;
+        const int r = rb + u * RG;
         if (src[u] >= 0 && src[u] != s0 + r) {
           *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv[u];
           *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv[u];
         }
-        if (src[u] >= 0 && pool) mm.add(kv[u]);
+        if (src[u] >= 0 && pool) {
+          mn = min16<T>(mn, kv[u], false);
+          mx = min16<T>(mx, kv[u], true);
+        }
       }
     }
   }
@@ -326,19 +318,34 @@ __global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args
     }
   }
   if (!pool) return;
-  float *sp = reinterpret_cast<float *>(s_src + a.bs);  // [2][rg][D]
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    sp[r0 * a.D + c * E + e] = mm.min_of(e);
-    sp[(rg + r0) * a.D + c * E + e] = mm.max_of(e);
+  for (int o = PC; o < 32; o <<= 1) {
+    mn = min16<T>(mn, shfl_xor16(mn, o), false);
+    mx = min16<T>(mx, shfl_xor16(mx, o), true);
+  }
+  // [min, max][warp row][PC]: at PC 64 (fp32, D 256) two warps hold a row
+  constexpr int WR = PC <= 32 ? 8 : 256 / PC;
+  uint4 *sp = reinterpret_cast<uint4 *>(s_src + (a.bs + 3) / 4 * 4);
+  const int wrow = PC <= 32 ? warp : r0;
+  if (PC > 32 || (tid & 31) < PC) {
+    sp[wrow * PC + c] = mn;
+    sp[(WR + wrow) * PC + c] = mx;
   }
   __syncthreads();
-  for (int i = tid; i < 2 * a.D; i += 256) {
-    const bool top = i >= a.D;
-    const int d = top ? i - a.D : i;
-    const float *s = sp + (top ? rg * a.D : 0) + d;
-    float x = s[0];
-    for (int r = 1; r < rg; ++r) x = top ? fmaxf(x, s[r * a.D]) : fminf(x, s[r * a.D]);
+  for (int i = tid; i < 2 * D; i += 256) {
+    const bool top = i >= D;
+    const int d = top ? i - D : i;
+    const T *s = reinterpret_cast<const T *>(sp + (top ? WR * PC : 0)) + d;
+    float x;
+#pragma unroll
+    for (int r = 0; r < WR; ++r) {
+      float y;
+      if constexpr (sizeof(T) == 4)
+        y = s[r * D];
+      else
+        y = Mma<T>::to_f(s[r * D]);
+      x = r == 0 ? y : top ? fmaxf(x, y) : fminf(x, y);
+    }
     (top ? a.kmax : a.kmin)[b * a.km_sb + h * a.km_sh + (long long)blk * a.km_sn + d] = x;
   }
 }
@@ -416,14 +423,22 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
     cudaLaunchKernelEx(&cfg, evict_pick_kernel<0>, *a, w, ipt);
   if (bsa_status s = check_launch("evict_pick")) return s;
   const unsigned grid = (unsigned)bh * w.nblk;
-  const int es = (int)elem_size(a->dtype), rg = 256 / (a->D * es / 16);
-  const size_t smem = (size_t)a->bs * 4 + 2ull * rg * a->D * 4;
-  if (a->dtype == BSA_BF16)
-    launch_after(evict_move_kernel<__nv_bfloat16>, grid, 256, smem, st, *a, w);
-  else if (a->dtype == BSA_F16)
-    launch_after(evict_move_kernel<__half>, grid, 256, smem, st, *a, w);
-  else
-    launch_after(evict_move_kernel<float>, grid, 256, smem, st, *a, w);
+  const size_t smem = (size_t)align_up(a->bs * 4, 16) + 2ull * 8 * a->D * elem_size(a->dtype);
+#define BSA_MOVE(T_)                                                                          \
+  switch (a->D) {                                                                             \
+    case 32: launch_after(evict_move_kernel<T_, 32>, grid, 256, smem, st, *a, w); break;      \
+    case 64: launch_after(evict_move_kernel<T_, 64>, grid, 256, smem, st, *a, w); break;      \
+    case 128: launch_after(evict_move_kernel<T_, 128>, grid, 256, smem, st, *a, w); break;    \
+    default: launch_after(evict_move_kernel<T_, 256>, grid, 256, smem, st, *a, w);            \
+  }
+  if (a->dtype == BSA_BF16) {
+    BSA_MOVE(__nv_bfloat16)
+  } else if (a->dtype == BSA_F16) {
+    BSA_MOVE(__half)
+  } else {
+    BSA_MOVE(float)
+  }
+#undef BSA_MOVE
   return check_launch("evict_move");
 }
 
