@@ -63,13 +63,13 @@ __device__ __forceinline__ int warp_prefix(int v, int *s, int *total) {
 }
 }  // namespace
 
-// IPT > 0: a thread's IPT keys stay in registers (up to 8 * 1024 * 16 slots per
-// head); IPT = 0: they are read again in every pass, for any length.  Warp w of a CTA
-// owns 32 * ipt consecutive slots, lane l of it slots l, l + 32, ..., so a rank among
-// them is a ballot, and one prefix over the warps per list.
+// Warp w of a CTA owns groups * 32 * IPT consecutive slots, in rows of 32: lane l of it
+// slots l, l + 32, ..., so a rank among them is a ballot, and one prefix over the warps
+// per list.  groups == 1: the IPT keys of a thread stay in registers (up to 8 * 1024 *
+// 16 slots per head); more: they are read again in every pass, for any length.
 template <int IPT>
 __global__ void __launch_bounds__(kPickThreads)
-    evict_pick_kernel(const bsa_evict_args a, const EvictWork w, const int ipt_) {
+    evict_pick_kernel(const bsa_evict_args a, const EvictWork w, const int groups) {
   cg::cluster_group cl = cg::this_cluster();
   const int nc = cl.num_blocks(), rank = cl.block_rank();
   const int bh = blockIdx.x / nc, b = bh / a.Hkv, h = bh % a.Hkv;
@@ -82,20 +82,22 @@ __global__ void __launch_bounds__(kPickThreads)
   const float *wt = a.weight + b * a.w_sb + h * a.w_sh;
   const int32_t *ps = a.pos + b * a.p_sb + h * a.p_sh;
   const int first_recent = a.seen - a.recent;
-  const int ipt = IPT > 0 ? IPT : ipt_;
-  const int base = (rank * 32 + warp) * 32 * ipt + lane;  // this lane's first slot
-  auto read = [&](int s) -> uint32_t {
-    return s < a.L ? evict_key(__ldg(wt + s), __ldg(ps + s), a.sink, first_recent) : 0u;
-  };
-  uint32_t kr[IPT > 0 ? IPT : 1];
-  if constexpr (IPT > 0)
+  const bool guards = a.sink > 0 || a.recent > 0;
+  const long long first = (long long)(rank * 32 + warp) * groups * (32 * IPT);  // this warp's first slot
+  uint32_t kr[IPT];
+  int base = 0;  // this lane's first slot of the group; slots past L get key 0, below every real one
+  auto load = [&](int g) {
+    base = (int)min(first + (long long)g * (32 * IPT), (long long)a.L) + lane;
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) kr[i] = read(base + 32 * i);
-  auto key = [&](int i) -> uint32_t {
-    if constexpr (IPT > 0)
-      return kr[i];
-    else
-      return read(base + 32 * i);
+    for (int i = 0; i < IPT; ++i) {
+      const int s = base + 32 * i;
+      kr[i] = s < a.L ? evict_key(__ldg(wt + s), guards ? __ldg(ps + s) : 0, a.sink, guards ? first_recent : 1) : 0u;
+    }
+  };
+  // rows of this group with base + 32 * i < end, as a bit mask
+  auto rows_below = [&](int end) {
+    const int n = min(max((end - base + 31) >> 5, 0), IPT);
+    return (1u << n) - 1u;
   };
   auto sync_all = [&] {
     if (nc > 1)
@@ -104,6 +106,7 @@ __global__ void __launch_bounds__(kPickThreads)
       __syncthreads();
   };
   for (int i = tid; i < 3 * kBins; i += kPickThreads) (&hist[0][0])[i] = 0;
+  load(0);
   __syncthreads();
 
   // ---- key of the budget-th best slot, 11 + 11 + 10 bits from the top
@@ -113,11 +116,14 @@ __global__ void __launch_bounds__(kPickThreads)
   for (int r3 = 0; r3 < 3; ++r3) {
     const int sh = r3 == 0 ? 21 : r3 == 1 ? 10 : 0, nb = r3 == 2 ? 1024 : 2048;
     int *hs = hist[r3];
+    for (int g = 0; g < groups; ++g) {
+      if (groups > 1) load(g);
 #pragma unroll
-    for (int i = 0; i < ipt; ++i) {
-      const uint32_t k = key(i);
-      if (base + 32 * i < a.L && (r3 == 0 || (k >> (sh + (r3 == 2 ? 10 : 11))) == prefix))
-        atomicAdd(&hs[(k >> sh) & (nb - 1)], 1);
+      for (int i = 0; i < IPT; ++i) {
+        const uint32_t k = kr[i];
+        if (k != 0u && (r3 == 0 || (k >> (sh + (r3 == 2 ? 10 : 11))) == prefix))
+          atomicAdd(&hs[(k >> sh) & (nb - 1)], 1);
+      }
     }
     sync_all();
     // bins from the top, two per thread; sums over the cluster
@@ -152,9 +158,12 @@ __global__ void __launch_bounds__(kPickThreads)
 
   // ---- equal keys before this warp's slots
   int eq = 0;
+  for (int g = 0; g < groups; ++g) {
+    if (groups > 1) load(g);
 #pragma unroll
-  for (int i = 0; i < ipt; ++i)
-    eq += __popc(__ballot_sync(0xffffffffu, base + 32 * i < a.L && key(i) == kth));
+    for (int i = 0; i < IPT; ++i) eq += kr[i] == kth;
+  }
+  eq = __reduce_add_sync(0xffffffffu, eq);
   int eq_total;
   int eq0 = warp_prefix(eq, s_scan[3], &eq_total);
   if (nc > 1) {
@@ -162,18 +171,33 @@ __global__ void __launch_bounds__(kPickThreads)
     cl.sync();
     for (int r = 0; r < rank; ++r) eq0 += cl.map_shared_rank(s_cnt, r)[0];
   }
+  // rows of the group that survive, as a bit mask; e: equal keys before the group
+  auto kept = [&](int &e) {
+    uint32_t keep = 0, same = 0;
+#pragma unroll
+    for (int i = 0; i < IPT; ++i) {
+      keep |= (uint32_t)(kr[i] > kth) << i;
+      same |= (uint32_t)(kr[i] == kth) << i;
+    }
+    if (__any_sync(0xffffffffu, same != 0u))
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) {
+        const unsigned m = __ballot_sync(0xffffffffu, (same >> i) & 1u);
+        if (((same >> i) & 1u) && e + __popc(m & below) < need) keep |= 1u << i;
+        e += __popc(m);
+      }
+    return keep;
+  };
   // ---- freed slots below the budget and survivors beyond it, in this warp
   int holes = 0, tails = 0, e = eq0;
-#pragma unroll
-  for (int i = 0; i < ipt; ++i) {
-    const int s = base + 32 * i;
-    const uint32_t k = key(i);
-    const unsigned same = __ballot_sync(0xffffffffu, s < a.L && k == kth);
-    const bool keep = k > kth || (k == kth && e + __popc(same & below) < need);
-    e += __popc(same);
-    holes += __popc(__ballot_sync(0xffffffffu, s < a.budget && !keep));
-    tails += __popc(__ballot_sync(0xffffffffu, s >= a.budget && s < a.L && keep));
+  for (int g = 0; g < groups; ++g) {
+    if (groups > 1) load(g);
+    const uint32_t keep = kept(e), low = rows_below(a.budget);
+    holes += __popc(low & ~keep);
+    tails += __popc(keep & ~low);
   }
+  holes = __reduce_add_sync(0xffffffffu, holes);
+  tails = __reduce_add_sync(0xffffffffu, tails);
   int hall, tall;
   int hb = warp_prefix(holes, s_scan[4], &hall), tb = warp_prefix(tails, s_scan[5], &tall);
   if (nc > 1) {
@@ -195,21 +219,26 @@ __global__ void __launch_bounds__(kPickThreads)
   int *off = w.off + (long long)bh * (w.nblk + 1);
   if (rank == 0 && tid == 0) off[w.nblk] = hall;
   e = eq0;
+  for (int g = 0; g < groups; ++g) {
+    if (groups > 1) load(g);
+    const uint32_t keep = kept(e), low = rows_below(a.budget);
+    const uint32_t fr = low & ~keep, sv = keep & ~low;
+    const int row0 = base - lane;
+    int blk = (row0 + a.bs - 1) / a.bs;  // the next block that starts in these rows
 #pragma unroll
-  for (int i = 0; i < ipt; ++i) {
-    const int s = base + 32 * i;
-    const uint32_t k = key(i);
-    const unsigned same = __ballot_sync(0xffffffffu, s < a.L && k == kth);
-    const bool keep = k > kth || (k == kth && e + __popc(same & below) < need);
-    e += __popc(same);
-    const bool fr = s < a.budget && !keep, sv = s >= a.budget && s < a.L && keep;
-    const unsigned fm = __ballot_sync(0xffffffffu, fr), sm = __ballot_sync(0xffffffffu, sv);
-    const int hr = hb + __popc(fm & below), tr = tb + __popc(sm & below);
-    hb += __popc(fm);
-    tb += __popc(sm);
-    if (s < a.budget && s % a.bs == 0) off[s / a.bs] = hr;
-    if (fr && hr < w.m_cap) hole[hr] = s;
-    if (sv && tr < w.m_cap) tail[tr] = s;
+    for (int i = 0; i < IPT; ++i) {
+      const int s = base + 32 * i;
+      const unsigned fm = __ballot_sync(0xffffffffu, (fr >> i) & 1u);
+      for (; blk < w.nblk && blk * a.bs < row0 + 32 * (i + 1); ++blk) {
+        const int at = blk * a.bs - (row0 + 32 * i);
+        if (lane == 0) off[blk] = hb + __popc(fm & ((1u << at) - 1u));
+      }
+      if ((fr >> i) & 1u) hole[hb + __popc(fm & below)] = s;
+      hb += __popc(fm);
+      const unsigned sm = __ballot_sync(0xffffffffu, (sv >> i) & 1u);
+      if ((sv >> i) & 1u) tail[tb + __popc(sm & below)] = s;
+      tb += __popc(sm);
+    }
   }
 }
 
@@ -404,6 +433,7 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
   while (nc < 8 && ((long long)nc * 16384 < a->L || ((long long)nc * 4096 < a->L && (long long)bh * nc * 2 <= 148)))
     nc *= 2;
   const int ipt = (int)((a->L + (long long)nc * kPickThreads - 1) / ((long long)nc * kPickThreads));
+  const int groups = std::max(1, (ipt + 15) / 16);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)bh * nc);
   cfg.blockDim = dim3(kPickThreads);
@@ -414,13 +444,13 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   if (ipt <= 1)
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<1>, *a, w, ipt);
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<1>, *a, w, 1);
   else if (ipt <= 4)
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<4>, *a, w, ipt);
-  else if (ipt <= 16)
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<16>, *a, w, ipt);
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<4>, *a, w, 1);
+  else if (ipt <= 8)
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<8>, *a, w, 1);
   else
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<0>, *a, w, ipt);
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<16>, *a, w, groups);
   if (bsa_status s = check_launch("evict_pick")) return s;
   const unsigned grid = (unsigned)bh * w.nblk;
   const size_t smem = (size_t)align_up(a->bs * 4, 16) + 2ull * 8 * a->D * elem_size(a->dtype);
