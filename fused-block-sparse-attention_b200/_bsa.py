@@ -627,6 +627,10 @@ _PACK = {"bsa_decode_weighted": _format(DecodeWeightedArgs), "bsa_evict": _forma
          "bsa_decode_prefix": _format(DecodePrefixArgs)}
 _packed_fn = {}
 
+# the current stream's handle without the Stream object (3 us a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
 
 def _launch(name, packed, dev):
     """Workspace and launch of entry point `name` (its argument struct as bytes) on CUDA
@@ -645,7 +649,7 @@ def _launch(name, packed, dev):
     if nbytes == 0:   # validation failed: the call reports why
         _check(run(packed, None, 0, None))
     ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-    st = run(packed, ws.data_ptr(), nbytes, torch.cuda.current_stream().cuda_stream)
+    st = run(packed, ws.data_ptr(), nbytes, _raw_stream(dev))
     if st:
         _check(st)
 
