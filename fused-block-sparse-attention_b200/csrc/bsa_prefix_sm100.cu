@@ -11,21 +11,22 @@
 // K/V tile: half the shared-memory fill per product.  NT = 1: up to 128 rows, or D 256,
 // whose O fills TMEM.  A tile's step is a chain S -> softmax -> PV, so what counts is
 // that the next S is there when a softmax ends:
-//   D 64, or NT = 1: steps of 128 keys; P has columns of its own, so S of the next step
-//     runs under the exponentials of this one.  Eight softmax warps per tile, half a row
-//     per thread; the halves exchange their maxima through shared memory.
-//   D 128 with two tiles ("half steps"): TMEM holds O and 128 columns per tile besides;
-//     steps of 64 keys use them as two S buffers, each overlaid by its own P, so S runs
-//     one step ahead.  (One buffer of 128 keys left S waiting for PV: 6600 cycles per
-//     128 keys and pair of tiles, tensor pipe 33% busy.)  Four warps per tile, a row per
-//     thread.
+//   NT = 1: steps of 128 keys; P has columns of its own, so S of the next step runs
+//     under the exponentials of this one.  Eight softmax warps, half a row per thread;
+//     the halves exchange their maxima through shared memory.
+//   NT = 2 ("half steps"): TMEM holds O and 128 columns per tile besides; steps of 64
+//     keys use them as two S buffers, each overlaid by its own P, so S runs one step
+//     ahead.  (One buffer of 128 keys left S waiting for PV: 6600 cycles per 128 keys
+//     and pair of tiles, tensor pipe 33% busy.)  Four warps per tile, a row per thread.
 //
 // K and V move as units of min(D, 128) columns x 128 keys in one ring, so that PV is
 // issued with N = 128: a 128x64x16 product costs as much tensor time as three quarters
-// of a 128x128x16 one.  Each tile has its issuing warp, S of the next step before
-// PV of this one: with one for both, the tensor pipe ran dry between the batches.
-// Softmax warps first, then the TMA producer, then the issuers, the first of which owns
-// TMEM.  Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the CTA runs
+// of a 128x128x16 one.  S and PV of each tile have an issuing warp of their own: a warp
+// that issues a product takes about as many cycles from the softmax warps of its SM
+// quarter as the product runs, so the issue is spread over the quarters, and with one
+// warp for all of it the tensor pipe ran dry between the batches.
+// Softmax warps first, then the TMA producer, then the issuers, the first of which
+// owns TMEM.  Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the CTA runs
 // on to its end.
 #include <type_traits>
 
@@ -39,6 +40,12 @@ namespace {
 constexpr int PX_KEYS = 128;
 constexpr int PX_CHUNK = PX_KEYS * 64 * 2;  // 16 KB: 128 rows x 64 columns
 constexpr float PX_RESCALE = 8.f;           // log2 units
+// f16 P: 2^7 larger (at most 2^15 with the lazy maximum), so that keys 2^-24 below the
+// largest still count; m is stored lower by as much.
+template <typename T>
+constexpr float px_shift() {
+  return std::is_same<T, __half>::value ? 7.f : 0.f;
+}
 
 template <int DP, int NT>
 struct PX {
@@ -47,10 +54,10 @@ struct PX {
   static constexpr int NU = NCH / UC;              // units per K or V tile
   static constexpr int UNIT = UC * PX_CHUNK;
   static constexpr int U = DP == 64 ? 10 : NT * NCH == 2 ? 6 : 5;  // ring units
-  static constexpr bool HALF = DP == 128 && NT == 2;
+  static constexpr bool HALF = NT == 2;
   static constexpr int KB = HALF ? 64 : 128;       // keys per step
   static constexpr int WPT = HALF ? 4 : 8;         // softmax warps per tile
-  static constexpr int WARPS = WPT * NT, THREADS = 32 * (WARPS + 1 + NT);
+  static constexpr int WARPS = WPT * NT, THREADS = 32 * (WARPS + 1 + 2 * NT);
   static constexpr int XCH = HALF ? 0 : NT * 2 * 4 * 2 * 32 * 4;
   static constexpr int SMEM = NT * NCH * PX_CHUNK + U * UNIT + XCH + 320;
   // TMEM columns of tile t (step parity b)
@@ -58,7 +65,7 @@ struct PX {
   static constexpr int P(int t, int b) { return HALF ? S(t, b) : 128 * NT + 64 * t; }
   static constexpr int O(int t) { return (HALF ? 256 : 192 * NT) + DP * t; }
   static constexpr uint32_t COLS = O(NT - 1) + DP <= 256 ? 256 : 512;
-  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 7 * NT) * 8 + 4 <= 320, "fits the SM");
+  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 7 * NT + 1) * 8 + 4 <= 320, "fits the SM");
 };
 }  // namespace
 
@@ -81,7 +88,8 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
   // second time before the first was seen
   uint64_t *r_full = bars, *r_empty = bars + U, *s_full = bars + 2 * U, *p_full = s_full + 2 * NT,
            *o_done = p_full + 2 * NT, *s_empty = o_done + 2 * NT;
-  uint32_t *tmem_sh = reinterpret_cast<uint32_t *>(s_empty + NT);
+  uint64_t *go = s_empty + NT;                   // half steps: tile 1 may start
+  uint32_t *tmem_sh = reinterpret_cast<uint32_t *>(go + 1);
 
   pdl_trigger();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -113,6 +121,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
       mbar_init(&s_empty[t], X::WPT);
     }
+    mbar_init(go, 1);
     fence_mbar_init();
   }
   if (warp == X::WARPS + 1) {
@@ -172,9 +181,11 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       if (HALF && j + 1 < ntiles) load(false, j + 1);
     }
   } else if (warp > X::WARPS) {
-    // ================= issuer of tile t: the whole warp runs the sequence, one elected
-    // lane (always the same) issues the products and commits
-    const int t = warp - X::WARPS - 1;
+    // ================= issuers: of S and of PV, one warp per tile each (warps + 1 ..: S of
+    // every tile, then PV).  The whole warp runs the sequence, one elected lane (always the
+    // same) issues the products and commits.
+    const int t = (warp - X::WARPS - 1) % NT;
+    const bool is_s = warp - X::WARPS - 1 < NT;
     const uint32_t on = tc05::elect_one();
     const uint64_t dq = tc05::sdesc(smem_u32(sQ), 16, 1024);
     const uint32_t sR0 = smem_u32(sR);
@@ -218,19 +229,22 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
       tc05::commit_if(on, &o_done[2 * t + b]);
     };
-    issue_s(0);
-    for (int j = 0; j < nsteps; ++j) {
-      if (j + 1 < nsteps) {
-        // the columns of S_{j+1}: free once S_j has been read; with half steps, once
-        // PV_{j-1}, whose P lies in them, is complete
-        if (!HALF)
-          wait(&s_empty[t], j & 1);
-        else if (j >= 1)
-          wait(&o_done[2 * t + ((j - 1) & 1)], ((j - 1) >> 1) & 1);
-        issue_s(j + 1);
+    if (is_s) {
+      // Half steps: the tiles run half a step apart, so that the exponentials of one fall
+      // between those of the other (the MUFU is half of a step when both wait for it).
+      if (HALF && t == 1) wait(go, 0);
+      for (int j = 0; j < nsteps; ++j) {
+        // the columns of S_j: free once S_{j-1} has been read; with half steps, once
+        // PV_{j-2}, whose P lies in them, is complete
+        if (!HALF && j >= 1) wait(&s_empty[t], (j - 1) & 1);
+        if (HALF && j >= 2) wait(&o_done[2 * t + (j & 1)], ((j - 2) >> 1) & 1);
+        issue_s(j);
       }
-      wait(&p_full[2 * t + (j & 1)], (j >> 1) & 1);
-      issue_pv(j);
+    } else {
+      for (int j = 0; j < nsteps; ++j) {
+        wait(&p_full[2 * t + (j & 1)], (j >> 1) & 1);
+        issue_pv(j);
+      }
     }
   } else {
     // ================= softmax
@@ -295,7 +309,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
         l *= alpha;
         need = true;
       }
-      const float off = m_used == -INFINITY ? 0.f : -m_used;
+      const float off = m_used == -INFINITY ? 0.f : px_shift<T>() - m_used;
       const float2 sc2 = make_float2(p.scale2, p.scale2), of2 = make_float2(off, off);
       uint32_t w[32];
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -308,6 +322,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
       const float2 st = add2(sum[0], sum[1]);
       l += st.x + st.y;
+      if (HALF && j == 0 && warp == 0 && lane == 0) tc05::mbar_arrive(go);
       const bool rescale = __any_sync(0xffffffffu, need) && j >= 1;
       // PV of the step before: has read its P (one P buffer), and O may be rescaled
       if (j >= 1 && (!HALF || rescale)) wait_pv(j - 1);
@@ -343,7 +358,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
         int rb, rh, rtt;
         at = (long long)split * p.rows + split_row(p, 0, hk, r0 + r, rb, rh, rtt);
         // a NaN sum with no maximum (every logit NaN) must not read as an empty row
-        if (hf == 0) p.pml[at] = make_float2(m_used == -INFINITY && isnan(l) ? l : m_used, l);
+        if (hf == 0) p.pml[at] = make_float2(m_used == -INFINITY && isnan(l) ? l : m_used - px_shift<T>(), l);
       }
 #pragma unroll 1
       for (int c = 0; c < OC; c += 32) {
