@@ -19,7 +19,7 @@
 //     ahead.  (One buffer of 128 keys left S waiting for PV: 6600 cycles per 128 keys
 //     and pair of tiles, tensor pipe 33% busy.)  Four warps per tile, a row per thread.
 //
-// K and V move as units of min(D, 128) columns x 128 keys in one ring, so that PV is
+// K and V move as units of min(D, 128) columns x one step's keys in one ring, so that PV is
 // issued with N = 128: a 128x64x16 product costs as much tensor time as three quarters
 // of a 128x128x16 one.  S and PV of each tile have an issuing warp of their own: a warp
 // that issues a product takes about as many cycles from the softmax warps of its SM
@@ -50,12 +50,13 @@ constexpr float px_shift() {
 template <int DP, int NT>
 struct PX {
   static constexpr int NCH = DP / 64;
-  static constexpr int UC = DP >= 128 ? 2 : 1;     // 64-column chunks per unit
-  static constexpr int NU = NCH / UC;              // units per K or V tile
-  static constexpr int UNIT = UC * PX_CHUNK;
-  static constexpr int U = DP == 64 ? 10 : NT * NCH == 2 ? 6 : 5;  // ring units
   static constexpr bool HALF = NT == 2;
   static constexpr int KB = HALF ? 64 : 128;       // keys per step
+  static constexpr int UC = DP >= 128 ? 2 : 1;     // 64-column chunks per unit
+  static constexpr int NU = NCH / UC;              // units per K or V step
+  static constexpr int CHUNK = KB * 64 * 2;        // a unit's KB rows x 64 columns
+  static constexpr int UNIT = UC * CHUNK;
+  static constexpr int U = HALF ? (DP == 64 ? 12 : 6) : DP == 256 ? 5 : 6;  // ring units
   static constexpr int WPT = HALF ? 4 : 8;         // softmax warps per tile
   static constexpr int WARPS = WPT * NT, THREADS = 32 * (WARPS + 1 + 2 * NT);
   static constexpr int XCH = HALF ? 0 : NT * 2 * 4 * 2 * 32 * 4;
@@ -97,8 +98,8 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
   const int r0 = rt * ROWS;
   const int nkt = (p.nkeys + PX_KEYS - 1) / PX_KEYS;
   const int j0 = blockIdx.y * cps;
-  const int ntiles = min(nkt, j0 + cps) - j0;    // >= 1 by the launcher's choice of splits
-  const int nsteps = HALF ? (min(p.nkeys, (j0 + ntiles) * PX_KEYS) - j0 * PX_KEYS + KB - 1) / KB : ntiles;
+  // this CTA's keys, at least one by the launcher's choice of splits, in steps of KB
+  const int nsteps = (min(p.nkeys, min(nkt, j0 + cps) * PX_KEYS) - j0 * PX_KEYS + KB - 1) / KB;
   const int split = p.split0 + blockIdx.y;
   // The swizzled layouts count on this alignment of the dynamic shared memory.
   if (smem_u32(smem) & 1023) {
@@ -152,33 +153,32 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
   __syncthreads();
   tc05::fence_after();
   const uint32_t tmem = *tmem_sh;
+  bool bad = false;  // a wait gave up
 
-  // Ring sequence, in tiles of NU units.  Half steps: K_0, V_0, K_1, V_1, ..., else
-  // K_0, K_1, V_0, K_2, V_1, ...: the order in which one row tile's products use them.
-  // k_at, v_at: position of step j's K and V.
-  auto k_at = [&](int j) { return (HALF ? 2 * (j >> 1) : j == 0 ? 0 : 2 * j - 1) * NU; };
-  auto v_at = [&](int j) { return (HALF ? 2 * (j >> 1) + 1 : j + 1 < nsteps ? 2 * j + 2 : 2 * j + 1) * NU; };
+  // Ring sequence, in steps of NU units: K_0, K_1, V_0, K_2, V_1, ...: S of the next
+  // step goes before PV of this one.  k_at, v_at: position of step j's K and V.
+  auto k_at = [&](int j) { return (j == 0 ? 0 : 2 * j - 1) * NU; };
+  auto v_at = [&](int j) { return (j + 1 < nsteps ? 2 * j + 2 : 2 * j + 1) * NU; };
   if (warp == X::WARPS) {
     // ================= TMA producer
     int n = 0;
     auto load = [&](bool isv, int j) {
       for (int u = 0; u < NU; ++u, ++n) {
         const int sl = n % U;
-        if (n >= U && !mbar_wait_warp(&r_empty[sl], ((n / U) - 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+        if (n >= U) bad |= !mbar_wait_warp(&r_empty[sl], ((n / U) - 1) & 1);
         if (tc05::elect_one()) {
           mbar_expect_tx(&r_full[sl], X::UNIT);
           for (int c = 0; c < UC; ++c)
-            tma_load_rhb(sR + sl * X::UNIT + c * PX_CHUNK, isv ? &tv : &tk, &r_full[sl], isv ? perm_v : perm_k,
-                         64 * (u * UC + c), (j0 + j) * PX_KEYS, hk, 0);
+            tma_load_rhb(sR + sl * X::UNIT + c * X::CHUNK, isv ? &tv : &tk, &r_full[sl], isv ? perm_v : perm_k,
+                         64 * (u * UC + c), j0 * PX_KEYS + j * KB, hk, 0);
         }
         __syncwarp();
       }
     };
     load(false, 0);
-    for (int j = 0; j < ntiles; ++j) {
-      if (!HALF && j + 1 < ntiles) load(false, j + 1);
+    for (int j = 0; j < nsteps; ++j) {
+      if (j + 1 < nsteps) load(false, j + 1);
       load(true, j);
-      if (HALF && j + 1 < ntiles) load(false, j + 1);
     }
   } else if (warp > X::WARPS) {
     // ================= issuers: of S and of PV, one warp per tile each (warps + 1 ..: S of
@@ -190,27 +190,25 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
     const uint64_t dq = tc05::sdesc(smem_u32(sQ), 16, 1024);
     const uint32_t sR0 = smem_u32(sR);
     auto wait = [&](uint64_t *bar, uint32_t parity) {
-      if (!mbar_wait_warp(bar, parity)) report(p.status, BSA_DEVERR_TIMEOUT);
+      bad |= !mbar_wait_warp(bar, parity);
       tc05::fence_after();
     };
-    // a unit is free once both tiles' last products on it are done
-    auto last_use = [&](int j) { return !HALF || (j & 1) || j == nsteps - 1; };
+    // a unit is free once every tile's products on it are done (r_empty counts the tiles)
     auto issue_s = [&](int j) {
       const int b = j & 1, n0 = k_at(j);
       const uint32_t ds = tc05::taddr(tmem, 0, b ? X::S(t, 1) : X::S(t, 0));
       for (int u = 0; u < NU; ++u) {
         const int sl = (n0 + u) % U;
-        if (!HALF || b == 0) wait(&r_full[sl], ((n0 + u) / U) & 1);  // once per unit
-        // half steps: the tile's upper 64 rows are 8 KB further on
-        const uint64_t dk = tc05::sdesc(sR0 + sl * X::UNIT, 16, 1024) + (HALF ? b * (64 * 128 >> 4) : 0);
+        wait(&r_full[sl], ((n0 + u) / U) & 1);
+        const uint64_t dk = tc05::sdesc(sR0 + sl * X::UNIT, 16, 1024);
         const uint64_t dqu = dq + (t * NCH + u * UC) * (PX_CHUNK >> 4);
 #pragma unroll
         for (int c = 0; c < UC; ++c)
 #pragma unroll
           for (int ks = 0; ks < 4; ++ks)
-            tc05::mma_f16_if(on, ds, dqu + c * (PX_CHUNK >> 4) + 2 * ks, dk + c * (PX_CHUNK >> 4) + 2 * ks, IDESC_S,
+            tc05::mma_f16_if(on, ds, dqu + c * (PX_CHUNK >> 4) + 2 * ks, dk + c * (X::CHUNK >> 4) + 2 * ks, IDESC_S,
                              (u > 0 || c > 0 || ks > 0) ? 1u : 0u);
-        if (last_use(j)) tc05::commit_if(on, &r_empty[sl]);
+        tc05::commit_if(on, &r_empty[sl]);
       }
       tc05::commit_if(on, &s_full[2 * t + b]);
     };
@@ -219,13 +217,13 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       const uint32_t ap = tc05::taddr(tmem, 0, b ? X::P(t, 1) : X::P(t, 0));
       for (int u = 0; u < NU; ++u) {
         const int sl = (n0 + u) % U;
-        if (!HALF || b == 0) wait(&r_full[sl], ((n0 + u) / U) & 1);  // once per unit
-        const uint64_t dv = tc05::sdesc(sR0 + sl * X::UNIT, PX_CHUNK, 1024) + (HALF ? b * (64 * 128 >> 4) : 0);
+        wait(&r_full[sl], ((n0 + u) / U) & 1);
+        const uint64_t dv = tc05::sdesc(sR0 + sl * X::UNIT, X::CHUNK, 1024);
 #pragma unroll
         for (int ks = 0; ks < KB / 16; ++ks)
           tc05::mma_f16_ts_if(on, tc05::taddr(tmem, 0, X::O(t) + 64 * UC * u), ap + 8 * ks, dv + 128 * ks, IDESC_PV,
                               (j > 0 || ks > 0) ? 1u : 0u);
-        if (last_use(j)) tc05::commit_if(on, &r_empty[sl]);
+        tc05::commit_if(on, &r_empty[sl]);
       }
       tc05::commit_if(on, &o_done[2 * t + b]);
     };
@@ -259,14 +257,14 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       return s_xch[(((par * NT + t) * 4 + quad) * 2 + half) * 32 + lane];
     };
     auto wait_pv = [&](int j) {
-      if (!mbar_wait(&o_done[2 * t + (j & 1)], (j >> 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      bad |= !mbar_wait(&o_done[2 * t + (j & 1)], (j >> 1) & 1);
       tc05::fence_after();
     };
     float m_used = -INFINITY, l = 0.f;
     for (int j = 0; j < nsteps; ++j) {
       const uint32_t ts = tmem + lane_base + (j & 1 ? X::S(t, 1) : X::S(t, 0)) + 64 * hf;
       const uint32_t tp = tmem + lane_base + (j & 1 ? X::P(t, 1) : X::P(t, 0)) + 32 * hf;
-      if (!mbar_wait(&s_full[2 * t + (j & 1)], (j >> 1) & 1)) report(p.status, BSA_DEVERR_TIMEOUT);
+      bad |= !mbar_wait(&s_full[2 * t + (j & 1)], (j >> 1) & 1);
       tc05::fence_after();
       if (!rows_here) {  // nothing to do but keep step; its P stays what it is
         __syncwarp();
@@ -374,6 +372,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
     }
   }
+  if (bad) report(p.status, BSA_DEVERR_TIMEOUT);
   tc05::fence_before();
   __syncthreads();
   if (warp == X::WARPS + 1) {
@@ -421,13 +420,14 @@ int prefix_sm100_splits(const bsa_decode_prefix_args *a) {
 }
 
 bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParams &p, cudaStream_t st) {
-  TensorMap4 mk, mv;
-  bsa_status s;
-  if ((s = make_tmap(&mk, a->pk.ptr, a->dtype, 1, a->Hkv, a->P, a->D, 0, a->pk.sh, a->pk.sl, 128, "pk"))) return s;
-  if ((s = make_tmap(&mv, a->pv.ptr, a->dtype, 1, a->Hkv, a->P, a->D, 0, a->pv.sh, a->pv.sl, 128, "pv"))) return s;
-  auto pk = [](const TensorMap4 &m) { return m.perm[0] | (m.perm[1] << 2) | (m.perm[2] << 4); };
   int nt, rtiles, cps, ns;
   prefix_shape(a->D, a->Hkv, p.R, a->P, nt, rtiles, cps, ns);
+  const int rows = nt == 2 ? 64 : 128;  // keys per unit
+  TensorMap4 mk, mv;
+  bsa_status s;
+  if ((s = make_tmap(&mk, a->pk.ptr, a->dtype, 1, a->Hkv, a->P, a->D, 0, a->pk.sh, a->pk.sl, rows, "pk"))) return s;
+  if ((s = make_tmap(&mv, a->pv.ptr, a->dtype, 1, a->Hkv, a->P, a->D, 0, a->pv.sh, a->pv.sl, rows, "pv"))) return s;
+  auto pk = [](const TensorMap4 &m) { return m.perm[0] | (m.perm[1] << 2) | (m.perm[2] << 4); };
   const int qvec = reinterpret_cast<uintptr_t>(a->q.ptr) % 16 == 0 && a->q.sb % 8 == 0 && a->q.sh % 8 == 0 &&
                    a->q.sl % 8 == 0;
   const dim3 grid((unsigned)(a->Hkv * rtiles), ns);
