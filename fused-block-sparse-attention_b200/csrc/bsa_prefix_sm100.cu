@@ -413,9 +413,10 @@ bool prefix_sm100_applicable(const bsa_decode_prefix_args *a) {
   return true;
 }
 
-int prefix_sm100_splits(const bsa_decode_prefix_args *a) {
+int prefix_sm100_splits(const bsa_decode_prefix_args *a, int *row_tiles) {
   int nt, rtiles, cps, ns;
   prefix_shape(a->D, a->Hkv, a->B * (a->Hq / a->Hkv) * a->T, a->P, nt, rtiles, cps, ns);
+  *row_tiles = nt;
   return ns;
 }
 

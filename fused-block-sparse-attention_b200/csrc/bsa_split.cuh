@@ -36,6 +36,7 @@ struct SplitParams {
   float *logits;        // optional [b*Hkv + hk][R][ncap]: x_j of each row
   long long ncap;
   int *live;            // with sel and logits: [b*Hkv + hk][1 + kk] count and live block ids
+  int after;            // launched beside the kernel before it, whose end it waits for at its own
   int32_t *status;
 };
 
