@@ -21,13 +21,12 @@
 //
 // K and V move as units of min(D, 128) columns x one step's keys in one ring, so that PV is
 // issued with N = 128: a 128x64x16 product costs as much tensor time as three quarters
-// of a 128x128x16 one.  S and PV of each tile have an issuing warp of their own: a warp
-// that issues a product takes about as many cycles from the softmax warps of its SM
-// quarter as the product runs, so the issue is spread over the quarters, and with one
+// of a 128x128x16 one.  S of each tile has an issuing warp, PV another: with one
 // warp for all of it the tensor pipe ran dry between the batches.
 // Softmax warps first, then the TMA producer, then the issuers, the first of which
 // owns TMEM.  Every wait is bounded; a timeout sets BSA_DEVERR_TIMEOUT and the CTA runs
 // on to its end.
+#include <algorithm>
 #include <type_traits>
 
 #include "bsa_host.h"
@@ -56,17 +55,17 @@ struct PX {
   static constexpr int NU = NCH / UC;              // units per K or V step
   static constexpr int CHUNK = KB * 64 * 2;        // a unit's KB rows x 64 columns
   static constexpr int UNIT = UC * CHUNK;
-  static constexpr int U = HALF ? (DP == 64 ? 12 : 6) : DP == 256 ? 5 : 6;  // ring units
+  static constexpr int U = HALF ? (DP == 64 ? 16 : 10) : DP == 256 ? 5 : 6;  // ring units
   static constexpr int WPT = HALF ? 4 : 8;         // softmax warps per tile
-  static constexpr int WARPS = WPT * NT, THREADS = 32 * (WARPS + 1 + 2 * NT);
+  static constexpr int WARPS = WPT * NT, THREADS = 32 * (WARPS + 2 + NT);
   static constexpr int XCH = HALF ? 0 : NT * 2 * 4 * 2 * 32 * 4;
-  static constexpr int SMEM = NT * NCH * PX_CHUNK + U * UNIT + XCH + 320;
+  static constexpr int SMEM = NT * NCH * PX_CHUNK + U * UNIT + XCH + 384;
   // TMEM columns of tile t (step parity b)
   static constexpr int S(int t, int b) { return 128 * t + (HALF ? 64 * b : 0); }
   static constexpr int P(int t, int b) { return HALF ? S(t, b) : 128 * NT + 64 * t; }
   static constexpr int O(int t) { return (HALF ? 256 : 192 * NT) + DP * t; }
   static constexpr uint32_t COLS = O(NT - 1) + DP <= 256 ? 256 : 512;
-  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 7 * NT + 1) * 8 + 4 <= 320, "fits the SM");
+  static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 7 * NT + 1) * 8 + 4 <= 384, "fits the SM");
 };
 }  // namespace
 
@@ -181,11 +180,11 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       load(true, j);
     }
   } else if (warp > X::WARPS) {
-    // ================= issuers: of S and of PV, one warp per tile each (warps + 1 ..: S of
-    // every tile, then PV).  The whole warp runs the sequence, one elected lane (always the
-    // same) issues the products and commits.
-    const int t = (warp - X::WARPS - 1) % NT;
-    const bool is_s = warp - X::WARPS - 1 < NT;
+    // ================= issuers: one warp per tile for S, one for every tile's PV.  The
+    // whole warp runs the sequence, one elected lane (always the same) issues the products
+    // and commits.
+    const int t_s = warp - X::WARPS - 1;
+    const bool is_s = t_s < NT;
     const uint32_t on = tc05::elect_one();
     const uint64_t dq = tc05::sdesc(smem_u32(sQ), 16, 1024);
     const uint32_t sR0 = smem_u32(sR);
@@ -194,7 +193,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       tc05::fence_after();
     };
     // a unit is free once every tile's products on it are done (r_empty counts the tiles)
-    auto issue_s = [&](int j) {
+    auto issue_s = [&](int t, int j) {
       const int b = j & 1, n0 = k_at(j);
       const uint32_t ds = tc05::taddr(tmem, 0, b ? X::S(t, 1) : X::S(t, 0));
       for (int u = 0; u < NU; ++u) {
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       }
       tc05::commit_if(on, &s_full[2 * t + b]);
     };
-    auto issue_pv = [&](int j) {
+    auto issue_pv = [&](int t, int j) {
       const int b = j & 1, n0 = v_at(j);
       const uint32_t ap = tc05::taddr(tmem, 0, b ? X::P(t, 1) : X::P(t, 0));
       for (int u = 0; u < NU; ++u) {
@@ -228,6 +227,7 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
       tc05::commit_if(on, &o_done[2 * t + b]);
     };
     if (is_s) {
+      const int t = t_s;
       // Half steps: the tiles run half a step apart, so that the exponentials of one fall
       // between those of the other (the MUFU is half of a step when both wait for it).
       if (HALF && t == 1) wait(go, 0);
@@ -236,13 +236,15 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
         // PV_{j-2}, whose P lies in them, is complete
         if (!HALF && j >= 1) wait(&s_empty[t], (j - 1) & 1);
         if (HALF && j >= 2) wait(&o_done[2 * t + (j & 1)], ((j - 2) >> 1) & 1);
-        issue_s(j);
+        issue_s(t, j);
       }
     } else {
-      for (int j = 0; j < nsteps; ++j) {
-        wait(&p_full[2 * t + (j & 1)], (j >> 1) & 1);
-        issue_pv(j);
-      }
+      for (int j = 0; j < nsteps; ++j)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          wait(&p_full[2 * t + (j & 1)], (j >> 1) & 1);
+          issue_pv(t, j);
+        }
     }
   } else {
     // ================= softmax
@@ -382,17 +384,27 @@ __global__ void __launch_bounds__(PX<DP, NT>::THREADS, 1)
 }
 
 namespace {
-// Row tiles of 128 or 256, and the splits of the prefix that fill the SMs (one CTA each).
-void prefix_shape(int D, int Hkv, int R, int P, int &nt, int &rtiles, int &cps, int &nsplit) {
-  nt = D <= 128 && R > 128 ? 2 : 1;
+// Row tiles of 128 or 256, and the splits of the prefix (one CTA per SM each).  The
+// kernel that reads the sequences' own slots starts on the SMs that this one leaves
+// free, so fewer splits than fill the SMs can be the faster whole: it is the split with
+// the least max(this kernel's time, all SM time / 148), in key tiles.  Measured: a tile
+// takes 2.4 us with two row tiles (D 128) and 1.8 us with one (D 256), and beside this
+// kernel an SM draws 46 GB/s of own slots; lengths are not known here, half of the
+// capacity is assumed.  Large batch (32768 keys, 128 sequences of up to 1024 slots,
+// D 128): 9, 8, 7, 6 splits 125, 122, 118, 115 us.
+void prefix_shape(const bsa_decode_prefix_args *a, int &nt, int &rtiles, int &cps, int &nsplit) {
+  const int R = a->B * (a->Hq / a->Hkv) * a->T;
+  nt = a->D <= 128 && R > 128 ? 2 : 1;
   rtiles = (R + 128 * nt - 1) / (128 * nt);
-  const long long items = (long long)Hkv * rtiles, nkt = (P + PX_KEYS - 1) / PX_KEYS;
+  const long long items = (long long)a->Hkv * rtiles, nkt = (a->P + PX_KEYS - 1) / PX_KEYS;
+  const double own = (double)a->B * a->Hkv * a->S * a->D * 2 / 46e3 / (nt == 2 ? 2.4 : 1.8);
   const int fixed = 3;  // prologue, first fill and epilogue of a CTA, in key tiles
-  long long best = -1;
+  double best = -1;
   cps = (int)nkt;
   for (long long s = 1; s <= nkt && s <= 148; ++s) {
     const long long c = (nkt + s - 1) / s, ns = (nkt + c - 1) / c;
-    const long long cost = ((items * ns + 147) / 148) * (c + fixed);
+    const double one = (double)((items * ns + 147) / 148) * (c + fixed);
+    const double cost = std::max(one, ((double)items * ns * (c + fixed) + own) / 148);
     if (best < 0 || cost < best) {
       best = cost;
       cps = (int)c;
@@ -413,16 +425,15 @@ bool prefix_sm100_applicable(const bsa_decode_prefix_args *a) {
   return true;
 }
 
-int prefix_sm100_splits(const bsa_decode_prefix_args *a, int *row_tiles) {
+int prefix_sm100_splits(const bsa_decode_prefix_args *a) {
   int nt, rtiles, cps, ns;
-  prefix_shape(a->D, a->Hkv, a->B * (a->Hq / a->Hkv) * a->T, a->P, nt, rtiles, cps, ns);
-  *row_tiles = nt;
+  prefix_shape(a, nt, rtiles, cps, ns);
   return ns;
 }
 
 bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParams &p, cudaStream_t st) {
   int nt, rtiles, cps, ns;
-  prefix_shape(a->D, a->Hkv, p.R, a->P, nt, rtiles, cps, ns);
+  prefix_shape(a, nt, rtiles, cps, ns);
   const int rows = nt == 2 ? 64 : 128;  // keys per unit
   TensorMap4 mk, mv;
   bsa_status s;

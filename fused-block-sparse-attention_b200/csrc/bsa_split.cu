@@ -14,6 +14,7 @@
 namespace bsa {
 
 namespace {
+constexpr int NW = 4;          // warps per CTA of the partial kernel
 constexpr int kMaxLive = 512;  // block ids of one selection row
 
 // K and V are read once: they leave L2 first, so that the logits stay there for the join.
@@ -97,11 +98,9 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 }  // namespace
 
 // ------------------------------------------------------------------ partial kernel
-// CTA = (K/V head group, 16*MT query rows, split); each of its NW warps takes every
-// NW-th chunk of KC keys and keeps its own m, l and O, so the warps meet only at
-// the end.  NW = 4; 2 beside the shared-prefix kernel with two row tiles, which leaves
-// 15 K registers and 60 KB of shared memory of an SM: the sequences' own slots are then
-// read while it computes.  A chunk's K and V rows arrive by 16-byte cp.async in a ring of NST
+// CTA = (K/V head group, 16*MT query rows, split); each of its NW = 4 warps takes every
+// fourth chunk of KC keys and keeps its own m, l and O, so the warps meet only at
+// the end.  A chunk's K and V rows arrive by 16-byte cp.async in a ring of NST
 // stages per warp, rows past the end zero-filled (never read).  S = Q K^T and
 // O += P V are mma.sync products with the query rows as M; 16 rows are mostly
 // padding in a decode step (grp = 8: half), which costs nothing while HBM is the
@@ -123,8 +122,8 @@ struct SplitCfg {
   static constexpr int KC = ES == 2 ? (D >= 128 ? 16 : 32) : (D == 256 ? 8 : 16);
   static constexpr int STAGE = KC * D * ES * 2;       // K and V of a chunk, bytes
   static constexpr int NST = STAGE <= 4096 ? 5 : 3;
-  static constexpr int MINB = STAGE >= 16384 ? 1 : 2; // CTAs of four warps per SM
-  static constexpr int ring(int nw) { return nw * NST * STAGE; }
+  static constexpr int MINB = STAGE >= 16384 ? 1 : 2; // CTAs per SM
+  static constexpr int RING = NW * NST * STAGE;
 };
 
 // Byte offset of 16-byte chunk `chunk` of a D-wide row: chunks are permuted within
@@ -140,8 +139,8 @@ __device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
     return row * (D * 4) + ((chunk ^ ((row & 6) ^ ((row & 1) << 2))) << 4);
 }
 
-template <typename T, int D, int MT, int NW>
-__global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB * 4 / NW)
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     split_mma_kernel(const SplitParams p, int rtiles, int min_chunks) {
   using C = SplitCfg<T, D>;
   constexpr bool F32 = C::ES == 4;
@@ -152,7 +151,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB * 4 / NW)
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
   uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
   uint8_t *ring = sm + ROWS * D * ES;
-  int *s_blk = reinterpret_cast<int *>(ring + C::ring(NW));  // with a selection: 3 * kMaxLive words
+  int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
   float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
   int *s_raw = s_blk + 2 * kMaxLive;
   // Launched to start beside the prefix kernel: its last CTA ends no earlier than that
@@ -776,32 +775,31 @@ constexpr int kMaxSplit = 296;
 constexpr int row_tiles(int D, int R) { return R > 16 && D >= 64 && D <= 128 ? 2 : 1; }
 
 template <typename T, int D>
-static int split_count_t(long long groups, int R, long long n, int nw) {
+static int split_count_t(long long groups, int R, long long n) {
   using C = SplitCfg<T, D>;
   const int rows = 16 * row_tiles(D, R);
-  const long long step = C::KC * nw;
-  return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, 148 * C::MINB * 4 / nw, 16 / nw,
-                      kMaxSplit);
+  const long long step = C::KC * NW;
+  return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, 148 * C::MINB, 4, kMaxSplit);
 }
 
-// Splits of the partial kernel (nw warps) for n keys, `groups` K/V head groups and R rows each.
-int split_count(int dtype, int D, long long groups, int R, long long n, int nw) {
+// Splits of the partial kernel for n keys, `groups` K/V head groups and R rows each.
+int split_count(int dtype, int D, long long groups, int R, long long n) {
   const bool f = dtype == BSA_F32;
   switch (D) {
-    case 32: return f ? split_count_t<float, 32>(groups, R, n, nw) : split_count_t<__half, 32>(groups, R, n, nw);
-    case 64: return f ? split_count_t<float, 64>(groups, R, n, nw) : split_count_t<__half, 64>(groups, R, n, nw);
-    case 128: return f ? split_count_t<float, 128>(groups, R, n, nw) : split_count_t<__half, 128>(groups, R, n, nw);
-    default: return f ? split_count_t<float, 256>(groups, R, n, nw) : split_count_t<__half, 256>(groups, R, n, nw);
+    case 32: return f ? split_count_t<float, 32>(groups, R, n) : split_count_t<__half, 32>(groups, R, n);
+    case 64: return f ? split_count_t<float, 64>(groups, R, n) : split_count_t<__half, 64>(groups, R, n);
+    case 128: return f ? split_count_t<float, 128>(groups, R, n) : split_count_t<__half, 128>(groups, R, n);
+    default: return f ? split_count_t<float, 256>(groups, R, n) : split_count_t<__half, 256>(groups, R, n);
   }
 }
 
-template <typename T, int D, int MT, int NW>
+template <typename T, int D, int MT>
 static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_t st) {
   using C = SplitCfg<T, D>;
   const int rtiles = (p.R + 16 * MT - 1) / (16 * MT);
-  const int base = 16 * MT * D * C::ES + C::ring(NW), most = base + 3 * kMaxLive * 4;
-  auto kern = split_mma_kernel<T, D, MT, NW>;
-  static_assert(C::ring(1) >= 16 * MT * D * 4, "the ring holds the warps' O for the join");
+  const int base = 16 * MT * D * C::ES + C::RING, most = base + 3 * kMaxLive * 4;
+  auto kern = split_mma_kernel<T, D, MT>;
+  static_assert(C::RING >= NW * 16 * MT * D * 4, "the ring holds the warps' O for the join");
   static_assert(C::KC * D * C::ES >= 16 * MT * C::KC * 4, "a chunk's K buffer holds its P");
   static std::atomic<uint64_t> done{0};
   allow_smem(reinterpret_cast<const void *>(kern), most, done);
@@ -814,31 +812,27 @@ static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_
   return check_launch("split_mma");
 }
 
-// nw = 2 is there for the 16-bit types at D <= 128 (beside the prefix kernel), 16 rows
-// per CTA: with 32 its registers would not fit.
 template <typename T, int D>
-static bsa_status launch_mma_d(const SplitParams &p, long long groups, int nw, cudaStream_t st) {
-  if constexpr (sizeof(T) == 2 && D <= 128)
-    if (nw == 2) return launch_mma<T, D, 1, 2>(p, groups, st);
+static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStream_t st) {
   if constexpr (row_tiles(D, 17) == 2)
-    if (row_tiles(D, p.R) == 2) return launch_mma<T, D, 2, 4>(p, groups, st);
-  return launch_mma<T, D, 1, 4>(p, groups, st);
+    if (row_tiles(D, p.R) == 2) return launch_mma<T, D, 2>(p, groups, st);
+  return launch_mma<T, D, 1>(p, groups, st);
 }
 
 template <int D>
-static bsa_status launch_split_d(int dtype, const SplitParams &p, long long groups, int nw, cudaStream_t st) {
-  if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D>(p, groups, nw, st);
-  if (dtype == BSA_F16) return launch_mma_d<__half, D>(p, groups, nw, st);
-  return launch_mma_d<float, D>(p, groups, nw, st);
+static bsa_status launch_split_d(int dtype, const SplitParams &p, long long groups, cudaStream_t st) {
+  if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D>(p, groups, st);
+  if (dtype == BSA_F16) return launch_mma_d<__half, D>(p, groups, st);
+  return launch_mma_d<float, D>(p, groups, st);
 }
 
-bsa_status launch_split(int dtype, int D, const SplitParams &p, int nw, cudaStream_t st) {
+bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStream_t st) {
   const long long groups = p.fold ? p.Hkv : (long long)p.B * p.Hkv;
   switch (D) {
-    case 32: return launch_split_d<32>(dtype, p, groups, nw, st);
-    case 64: return launch_split_d<64>(dtype, p, groups, nw, st);
-    case 128: return launch_split_d<128>(dtype, p, groups, nw, st);
-    default: return launch_split_d<256>(dtype, p, groups, nw, st);
+    case 32: return launch_split_d<32>(dtype, p, groups, st);
+    case 64: return launch_split_d<64>(dtype, p, groups, st);
+    case 128: return launch_split_d<128>(dtype, p, groups, st);
+    default: return launch_split_d<256>(dtype, p, groups, st);
   }
 }
 
@@ -902,7 +896,7 @@ WeightedPlan weighted_plan(const bsa_decode_weighted_args *a) {
   WeightedPlan w;
   const int R = (a->Hq / a->Hkv) * a->T;
   const long long n = a->sel ? (long long)a->kk * a->bs : a->L;
-  w.nsplit = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, n, 4);
+  w.nsplit = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, n);
   w.ncap = (n + 31) / 32 * 32;
   w.rows = (long long)a->B * a->Hq * a->T;
   w.o_po = 0;
@@ -962,7 +956,7 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
   p.ncap = w.ncap;
   p.live = a->sel ? reinterpret_cast<int *>(base + w.o_lv) : nullptr;
   p.status = a->status;
-  if (bsa_status s = launch_split(a->dtype, a->D, p, 4, st)) return s;
+  if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
   JoinParams j{};
   j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
   j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;
@@ -975,25 +969,22 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
 
 // ------------------------------------------------------------------ decode_prefix
 bool prefix_sm100_applicable(const bsa_decode_prefix_args *a);
-int prefix_sm100_splits(const bsa_decode_prefix_args *a, int *row_tiles);
+int prefix_sm100_splits(const bsa_decode_prefix_args *a);
 bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParams &p, cudaStream_t st);
 
 namespace {
 struct PrefixPlan {
   bool tc;     // the prefix on the tensor-memory kernel
   int np, ns;  // splits of the prefix and of the own slots
-  int nw;      // warps per CTA for the own slots
   long long rows;
   size_t o_ml, bytes;
 };
 PrefixPlan prefix_plan(const bsa_decode_prefix_args *a) {
   PrefixPlan w;
   const int R = (a->Hq / a->Hkv) * a->T;
-  int nt = 1;
   w.tc = prefix_sm100_applicable(a);
-  w.np = w.tc ? prefix_sm100_splits(a, &nt) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P, 4) : 0;
-  w.nw = nt == 2 && R <= 16 ? 2 : 4;
-  w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S, w.nw);
+  w.np = w.tc ? prefix_sm100_splits(a) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P) : 0;
+  w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S);
   w.rows = (long long)a->B * a->Hq * a->T;
   w.o_ml = align_up((size_t)(w.np + w.ns) * w.rows * a->D * 4, 256);
   w.bytes = align_up(w.o_ml + (size_t)(w.np + w.ns) * w.rows * 8, 256);
@@ -1038,7 +1029,7 @@ bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes
     p.R = a->B * p.grp * a->T;
     p.nkeys = a->P;
     p.split0 = 0, p.nsplit = w.np;
-    if (bsa_status s = w.tc ? launch_prefix_sm100(a, p, st) : launch_split(a->dtype, a->D, p, 4, st)) return s;
+    if (bsa_status s = w.tc ? launch_prefix_sm100(a, p, st) : launch_split(a->dtype, a->D, p, st)) return s;
   }
   p.k = a->k.ptr, p.k_sb = a->k.sb, p.k_sh = a->k.sh, p.k_sl = a->k.sl;
   p.v = a->v.ptr, p.v_sb = a->v.sb, p.v_sh = a->v.sh, p.v_sl = a->v.sl;
@@ -1049,7 +1040,7 @@ bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes
   p.causal = 1;
   p.split0 = w.np, p.nsplit = w.ns;
   p.after = a->P > 0;
-  if (bsa_status s = launch_split(a->dtype, a->D, p, w.nw, st)) return s;
+  if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
   JoinParams j{};
   j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
   j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;
