@@ -1,9 +1,9 @@
 // Split-key attention of few query rows (decode steps) in bf16 / f16 / fp32, the
 // join of the splits, and the running sum of every slot's attention weight.
 //
-//   split_mma_kernel   partial softmax and O of one split; one warp streams its own keys
-//   split_join_kernel  joins the splits of every row; with weights, also adds
-//                      sum over the rows of p = 2^(x - lse) to each slot's sum
+//   split_mma_kernel, split_f32_kernel   partial softmax and O of one split
+//   split_join_kernel   joins the splits of every row; with weights, also adds the sum
+//                       over the rows of p = 2^(x - lse) to each slot's sum
 // The kernels are bound by reading K and V once (HBM).
 #include <algorithm>
 #include <cmath>
@@ -97,34 +97,45 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 }
 }  // namespace
 
-// ------------------------------------------------------------------ partial kernel
-// CTA = (K/V head group, 16*MT query rows, split); each of its NW = 4 warps takes every
-// fourth chunk of KC keys and keeps its own m, l and O, so the warps meet only at
-// the end.  A chunk's K and V rows arrive by 16-byte cp.async in a ring of NST
-// stages per warp, rows past the end zero-filled (never read).  S = Q K^T and
-// O += P V are mma.sync products with the query rows as M; 16 rows are mostly
-// padding in a decode step (grp = 8: half), which costs nothing while HBM is the
-// bound: 8 KB of keys take 350 cycles of the SM's share of HBM, their products 64
-// (bf16, D 128) or 190 (fp32).
-// 16-bit types (m16n8k16): P is split in two 16-bit terms (p = hi + lo, hi = round(p),
-// lo = round(p - hi)), so its rounding does not add to the output's; the extra products
-// are free here.  fp32 (m16n8k8 on tf32 terms): a contraction may take its index in any
-// order, so a thread's 16-byte piece of a K row feeds two k-steps (its dims 4t .. 4t+3
-// stand for k = t, t + 4 of each), S's accumulator layout is P's operand layout (keys
-// 2t, 2t + 1 stand for k = t, t + 4), and a 16-byte piece of a V row feeds four column
-// tiles (tile e holds columns 4j + e of a group of 32).
-// Keys that some rows of the tile must not see (the newest T - 1) are multiplied
-// one by one in fp32 and skipped where p = 0: an infinity or NaN in a masked V row
-// never reaches a row that does not see it.
+// ------------------------------------------------------------------ partial kernels
+// CTA = (K/V head group, a tile of query rows, split); each of its NW = 4 warps takes
+// every fourth chunk of KC keys and keeps its own m, l and O, so the warps meet only at
+// the end.  A chunk's K and V rows arrive by 16-byte cp.async in a ring of NST stages
+// per warp, rows past the end zero-filled (never read).  Keys that some rows of the tile
+// must not see (the newest T - 1) are multiplied one by one in fp32 and skipped where
+// p = 0: an infinity or NaN in a masked V row never reaches a row that does not see it.
+//
+// 16-bit types, split_mma_kernel: the keys are M of the m16n8k16 products and the query
+// rows N, eight at a time: S^T = K Q^T, O^T += V^T P^T.  A decode step has few rows (a
+// head group, times the new tokens), and with the rows as M half of every product and of
+// O's registers was padding; 480 instructions per 16 keys at D 128 kept the warps from
+// drawing their share of HBM.  P^T reaches its operand layout by movmatrix, in two 16-bit
+// terms (p = hi + lo, hi = round(p), lo = round(p - hi)), so its rounding does not add to
+// the output's; the extra products are free under HBM's time.
+//
+// fp32, split_f32_kernel: rows as M, m16n8k8 on tf32 terms (above).  A contraction may
+// take its index in any order, so a thread's 16-byte piece of a K row feeds two k-steps
+// (its dims 4t .. 4t+3 stand for k = t, t + 4 of each), S's accumulator layout is P's
+// operand layout (keys 2t, 2t + 1 stand for k = t, t + 4), and a 16-byte piece of a V
+// row feeds four column tiles (tile e holds columns 4j + e of a group of 32).
 template <typename T, int D>
 struct SplitCfg {
-  static constexpr int ES = sizeof(T);
+  static constexpr int ES = sizeof(T), E16 = 16 / ES;
   static constexpr int KC = ES == 2 ? (D >= 128 ? 16 : 32) : (D == 256 ? 8 : 16);
   static constexpr int STAGE = KC * D * ES * 2;       // K and V of a chunk, bytes
   static constexpr int NST = STAGE <= 4096 ? 5 : 3;
   static constexpr int MINB = STAGE >= 16384 ? 1 : 2; // CTAs per SM
   static constexpr int RING = NW * NST * STAGE;
+  // most rows per CTA: O fits the registers, P a chunk of K
+  static constexpr int MAXROWS = ES == 2 ? (D == 64 || D == 128 ? 32 : 16) : (D >= 64 && D <= 128 ? 32 : 16);
 };
+
+// Rows per CTA for R query rows.
+template <typename T, int D>
+constexpr int split_rows(int R) {
+  using C = SplitCfg<T, D>;
+  return C::ES == 2 && R <= 8 ? 8 : R <= 16 || C::MAXROWS == 16 ? 16 : 32;
+}
 
 // Byte offset of 16-byte chunk `chunk` of a D-wide row: chunks are permuted within
 // 128 bytes so that the eight rows (16-bit: ldmatrix) or two / four rows (fp32: the
@@ -139,129 +150,443 @@ __device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
     return row * (D * 4) + ((chunk ^ ((row & 6) ^ ((row & 1) << 2))) << 4);
 }
 
-template <typename T, int D, int MT>
+// What a CTA works on.
+struct Span {
+  int b, hk, grpid, r0, len, c_lo, c_hi, split;
+};
+
+// Row tile, length, live blocks and chunk range of this CTA.  False: nothing to see
+// (the rows' m is written as -inf and the join skips the split).
+template <int KC, int ROWS>
+__device__ __forceinline__ bool split_span(const SplitParams &p, int rtiles, int min_chunks, Span &s, int *s_blk,
+                                           float *s_gate, int *s_raw, int *s_n) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rt = blockIdx.x % rtiles;
+  s.grpid = blockIdx.x / rtiles;
+  s.b = p.fold ? 0 : s.grpid / p.Hkv;
+  s.hk = s.grpid % p.Hkv;
+  s.r0 = rt * ROWS;
+  s.len = p.nkeys;
+  if (p.lens) {
+    s.len = __ldg(p.lens + s.b);
+    if (s.len < 0 || s.len > p.nkeys) {
+      if (tid == 0) report(p.status, BSA_DEVERR_INDEX);
+      s.len = s.len < 0 ? 0 : p.nkeys;
+    }
+  }
+  int nv = s.len;  // virtual keys: the slots, or those of the live blocks one after another
+  if (p.sel) {
+    if (warp == 0) {
+      const int n = build_live(p, s.b, s.hk, s.len, s_blk, s_gate, s_raw);
+      if (lane == 0) *s_n = n;
+      if (p.live && blockIdx.y == 0 && rt == 0) {
+        __syncwarp();
+        int *lv = p.live + (long long)s.grpid * (1 + p.kk);
+        for (int i = lane; i < n; i += 32) lv[1 + i] = s_blk[i];
+        if (lane == 0) lv[0] = n;
+      }
+    }
+    __syncthreads();
+    nv = *s_n * p.bs;
+  }
+  const int nch = (nv + KC - 1) / KC;
+  const int cps = max(min_chunks, (nch + p.nsplit - 1) / p.nsplit);
+  s.c_lo = min(nch, (int)blockIdx.y * cps);
+  s.c_hi = min(nch, s.c_lo + cps);
+  s.split = p.split0 + blockIdx.y;
+  if (s.c_lo < s.c_hi) return true;
+  for (int r = tid; r < ROWS && s.r0 + r < p.R; r += blockDim.x) {
+    int rb, rh, rtt;
+    const long long gr = split_row(p, s.b, s.hk, s.r0 + r, rb, rh, rtt);
+    p.pml[(long long)s.split * p.rows + gr] = make_float2(-INFINITY, 0.f);
+  }
+  return false;
+}
+
+// First key of chunk c, and its gate.
+template <int KC>
+__device__ __forceinline__ int split_key(const SplitParams &p, const int *s_blk, const float *s_gate, int c,
+                                         float &gate) {
+  const int j = c * KC;
+  if (!p.sel) {
+    gate = 0.f;
+    return j;
+  }
+  const int i = j / p.bs;
+  gate = s_gate[i];
+  return s_blk[i] * p.bs + (j - i * p.bs);
+}
+
+// K and V rows [key0, key0 + KC) of one chunk into a stage, by one warp.
+template <typename T, int D>
+__device__ __forceinline__ void split_load(const T *kb, const T *vb, int64_t ksl, int64_t vsl, int key0, int len,
+                                           uint32_t stage, uint64_t policy) {
+  using C = SplitCfg<T, D>;
+  constexpr int CPR = D / C::E16;                    // 16-byte pieces per row
+  constexpr int IT = C::KC * CPR / 32;
+  const int lane = threadIdx.x & 31;
+  const uint32_t dv = stage + C::KC * D * C::ES;
+#pragma unroll
+  for (int it = 0; it < IT; ++it) {
+    const int i = it * 32 + lane, row = i / CPR, ch = i % CPR;
+    const bool ok = key0 + row < len;
+    const int64_t key = ok ? key0 + row : 0;
+    const uint32_t off = sw_off<C::ES, D>(row, ch);
+    cp16(stage + off, kb + key * ksl + ch * C::E16, ok, policy);
+    cp16(dv + off, vb + key * vsl + ch * C::E16, ok, policy);
+  }
+}
+
+// The query rows of the tile into shared memory (swizzled), zeros past R.
+template <typename T, int D, int ROWS>
+__device__ __forceinline__ void split_queries(const SplitParams &p, const Span &s, uint8_t *sQ) {
+  constexpr int E16 = SplitCfg<T, D>::E16, CPR = D / E16;
+  for (int i = threadIdx.x; i < ROWS * CPR; i += blockDim.x) {
+    const int r = i / CPR, ch = i % CPR;
+    alignas(16) T e[E16];
+    *reinterpret_cast<uint4 *>(e) = make_uint4(0, 0, 0, 0);
+    if (s.r0 + r < p.R) {
+      int rb, rh, rtt;
+      split_row(p, s.b, s.hk, s.r0 + r, rb, rh, rtt);
+      const T *qp = reinterpret_cast<const T *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + ch * E16;
+#pragma unroll
+      for (int x = 0; x < E16; ++x) e[x] = qp[x];
+    }
+    *reinterpret_cast<uint4 *>(sQ + sw_off<sizeof(T), D>(r, ch)) = *reinterpret_cast<uint4 *>(e);
+  }
+}
+
+// Sum of the warps' O (so: [warp][ROWS][STRIDE], scaled to the common maximum) and their
+// (m, l), to the split's place.
+template <int D, int ROWS, int STRIDE>
+__device__ __forceinline__ void split_write(const SplitParams &p, const Span &s, const float *so,
+                                            const float (*s_m)[ROWS], const float (*s_l)[ROWS]) {
+  const int nr = min(ROWS, p.R - s.r0);
+  for (int i = threadIdx.x; i < nr * (D / 4); i += blockDim.x) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    float4 o = *reinterpret_cast<const float4 *>(so + r * STRIDE + d);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      const float4 x = *reinterpret_cast<const float4 *>(so + (w * ROWS + r) * STRIDE + d);
+      o.x += x.x;
+      o.y += x.y;
+      o.z += x.z;
+      o.w += x.w;
+    }
+    int rb, rh, rtt;
+    const long long at = (long long)s.split * p.rows + split_row(p, s.b, s.hk, s.r0 + r, rb, rh, rtt);
+    *reinterpret_cast<float4 *>(p.po + at * D + d) = o;
+    if (d == 0) {
+      float M = s_m[0][r], L = 0.f;
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M = fmax_nan(M, s_m[w][r]);
+#pragma unroll
+      for (int w = 0; w < NW; ++w) L += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2(s_m[w][r] - M);
+      p.pml[at] = make_float2(M, L);
+    }
+  }
+}
+
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {  // 8x8 of 16 bits, transposed over the warp
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
+
+// ------------------------------------------------------------------ bf16 / f16
+template <typename T, int D, int NR>
 __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     split_mma_kernel(const SplitParams p, int rtiles, int min_chunks) {
   using C = SplitCfg<T, D>;
-  constexpr bool F32 = C::ES == 4;
-  constexpr int ES = C::ES, E16 = 16 / ES;            // elements per 16 bytes
-  constexpr int KC = C::KC, NST = C::NST, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
+  constexpr int KC = C::KC, NST = C::NST, KS = D / 16, KT = KC / 16, ROWS = 8 * NR, SO = D + 4;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int s_n;
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
   uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
-  uint8_t *ring = sm + ROWS * D * ES;
+  uint8_t *ring = sm + ROWS * D * 2;
   int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
   float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
-  int *s_raw = s_blk + 2 * kMaxLive;
   // Launched to start beside the prefix kernel: its last CTA ends no earlier than that
   // kernel, so that waiting for this grid is waiting for both.
   const bool last = p.after && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, tq = lane & 3;
   pdl_trigger();  // the join may take its place on the SMs; it waits for this grid
-  const int rt = blockIdx.x % rtiles, grpid = blockIdx.x / rtiles;
-  const int b = p.fold ? 0 : grpid / p.Hkv, hk = grpid % p.Hkv;
-  const int r0 = rt * ROWS;
-
-  int len = p.nkeys;
-  if (p.lens) {
-    len = __ldg(p.lens + b);
-    if (len < 0 || len > p.nkeys) {
-      if (tid == 0) report(p.status, BSA_DEVERR_INDEX);
-      len = len < 0 ? 0 : p.nkeys;
-    }
-  }
-  int nv = len;  // virtual keys: the slots, or those of the live blocks one after another
-  if (p.sel) {
-    if (warp == 0) {
-      const int n = build_live(p, b, hk, len, s_blk, s_gate, s_raw);
-      if (lane == 0) s_n = n;
-      if (p.live && blockIdx.y == 0 && rt == 0) {
-        __syncwarp();
-        int *lv = p.live + (long long)grpid * (1 + p.kk);
-        for (int i = lane; i < n; i += 32) lv[1 + i] = s_blk[i];
-        if (lane == 0) lv[0] = n;
-      }
-    }
-    __syncthreads();
-    nv = s_n * p.bs;
-  }
-  const int nch = (nv + KC - 1) / KC;
-  const int cps = max(min_chunks, (nch + p.nsplit - 1) / p.nsplit);
-  const int c_lo = min(nch, (int)blockIdx.y * cps), c_hi = min(nch, c_lo + cps);
-  const int split = p.split0 + blockIdx.y;
-  if (c_lo >= c_hi) {  // nothing to see here: the join skips this split
-    for (int r = tid; r < ROWS && r0 + r < p.R; r += blockDim.x) {
-      int rb, rh, rtt;
-      const long long gr = split_row(p, b, hk, r0 + r, rb, rh, rtt);
-      p.pml[(long long)split * p.rows + gr] = make_float2(-INFINITY, 0.f);
-    }
+  Span sp;
+  if (!split_span<KC, ROWS>(p, rtiles, min_chunks, sp, s_blk, s_gate, s_blk + 2 * kMaxLive, &s_n)) {
     if (last) pdl_wait();
     return;
   }
-
-  const T *kb_ = reinterpret_cast<const T *>(p.k) + (p.fold ? 0 : b * p.k_sb) + hk * p.k_sh;
-  const T *vb_ = reinterpret_cast<const T *>(p.v) + (p.fold ? 0 : b * p.v_sb) + hk * p.v_sh;
+  const int len = sp.len, r0 = sp.r0;
+  const T *kb_ = reinterpret_cast<const T *>(p.k) + (p.fold ? 0 : sp.b * p.k_sb) + sp.hk * p.k_sh;
+  const T *vb_ = reinterpret_cast<const T *>(p.v) + (p.fold ? 0 : sp.b * p.v_sb) + sp.hk * p.v_sh;
   uint8_t *wring = ring + warp * NST * C::STAGE;
+  const uint32_t wr0 = smem_u32(wring);
   const uint64_t policy = evict_first_policy();
-  // first key of chunk c, and its gate
-  auto key_of = [&](int c, float &gate) -> int {
-    const int j = c * KC;
-    if (!p.sel) {
-      gate = 0.f;
-      return j;
-    }
-    const int i = j / p.bs;
-    gate = s_gate[i];
-    return s_blk[i] * p.bs + (j - i * p.bs);
-  };
   auto load = [&](int c, int st) {
-    if (c < c_hi) {
+    if (c < sp.c_hi) {
       float gt;
-      const int key0 = key_of(c, gt);
-      const uint32_t dk = smem_u32(wring + st * C::STAGE), dv = dk + KC * D * ES;
-#pragma unroll
-      for (int it = 0; it < KC * D / E16 / 32; ++it) {
-        const int i = it * 32 + lane, row = i / (D / E16), ch = i % (D / E16);
-        const bool ok = key0 + row < len;
-        const long long key = ok ? key0 + row : 0;
-        const uint32_t off = sw_off<ES, D>(row, ch);
-        cp16(dk + off, kb_ + key * p.k_sl + ch * E16, ok, policy);
-        cp16(dv + off, vb_ + key * p.v_sl + ch * E16, ok, policy);
-      }
+      const int key0 = split_key<KC>(p, s_blk, s_gate, c, gt);
+      split_load<T, D>(kb_, vb_, p.k_sl, p.v_sl, key0, len, wr0 + st * C::STAGE, policy);
     }
     cp_commit();
   };
 #pragma unroll
-  for (int s = 0; s < NST - 1; ++s) load(c_lo + warp + s * NW, s);
-
-  // query rows, zeros past R
-  for (int i = tid; i < ROWS * (D / E16); i += blockDim.x) {
-    const int r = i / (D / E16), ch = i % (D / E16);
-    alignas(16) T e[E16];
-    *reinterpret_cast<uint4 *>(e) = make_uint4(0, 0, 0, 0);
-    if (r0 + r < p.R) {
-      int rb, rh, rtt;
-      split_row(p, b, hk, r0 + r, rb, rh, rtt);
-      const T *qp = reinterpret_cast<const T *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + ch * E16;
-#pragma unroll
-      for (int x = 0; x < E16; ++x) e[x] = qp[x];
-    }
-    *reinterpret_cast<uint4 *>(sQ + sw_off<ES, D>(r, ch)) = *reinterpret_cast<uint4 *>(e);
-  }
+  for (int s = 0; s < NST - 1; ++s) load(sp.c_lo + warp + s * NW, s);
+  split_queries<T, D, ROWS>(p, sp, sQ);
   __syncthreads();
 
-  constexpr bool QREG = !F32 && D <= 128 && MT == 1;
-  const uint32_t qa = smem_u32(sQ);
-  uint32_t qf[QREG ? KS : 1][4];
-  auto ldq = [&](int mt, int ks, uint32_t *a) {
-    const int row = mt * 16 + (lane & 15), ch = ks * 2 + (lane >> 4);
-    ldsm_x4(qa + sw_off<ES, D>(row, ch), a[0], a[1], a[2], a[3]);
-  };
-  if constexpr (QREG)
+  // Q^T as the second operand: (dims 2t, 2t+1 and 8 further; row g)
+  uint32_t qf[NR][KS][2];
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) ldq(0, ks, qf[ks]);
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        qf[n][ks][h] = *reinterpret_cast<const uint32_t *>(sQ + sw_off<2, D>(n * 8 + g, ks * 2 + h) + tq * 4);
+
+  float acc[NR][KS][4], m[NR][2], l[NR][2];  // O^T: dims g, g + 8 of tile ks; rows 2t, 2t + 1 of group n
+  int qlast[NR][2];                          // newest key that the row sees
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][ks][e] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[n][h] = -INFINITY;
+      l[n][h] = 0.f;
+      const int r = r0 + n * 8 + 2 * tq + h;
+      qlast[n][h] = p.causal ? len - p.T + r % p.T : len - 1;
+    }
+  }
+  const int all_see = p.causal ? len - p.T : len - 1;  // newest key that every row sees
+  float *lg = p.logits ? p.logits + ((long long)sp.grpid * p.ncap + g) * p.rpad + r0 + 2 * tq : nullptr;
+  // lane parts of the ldmatrix addresses
+  const int krow = (lane & 7) + ((lane >> 3) & 1) * 8, kch = lane >> 4;
+  const int vrow = (lane & 7) + (lane >> 4) * 8, vch = (lane >> 3) & 1;
+
+  int st = 0;
+  for (int c = sp.c_lo + warp; c < sp.c_hi; c += NW) {
+    cp_wait<NST - 2>();
+    __syncwarp();
+    {
+      int nst = st + NST - 1;
+      if (nst >= NST) nst -= NST;
+      load(c + (NST - 1) * NW, nst);
+    }
+    const uint32_t ka = wr0 + st * C::STAGE, va = ka + KC * D * 2;
+    float gate;
+    const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
+    // ---- S^T = K Q^T
+    float s[KT][NR][4];  // keys g, g + 8 of tile kt; rows 2t, 2t + 1
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t a[4];
+        ldsm_x4(ka + sw_off<2, D>(kt * 16 + krow, ks * 2 + kch), a[0], a[1], a[2], a[3]);
+#pragma unroll
+        for (int n = 0; n < NR; ++n) Mma<T>::run(s[kt][n], a, qf[n][ks][0], qf[n][ks][1]);
+      }
+    // ---- online softmax (log2 domain); masked and missing keys are -inf
+    const bool masked = key0 + KC - 1 > all_see;
+    const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float x = fmaf(s[kt][n][e], p.scale2, gate);
+          if (masked && key0 + kt * 16 + g + 8 * (e >> 1) > qlast[n][e & 1]) x = -INFINITY;
+          s[kt][n][e] = x;
+          mx[e & 1] = fmax_nan(mx[e & 1], x);
+        }
+      if (lg && r0 + n * 8 < p.R) {  // rows are padded to rpad: whole groups of eight
+        float *lp = lg + (long long)c * KC * p.rpad + n * 8;
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2 *>(lp + (long long)(kt * 16 + 8 * h) * p.rpad) =
+                make_float2(s[kt][n][2 * h], s[kt][n][2 * h + 1]);
+      }
+      float al[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
+        const float mn = fmax_nan(m[n][h], mx[h]);
+        al[h] = mn == -INFINITY ? 1.f : ex2(m[n][h] - mn);
+        m[n][h] = mn;
+      }
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+        l[n][0] *= al[0];
+        l[n][1] *= al[1];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][ks][e] *= al[e & 1];
+      }
+      const float off[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          s[kt][n][e] = ex2(s[kt][n][e] - off[e & 1]);
+          l[n][e & 1] += s[kt][n][e];
+        }
+    }
+    // ---- O^T += V^T P^T
+    if (!mixed) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) {
+        uint32_t hi[NR][2], lo[NR][2];
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float x = s[kt][n][2 * h], y = s[kt][n][2 * h + 1];
+            const uint32_t u = Mma<T>::pack(x, y);
+            const T *ht = reinterpret_cast<const T *>(&u);
+            hi[n][h] = movmatrix(u);
+            lo[n][h] = movmatrix(Mma<T>::pack(x - Mma<T>::to_f(ht[0]), y - Mma<T>::to_f(ht[1])));
+          }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          uint32_t a[4];
+          ldsm_x4_t(va + sw_off<2, D>(kt * 16 + vrow, ks * 2 + vch), a[0], a[1], a[2], a[3]);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            Mma<T>::run(acc[n][ks], a, hi[n][0], hi[n][1]);
+            Mma<T>::run(acc[n][ks], a, lo[n][0], lo[n][1]);
+          }
+        }
+      }
+    } else {
+      // P through the chunk's K buffer (its reads are done), then key by key
+      __syncwarp();
+      float *sp_ = reinterpret_cast<float *>(wring + st * C::STAGE);  // [KC][ROWS]
+      const uint8_t *sv = wring + st * C::STAGE + KC * D * 2;
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            sp_[(kt * 16 + g + 8 * (e >> 1)) * ROWS + n * 8 + 2 * tq + (e & 1)] = s[kt][n][e];
+      __syncwarp();
+#pragma unroll 1
+      for (int k = 0; k < KC && key0 + k < len; ++k) {
+#pragma unroll
+        for (int n = 0; n < NR; ++n) {
+          const float2 pk = *reinterpret_cast<const float2 *>(sp_ + k * ROWS + n * 8 + 2 * tq);
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            const float v0 = Mma<T>::to_f(*reinterpret_cast<const T *>(sv + sw_off<2, D>(k, ks * 2) + g * 2));
+            const float v1 = Mma<T>::to_f(*reinterpret_cast<const T *>(sv + sw_off<2, D>(k, ks * 2 + 1) + g * 2));
+            if (pk.x != 0.f) {
+              acc[n][ks][0] = fmaf(pk.x, v0, acc[n][ks][0]);
+              acc[n][ks][2] = fmaf(pk.x, v1, acc[n][ks][2]);
+            }
+            if (pk.y != 0.f) {
+              acc[n][ks][1] = fmaf(pk.y, v0, acc[n][ks][1]);
+              acc[n][ks][3] = fmaf(pk.y, v1, acc[n][ks][3]);
+            }
+          }
+        }
+      }
+      __syncwarp();
+    }
+    if (++st == NST) st = 0;
+  }
+
+  // ---- join the four warps
+  cp_wait<0>();
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], o);
+      if (g == 0) {
+        s_m[warp][n * 8 + 2 * tq + h] = m[n][h];
+        s_l[warp][n * 8 + 2 * tq + h] = l[n][h];
+      }
+    }
+  __syncthreads();
+  float *so = reinterpret_cast<float *>(ring);  // [warp][ROWS][SO]; SO: rows 2t apart in banks
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = n * 8 + 2 * tq + h;
+      float M = s_m[0][r];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) M = fmax_nan(M, s_m[w][r]);
+      const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - M);
+      float *op = so + (warp * ROWS + r) * SO + g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        op[ks * 16] = acc[n][ks][h] * f;
+        op[ks * 16 + 8] = acc[n][ks][2 + h] * f;
+      }
+    }
+  __syncthreads();
+  split_write<D, ROWS, SO>(p, sp, so, s_m, s_l);
+  if (last) pdl_wait();
+}
+
+// ------------------------------------------------------------------ fp32
+template <int D, int MT>
+__global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
+    split_f32_kernel(const SplitParams p, int rtiles, int min_chunks) {
+  using C = SplitCfg<float, D>;
+  constexpr int KC = C::KC, NST = C::NST, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int s_n;
+  __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
+  uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
+  uint8_t *ring = sm + ROWS * D * 4;
+  int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
+  float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
+  const bool last = p.after && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, tq = lane & 3;
+  pdl_trigger();
+  Span sp;
+  if (!split_span<KC, ROWS>(p, rtiles, min_chunks, sp, s_blk, s_gate, s_blk + 2 * kMaxLive, &s_n)) {
+    if (last) pdl_wait();
+    return;
+  }
+  const int len = sp.len, r0 = sp.r0;
+  const float *kb_ = reinterpret_cast<const float *>(p.k) + (p.fold ? 0 : sp.b * p.k_sb) + sp.hk * p.k_sh;
+  const float *vb_ = reinterpret_cast<const float *>(p.v) + (p.fold ? 0 : sp.b * p.v_sb) + sp.hk * p.v_sh;
+  uint8_t *wring = ring + warp * NST * C::STAGE;
+  const uint32_t wr0 = smem_u32(wring);
+  const uint64_t policy = evict_first_policy();
+  auto load = [&](int c, int st) {
+    if (c < sp.c_hi) {
+      float gt;
+      const int key0 = split_key<KC>(p, s_blk, s_gate, c, gt);
+      split_load<float, D>(kb_, vb_, p.k_sl, p.v_sl, key0, len, wr0 + st * C::STAGE, policy);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < NST - 1; ++s) load(sp.c_lo + warp + s * NW, s);
+  split_queries<float, D, ROWS>(p, sp, sQ);
+  __syncthreads();
 
   float acc[MT][NT][4], m[MT][2], l[MT][2];
   int qlast[MT][2];  // newest key that the row sees
@@ -282,7 +607,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
   const int all_see = p.causal ? len - p.T : len - 1;  // newest key that every row sees
 
   int st = 0;
-  for (int c = c_lo + warp; c < c_hi; c += NW) {
+  for (int c = sp.c_lo + warp; c < sp.c_hi; c += NW) {
     cp_wait<NST - 2>();
     __syncwarp();
     {
@@ -290,10 +615,9 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
       if (nst >= NST) nst -= NST;
       load(c + (NST - 1) * NW, nst);
     }
-    const uint32_t ka = smem_u32(wring + st * C::STAGE), va = ka + KC * D * ES;
-    const uint8_t *sk = wring + st * C::STAGE, *sv = sk + KC * D * ES;
+    const uint8_t *sk = wring + st * C::STAGE, *sv = sk + KC * D * 4;
     float gate;
-    const int key0 = key_of(c, gate);
+    const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
     // ---- S = Q K^T
     float s[MT][KC / 8][4];
 #pragma unroll
@@ -302,66 +626,39 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
       for (int n = 0; n < KC / 8; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
-    if constexpr (!F32) {
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        uint32_t a[MT][4];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          if constexpr (QREG) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) a[mt][e] = qf[ks][e];
-          } else {
-            ldq(mt, ks, a[mt]);
-          }
-        }
-#pragma unroll
-        for (int n2 = 0; n2 < KC / 16; ++n2) {
-          uint32_t b0, b1, b2, b3;
-          const int row = n2 * 16 + (lane & 7) + ((lane >> 4) << 3), ch = ks * 2 + ((lane >> 3) & 1);
-          ldsm_x4(ka + sw_off<ES, D>(row, ch), b0, b1, b2, b3);
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            Mma<T>::run(s[mt][2 * n2], a[mt], b0, b1);
-            Mma<T>::run(s[mt][2 * n2 + 1], a[mt], b2, b3);
-          }
-        }
-      }
-    } else {
 #pragma unroll 4
-      for (int ks = 0; ks < KS; ++ks) {  // 16 dims: two k-steps
-        uint32_t ah[MT][2][4], al[MT][2][4];
+    for (int ks = 0; ks < KS; ++ks) {  // 16 dims: two k-steps
+      uint32_t ah[MT][2][4], al[MT][2][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float4 x = *reinterpret_cast<const float4 *>(sQ + sw_off<ES, D>(mt * 16 + g, ks * 4 + tq));
-          const float4 y = *reinterpret_cast<const float4 *>(sQ + sw_off<ES, D>(mt * 16 + g + 8, ks * 4 + tq));
-          tf32_split(x.x, ah[mt][0][0], al[mt][0][0]);
-          tf32_split(y.x, ah[mt][0][1], al[mt][0][1]);
-          tf32_split(x.y, ah[mt][0][2], al[mt][0][2]);
-          tf32_split(y.y, ah[mt][0][3], al[mt][0][3]);
-          tf32_split(x.z, ah[mt][1][0], al[mt][1][0]);
-          tf32_split(y.z, ah[mt][1][1], al[mt][1][1]);
-          tf32_split(x.w, ah[mt][1][2], al[mt][1][2]);
-          tf32_split(y.w, ah[mt][1][3], al[mt][1][3]);
-        }
+      for (int mt = 0; mt < MT; ++mt) {
+        const float4 x = *reinterpret_cast<const float4 *>(sQ + sw_off<4, D>(mt * 16 + g, ks * 4 + tq));
+        const float4 y = *reinterpret_cast<const float4 *>(sQ + sw_off<4, D>(mt * 16 + g + 8, ks * 4 + tq));
+        tf32_split(x.x, ah[mt][0][0], al[mt][0][0]);
+        tf32_split(y.x, ah[mt][0][1], al[mt][0][1]);
+        tf32_split(x.y, ah[mt][0][2], al[mt][0][2]);
+        tf32_split(y.y, ah[mt][0][3], al[mt][0][3]);
+        tf32_split(x.z, ah[mt][1][0], al[mt][1][0]);
+        tf32_split(y.z, ah[mt][1][1], al[mt][1][1]);
+        tf32_split(x.w, ah[mt][1][2], al[mt][1][2]);
+        tf32_split(y.w, ah[mt][1][3], al[mt][1][3]);
+      }
 #pragma unroll
-        for (int n = 0; n < KC / 8; ++n) {
-          const float4 k4 = *reinterpret_cast<const float4 *>(sk + sw_off<ES, D>(n * 8 + g, ks * 4 + tq));
-          uint32_t bh[4], bl[4];
-          tf32_split(k4.x, bh[0], bl[0]);
-          tf32_split(k4.y, bh[1], bl[1]);
-          tf32_split(k4.z, bh[2], bl[2]);
-          tf32_split(k4.w, bh[3], bl[3]);
+      for (int n = 0; n < KC / 8; ++n) {
+        const float4 k4 = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(n * 8 + g, ks * 4 + tq));
+        uint32_t bh[4], bl[4];
+        tf32_split(k4.x, bh[0], bl[0]);
+        tf32_split(k4.y, bh[1], bl[1]);
+        tf32_split(k4.z, bh[2], bl[2]);
+        tf32_split(k4.w, bh[3], bl[3]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int k2 = 0; k2 < 2; ++k2) {
-              const uint32_t *xh = ah[mt][k2], *xl = al[mt][k2];
-              mma_tf32(s[mt][n], xl[0], xl[1], xl[2], xl[3], bh[2 * k2], bh[2 * k2 + 1]);
-              mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bl[2 * k2], bl[2 * k2 + 1]);
-              mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bh[2 * k2], bh[2 * k2 + 1]);
-            }
-        }
+          for (int k2 = 0; k2 < 2; ++k2) {
+            const uint32_t *xh = ah[mt][k2], *xl = al[mt][k2];
+            mma_tf32(s[mt][n], xl[0], xl[1], xl[2], xl[3], bh[2 * k2], bh[2 * k2 + 1]);
+            mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bl[2 * k2], bl[2 * k2 + 1]);
+            mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bh[2 * k2], bh[2 * k2 + 1]);
+          }
       }
     }
     // ---- online softmax (log2 domain); masked and missing keys are -inf
@@ -384,10 +681,12 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
         for (int h = 0; h < 2; ++h) {
           const int r = r0 + mt * 16 + g + 8 * h;
           if (r < p.R) {
-            float *lp = p.logits + ((long long)grpid * p.R + r) * p.ncap + (long long)c * KC + tq * 2;
+            float *lp = p.logits + ((long long)sp.grpid * p.ncap + (long long)c * KC + tq * 2) * p.rpad + r;
 #pragma unroll
-            for (int n = 0; n < KC / 8; ++n)
-              *reinterpret_cast<float2 *>(lp + n * 8) = make_float2(s[mt][n][2 * h], s[mt][n][2 * h + 1]);
+            for (int n = 0; n < KC / 8; ++n) {
+              lp[(long long)(n * 8) * p.rpad] = s[mt][n][2 * h];
+              lp[(long long)(n * 8 + 1) * p.rpad] = s[mt][n][2 * h + 1];
+            }
           }
         }
       }
@@ -419,61 +718,32 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     }
     // ---- O += P V
     if (!mixed) {
-      if constexpr (F32) {
 #pragma unroll
-        for (int k8 = 0; k8 < KC / 8; ++k8) {
-          uint32_t ph[MT][4], pl[MT][4];
+      for (int k8 = 0; k8 < KC / 8; ++k8) {
+        uint32_t ph[MT][4], pl[MT][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            tf32_split(s[mt][k8][0], ph[mt][0], pl[mt][0]);
-            tf32_split(s[mt][k8][2], ph[mt][1], pl[mt][1]);
-            tf32_split(s[mt][k8][1], ph[mt][2], pl[mt][2]);
-            tf32_split(s[mt][k8][3], ph[mt][3], pl[mt][3]);
-          }
-#pragma unroll
-          for (int cg = 0; cg < D / 32; ++cg) {
-            const float4 v0 = *reinterpret_cast<const float4 *>(sv + sw_off<ES, D>(k8 * 8 + 2 * tq, cg * 8 + g));
-            const float4 v1 = *reinterpret_cast<const float4 *>(sv + sw_off<ES, D>(k8 * 8 + 2 * tq + 1, cg * 8 + g));
-            const float x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t h0, l0, h1, l1;
-              tf32_split(x0[e], h0, l0);
-              tf32_split(x1[e], h1, l1);
-#pragma unroll
-              for (int mt = 0; mt < MT; ++mt) {
-                float *c = acc[mt][cg * 4 + e];
-                mma_tf32(c, pl[mt][0], pl[mt][1], pl[mt][2], pl[mt][3], h0, h1);
-                mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], l0, l1);
-                mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], h0, h1);
-              }
-            }
-          }
+        for (int mt = 0; mt < MT; ++mt) {
+          tf32_split(s[mt][k8][0], ph[mt][0], pl[mt][0]);
+          tf32_split(s[mt][k8][2], ph[mt][1], pl[mt][1]);
+          tf32_split(s[mt][k8][1], ph[mt][2], pl[mt][2]);
+          tf32_split(s[mt][k8][3], ph[mt][3], pl[mt][3]);
         }
-      } else {
 #pragma unroll
-        for (int k2 = 0; k2 < KC / 16; ++k2) {
-          uint32_t hi[MT][4], lo[MT][4];
+        for (int cg = 0; cg < D / 32; ++cg) {
+          const float4 v0 = *reinterpret_cast<const float4 *>(sv + sw_off<4, D>(k8 * 8 + 2 * tq, cg * 8 + g));
+          const float4 v1 = *reinterpret_cast<const float4 *>(sv + sw_off<4, D>(k8 * 8 + 2 * tq + 1, cg * 8 + g));
+          const float x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = s[mt][2 * k2 + (e >> 1)][2 * (e & 1)], y = s[mt][2 * k2 + (e >> 1)][2 * (e & 1) + 1];
-              hi[mt][e] = Mma<T>::pack(x, y);
-              const T *ht = reinterpret_cast<const T *>(&hi[mt][e]);
-              lo[mt][e] = Mma<T>::pack(x - Mma<T>::to_f(ht[0]), y - Mma<T>::to_f(ht[1]));
-            }
-#pragma unroll
-          for (int n2 = 0; n2 < NT / 2; ++n2) {
-            uint32_t b0, b1, b2, b3;
-            const int row = k2 * 16 + (lane & 15), ch = n2 * 2 + (lane >> 4);
-            ldsm_x4_t(va + sw_off<ES, D>(row, ch), b0, b1, b2, b3);
+          for (int e = 0; e < 4; ++e) {
+            uint32_t h0, l0, h1, l1;
+            tf32_split(x0[e], h0, l0);
+            tf32_split(x1[e], h1, l1);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              Mma<T>::run(acc[mt][2 * n2], hi[mt], b0, b1);
-              Mma<T>::run(acc[mt][2 * n2 + 1], hi[mt], b2, b3);
-              Mma<T>::run(acc[mt][2 * n2], lo[mt], b0, b1);
-              Mma<T>::run(acc[mt][2 * n2 + 1], lo[mt], b2, b3);
+              float *c = acc[mt][cg * 4 + e];
+              mma_tf32(c, pl[mt][0], pl[mt][1], pl[mt][2], pl[mt][3], h0, h1);
+              mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], l0, l1);
+              mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], h0, h1);
             }
           }
         }
@@ -481,32 +751,26 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     } else {
       // P through the chunk's K buffer (its reads are done), then key by key
       __syncwarp();
-      float *sp = reinterpret_cast<float *>(wring + st * C::STAGE);  // [ROWS][KC]
+      float *sp_ = reinterpret_cast<float *>(wring + st * C::STAGE);  // [ROWS][KC]
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
         for (int n = 0; n < KC / 8; ++n)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            sp[(mt * 16 + g + 8 * (e >> 1)) * KC + n * 8 + tq * 2 + (e & 1)] = s[mt][n][e];
+            sp_[(mt * 16 + g + 8 * (e >> 1)) * KC + n * 8 + tq * 2 + (e & 1)] = s[mt][n][e];
       __syncwarp();
 #pragma unroll 1
       for (int k = 0; k < KC && key0 + k < len; ++k) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const float pa = sp[(mt * 16 + g) * KC + k], pb = sp[(mt * 16 + g + 8) * KC + k];
+          const float pa = sp_[(mt * 16 + g) * KC + k], pb = sp_[(mt * 16 + g + 8) * KC + k];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            float v0, v1;  // this thread's two columns of tile n
-            if constexpr (F32) {
-              const int ch = (n >> 2) * 8 + 2 * tq;
-              v0 = *reinterpret_cast<const float *>(sv + sw_off<ES, D>(k, ch) + (n & 3) * 4);
-              v1 = *reinterpret_cast<const float *>(sv + sw_off<ES, D>(k, ch + 1) + (n & 3) * 4);
-            } else {
-              const T *vp = reinterpret_cast<const T *>(sv + sw_off<ES, D>(k, n) + tq * 4);
-              v0 = Mma<T>::to_f(vp[0]);
-              v1 = Mma<T>::to_f(vp[1]);
-            }
+            // this thread's two columns of tile n
+            const int ch = (n >> 2) * 8 + 2 * tq;
+            const float v0 = *reinterpret_cast<const float *>(sv + sw_off<4, D>(k, ch) + (n & 3) * 4);
+            const float v1 = *reinterpret_cast<const float *>(sv + sw_off<4, D>(k, ch + 1) + (n & 3) * 4);
             if (pa != 0.f) {
               acc[mt][n][0] = fmaf(pa, v0, acc[mt][n][0]);
               acc[mt][n][1] = fmaf(pa, v1, acc[mt][n][1]);
@@ -547,46 +811,15 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
 #pragma unroll
       for (int w = 1; w < NW; ++w) M = fmax_nan(M, s_m[w][r]);
       const float f = m[mt][h] == -INFINITY ? 0.f : ex2(m[mt][h] - M);
-      if (r0 + r < p.R) {
-        float *op = so + (warp * ROWS + r) * D;
+      float *op = so + (warp * ROWS + r) * D + tq * 8;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const float x = acc[mt][n][2 * h] * f, y = acc[mt][n][2 * h + 1] * f;
-          if constexpr (F32) {
-            op[(n >> 2) * 32 + tq * 8 + (n & 3)] = x;
-            op[(n >> 2) * 32 + tq * 8 + 4 + (n & 3)] = y;
-          } else {
-            *reinterpret_cast<float2 *>(op + n * 8 + tq * 2) = make_float2(x, y);
-          }
-        }
+      for (int n = 0; n < NT; ++n) {
+        op[(n >> 2) * 32 + (n & 3)] = acc[mt][n][2 * h] * f;
+        op[(n >> 2) * 32 + 4 + (n & 3)] = acc[mt][n][2 * h + 1] * f;
       }
     }
   __syncthreads();
-  const int nr = min(ROWS, p.R - r0);
-  for (int i = tid; i < nr * (D / 4); i += blockDim.x) {
-    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
-    float4 o = *reinterpret_cast<const float4 *>(so + r * D + d);
-#pragma unroll
-    for (int w = 1; w < NW; ++w) {
-      const float4 x = *reinterpret_cast<const float4 *>(so + (w * ROWS + r) * D + d);
-      o.x += x.x;
-      o.y += x.y;
-      o.z += x.z;
-      o.w += x.w;
-    }
-    int rb, rh, rtt;
-    const long long at = (long long)split * p.rows + split_row(p, b, hk, r0 + r, rb, rh, rtt);
-    *reinterpret_cast<float4 *>(p.po + at * D + d) = o;
-    if (d == 0) {
-      float M = s_m[0][r], L = 0.f;
-#pragma unroll
-      for (int w = 1; w < NW; ++w) M = fmax_nan(M, s_m[w][r]);
-#pragma unroll
-      for (int w = 0; w < NW; ++w)
-        L += s_m[w][r] == -INFINITY ? 0.f : s_l[w][r] * ex2(s_m[w][r] - M);
-      p.pml[at] = make_float2(M, L);
-    }
-  }
+  split_write<D, ROWS, D>(p, sp, so, s_m, s_l);
   if (last) pdl_wait();
 }
 
@@ -598,24 +831,84 @@ struct JoinParams {
   long long rows;
   const float *po;
   const float2 *pml;
-  const float *logits;  // with weights
+  const float *logits;  // with weights: [b*Hkv + hk][ncap][rpad]
   long long ncap;
+  int rpad;
   const int *live;
   int kk, bs, L;
   float *weight;
   int64_t w_sb, w_sh;
-  int wtiles;           // weight blocks per (b, hk); they follow the row blocks
+  int wtiles, kpb;      // weight blocks per (b, hk) and slots of each; they follow the row blocks
 };
 
 constexpr int kJoinThreads = 256;
 
 // Row blocks: 8 / wpr query rows each.  A row's columns take D/4 lanes; the remaining
 // lanes of its warps, and its wpr warps, take splits side by side.  Weight blocks:
-// 1024 slots of one (b, hk), four per thread: lse of its R rows from the splits'
-// (m, l), then the sum over the rows, in row order, of 2^(x - m) / l.
+// kpb slots of one (b, hk): lse of its R rows from the splits' (m, l), then the sum over
+// the rows of 2^(x - m) / l, four rows to a lane and LPK lanes to a slot, so that a warp
+// reads whole lines of the logits.
+// 2^(x - m) f, and 0 where f is: a row that saw nothing or padding, whatever its x holds.
+__device__ __forceinline__ float join_p(float x, float m, float f) { return f == 0.f ? 0.f : ex2(x - m) * f; }
+
+template <int LPK>
+__device__ __forceinline__ void join_weights(const JoinParams &p, int bh, int b, int hk, int tile, const float *sj) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int KPW = 32 / LPK;  // slots per warp and step
+  const int sub = lane % LPK;
+  const int *lv = p.live ? p.live + (long long)bh * (1 + p.kk) : nullptr;
+  const long long nv = lv ? (long long)lv[0] * p.bs : p.L;
+  float *wp = p.weight + b * p.w_sb + hk * p.w_sh;
+  const float *lg = p.logits + (long long)bh * p.ncap * p.rpad;
+  const long long j0 = (long long)tile * p.kpb;
+  // this lane's first four rows (none when there are fewer)
+  float4 m4 = make_float4(0, 0, 0, 0), f4 = m4;
+  const bool rows = sub * 4 < p.rpad;
+  if (rows) {
+    m4 = *reinterpret_cast<const float4 *>(sj + sub * 4);
+    f4 = *reinterpret_cast<const float4 *>(sj + p.rpad + sub * 4);
+  }
+  constexpr int U = 4, STEP = KPW * (kJoinThreads / 32);  // slots in flight per lane group, slots per step
+  for (int i = 0; i < p.kpb; i += U * STEP) {
+    float4 x4[U];
+    float w0[U];
+    long long key[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long jw = j0 + i + u * STEP + warp * KPW;  // the warp's slots lie in one block of 32
+      const long long j = jw + lane / LPK;
+      key[u] = j;
+      if (lv && jw < nv) {
+        const long long blk = jw / p.bs;
+        key[u] = (long long)lv[1 + blk] * p.bs + (j - blk * p.bs);
+      }
+      if (i + u * STEP >= p.kpb || j >= nv || key[u] >= p.L) key[u] = -1;
+      x4[u] = make_float4(0, 0, 0, 0);
+      if (key[u] >= 0 && rows) x4[u] = __ldcs(reinterpret_cast<const float4 *>(lg + j * p.rpad + sub * 4));
+      w0[u] = key[u] >= 0 && sub == 0 ? wp[key[u]] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float w = (join_p(x4[u].x, m4.x, f4.x) + join_p(x4[u].y, m4.y, f4.y)) +
+                (join_p(x4[u].z, m4.z, f4.z) + join_p(x4[u].w, m4.w, f4.w));
+      if (LPK == 8 && key[u] >= 0) {  // more than 32 rows
+        const float *x = lg + (j0 + i + u * STEP + warp * KPW + lane / LPK) * p.rpad;
+        for (int r = (sub + LPK) * 4; r < p.rpad; r += LPK * 4) {
+          const float4 y4 = __ldcs(reinterpret_cast<const float4 *>(x + r));
+          w += (join_p(y4.x, sj[r], sj[p.rpad + r]) + join_p(y4.y, sj[r + 1], sj[p.rpad + r + 1])) +
+               (join_p(y4.z, sj[r + 2], sj[p.rpad + r + 2]) + join_p(y4.w, sj[r + 3], sj[p.rpad + r + 3]));
+        }
+      }
+#pragma unroll
+      for (int o = 1; o < LPK; o <<= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
+      if (key[u] >= 0 && sub == 0) wp[key[u]] = w0[u] + w;
+    }
+  }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinParams p, const int wpr) {
-  extern __shared__ float sj[];
+  extern __shared__ __align__(16) float sj[];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rpb = 8 / wpr;
   const long long rblocks = (p.rows + rpb - 1) / rpb;
@@ -718,39 +1011,18 @@ __global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinPara
 #pragma unroll
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     if (lane == 0) {  // offset and factor of the row
-      sj[2 * r] = l == 0.f ? INFINITY : m;
-      sj[2 * r + 1] = l == 0.f ? 0.f : 1.f / l;
+      sj[r] = m;
+      sj[p.rpad + r] = l == 0.f ? 0.f : 1.f / l;
     }
   }
+  for (int r = p.R + tid; r < p.rpad; r += kJoinThreads) sj[r] = sj[p.rpad + r] = 0.f;
   __syncthreads();
-  const int *lv = p.live ? p.live + (long long)bh * (1 + p.kk) : nullptr;
-  const long long nv = lv ? (long long)lv[0] * p.bs : p.L;
-  const long long j = tile * 1024LL + tid * 4;  // the row length ncap is a multiple of 4
-  if (j >= nv) return;
-  const float *lg = p.logits + (long long)bh * p.R * p.ncap + j;
-  long long key = j;
-  if (lv) {  // four slots of one block: bs is a multiple of 4
-    const long long blk = j / p.bs;
-    key = (long long)lv[1 + blk] * p.bs + (j - blk * p.bs);
-  }
-  float *wp = p.weight + b * p.w_sb + hk * p.w_sh + key;
-  float w0[4];
-#pragma unroll
-  for (int e = 0; e < 4; ++e) w0[e] = key + e < p.L ? wp[e] : 0.f;
-  float4 w = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-  for (int r = 0; r < p.R; ++r) {
-    const float4 x = *reinterpret_cast<const float4 *>(lg + (long long)r * p.ncap);
-    const float m = sj[2 * r], f = sj[2 * r + 1];
-    w.x = fmaf(ex2(x.x - m), f, w.x);
-    w.y = fmaf(ex2(x.y - m), f, w.y);
-    w.z = fmaf(ex2(x.z - m), f, w.z);
-    w.w = fmaf(ex2(x.w - m), f, w.w);
-  }
-  if (key < p.L) wp[0] = w0[0] + w.x;
-  if (key + 1 < p.L) wp[1] = w0[1] + w.y;
-  if (key + 2 < p.L) wp[2] = w0[2] + w.z;
-  if (key + 3 < p.L) wp[3] = w0[3] + w.w;
+  if (p.rpad == 8)
+    join_weights<2>(p, bh, b, hk, tile, sj);
+  else if (p.rpad == 16)
+    join_weights<4>(p, bh, b, hk, tile, sj);
+  else
+    join_weights<8>(p, bh, b, hk, tile, sj);
 }
 
 // ------------------------------------------------------------------ launchers
@@ -771,13 +1043,10 @@ static int choose_split(long long groups, long long steps, int slots, int fixed,
 
 constexpr int kMaxSplit = 296;
 
-// Row tiles of 16 or 32: two tiles share a chunk's fragments where O fits the registers.
-constexpr int row_tiles(int D, int R) { return R > 16 && D >= 64 && D <= 128 ? 2 : 1; }
-
 template <typename T, int D>
 static int split_count_t(long long groups, int R, long long n) {
   using C = SplitCfg<T, D>;
-  const int rows = 16 * row_tiles(D, R);
+  const int rows = split_rows<T, D>(R);
   const long long step = C::KC * NW;
   return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, 148 * C::MINB, 4, kMaxSplit);
 }
@@ -793,14 +1062,18 @@ int split_count(int dtype, int D, long long groups, int R, long long n) {
   }
 }
 
-template <typename T, int D, int MT>
-static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_t st) {
+template <typename T, int D, int ROWS>
+static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream_t st) {
   using C = SplitCfg<T, D>;
-  const int rtiles = (p.R + 16 * MT - 1) / (16 * MT);
-  const int base = 16 * MT * D * C::ES + C::RING, most = base + 3 * kMaxLive * 4;
-  auto kern = split_mma_kernel<T, D, MT>;
-  static_assert(C::RING >= NW * 16 * MT * D * 4, "the ring holds the warps' O for the join");
-  static_assert(C::KC * D * C::ES >= 16 * MT * C::KC * 4, "a chunk's K buffer holds its P");
+  const int rtiles = (p.R + ROWS - 1) / ROWS;
+  const int base = ROWS * D * C::ES + C::RING, most = base + 3 * kMaxLive * 4;
+  static_assert(C::RING >= NW * ROWS * (D + 4) * 4, "the ring holds the warps' O for the join");
+  static_assert(C::KC * D * C::ES >= ROWS * C::KC * 4, "a chunk's K buffer holds its P");
+  void (*kern)(const SplitParams, int, int);
+  if constexpr (C::ES == 2)
+    kern = split_mma_kernel<T, D, ROWS / 8>;
+  else
+    kern = split_f32_kernel<D, ROWS / 16>;
   static std::atomic<uint64_t> done{0};
   allow_smem(reinterpret_cast<const void *>(kern), most, done);
   const dim3 grid((unsigned)(groups * rtiles), p.nsplit);
@@ -809,14 +1082,17 @@ static bsa_status launch_mma(const SplitParams &p, long long groups, cudaStream_
     launch_after(kern, grid, NW * 32, smem, st, p, rtiles, NW);
   else
     kern<<<grid, NW * 32, smem, st>>>(p, rtiles, NW);
-  return check_launch("split_mma");
+  return check_launch("split");
 }
 
 template <typename T, int D>
 static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStream_t st) {
-  if constexpr (row_tiles(D, 17) == 2)
-    if (row_tiles(D, p.R) == 2) return launch_mma<T, D, 2>(p, groups, st);
-  return launch_mma<T, D, 1>(p, groups, st);
+  const int rows = split_rows<T, D>(p.R);
+  if constexpr (sizeof(T) == 2)
+    if (rows == 8) return launch_rows<T, D, 8>(p, groups, st);
+  if constexpr (SplitCfg<T, D>::MAXROWS == 32)
+    if (rows == 32) return launch_rows<T, D, 32>(p, groups, st);
+  return launch_rows<T, D, 16>(p, groups, st);
 }
 
 template <int D>
@@ -842,7 +1118,7 @@ static void launch_join_t(const JoinParams &p, cudaStream_t st) {
   const int wpr = p.nsplit <= 8 ? 1 : p.nsplit <= 16 ? 2 : p.nsplit <= 32 ? 4 : 8;
   const long long rblocks = (p.rows * wpr + 7) / 8;
   const dim3 grid((unsigned)(rblocks + (p.weight ? (long long)p.B * p.Hkv * p.wtiles : 0)));
-  const size_t smem = std::max<size_t>((8 * p.D + 8) * 4, p.weight ? (size_t)p.R * 8 : 0);
+  const size_t smem = std::max<size_t>((8 * p.D + 8) * 4, p.weight ? (size_t)p.rpad * 8 : 0);
   switch (p.D) {
     case 32: return launch_after(split_join_kernel<T, 32>, grid, kJoinThreads, smem, st, p, wpr);
     case 64: return launch_after(split_join_kernel<T, 64>, grid, kJoinThreads, smem, st, p, wpr);
@@ -889,6 +1165,7 @@ namespace {
 constexpr int kMaxWeightRows = 4096;
 struct WeightedPlan {
   int nsplit;
+  int rpad;
   long long ncap, rows;
   size_t o_po, o_ml, o_lg, o_lv, bytes;
 };
@@ -898,11 +1175,12 @@ WeightedPlan weighted_plan(const bsa_decode_weighted_args *a) {
   const long long n = a->sel ? (long long)a->kk * a->bs : a->L;
   w.nsplit = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, n);
   w.ncap = (n + 31) / 32 * 32;
+  w.rpad = (R + 7) / 8 * 8;
   w.rows = (long long)a->B * a->Hq * a->T;
   w.o_po = 0;
   w.o_ml = align_up((size_t)w.nsplit * w.rows * a->D * 4, 256);
   w.o_lg = align_up(w.o_ml + (size_t)w.nsplit * w.rows * 8, 256);
-  w.o_lv = align_up(w.o_lg + (size_t)w.rows * w.ncap * 4, 256);
+  w.o_lv = align_up(w.o_lg + (size_t)a->B * a->Hkv * w.rpad * w.ncap * 4, 256);
   w.bytes = align_up(w.o_lv + (a->sel ? (size_t)a->B * a->Hkv * (1 + a->kk) * 4 : 0), 256);
   return w;
 }
@@ -954,6 +1232,7 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
   p.pml = reinterpret_cast<float2 *>(base + w.o_ml);
   p.logits = reinterpret_cast<float *>(base + w.o_lg);
   p.ncap = w.ncap;
+  p.rpad = w.rpad;
   p.live = a->sel ? reinterpret_cast<int *>(base + w.o_lv) : nullptr;
   p.status = a->status;
   if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
@@ -961,9 +1240,13 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
   j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
   j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;
   j.nsplit = w.nsplit, j.R = p.R, j.rows = w.rows, j.po = p.po, j.pml = p.pml;
-  j.logits = p.logits, j.ncap = w.ncap, j.live = p.live, j.kk = p.kk, j.bs = a->bs, j.L = a->L;
+  j.logits = p.logits, j.ncap = w.ncap, j.rpad = w.rpad, j.live = p.live, j.kk = p.kk, j.bs = a->bs, j.L = a->L;
   j.weight = a->weight, j.w_sb = a->weight_sb, j.w_sh = a->weight_sh;
-  j.wtiles = (int)((w.ncap + 1023) / 1024);
+  // slots per weight block: enough work to hide the lse of its rows, unless few blocks
+  // come of it
+  const long long heads = (long long)a->B * a->Hkv;
+  j.kpb = heads * (w.ncap / 1024) >= 148 ? 1024 : heads * (w.ncap / 512) >= 148 ? 512 : 256;
+  j.wtiles = (int)((w.ncap + j.kpb - 1) / j.kpb);
   return launch_join(a->dtype, j, st);
 }
 

@@ -33,8 +33,9 @@ struct SplitParams {
   long long rows;       // B*Hq*T
   float *po;            // [split][rows][D]
   float2 *pml;          // [split][rows] (m, l); m = -inf: nothing visible, O not written
-  float *logits;        // optional [b*Hkv + hk][R][ncap]: x_j of each row
+  float *logits;        // optional [b*Hkv + hk][ncap][rpad]: x_j of each row
   long long ncap;
+  int rpad;             // rows padded to a multiple of 8
   int *live;            // with sel and logits: [b*Hkv + hk][1 + kk] count and live block ids
   int after;            // launched beside the kernel before it, whose end it waits for at its own
   int32_t *status;
