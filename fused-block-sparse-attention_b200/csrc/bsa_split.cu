@@ -846,64 +846,80 @@ constexpr int kJoinThreads = 256;
 // Row blocks: 8 / wpr query rows each.  A row's columns take D/4 lanes; the remaining
 // lanes of its warps, and its wpr warps, take splits side by side.  Weight blocks:
 // kpb slots of one (b, hk): lse of its R rows from the splits' (m, l), then the sum over
-// the rows of 2^(x - m) / l, four rows to a lane and LPK lanes to a slot, so that a warp
-// reads whole lines of the logits.
+// the rows of 2^(x - m) / l, eight rows to a lane and LPK lanes to a slot, so that a
+// warp reads whole lines of the logits.
 // 2^(x - m) f, and 0 where f is: a row that saw nothing or padding, whatever its x holds.
 __device__ __forceinline__ float join_p(float x, float m, float f) { return f == 0.f ? 0.f : ex2(x - m) * f; }
 
-template <int LPK>
+template <int LPK, bool SEL>
 __device__ __forceinline__ void join_weights(const JoinParams &p, int bh, int b, int hk, int tile, const float *sj) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  constexpr int KPW = 32 / LPK;  // slots per warp and step
-  const int sub = lane % LPK;
-  const int *lv = p.live ? p.live + (long long)bh * (1 + p.kk) : nullptr;
-  const long long nv = lv ? (long long)lv[0] * p.bs : p.L;
+  constexpr int KPW = 32 / LPK, STEP = KPW * (kJoinThreads / 32);  // slots of a warp, of the CTA per step
+  constexpr int U = 4;                                             // steps in flight
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % LPK;
+  const int *lv = SEL ? p.live + (long long)bh * (1 + p.kk) : nullptr;
+  const int nv = SEL ? lv[0] * p.bs : p.L;       // (virtual) slots
+  const int jw0 = tile * p.kpb + warp * KPW;     // the warp's first slot
+  const int end = min(nv, tile * p.kpb + p.kpb);
   float *wp = p.weight + b * p.w_sb + hk * p.w_sh;
-  const float *lg = p.logits + (long long)bh * p.ncap * p.rpad;
-  const long long j0 = (long long)tile * p.kpb;
-  // this lane's first four rows (none when there are fewer)
-  float4 m4 = make_float4(0, 0, 0, 0), f4 = m4;
-  const bool rows = sub * 4 < p.rpad;
-  if (rows) {
-    m4 = *reinterpret_cast<const float4 *>(sj + sub * 4);
-    f4 = *reinterpret_cast<const float4 *>(sj + p.rpad + sub * 4);
+  const float *lg = p.logits + ((long long)bh * p.ncap + jw0 + lane / LPK) * p.rpad + sub * 8;
+  const int step = STEP * p.rpad;
+  // this lane's first eight rows (none when there are fewer)
+  float m8[8], f8[8];
+  const bool rows = sub * 8 < p.rpad;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    m8[e] = rows ? sj[sub * 8 + e] : 0.f;
+    f8[e] = rows ? sj[p.rpad + sub * 8 + e] : 0.f;
   }
-  constexpr int U = 4, STEP = KPW * (kJoinThreads / 32);  // slots in flight per lane group, slots per step
-  for (int i = 0; i < p.kpb; i += U * STEP) {
-    float4 x4[U];
+  for (int jw = jw0; jw < end; jw += U * STEP, lg += U * step) {
+    float4 x4[U][2];
     float w0[U];
-    long long key[U];
+    int key[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const long long jw = j0 + i + u * STEP + warp * KPW;  // the warp's slots lie in one block of 32
-      const long long j = jw + lane / LPK;
+      const int j = jw + u * STEP + lane / LPK;
+      const bool in = j < end;
       key[u] = j;
-      if (lv && jw < nv) {
-        const long long blk = jw / p.bs;
-        key[u] = (long long)lv[1 + blk] * p.bs + (j - blk * p.bs);
+      if (SEL && in) {  // the warp's slots lie in one block (bs is a multiple of 32)
+        const int blk = (jw + u * STEP) / p.bs;
+        key[u] = lv[1 + blk] * p.bs + (j - blk * p.bs);
       }
-      if (i + u * STEP >= p.kpb || j >= nv || key[u] >= p.L) key[u] = -1;
-      x4[u] = make_float4(0, 0, 0, 0);
-      if (key[u] >= 0 && rows) x4[u] = __ldcs(reinterpret_cast<const float4 *>(lg + j * p.rpad + sub * 4));
-      w0[u] = key[u] >= 0 && sub == 0 ? wp[key[u]] : 0.f;
+      const bool live = in && (!SEL || key[u] < p.L);
+      x4[u][0] = x4[u][1] = make_float4(0, 0, 0, 0);
+      w0[u] = 0.f;
+      if (live && rows) {
+        x4[u][0] = __ldcs(reinterpret_cast<const float4 *>(lg + u * step));
+        x4[u][1] = __ldcs(reinterpret_cast<const float4 *>(lg + u * step + 4));
+      }
+      if (live && sub == 0) w0[u] = wp[key[u]];
+      if (!live) key[u] = -1;
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      float w = (join_p(x4[u].x, m4.x, f4.x) + join_p(x4[u].y, m4.y, f4.y)) +
-                (join_p(x4[u].z, m4.z, f4.z) + join_p(x4[u].w, m4.w, f4.w));
-      if (LPK == 8 && key[u] >= 0) {  // more than 32 rows
-        const float *x = lg + (j0 + i + u * STEP + warp * KPW + lane / LPK) * p.rpad;
-        for (int r = (sub + LPK) * 4; r < p.rpad; r += LPK * 4) {
-          const float4 y4 = __ldcs(reinterpret_cast<const float4 *>(x + r));
-          w += (join_p(y4.x, sj[r], sj[p.rpad + r]) + join_p(y4.y, sj[r + 1], sj[p.rpad + r + 1])) +
-               (join_p(y4.z, sj[r + 2], sj[p.rpad + r + 2]) + join_p(y4.w, sj[r + 3], sj[p.rpad + r + 3]));
+      float w = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w += (join_p(x4[u][h].x, m8[4 * h], f8[4 * h]) + join_p(x4[u][h].y, m8[4 * h + 1], f8[4 * h + 1])) +
+             (join_p(x4[u][h].z, m8[4 * h + 2], f8[4 * h + 2]) + join_p(x4[u][h].w, m8[4 * h + 3], f8[4 * h + 3]));
+      if (LPK == 4 && key[u] >= 0)  // more than 32 rows
+        for (int r = LPK * 8; r + sub * 8 < p.rpad; r += LPK * 8) {
+          const float *x = lg + u * step + r, *sm = sj + r + sub * 8, *sf = sm + p.rpad;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) w += join_p(x[e], sm[e], sf[e]);
         }
-      }
 #pragma unroll
       for (int o = 1; o < LPK; o <<= 1) w += __shfl_xor_sync(0xffffffffu, w, o);
       if (key[u] >= 0 && sub == 0) wp[key[u]] = w0[u] + w;
     }
   }
+}
+
+template <int LPK>
+__device__ __forceinline__ void join_weights(const JoinParams &p, int bh, int b, int hk, int tile, const float *sj) {
+  if (p.live)
+    join_weights<LPK, true>(p, bh, b, hk, tile, sj);
+  else
+    join_weights<LPK, false>(p, bh, b, hk, tile, sj);
 }
 
 template <typename T, int D>
@@ -1018,11 +1034,11 @@ __global__ void __launch_bounds__(kJoinThreads) split_join_kernel(const JoinPara
   for (int r = p.R + tid; r < p.rpad; r += kJoinThreads) sj[r] = sj[p.rpad + r] = 0.f;
   __syncthreads();
   if (p.rpad == 8)
-    join_weights<2>(p, bh, b, hk, tile, sj);
+    join_weights<1>(p, bh, b, hk, tile, sj);
   else if (p.rpad == 16)
-    join_weights<4>(p, bh, b, hk, tile, sj);
+    join_weights<2>(p, bh, b, hk, tile, sj);
   else
-    join_weights<8>(p, bh, b, hk, tile, sj);
+    join_weights<4>(p, bh, b, hk, tile, sj);
 }
 
 // ------------------------------------------------------------------ launchers
