@@ -63,18 +63,30 @@ __device__ __forceinline__ int warp_prefix(int v, int *s, int *total) {
 }
 }  // namespace
 
-// Warp w of a CTA owns groups * 32 * IPT consecutive slots, in rows of 32: lane l of it
-// slots l, l + 32, ..., so a rank among them is a ballot, and one prefix over the warps
-// per list.  groups == 1: the IPT keys of a thread stay in registers (up to 8 * 1024 *
-// 16 slots per head); more: they are read again in every pass, for any length.
+// Exclusive prefix over the lanes of a warp, and its total.
+__device__ __forceinline__ int lane_prefix(int v, int *total) {
+  const int lane = threadIdx.x & 31;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  *total = __shfl_sync(0xffffffffu, x, 31);
+  return x - v;
+}
+
+// Lane l of warp w owns IPT consecutive slots of each of `groups` runs of 32 * IPT, so a
+// rank is a bit count in the lane, one prefix over the lanes and one over the warps, not
+// a ballot per row of 32 slots.  groups == 1: the keys stay in registers (up to 8 * 1024
+// * 16 slots per head); more: they are read again in every pass, for any length.
 template <int IPT>
 __global__ void __launch_bounds__(kPickThreads)
-    evict_pick_kernel(const bsa_evict_args a, const EvictWork w, const int groups) {
+    evict_pick_kernel(const bsa_evict_args a, const EvictWork w, const int groups, const int vec) {
   cg::cluster_group cl = cg::this_cluster();
   const int nc = cl.num_blocks(), rank = cl.block_rank();
   const int bh = blockIdx.x / nc, b = bh / a.Hkv, h = bh % a.Hkv;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const unsigned below = (1u << lane) - 1u;
   pdl_trigger();
   __shared__ int hist[3][kBins];
   __shared__ int s_scan[6][32];
@@ -87,18 +99,30 @@ __global__ void __launch_bounds__(kPickThreads)
   uint32_t kr[IPT];
   int base = 0;  // this lane's first slot of the group; slots past L get key 0, below every real one
   auto load = [&](int g) {
-    base = (int)min(first + (long long)g * (32 * IPT), (long long)a.L) + lane;
+    base = (int)min(first + (long long)g * (32 * IPT) + lane * IPT, (long long)a.L);
+    if (vec && base + IPT <= a.L) {
+      float4 x[IPT / 4];
+      int4 y[IPT / 4];
 #pragma unroll
-    for (int i = 0; i < IPT; ++i) {
-      const int s = base + 32 * i;
-      kr[i] = s < a.L ? evict_key(__ldg(wt + s), guards ? __ldg(ps + s) : 0, a.sink, guards ? first_recent : 1) : 0u;
+      for (int i = 0; i < IPT / 4; ++i) {
+        x[i] = __ldg(reinterpret_cast<const float4 *>(wt + base) + i);
+        y[i] = guards ? __ldg(reinterpret_cast<const int4 *>(ps + base) + i) : make_int4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < IPT; ++i)
+        kr[i] = evict_key(reinterpret_cast<const float *>(x)[i], reinterpret_cast<const int *>(y)[i], a.sink,
+                          guards ? first_recent : 1);
+    } else {
+#pragma unroll
+      for (int i = 0; i < IPT; ++i) {
+        const int s = base + i;
+        kr[i] = s < a.L ? evict_key(__ldg(wt + s), guards ? __ldg(ps + s) : 0, a.sink, guards ? first_recent : 1)
+                        : 0u;
+      }
     }
   };
-  // rows of this group with base + 32 * i < end, as a bit mask
-  auto rows_below = [&](int end) {
-    const int n = min(max((end - base + 31) >> 5, 0), IPT);
-    return (1u << n) - 1u;
-  };
+  // the lane's slots below `end`, as a bit mask
+  auto below = [&](int end) { return (1u << min(max(end - base, 0), IPT)) - 1u; };
   auto sync_all = [&] {
     if (nc > 1)
       cl.sync();
@@ -129,20 +153,21 @@ __global__ void __launch_bounds__(kPickThreads)
     // bins from the top, two per thread; sums over the cluster
     int c0 = 0, c1 = 0;
     const int b0 = nb - 1 - 2 * tid, b1 = b0 - 1;
-    if (b1 >= 0)
-      for (int r = 0; r < nc; ++r) {
-        const int *hr = cl.map_shared_rank(hs, r);
-        c0 += hr[b0];
-        c1 += hr[b1];
+    if (b1 >= 0) {
+      if (nc > 1) {
+        for (int r = 0; r < nc; ++r) {
+          const int *hr = cl.map_shared_rank(hs, r);
+          c0 += hr[b0];
+          c1 += hr[b1];
+        }
+      } else {
+        c0 = hs[b0];
+        c1 = hs[b1];
       }
-    int x = c0 + c1;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
     }
-    int total;
-    const int before = warp_prefix(__shfl_sync(0xffffffffu, x, 31), s_scan[r3], &total) + x - c0 - c1;
+    int wsum, total;
+    const int lp = lane_prefix(c0 + c1, &wsum);
+    const int before = warp_prefix(wsum, s_scan[r3], &total) + lp;
     if (before < need && before + c0 >= need) {
       s_bin[r3] = b0;
       s_need[r3] = need - before;
@@ -171,7 +196,7 @@ __global__ void __launch_bounds__(kPickThreads)
     cl.sync();
     for (int r = 0; r < rank; ++r) eq0 += cl.map_shared_rank(s_cnt, r)[0];
   }
-  // rows of the group that survive, as a bit mask; e: equal keys before the group
+  // the lane's slots of the group that survive, as a bit mask; e: equal keys before the group
   auto kept = [&](int &e) {
     uint32_t keep = 0, same = 0;
 #pragma unroll
@@ -179,20 +204,19 @@ __global__ void __launch_bounds__(kPickThreads)
       keep |= (uint32_t)(kr[i] > kth) << i;
       same |= (uint32_t)(kr[i] == kth) << i;
     }
-    if (__any_sync(0xffffffffu, same != 0u))
-#pragma unroll
-      for (int i = 0; i < IPT; ++i) {
-        const unsigned m = __ballot_sync(0xffffffffu, (same >> i) & 1u);
-        if (((same >> i) & 1u) && e + __popc(m & below) < need) keep |= 1u << i;
-        e += __popc(m);
-      }
+    if (__any_sync(0xffffffffu, same != 0u)) {
+      int sum;
+      int before = e + lane_prefix(__popc(same), &sum);
+      for (uint32_t s = same; s != 0u && before < need; s &= s - 1u, ++before) keep |= s & (0u - s);
+      e += sum;
+    }
     return keep;
   };
   // ---- freed slots below the budget and survivors beyond it, in this warp
   int holes = 0, tails = 0, e = eq0;
   for (int g = 0; g < groups; ++g) {
     if (groups > 1) load(g);
-    const uint32_t keep = kept(e), low = rows_below(a.budget);
+    const uint32_t keep = kept(e), low = below(a.budget);
     holes += __popc(low & ~keep);
     tails += __popc(keep & ~low);
   }
@@ -221,24 +245,17 @@ __global__ void __launch_bounds__(kPickThreads)
   e = eq0;
   for (int g = 0; g < groups; ++g) {
     if (groups > 1) load(g);
-    const uint32_t keep = kept(e), low = rows_below(a.budget);
+    const uint32_t keep = kept(e), low = below(a.budget);
     const uint32_t fr = low & ~keep, sv = keep & ~low;
-    const int row0 = base - lane;
-    int blk = (row0 + a.bs - 1) / a.bs;  // the next block that starts in these rows
-#pragma unroll
-    for (int i = 0; i < IPT; ++i) {
-      const int s = base + 32 * i;
-      const unsigned fm = __ballot_sync(0xffffffffu, (fr >> i) & 1u);
-      for (; blk < w.nblk && blk * a.bs < row0 + 32 * (i + 1); ++blk) {
-        const int at = blk * a.bs - (row0 + 32 * i);
-        if (lane == 0) off[blk] = hb + __popc(fm & ((1u << at) - 1u));
-      }
-      if ((fr >> i) & 1u) hole[hb + __popc(fm & below)] = s;
-      hb += __popc(fm);
-      const unsigned sm = __ballot_sync(0xffffffffu, (sv >> i) & 1u);
-      if ((sv >> i) & 1u) tail[tb + __popc(sm & below)] = s;
-      tb += __popc(sm);
-    }
+    int nh, nt;
+    int hr = hb + lane_prefix(__popc(fr), &nh), tr = tb + lane_prefix(__popc(sv), &nt);
+    // blocks that start in this lane's slots
+    for (int blk = (base + a.bs - 1) / a.bs; blk < w.nblk && blk * a.bs < base + IPT; ++blk)
+      off[blk] = hr + __popc(fr & ((1u << (blk * a.bs - base)) - 1u));
+    for (uint32_t m = fr; m != 0u; m &= m - 1u) hole[hr++] = base + __ffs(m) - 1;
+    for (uint32_t m = sv; m != 0u; m &= m - 1u) tail[tr++] = base + __ffs(m) - 1;
+    hb += nh;
+    tb += nt;
   }
 }
 
@@ -427,13 +444,15 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
   const size_t need = evict_plan(a, &w, static_cast<uint8_t *>(ws));
   if (!ws || ws_bytes < need) return fail(BSA_ERR_WORKSPACE, "evict: workspace too small");
   const int bh = a->B * a->Hkv;
-  // CTAs per (b, head): enough that a thread's slots fit its registers (16), up to one
-  // per 4096 slots while all fit the SMs at once; at most 8, the portable cluster size
+  // CTAs per (b, head): as few as hold its slots in registers (16 per thread), at most 8,
+  // the portable cluster size: a pass over a cluster costs twice the barrier of one CTA
   int nc = 1;
-  while (nc < 8 && ((long long)nc * 16384 < a->L || ((long long)nc * 4096 < a->L && (long long)bh * nc * 2 <= 148)))
-    nc *= 2;
+  while (nc < 8 && (long long)nc * 16 * kPickThreads < a->L) nc *= 2;
   const int ipt = (int)((a->L + (long long)nc * kPickThreads - 1) / ((long long)nc * kPickThreads));
   const int groups = std::max(1, (ipt + 15) / 16);
+  // 16-byte loads of the sums and positions
+  const int vec = !(reinterpret_cast<uintptr_t>(a->weight) % 16 || reinterpret_cast<uintptr_t>(a->pos) % 16 ||
+                    a->w_sb % 4 || a->w_sh % 4 || a->p_sb % 4 || a->p_sh % 4);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)bh * nc);
   cfg.blockDim = dim3(kPickThreads);
@@ -443,14 +462,12 @@ bsa_status run_evict(const bsa_evict_args *a, void *ws, size_t ws_bytes, cudaStr
   at.val.clusterDim.x = nc, at.val.clusterDim.y = 1, at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (ipt <= 1)
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<1>, *a, w, 1);
-  else if (ipt <= 4)
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<4>, *a, w, 1);
+  if (ipt <= 4)
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<4>, *a, w, 1, vec);
   else if (ipt <= 8)
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<8>, *a, w, 1);
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<8>, *a, w, 1, vec);
   else
-    cudaLaunchKernelEx(&cfg, evict_pick_kernel<16>, *a, w, groups);
+    cudaLaunchKernelEx(&cfg, evict_pick_kernel<16>, *a, w, groups, vec);
   if (bsa_status s = check_launch("evict_pick")) return s;
   const unsigned grid = (unsigned)bh * w.nblk;
   const size_t smem = (size_t)align_up(a->bs * 4, 16) + 2ull * 8 * a->D * elem_size(a->dtype);
