@@ -297,11 +297,12 @@ __device__ __forceinline__ uint4 shfl_xor16(uint4 a, int o) {
 // owns one piece column (PC <= 32: its warp holds 32 / PC rows side by side) and every
 // RG-th row.  A block is a few rows per thread behind a chain of dependent loads
 // (offsets, lists, rows), so CTAs side by side hide it: min and max stay in the row's
-// type and are joined by shuffles, which leaves room for five CTAs per SM and takes
+// type and are joined by shuffles, which leaves room for six CTAs per SM and takes
 // most of the instructions out (an fp32 min / max through shared memory: 42% of the
-// issue slots at half the HBM rate).
+// issue slots at half the HBM rate).  Rows pass through once: streaming loads and
+// stores (a prompt to a quarter: 112 -> 102 us).
 template <typename T, int D>
-__global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args a, const EvictWork w) {
+__global__ void __launch_bounds__(256, 6) evict_move_kernel(const bsa_evict_args a, const EvictWork w) {
   constexpr int E = 16 / sizeof(T), PC = D / E, RG = 256 / PC;
   extern __shared__ int s_src[];  // [bs] source slot, then per warp the min and the max
   const int blk = blockIdx.x % w.nblk, bh = blockIdx.x / w.nblk;
@@ -334,16 +335,16 @@ __global__ void __launch_bounds__(256, 5) evict_move_kernel(const bsa_evict_args
         const int r = rb + u * RG;
         src[u] = r < rows ? s_src[r] : -1;
         if (src[u] >= 0 && (pool || src[u] != s0 + r))
-          kv[u] = *reinterpret_cast<const uint4 *>(kp + (long long)src[u] * a.k.sl);
+          kv[u] = __ldcs(reinterpret_cast<const uint4 *>(kp + (long long)src[u] * a.k.sl));
         if (src[u] >= 0 && src[u] != s0 + r)
-          vv[u] = *reinterpret_cast<const uint4 *>(vp + (long long)src[u] * a.v.sl);
+          vv[u] = __ldcs(reinterpret_cast<const uint4 *>(vp + (long long)src[u] * a.v.sl));
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int r = rb + u * RG;
         if (src[u] >= 0 && src[u] != s0 + r) {
-          *reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl) = kv[u];
-          *reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl) = vv[u];
+          __stcs(reinterpret_cast<uint4 *>(kp + (long long)(s0 + r) * a.k.sl), kv[u]);
+          __stcs(reinterpret_cast<uint4 *>(vp + (long long)(s0 + r) * a.v.sl), vv[u]);
         }
         if (src[u] >= 0 && pool) {
           mn = min16<T>(mn, kv[u], false);
