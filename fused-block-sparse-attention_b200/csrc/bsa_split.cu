@@ -7,6 +7,7 @@
 // The kernels are bound by reading K and V once (HBM).
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "bsa_host.h"
 #include "bsa_split.cuh"
@@ -41,8 +42,7 @@ __device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) 
 }
 __device__ __forceinline__ void mma_tf32(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -123,7 +123,7 @@ struct SplitCfg {
   static constexpr int ES = sizeof(T), E16 = 16 / ES;
   static constexpr int KC = ES == 2 ? (D >= 128 ? 16 : 32) : (D == 256 ? 8 : 16);
   static constexpr int STAGE = KC * D * ES * 2;       // K and V of a chunk, bytes
-  static constexpr int NST = STAGE <= 4096 ? 5 : 3;
+  static constexpr int NST = STAGE <= 4096 ? 5 : ES == 4 && STAGE == 16384 ? 2 : 3;  // fp32: Q takes twice its size
   static constexpr int MINB = STAGE >= 16384 ? 1 : 2; // CTAs per SM
   static constexpr int RING = NW * NST * STAGE;
   // most rows per CTA: O fits the registers, P a chunk of K
@@ -287,6 +287,20 @@ __device__ __forceinline__ void split_write(const SplitParams &p, const Span &s,
   }
 }
 
+// m16n8k16 product that the compiler may move: with one or two warps per SM quarter the
+// order of independent products is what hides their latency.
+template <typename T>
+__device__ __forceinline__ void mma16(float *c, const uint32_t *a, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {  // 8x8 of 16 bits, transposed over the warp
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -382,12 +396,16 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
     // ---- S^T = K Q^T
     float s[KT][NR][4];  // keys g, g + 8 of tile kt; rows 2t, 2t + 1
+    constexpr int PS = KT * NR >= 4 ? 1 : 2;  // partial sums over the dims: independent chains
+    float s2[PS][KT][NR][4];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int q = 0; q < PS; ++q)
 #pragma unroll
-      for (int n = 0; n < NR; ++n)
+      for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[kt][n][e] = 0.f;
+        for (int n = 0; n < NR; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s2[q][kt][n][e] = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
@@ -395,8 +413,14 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
         uint32_t a[4];
         ldsm_x4(ka + sw_off<2, D>(kt * 16 + krow, ks * 2 + kch), a[0], a[1], a[2], a[3]);
 #pragma unroll
-        for (int n = 0; n < NR; ++n) Mma<T>::run(s[kt][n], a, qf[n][ks][0], qf[n][ks][1]);
+        for (int n = 0; n < NR; ++n) mma16<T>(s2[ks % PS][kt][n], a, qf[n][ks][0], qf[n][ks][1]);
       }
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[kt][n][e] = PS == 2 ? s2[0][kt][n][e] + s2[PS - 1][kt][n][e] : s2[0][kt][n][e];
     // ---- online softmax (log2 domain); masked and missing keys are -inf
     const bool masked = key0 + KC - 1 > all_see;
     const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
@@ -468,8 +492,8 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
           ldsm_x4_t(va + sw_off<2, D>(kt * 16 + vrow, ks * 2 + vch), a[0], a[1], a[2], a[3]);
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
-            Mma<T>::run(acc[n][ks], a, hi[n][0], hi[n][1]);
-            Mma<T>::run(acc[n][ks], a, lo[n][0], lo[n][1]);
+            mma16<T>(acc[n][ks], a, hi[n][0], hi[n][1]);
+            mma16<T>(acc[n][ks], a, lo[n][0], lo[n][1]);
           }
         }
       }
@@ -556,8 +580,8 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int s_n;
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
-  uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
-  uint8_t *ring = sm + ROWS * D * 4;
+  uint8_t *sQ = sm;                                   // [hi, lo][ROWS][D] swizzled
+  uint8_t *ring = sm + 2 * ROWS * D * 4;
   int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
   float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
   const bool last = p.after && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
@@ -586,6 +610,17 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s) load(sp.c_lo + warp + s * NW, s);
   split_queries<float, D, ROWS>(p, sp, sQ);
+  __syncthreads();
+  for (int i = tid; i < ROWS * D / 4; i += blockDim.x) {  // tf32 terms of Q, once
+    uint4 hi, lo;
+    const float4 x = reinterpret_cast<const float4 *>(sQ)[i];
+    tf32_split(x.x, hi.x, lo.x);
+    tf32_split(x.y, hi.y, lo.y);
+    tf32_split(x.z, hi.z, lo.z);
+    tf32_split(x.w, hi.w, lo.w);
+    reinterpret_cast<uint4 *>(sQ)[i] = hi;
+    reinterpret_cast<uint4 *>(sQ + ROWS * D * 4)[i] = lo;
+  }
   __syncthreads();
 
   float acc[MT][NT][4], m[MT][2], l[MT][2];
@@ -619,48 +654,53 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
     float gate;
     const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
     // ---- S = Q K^T
-    float s[MT][KC / 8][4];
+    float s[MT][KC / 8][4], s3[2][MT][KC / 8][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int n = 0; n < KC / 8; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[mt][n][e] = s3[0][mt][n][e] = s3[1][mt][n][e] = 0.f;
 #pragma unroll 4
     for (int ks = 0; ks < KS; ++ks) {  // 16 dims: two k-steps
-      uint32_t ah[MT][2][4], al[MT][2][4];
+      uint4 ah[MT][2], al[MT][2];      // rows g, g + 8: dims 4t .. 4t + 3
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const float4 x = *reinterpret_cast<const float4 *>(sQ + sw_off<4, D>(mt * 16 + g, ks * 4 + tq));
-        const float4 y = *reinterpret_cast<const float4 *>(sQ + sw_off<4, D>(mt * 16 + g + 8, ks * 4 + tq));
-        tf32_split(x.x, ah[mt][0][0], al[mt][0][0]);
-        tf32_split(y.x, ah[mt][0][1], al[mt][0][1]);
-        tf32_split(x.y, ah[mt][0][2], al[mt][0][2]);
-        tf32_split(y.y, ah[mt][0][3], al[mt][0][3]);
-        tf32_split(x.z, ah[mt][1][0], al[mt][1][0]);
-        tf32_split(y.z, ah[mt][1][1], al[mt][1][1]);
-        tf32_split(x.w, ah[mt][1][2], al[mt][1][2]);
-        tf32_split(y.w, ah[mt][1][3], al[mt][1][3]);
-      }
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t off = sw_off<4, D>(mt * 16 + g + 8 * h, ks * 4 + tq);
+          ah[mt][h] = *reinterpret_cast<const uint4 *>(sQ + off);
+          al[mt][h] = *reinterpret_cast<const uint4 *>(sQ + ROWS * D * 4 + off);
+        }
+      uint32_t bh[KC / 8][4], bl[KC / 8][4];
 #pragma unroll
       for (int n = 0; n < KC / 8; ++n) {
         const float4 k4 = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(n * 8 + g, ks * 4 + tq));
-        uint32_t bh[4], bl[4];
-        tf32_split(k4.x, bh[0], bl[0]);
-        tf32_split(k4.y, bh[1], bl[1]);
-        tf32_split(k4.z, bh[2], bl[2]);
-        tf32_split(k4.w, bh[3], bl[3]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int k2 = 0; k2 < 2; ++k2) {
-            const uint32_t *xh = ah[mt][k2], *xl = al[mt][k2];
-            mma_tf32(s[mt][n], xl[0], xl[1], xl[2], xl[3], bh[2 * k2], bh[2 * k2 + 1]);
-            mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bl[2 * k2], bl[2 * k2 + 1]);
-            mma_tf32(s[mt][n], xh[0], xh[1], xh[2], xh[3], bh[2 * k2], bh[2 * k2 + 1]);
-          }
+        tf32_split(k4.x, bh[n][0], bl[n][0]);
+        tf32_split(k4.y, bh[n][1], bl[n][1]);
+        tf32_split(k4.z, bh[n][2], bl[n][2]);
+        tf32_split(k4.w, bh[n][3], bl[n][3]);
       }
+      // the three terms of every sum apart, so that consecutive products are independent
+#pragma unroll
+      for (int n = 0; n < KC / 8; ++n)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const uint4 *xh = ah[mt], *xl = al[mt];
+          mma_tf32(s3[0][mt][n], xl[0].x, xl[1].x, xl[0].y, xl[1].y, bh[n][0], bh[n][1]);
+          mma_tf32(s3[1][mt][n], xh[0].x, xh[1].x, xh[0].y, xh[1].y, bl[n][0], bl[n][1]);
+          mma_tf32(s[mt][n], xh[0].x, xh[1].x, xh[0].y, xh[1].y, bh[n][0], bh[n][1]);
+          mma_tf32(s3[0][mt][n], xl[0].z, xl[1].z, xl[0].w, xl[1].w, bh[n][2], bh[n][3]);
+          mma_tf32(s3[1][mt][n], xh[0].z, xh[1].z, xh[0].w, xh[1].w, bl[n][2], bl[n][3]);
+          mma_tf32(s[mt][n], xh[0].z, xh[1].z, xh[0].w, xh[1].w, bh[n][2], bh[n][3]);
+        }
     }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < KC / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][n][e] += s3[0][mt][n][e] + s3[1][mt][n][e];
     // ---- online softmax (log2 domain); masked and missing keys are -inf
     const bool masked = key0 + KC - 1 > all_see;
     const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
@@ -1082,7 +1122,7 @@ template <typename T, int D, int ROWS>
 static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream_t st) {
   using C = SplitCfg<T, D>;
   const int rtiles = (p.R + ROWS - 1) / ROWS;
-  const int base = ROWS * D * C::ES + C::RING, most = base + 3 * kMaxLive * 4;
+  const int base = ROWS * D * C::ES * (C::ES == 4 ? 2 : 1) + C::RING, most = base + 3 * kMaxLive * 4;
   static_assert(C::RING >= NW * ROWS * (D + 4) * 4, "the ring holds the warps' O for the join");
   static_assert(C::KC * D * C::ES >= ROWS * C::KC * 4, "a chunk's K buffer holds its P");
   void (*kern)(const SplitParams, int, int);
