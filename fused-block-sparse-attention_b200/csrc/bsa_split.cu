@@ -31,20 +31,18 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live, u
                : "memory");
 }
 
-// fp32 products on the tensor cores: x = hi + lo with hi and lo rounded to tf32 (11
-// bits each), x y = hi hi' + hi lo' + lo hi' up to 2^-21 |x y| (lo lo' and lo's own
-// rounding are dropped).  lo of an infinity is 0, so that hi carries it alone.
-__device__ __forceinline__ uint32_t tf32_rn(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
-__device__ __forceinline__ void tf32_split(float x, uint32_t &hi, uint32_t &lo) {
-  hi = tf32_rn(x);
-  const float d = x - __uint_as_float(hi);
-  lo = isinf(x) ? 0u : tf32_rn(d);
-}
-__device__ __forceinline__ void mma_tf32(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// fp32 products on the tensor cores: x = x1 + x2 + x3, each the bf16 rounding of what is
+// left (8 bits each, so all 24), and x y = x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1 up
+// to 2^-23 |x y| (the other three).  Six bf16 products take the time of one and a half
+// tf32 ones (mma.sync, measured 300 against 80 TFLOP/s), of which two-term tf32 splits
+// need three.  The terms of two neighbours, packed; an infinity is its own first term.
+__device__ __forceinline__ void split3(float x, float y, uint32_t *u) {
+  u[0] = Mma<__nv_bfloat16>::pack(x, y);
+  float x1 = __uint_as_float(u[0] << 16), y1 = __uint_as_float(u[0] & 0xffff0000u);
+  const float rx = x == x1 ? 0.f : x - x1, ry = y == y1 ? 0.f : y - y1;
+  u[1] = Mma<__nv_bfloat16>::pack(rx, ry);
+  x1 = __uint_as_float(u[1] << 16), y1 = __uint_as_float(u[1] & 0xffff0000u);
+  u[2] = Mma<__nv_bfloat16>::pack(rx - x1, ry - y1);
 }
 // Maximum that keeps a NaN: a row with a NaN logit ends as NaN, not as an empty row.
 __device__ __forceinline__ float fmax_nan(float a, float b) {
@@ -59,7 +57,8 @@ __device__ __forceinline__ void cp_wait() {
 }
 
 // Live block ids (and gates) of one selection row: the first occurrence of each id
-// that holds slots before L, unless its gate is -inf; in slot order; by one warp.  Returns their count.
+// that holds slots before L, unless its gate is -inf; in slot order; by one warp.
+// Returns their count.
 __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_blk, float *s_gate,
                           int *s_raw) {
   const int lane = threadIdx.x & 31;
@@ -113,28 +112,27 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 // terms (p = hi + lo, hi = round(p), lo = round(p - hi)), so its rounding does not add to
 // the output's; the extra products are free under HBM's time.
 //
-// fp32, split_f32_kernel: rows as M, m16n8k8 on tf32 terms (above).  A contraction may
-// take its index in any order, so a thread's 16-byte piece of a K row feeds two k-steps
-// (its dims 4t .. 4t+3 stand for k = t, t + 4 of each), S's accumulator layout is P's
-// operand layout (keys 2t, 2t + 1 stand for k = t, t + 4), and a 16-byte piece of a V
-// row feeds four column tiles (tile e holds columns 4j + e of a group of 32).
+// fp32, split_f32_kernel: the same on three bf16 terms of every operand (above).  A
+// contraction may take its index in any order and O's rows any place, so a thread's
+// 16-byte piece of a K row is its two pairs of a k-step (dims 4t .. 4t+3), and 16-byte
+// pieces of V rows feed four tiles of O (tile e holds columns 4j + e of a group).
 template <typename T, int D>
 struct SplitCfg {
   static constexpr int ES = sizeof(T), E16 = 16 / ES;
-  static constexpr int KC = ES == 2 ? (D >= 128 ? 16 : 32) : (D == 256 ? 8 : 16);
+  static constexpr int KC = ES == 2 && D <= 64 ? 32 : 16;
   static constexpr int STAGE = KC * D * ES * 2;       // K and V of a chunk, bytes
-  static constexpr int NST = STAGE <= 4096 ? 5 : ES == 4 && STAGE == 16384 ? 2 : 3;  // fp32: Q takes twice its size
+  static constexpr int NST = STAGE <= 4096 ? 5 : STAGE == 32768 ? 1 : 3;
   static constexpr int MINB = STAGE >= 16384 ? 1 : 2; // CTAs per SM
   static constexpr int RING = NW * NST * STAGE;
   // most rows per CTA: O fits the registers, P a chunk of K
-  static constexpr int MAXROWS = ES == 2 ? (D == 64 || D == 128 ? 32 : 16) : (D >= 64 && D <= 128 ? 32 : 16);
+  static constexpr int MAXROWS = D == 256 || (ES == 2 && D == 32) ? 16 : 32;
 };
 
 // Rows per CTA for R query rows.
 template <typename T, int D>
 constexpr int split_rows(int R) {
   using C = SplitCfg<T, D>;
-  return C::ES == 2 && R <= 8 ? 8 : R <= 16 || C::MAXROWS == 16 ? 16 : 32;
+  return R <= 8 ? 8 : R <= 16 || C::MAXROWS == 16 ? 16 : 32;
 }
 
 // Byte offset of 16-byte chunk `chunk` of a D-wide row: chunks are permuted within
@@ -572,16 +570,17 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
 }
 
 // ------------------------------------------------------------------ fp32
-template <int D, int MT>
+template <int D, int NR>
 __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
     split_f32_kernel(const SplitParams p, int rtiles, int min_chunks) {
   using C = SplitCfg<float, D>;
-  constexpr int KC = C::KC, NST = C::NST, NT = D / 8, KS = D / 16, ROWS = 16 * MT;
+  constexpr int KC = C::KC, NST = C::NST, KS = D / 16, ROWS = 8 * NR, SO = D + 4;
+  constexpr int VW = D >= 64 ? 4 : 2, VG = D / (16 * VW);  // columns per piece of V, column groups
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int s_n;
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
-  uint8_t *sQ = sm;                                   // [hi, lo][ROWS][D] swizzled
-  uint8_t *ring = sm + 2 * ROWS * D * 4;
+  uint8_t *sQ = sm;                                   // fp32 rows first, then three bf16 terms [ROWS][D]
+  uint8_t *ring = sm + 3 * ROWS * D * 2;
   int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
   float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
   const bool last = p.after && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
@@ -609,43 +608,66 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   };
 #pragma unroll
   for (int s = 0; s < NST - 1; ++s) load(sp.c_lo + warp + s * NW, s);
-  split_queries<float, D, ROWS>(p, sp, sQ);
-  __syncthreads();
-  for (int i = tid; i < ROWS * D / 4; i += blockDim.x) {  // tf32 terms of Q, once
-    uint4 hi, lo;
-    const float4 x = reinterpret_cast<const float4 *>(sQ)[i];
-    tf32_split(x.x, hi.x, lo.x);
-    tf32_split(x.y, hi.y, lo.y);
-    tf32_split(x.z, hi.z, lo.z);
-    tf32_split(x.w, hi.w, lo.w);
-    reinterpret_cast<uint4 *>(sQ)[i] = hi;
-    reinterpret_cast<uint4 *>(sQ + ROWS * D * 4)[i] = lo;
+  // the three terms of Q, in a thread's order: row g, dims 4t .. 4t+3 of a k-step
+  for (int i = tid; i < ROWS * (D / 4); i += blockDim.x) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (r0 + r < p.R) {
+      int rb, rh, rtt;
+      split_row(p, sp.b, sp.hk, r0 + r, rb, rh, rtt);
+      const float *qp = reinterpret_cast<const float *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = qp[e];
+    }
+    uint32_t u[3], w[3];
+    split3(x[0], x[1], u);
+    split3(x[2], x[3], w);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      *reinterpret_cast<uint2 *>(sQ + k * ROWS * D * 2 + sw_off<2, D>(r, d / 8) + (d & 4) * 2) = make_uint2(u[k], w[k]);
   }
   __syncthreads();
+  auto ldq = [&](int k, int n, int ks) {
+    return *reinterpret_cast<const uint2 *>(sQ + k * ROWS * D * 2 + sw_off<2, D>(n * 8 + g, ks * 2 + (tq >> 1)) +
+                                            (tq & 1) * 8);
+  };
+  constexpr bool QREG = NR == 1 && D <= 128;
+  uint2 qf[QREG ? KS : 1][3];
+  if constexpr (QREG)
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) qf[ks][k] = ldq(k, 0, ks);
 
-  float acc[MT][NT][4], m[MT][2], l[MT][2];
-  int qlast[MT][2];  // newest key that the row sees
+  // O^T: tile (v, e) holds columns v * 16 VW + VW g + e (and 8 VW further) x rows 2t, 2t + 1
+  float acc[NR][KS][4], m[NR][2], l[NR][2];
+  int qlast[NR][2];  // newest key that the row sees
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt) {
+  for (int n = 0; n < NR; ++n) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
+    for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) acc[mt][n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) acc[n][ks][e] = 0.f;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      m[mt][h] = -INFINITY;
-      l[mt][h] = 0.f;
-      const int r = r0 + mt * 16 + g + 8 * h;
-      qlast[mt][h] = p.causal ? len - p.T + r % p.T : len - 1;
+      m[n][h] = -INFINITY;
+      l[n][h] = 0.f;
+      const int r = r0 + n * 8 + 2 * tq + h;
+      qlast[n][h] = p.causal ? len - p.T + r % p.T : len - 1;
     }
   }
   const int all_see = p.causal ? len - p.T : len - 1;  // newest key that every row sees
+  float *lg = p.logits ? p.logits + ((long long)sp.grpid * p.ncap + g) * p.rpad + r0 + 2 * tq : nullptr;
 
   int st = 0;
   for (int c = sp.c_lo + warp; c < sp.c_hi; c += NW) {
-    cp_wait<NST - 2>();
-    __syncwarp();
-    {
+    if constexpr (NST == 1) {
+      load(c, 0);  // D 256: a chunk is 32 KB, the other warps cover its way
+      cp_wait<0>();
+      __syncwarp();
+    } else {
+      cp_wait<NST - 2>();
+      __syncwarp();
       int nst = st + NST - 1;
       if (nst >= NST) nst -= NST;
       load(c + (NST - 1) * NW, nst);
@@ -653,213 +675,200 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
     const uint8_t *sk = wring + st * C::STAGE, *sv = sk + KC * D * 4;
     float gate;
     const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
-    // ---- S = Q K^T
-    float s[MT][KC / 8][4], s3[2][MT][KC / 8][4];
+    // ---- S^T = K Q^T
+    float s[NR][4], sr[NR][4];  // keys g, g + 8; rows 2t, 2t + 1: the leading products, the others
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int n = 0; n < NR; ++n)
 #pragma unroll
-      for (int n = 0; n < KC / 8; ++n)
+      for (int e = 0; e < 4; ++e) s[n][e] = sr[n][e] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][n][e] = s3[0][mt][n][e] = s3[1][mt][n][e] = 0.f;
-#pragma unroll 4
-    for (int ks = 0; ks < KS; ++ks) {  // 16 dims: two k-steps
-      uint4 ah[MT][2], al[MT][2];      // rows g, g + 8: dims 4t .. 4t + 3
+    for (int ks = 0; ks < KS; ++ks) {
+      uint32_t a[3][4], u[3];
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t off = sw_off<4, D>(mt * 16 + g + 8 * h, ks * 4 + tq);
-          ah[mt][h] = *reinterpret_cast<const uint4 *>(sQ + off);
-          al[mt][h] = *reinterpret_cast<const uint4 *>(sQ + ROWS * D * 4 + off);
-        }
-      uint32_t bh[KC / 8][4], bl[KC / 8][4];
-#pragma unroll
-      for (int n = 0; n < KC / 8; ++n) {
-        const float4 k4 = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(n * 8 + g, ks * 4 + tq));
-        tf32_split(k4.x, bh[n][0], bl[n][0]);
-        tf32_split(k4.y, bh[n][1], bl[n][1]);
-        tf32_split(k4.z, bh[n][2], bl[n][2]);
-        tf32_split(k4.w, bh[n][3], bl[n][3]);
+      for (int h = 0; h < 2; ++h) {
+        const float4 x = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(g + 8 * h, ks * 4 + tq));
+        split3(x.x, x.y, u);
+        a[0][h] = u[0], a[1][h] = u[1], a[2][h] = u[2];
+        split3(x.z, x.w, u);
+        a[0][2 + h] = u[0], a[1][2 + h] = u[1], a[2][2 + h] = u[2];
       }
-      // the three terms of every sum apart, so that consecutive products are independent
 #pragma unroll
-      for (int n = 0; n < KC / 8; ++n)
+      for (int n = 0; n < NR; ++n) {
+        uint2 q[3];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const uint4 *xh = ah[mt], *xl = al[mt];
-          mma_tf32(s3[0][mt][n], xl[0].x, xl[1].x, xl[0].y, xl[1].y, bh[n][0], bh[n][1]);
-          mma_tf32(s3[1][mt][n], xh[0].x, xh[1].x, xh[0].y, xh[1].y, bl[n][0], bl[n][1]);
-          mma_tf32(s[mt][n], xh[0].x, xh[1].x, xh[0].y, xh[1].y, bh[n][0], bh[n][1]);
-          mma_tf32(s3[0][mt][n], xl[0].z, xl[1].z, xl[0].w, xl[1].w, bh[n][2], bh[n][3]);
-          mma_tf32(s3[1][mt][n], xh[0].z, xh[1].z, xh[0].w, xh[1].w, bl[n][2], bl[n][3]);
-          mma_tf32(s[mt][n], xh[0].z, xh[1].z, xh[0].w, xh[1].w, bh[n][2], bh[n][3]);
+        for (int k = 0; k < 3; ++k) {
+          if constexpr (QREG)
+            q[k] = qf[ks][k];
+          else
+            q[k] = ldq(k, n, ks);
         }
+        mma16<__nv_bfloat16>(s[n], a[0], q[0].x, q[0].y);
+        mma16<__nv_bfloat16>(sr[n], a[2], q[0].x, q[0].y);
+        mma16<__nv_bfloat16>(sr[n], a[0], q[2].x, q[2].y);
+        mma16<__nv_bfloat16>(sr[n], a[1], q[1].x, q[1].y);
+        mma16<__nv_bfloat16>(sr[n], a[1], q[0].x, q[0].y);
+        mma16<__nv_bfloat16>(sr[n], a[0], q[1].x, q[1].y);
+      }
     }
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int n = 0; n < KC / 8; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s[mt][n][e] += s3[0][mt][n][e] + s3[1][mt][n][e];
     // ---- online softmax (log2 domain); masked and missing keys are -inf
     const bool masked = key0 + KC - 1 > all_see;
     const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int n = 0; n < NR; ++n) {
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int n = 0; n < KC / 8; ++n)
-#pragma unroll
         for (int e = 0; e < 4; ++e) {
-          float x = fmaf(s[mt][n][e], p.scale2, gate);
-          if (masked && key0 + n * 8 + tq * 2 + (e & 1) > qlast[mt][e >> 1]) x = -INFINITY;
-          s[mt][n][e] = x;
-          mx[e >> 1] = fmax_nan(mx[e >> 1], x);
+          float x = fmaf(s[n][e] + sr[n][e], p.scale2, gate);
+          if (masked && key0 + g + 8 * (e >> 1) > qlast[n][e & 1]) x = -INFINITY;
+          s[n][e] = x;
+          mx[e & 1] = fmax_nan(mx[e & 1], x);
         }
-      if (p.logits) {
+      if (lg && r0 + n * 8 < p.R) {  // rows are padded to rpad: whole groups of eight
+        float *lp = lg + (long long)c * KC * p.rpad + n * 8;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = r0 + mt * 16 + g + 8 * h;
-          if (r < p.R) {
-            float *lp = p.logits + ((long long)sp.grpid * p.ncap + (long long)c * KC + tq * 2) * p.rpad + r;
-#pragma unroll
-            for (int n = 0; n < KC / 8; ++n) {
-              lp[(long long)(n * 8) * p.rpad] = s[mt][n][2 * h];
-              lp[(long long)(n * 8 + 1) * p.rpad] = s[mt][n][2 * h + 1];
-            }
-          }
-        }
+          for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<float2 *>(lp + (long long)(8 * h) * p.rpad) =
+                make_float2(s[n][2 * h], s[n][2 * h + 1]);
       }
       float al[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-        mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-        const float mn = fmax_nan(m[mt][h], mx[h]);
-        al[h] = mn == -INFINITY ? 1.f : ex2(m[mt][h] - mn);
-        m[mt][h] = mn;
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
+        const float mn = fmax_nan(m[n][h], mx[h]);
+        al[h] = mn == -INFINITY ? 1.f : ex2(m[n][h] - mn);
+        m[n][h] = mn;
       }
       if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+        l[n][0] *= al[0];
+        l[n][1] *= al[1];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) l[mt][h] *= al[h];
+        for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[mt][n][e] *= al[e >> 1];
+          for (int e = 0; e < 4; ++e) acc[n][ks][e] *= al[e & 1];
       }
-      const float off[2] = {m[mt][0] == -INFINITY ? 0.f : m[mt][0], m[mt][1] == -INFINITY ? 0.f : m[mt][1]};
-#pragma unroll
-      for (int n = 0; n < KC / 8; ++n)
+      const float off[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          s[mt][n][e] = ex2(s[mt][n][e] - off[e >> 1]);
-          l[mt][e >> 1] += s[mt][n][e];
+          s[n][e] = ex2(s[n][e] - off[e & 1]);
+          l[n][e & 1] += s[n][e];
         }
     }
-    // ---- O += P V
+    // ---- O^T += V^T P^T
     if (!mixed) {
+      uint32_t pb[NR][2][3];
 #pragma unroll
-      for (int k8 = 0; k8 < KC / 8; ++k8) {
-        uint32_t ph[MT][4], pl[MT][4];
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          tf32_split(s[mt][k8][0], ph[mt][0], pl[mt][0]);
-          tf32_split(s[mt][k8][2], ph[mt][1], pl[mt][1]);
-          tf32_split(s[mt][k8][1], ph[mt][2], pl[mt][2]);
-          tf32_split(s[mt][k8][3], ph[mt][3], pl[mt][3]);
+        for (int h = 0; h < 2; ++h) {
+          split3(s[n][2 * h], s[n][2 * h + 1], pb[n][h]);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) pb[n][h][k] = movmatrix(pb[n][h][k]);
         }
 #pragma unroll
-        for (int cg = 0; cg < D / 32; ++cg) {
-          const float4 v0 = *reinterpret_cast<const float4 *>(sv + sw_off<4, D>(k8 * 8 + 2 * tq, cg * 8 + g));
-          const float4 v1 = *reinterpret_cast<const float4 *>(sv + sw_off<4, D>(k8 * 8 + 2 * tq + 1, cg * 8 + g));
-          const float x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
+      for (int v = 0; v < VG; ++v) {
+        float x[4][2][VW];  // keys 2t, 2t+1, 2t+8, 2t+9; columns and those 8 VW further
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t h0, l0, h1, l1;
-            tf32_split(x0[e], h0, l0);
-            tf32_split(x1[e], h1, l1);
+        for (int q = 0; q < 4; ++q)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-              float *c = acc[mt][cg * 4 + e];
-              mma_tf32(c, pl[mt][0], pl[mt][1], pl[mt][2], pl[mt][3], h0, h1);
-              mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], l0, l1);
-              mma_tf32(c, ph[mt][0], ph[mt][1], ph[mt][2], ph[mt][3], h0, h1);
-            }
+          for (int h = 0; h < 2; ++h) {
+            const int key = 2 * tq + (q & 1) + (q >> 1) * 8, col = (v * 2 + h) * 8 * VW + VW * g;
+            const uint8_t *at = sv + sw_off<4, D>(key, col >> 2) + (col & 3) * 4;
+            if constexpr (VW == 4)
+              *reinterpret_cast<float4 *>(x[q][h]) = *reinterpret_cast<const float4 *>(at);
+            else
+              *reinterpret_cast<float2 *>(x[q][h]) = *reinterpret_cast<const float2 *>(at);
+          }
+#pragma unroll
+        for (int e = 0; e < VW; ++e) {
+          uint32_t a[3][4], u[3];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            split3(x[0][h][e], x[1][h][e], u);
+            a[0][h] = u[0], a[1][h] = u[1], a[2][h] = u[2];
+            split3(x[2][h][e], x[3][h][e], u);
+            a[0][2 + h] = u[0], a[1][2 + h] = u[1], a[2][2 + h] = u[2];
+          }
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            float *o = acc[n][v * VW + e];
+            mma16<__nv_bfloat16>(o, a[2], pb[n][0][0], pb[n][1][0]);
+            mma16<__nv_bfloat16>(o, a[0], pb[n][0][2], pb[n][1][2]);
+            mma16<__nv_bfloat16>(o, a[1], pb[n][0][1], pb[n][1][1]);
+            mma16<__nv_bfloat16>(o, a[1], pb[n][0][0], pb[n][1][0]);
+            mma16<__nv_bfloat16>(o, a[0], pb[n][0][1], pb[n][1][1]);
+            mma16<__nv_bfloat16>(o, a[0], pb[n][0][0], pb[n][1][0]);
           }
         }
       }
     } else {
       // P through the chunk's K buffer (its reads are done), then key by key
       __syncwarp();
-      float *sp_ = reinterpret_cast<float *>(wring + st * C::STAGE);  // [ROWS][KC]
+      float *sp_ = reinterpret_cast<float *>(wring + st * C::STAGE);  // [KC][ROWS]
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
+      for (int n = 0; n < NR; ++n)
 #pragma unroll
-        for (int n = 0; n < KC / 8; ++n)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            sp_[(mt * 16 + g + 8 * (e >> 1)) * KC + n * 8 + tq * 2 + (e & 1)] = s[mt][n][e];
+        for (int e = 0; e < 4; ++e) sp_[(g + 8 * (e >> 1)) * ROWS + n * 8 + 2 * tq + (e & 1)] = s[n][e];
       __syncwarp();
 #pragma unroll 1
       for (int k = 0; k < KC && key0 + k < len; ++k) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          const float pa = sp_[(mt * 16 + g) * KC + k], pb = sp_[(mt * 16 + g + 8) * KC + k];
+        for (int n = 0; n < NR; ++n) {
+          const float2 pk = *reinterpret_cast<const float2 *>(sp_ + k * ROWS + n * 8 + 2 * tq);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            // this thread's two columns of tile n
-            const int ch = (n >> 2) * 8 + 2 * tq;
-            const float v0 = *reinterpret_cast<const float *>(sv + sw_off<4, D>(k, ch) + (n & 3) * 4);
-            const float v1 = *reinterpret_cast<const float *>(sv + sw_off<4, D>(k, ch + 1) + (n & 3) * 4);
-            if (pa != 0.f) {
-              acc[mt][n][0] = fmaf(pa, v0, acc[mt][n][0]);
-              acc[mt][n][1] = fmaf(pa, v1, acc[mt][n][1]);
+          for (int ks = 0; ks < KS; ++ks) {
+            const int c0 = (ks / VW) * 16 * VW + VW * g + ks % VW, c1 = c0 + 8 * VW;
+            const float v0 = *reinterpret_cast<const float *>(sv + sw_off<4, D>(k, c0 >> 2) + (c0 & 3) * 4);
+            const float v1 = *reinterpret_cast<const float *>(sv + sw_off<4, D>(k, c1 >> 2) + (c1 & 3) * 4);
+            if (pk.x != 0.f) {
+              acc[n][ks][0] = fmaf(pk.x, v0, acc[n][ks][0]);
+              acc[n][ks][2] = fmaf(pk.x, v1, acc[n][ks][2]);
             }
-            if (pb != 0.f) {
-              acc[mt][n][2] = fmaf(pb, v0, acc[mt][n][2]);
-              acc[mt][n][3] = fmaf(pb, v1, acc[mt][n][3]);
+            if (pk.y != 0.f) {
+              acc[n][ks][1] = fmaf(pk.y, v0, acc[n][ks][1]);
+              acc[n][ks][3] = fmaf(pk.y, v1, acc[n][ks][3]);
             }
           }
         }
       }
-      __syncwarp();
     }
+    __syncwarp();
     if (++st == NST) st = 0;
   }
 
   // ---- join the four warps
   cp_wait<0>();
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
-      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
-      if (tq == 0) {
-        s_m[warp][mt * 16 + g + 8 * h] = m[mt][h];
-        s_l[warp][mt * 16 + g + 8 * h] = l[mt][h];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], o);
+      if (g == 0) {
+        s_m[warp][n * 8 + 2 * tq + h] = m[n][h];
+        s_l[warp][n * 8 + 2 * tq + h] = l[n][h];
       }
     }
   __syncthreads();
-  float *so = reinterpret_cast<float *>(ring);  // [warp][ROWS][D]
+  float *so = reinterpret_cast<float *>(ring);  // [warp][ROWS][SO]; SO: rows 2t apart in banks
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+  for (int n = 0; n < NR; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = mt * 16 + g + 8 * h;
+      const int r = n * 8 + 2 * tq + h;
       float M = s_m[0][r];
 #pragma unroll
       for (int w = 1; w < NW; ++w) M = fmax_nan(M, s_m[w][r]);
-      const float f = m[mt][h] == -INFINITY ? 0.f : ex2(m[mt][h] - M);
-      float *op = so + (warp * ROWS + r) * D + tq * 8;
+      const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - M);
+      float *op = so + (warp * ROWS + r) * SO + VW * g;
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        op[(n >> 2) * 32 + (n & 3)] = acc[mt][n][2 * h] * f;
-        op[(n >> 2) * 32 + 4 + (n & 3)] = acc[mt][n][2 * h + 1] * f;
+      for (int ks = 0; ks < KS; ++ks) {
+        op[(ks / VW) * 16 * VW + ks % VW] = acc[n][ks][h] * f;
+        op[(ks / VW) * 16 * VW + 8 * VW + ks % VW] = acc[n][ks][2 + h] * f;
       }
     }
   __syncthreads();
-  split_write<D, ROWS, D>(p, sp, so, s_m, s_l);
+  split_write<D, ROWS, SO>(p, sp, so, s_m, s_l);
   if (last) pdl_wait();
 }
 
@@ -1122,14 +1131,14 @@ template <typename T, int D, int ROWS>
 static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream_t st) {
   using C = SplitCfg<T, D>;
   const int rtiles = (p.R + ROWS - 1) / ROWS;
-  const int base = ROWS * D * C::ES * (C::ES == 4 ? 2 : 1) + C::RING, most = base + 3 * kMaxLive * 4;
+  const int base = ROWS * D * (C::ES == 4 ? 6 : 2) + C::RING, most = base + 3 * kMaxLive * 4;
   static_assert(C::RING >= NW * ROWS * (D + 4) * 4, "the ring holds the warps' O for the join");
   static_assert(C::KC * D * C::ES >= ROWS * C::KC * 4, "a chunk's K buffer holds its P");
   void (*kern)(const SplitParams, int, int);
   if constexpr (C::ES == 2)
     kern = split_mma_kernel<T, D, ROWS / 8>;
   else
-    kern = split_f32_kernel<D, ROWS / 16>;
+    kern = split_f32_kernel<D, ROWS / 8>;
   static std::atomic<uint64_t> done{0};
   allow_smem(reinterpret_cast<const void *>(kern), most, done);
   const dim3 grid((unsigned)(groups * rtiles), p.nsplit);
@@ -1144,8 +1153,7 @@ static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream
 template <typename T, int D>
 static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStream_t st) {
   const int rows = split_rows<T, D>(p.R);
-  if constexpr (sizeof(T) == 2)
-    if (rows == 8) return launch_rows<T, D, 8>(p, groups, st);
+  if (rows == 8) return launch_rows<T, D, 8>(p, groups, st);
   if constexpr (SplitCfg<T, D>::MAXROWS == 32)
     if (rows == 32) return launch_rows<T, D, 32>(p, groups, st);
   return launch_rows<T, D, 16>(p, groups, st);

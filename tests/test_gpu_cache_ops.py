@@ -3,8 +3,8 @@
 
 Tolerances.  A logit of the kernels is a dot product of D exact products in fp32; at
 most n = 8 + D/8 roundings of 2^-23 (the tensor cores truncate) touch a partial sum,
-none of which exceeds |q||k| (fp32 operands: three tf32 products for every eight dims,
-3D/8 roundings, and 2^-21 of |q||k| in dropped terms, n = 8 + 3D/8), so in natural units it is off by at most
+none of which exceeds |q||k| (fp32 operands: six bf16 products for every sixteen dims,
+3D/8 roundings, and 2^-23 of |q||k| in dropped terms, n = 8 + 3D/8), so in natural units it is off by at most
 d = n 2^-23 |q||k| scale; the offset, the base change and ex2 add at most 2^-18 to the
 exponent's effect for logits up to 2^5.  A softmax weight is then off by a factor within
 1 +- e, e = 2 d + 2^-18, and with sum p = 1 the output by at most 2 e max|v| plus 2^-15
