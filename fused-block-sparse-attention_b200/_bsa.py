@@ -569,16 +569,14 @@ def decode(q, k, v, sel, gate=None, *, bs, L=None, mask_mode=MASK_TOKEN, scale=N
 
 
 def _same_device(names, first, *ts):
-    """Every tensor given (None: absent) lives on first's CUDA device.  Returns its index."""
+    """Raises unless every tensor given (None: absent) lives on first's CUDA device."""
     dev = first.get_device()
     if dev < 0:
         _need_cuda(first)
-    for i, t in enumerate(ts):
+    for name, t in zip(names, ts):
         if t is not None and t.get_device() != dev:
             _need_cuda(t)
-            raise BsaShapeError(ERR_ARG, "%s is on %s, the first operand on %s" %
-                                (names[i], t.device, first.device))
-    return dev
+            raise BsaShapeError(ERR_ARG, "%s is on %s, the first operand on %s" % (name, t.device, first.device))
 
 
 def _cache_operand(t, name, shape, st, B, Hkv, D, dtype):
@@ -594,26 +592,30 @@ def _cache_operand(t, name, shape, st, B, Hkv, D, dtype):
 def _row_operand(t, name, B, Hkv, n, dtype):
     """Strides of a (B, Hkv, >= n) per-slot tensor with unit stride along the slots."""
     shape, st = t.shape, t.stride()
+    if len(shape) == 3 and shape[0] == B and shape[1] == Hkv and shape[2] >= n and t.dtype is dtype and \
+            (st[2] == 1 or shape[2] <= 1):
+        return st
     if len(shape) != 3 or shape[0] != B or shape[1] != Hkv or shape[2] < n:
         raise BsaShapeError(ERR_SHAPE, "%s must be (%d, %d, >= %d); got %s" % (name, B, Hkv, n, tuple(shape)))
     if t.dtype != dtype:
         raise BsaError(ERR_DTYPE, "%s must be %s; got %s" % (name, dtype, t.dtype))
-    if shape[2] > 1 and st[2] != 1:
-        raise BsaError(ERR_STRIDE, "%s must have unit stride along the slots" % name)
-    return st
+    raise BsaError(ERR_STRIDE, "%s must have unit stride along the slots" % name)
 
 
-def _query_out(q, out):
-    """(q with unit stride along D, o) of a decode step."""
-    if q.dim() != 4:
+def _query_out(q, shape, out):
+    """(q with unit stride along D, its strides, o, o's strides) of a decode step."""
+    if len(shape) != 4:
         raise BsaShapeError(ERR_SHAPE, "q must be (B, Hq, T, D)")
-    if q.stride(3) != 1:
+    st = q.stride()
+    if st[3] != 1:
         q = q.contiguous()
+        st = q.stride()
     if out is None:
-        return q, torch.empty_like(q, memory_format=torch.contiguous_format)
-    if out.shape != q.shape or out.dtype != q.dtype or out.stride(3) != 1:
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+        return q, st, o, o.stride()
+    if out.shape != shape or out.dtype != q.dtype or out.stride(3) != 1:
         raise BsaShapeError(ERR_SHAPE, "out must have q's shape and dtype and unit stride along D")
-    return q, out
+    return q, st, out, out.stride()
 
 
 def _format(cls):
@@ -625,6 +627,7 @@ def _format(cls):
 
 _PACK = {"bsa_decode_weighted": _format(DecodeWeightedArgs), "bsa_evict": _format(EvictArgs),
          "bsa_decode_prefix": _format(DecodePrefixArgs)}
+_pack_weighted, _pack_evict, _pack_prefix = (_PACK[n].pack for n in _PACK)
 _packed_fn = {}
 
 # the current stream's handle without the Stream object (3 us a call)
@@ -632,24 +635,25 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda dev: torch.cuda.current_stream(dev).cuda_stream)
 
 
-def _launch(name, packed, dev):
-    """Workspace and launch of entry point `name` (its argument struct as bytes) on CUDA
-    device `dev` and its current stream."""
+def _launch(name, packed, like):
+    """Workspace and launch of entry point `name` (its argument struct as bytes) on the
+    CUDA device of `like` and its current stream."""
+    dev = like.get_device()
     if dev != torch.cuda.current_device():
         with torch.cuda.device(dev):
-            return _launch(name, packed, dev)
-    if name not in _packed_fn:
+            return _launch(name, packed, like)
+    fn = _packed_fn.get(name)
+    if fn is None:
         run, size = lib()[name], lib()[name + "_workspace"]
         run.restype, size.restype = ctypes.c_int, ctypes.c_size_t
         run.argtypes = [ctypes.c_char_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]
         size.argtypes = [ctypes.c_char_p]
-        _packed_fn[name] = run, size
-    run, size = _packed_fn[name]
-    nbytes = size(packed)
+        fn = _packed_fn[name] = run, size
+    nbytes = fn[1](packed)
     if nbytes == 0:   # validation failed: the call reports why
-        _check(run(packed, None, 0, None))
-    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-    st = run(packed, ws.data_ptr(), nbytes, _raw_stream(dev))
+        _check(fn[0](packed, None, 0, None))
+    ws = like.new_empty(nbytes >> 1)    # at least nbytes: no element is smaller than two
+    st = fn[0](packed, ws.data_ptr(), nbytes, _raw_stream(dev))
     if st:
         _check(st)
 
@@ -661,14 +665,20 @@ def decode_weighted(q, k, v, weight, sel=None, gate=None, *, bs=None, L=None, sc
     sum over hk's query heads and the T rows of their softmax weight on slot j.
     sel: int32 (B, kk) or (B, 1 or Hkv, kk) ids of blocks of bs slots (None: every
     slot), TOKEN masks; gate: optional fp32 like sel.  Returns o (B, Hq, T, D)."""
-    dev = _same_device(("k", "v", "weight", "sel", "gate", "out"), q, k, v, weight, sel, gate, out)
-    q, o = _query_out(q, out)
-    B, Hq, T, D = q.shape
+    dev = q.get_device()
+    if dev < 0 or not (k.get_device() == v.get_device() == weight.get_device() == dev) or \
+            sel is not None or out is not None:
+        _same_device(("k", "v", "weight", "sel", "gate", "out"), q, k, v, weight, sel, gate, out)
+    shape, dt = q.shape, q.dtype
+    q, qst, o, ost = _query_out(q, shape, out)
+    B, Hq, T, D = shape
     ks, vs, kst, vst = k.shape, v.shape, k.stride(), v.stride()
-    Hkv, dt = ks[1] if len(ks) == 4 else -1, q.dtype
-    _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
-    _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
-    cap = min(ks[2], vs[2])
+    if ks != vs or len(ks) != 4 or ks[0] != B or ks[3] != D or kst[3] != 1 or vst[3] != 1 or \
+            k.dtype is not dt or v.dtype is not dt:   # what is wrong, or only an unequal room
+        Hkv = ks[1] if len(ks) == 4 else -1
+        _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
+        _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
+    Hkv, cap = ks[1], min(ks[2], vs[2])
     L = cap if L is None else int(L)
     if L > cap:
         raise BsaShapeError(ERR_SHAPE, "decode_weighted: L = %d is more than k and v hold" % L)
@@ -694,10 +704,11 @@ def decode_weighted(q, k, v, weight, sel=None, gate=None, *, bs=None, L=None, sc
             g_ptr, g_sb, g_sh = gate.data_ptr(), gst[0], gst[1] if s_sh or (len(ss) == 3 and ss[1] > 1) else 0
     elif gate is not None:
         raise BsaShapeError(ERR_ARG, "decode_weighted: a gate needs a selection")
-    _launch("bsa_decode_weighted", _PACK["bsa_decode_weighted"].pack(
+    _launch("bsa_decode_weighted", _pack_weighted(
         _dtype(q), B, Hq, Hkv, L, D, bs if sel is not None else 0, T, kk, D ** -0.5 if scale is None else scale,
-        q.data_ptr(), *q.stride()[:3], k.data_ptr(), *kst[:3], v.data_ptr(), *vst[:3], o.data_ptr(),
-        *o.stride()[:3], s_ptr, s_sb, s_sh, g_ptr, g_sb, g_sh, weight.data_ptr(), wst[0], wst[1], status), dev)
+        q.data_ptr(), qst[0], qst[1], qst[2], k.data_ptr(), kst[0], kst[1], kst[2],
+        v.data_ptr(), vst[0], vst[1], vst[2], o.data_ptr(), ost[0], ost[1], ost[2],
+        s_ptr, s_sb, s_sh, g_ptr, g_sb, g_sh, weight.data_ptr(), wst[0], wst[1], status), q)
     return o
 
 
@@ -711,15 +722,19 @@ def evict(k, v, weight, pos, *, budget, L=None, seen=None, recent=0, sink=0, kmi
     weight / pos follow (into weight_out / pos_out when given), and kmin / kmax (fp32
     (B, Hkv, >= ceil(budget / bs), D), both or none) of the changed blocks of bs slots
     are pooled anew."""
-    dev = _same_device(("v", "weight", "pos", "kmin", "kmax", "weight_out", "pos_out"), k, v, weight, pos,
-                       kmin, kmax, weight_out, pos_out)
-    ks, vs, kst, vst = k.shape, v.shape, k.stride(), v.stride()
+    dev = k.get_device()
+    if dev < 0 or not (v.get_device() == weight.get_device() == pos.get_device() == dev) or \
+            weight_out is not None or kmin is not None:
+        _same_device(("v", "weight", "pos", "kmin", "kmax", "weight_out", "pos_out"), k, v, weight, pos,
+                     kmin, kmax, weight_out, pos_out)
+    ks, vs, kst, vst, dt = k.shape, v.shape, k.stride(), v.stride(), k.dtype
     if len(ks) != 4:
         raise BsaShapeError(ERR_SHAPE, "k must be (B, Hkv, >= L, D)")
     B, Hkv, cap, D = ks
-    _cache_operand(k, "k", ks, kst, B, Hkv, D, k.dtype)
-    _cache_operand(v, "v", vs, vst, B, Hkv, D, k.dtype)
-    cap = min(cap, vs[2])
+    if ks != vs or kst[3] != 1 or vst[3] != 1 or v.dtype is not dt:
+        _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
+        _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
+        cap = min(cap, vs[2])
     L = cap if L is None else int(L)
     if L > cap:
         raise BsaShapeError(ERR_SHAPE, "evict: L = %d is more than k and v hold" % L)
@@ -729,6 +744,8 @@ def evict(k, v, weight, pos, *, budget, L=None, seen=None, recent=0, sink=0, kmi
                                        "within the budget")
     if bs is not None and not 0 < bs <= 1024:
         raise BsaShapeError(ERR_SHAPE, "evict: bs must lie in 1 .. 1024")
+    if pos_out is not None and pos_out.get_device() != dev:
+        _same_device(("pos_out",), k, pos_out)
     wst = _row_operand(weight, "weight", B, Hkv, L, torch.float32)
     pst = _row_operand(pos, "pos", B, Hkv, L, torch.int32)
     wo, wost, po, post = weight, wst, pos, pst
@@ -741,20 +758,18 @@ def evict(k, v, weight, pos, *, budget, L=None, seen=None, recent=0, sink=0, kmi
     if kmin is not None and kmax is not None:
         if bs is None:
             raise BsaShapeError(ERR_ARG, "evict: kmin and kmax need bs")
-        kmst = kmin.stride()
-        for name, t in (("kmin", kmin), ("kmax", kmax)):
-            s, st = t.shape, t.stride()
-            _cache_operand(t, name, s, st, B, Hkv, D, torch.float32)
-            if s[2] * bs < budget or st != kmst:
-                raise BsaShapeError(ERR_SHAPE, "evict: kmin and kmax need one layout and ceil(budget / bs) blocks")
+        kmst, s = kmin.stride(), kmin.shape
+        _cache_operand(kmin, "kmin", s, kmst, B, Hkv, D, torch.float32)
+        if kmax.shape != s or kmax.dtype is not torch.float32 or s[2] * bs < budget or kmax.stride() != kmst:
+            raise BsaShapeError(ERR_SHAPE, "evict: kmin and kmax need one layout and ceil(budget / bs) blocks")
         km, kx = kmin.data_ptr(), kmax.data_ptr()
     elif kmin is not None or kmax is not None:
         raise BsaShapeError(ERR_ARG, "evict: kmin and kmax go together")
-    _launch("bsa_evict", _PACK["bsa_evict"].pack(
+    _launch("bsa_evict", _pack_evict(
         _dtype(k), B, Hkv, L, D, 64 if bs is None else bs, budget, recent, sink, seen,
-        k.data_ptr(), *kst[:3], v.data_ptr(), *vst[:3], weight.data_ptr(), wst[0], wst[1],
-        pos.data_ptr(), pst[0], pst[1], wo.data_ptr(), wost[0], wost[1], po.data_ptr(), post[0], post[1],
-        km, kx, *kmst[:3]), dev)
+        k.data_ptr(), kst[0], kst[1], kst[2], v.data_ptr(), vst[0], vst[1], vst[2],
+        weight.data_ptr(), wst[0], wst[1], pos.data_ptr(), pst[0], pst[1],
+        wo.data_ptr(), wost[0], wost[1], po.data_ptr(), post[0], post[1], km, kx, kmst[0], kmst[1], kmst[2]), k)
 
 
 def decode_prefix(q, pk, pv, k, v, lens, *, scale=None, out=None):
@@ -762,28 +777,34 @@ def decode_prefix(q, pk, pv, k, v, lens, *, scale=None, out=None):
     pk, pv (Hkv, P, D): the prefix, read once for the batch; k, v (B, Hkv, S, D): each
     sequence's own slots, lens int32 (B,) of them in use, the T new tokens last.  Row t
     sees the prefix and the own slots j <= lens[b] - T + t.  Returns o (B, Hq, T, D)."""
-    dev = _same_device(("pk", "pv", "k", "v", "lens", "out"), q, pk, pv, k, v, lens, out)
-    q, o = _query_out(q, out)
-    B, Hq, T, D = q.shape
+    dev = q.get_device()
+    if dev < 0 or out is not None or not (pk.get_device() == pv.get_device() == k.get_device() == v.get_device() ==
+                                          lens.get_device() == dev):
+        _same_device(("pk", "pv", "k", "v", "lens", "out"), q, pk, pv, k, v, lens, out)
+    shape, dt = q.shape, q.dtype
+    q, qst, o, ost = _query_out(q, shape, out)
+    B, Hq, T, D = shape
     ks, vs, ps, kst, vst, pkst, pvst = k.shape, v.shape, pk.shape, k.stride(), v.stride(), pk.stride(), pv.stride()
     if len(ks) != 4 or len(ps) != 3 or pv.shape != ps:
         raise BsaShapeError(ERR_SHAPE, "decode_prefix: k, v must be (B, Hkv, S, D) and pk, pv (Hkv, P, D)")
-    Hkv, S, dt = ks[1], ks[2], q.dtype
-    _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
-    _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
-    if vs[2] != S:
-        raise BsaShapeError(ERR_SHAPE, "decode_prefix: k and v hold different numbers of slots")
-    _cache_operand(pk, "pk", (1, *ps), (0, *pkst), 1, Hkv, D, dt)
-    _cache_operand(pv, "pv", (1, *ps), (0, *pvst), 1, Hkv, D, dt)
-    if lens.dim() != 1 or lens.shape[0] != B or lens.is_floating_point():
+    Hkv, S = ks[1], ks[2]
+    if ks != vs or ks[0] != B or ks[3] != D or ps[0] != Hkv or ps[2] != D or kst[3] != 1 or vst[3] != 1 or \
+            pkst[2] != 1 or pvst[2] != 1 or not (k.dtype is v.dtype is pk.dtype is pv.dtype is dt):
+        _cache_operand(k, "k", ks, kst, B, Hkv, D, dt)
+        _cache_operand(v, "v", vs, vst, B, Hkv, D, dt)
+        if vs[2] != S:
+            raise BsaShapeError(ERR_SHAPE, "decode_prefix: k and v hold different numbers of slots")
+        _cache_operand(pk, "pk", (1, *ps), (0, *pkst), 1, Hkv, D, dt)
+        _cache_operand(pv, "pv", (1, *ps), (0, *pvst), 1, Hkv, D, dt)
+    if lens.shape != (B,) or lens.is_floating_point():
         raise BsaShapeError(ERR_SHAPE, "decode_prefix: lens must be (B,) whole numbers")
-    if lens.dtype != torch.int32 or not lens.is_contiguous():
+    if lens.dtype is not torch.int32 or not lens.is_contiguous():
         lens = lens.to(torch.int32).contiguous()
-    _launch("bsa_decode_prefix", _PACK["bsa_decode_prefix"].pack(
+    _launch("bsa_decode_prefix", _pack_prefix(
         _dtype(q), B, Hq, Hkv, D, ps[1], S, T, D ** -0.5 if scale is None else scale,
-        q.data_ptr(), *q.stride()[:3], pk.data_ptr(), 0, pkst[0], pkst[1], pv.data_ptr(), 0, pvst[0], pvst[1],
-        k.data_ptr(), *kst[:3], v.data_ptr(), *vst[:3], o.data_ptr(), *o.stride()[:3], lens.data_ptr(),
-        status_tensor(dev).data_ptr()), dev)
+        q.data_ptr(), qst[0], qst[1], qst[2], pk.data_ptr(), 0, pkst[0], pkst[1], pv.data_ptr(), 0, pvst[0], pvst[1],
+        k.data_ptr(), kst[0], kst[1], kst[2], v.data_ptr(), vst[0], vst[1], vst[2],
+        o.data_ptr(), ost[0], ost[1], ost[2], lens.data_ptr(), status_tensor(dev).data_ptr()), q)
     return o
 
 

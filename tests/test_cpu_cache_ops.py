@@ -129,7 +129,7 @@ def bsa(monkeypatch):
     structs = {"bsa_decode_weighted": _bsa.DecodeWeightedArgs, "bsa_evict": _bsa.EvictArgs,
                "bsa_decode_prefix": _bsa.DecodePrefixArgs}
     monkeypatch.setattr(_bsa, "_launch",
-                        lambda name, a, dev: calls.append((name, structs[name].from_buffer_copy(a))))
+                        lambda name, a, like: calls.append((name, structs[name].from_buffer_copy(a))))
     _bsa.test_calls = calls
     return _bsa
 
