@@ -5,12 +5,16 @@
 //   split_join_kernel   joins the splits of every row; with weights, also adds the sum
 //                       over the rows of p = 2^(x - lse) to each slot's sum
 // The kernels are bound by reading K and V once (HBM).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
 
 #include "bsa_host.h"
 #include "bsa_split.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace bsa {
 
@@ -148,14 +152,14 @@ __device__ __forceinline__ uint32_t sw_off(int row, int chunk) {
     return row * (D * 4) + ((chunk ^ ((row & 6) ^ ((row & 1) << 2))) << 4);
 }
 
-// What a CTA works on.
+// What a CTA works on; chunks [0, nch2) are those of the shared keys (one launch only).
 struct Span {
-  int b, hk, grpid, r0, len, c_lo, c_hi, split;
+  int b, hk, grpid, r0, len, nch2, c_lo, c_hi, split;
 };
 
 // Row tile, length, live blocks and chunk range of this CTA.  False: nothing to see
 // (the rows' m is written as -inf and the join skips the split).
-template <int KC, int ROWS>
+template <int KC, int ROWS, bool CL>
 __device__ __forceinline__ bool split_span(const SplitParams &p, int rtiles, int min_chunks, Span &s, int *s_blk,
                                            float *s_gate, int *s_raw, int *s_n) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -187,12 +191,13 @@ __device__ __forceinline__ bool split_span(const SplitParams &p, int rtiles, int
     __syncthreads();
     nv = *s_n * p.bs;
   }
-  const int nch = (nv + KC - 1) / KC;
+  s.nch2 = CL ? (p.n2 + KC - 1) / KC : 0;
+  const int nch = s.nch2 + (nv + KC - 1) / KC;
   const int cps = max(min_chunks, (nch + p.nsplit - 1) / p.nsplit);
   s.c_lo = min(nch, (int)blockIdx.y * cps);
   s.c_hi = min(nch, s.c_lo + cps);
   s.split = p.split0 + blockIdx.y;
-  if (s.c_lo < s.c_hi) return true;
+  if (CL || s.c_lo < s.c_hi) return true;
   for (int r = tid; r < ROWS && s.r0 + r < p.R; r += blockDim.x) {
     int rb, rh, rtt;
     const long long gr = split_row(p, s.b, s.hk, s.r0 + r, rb, rh, rtt);
@@ -299,6 +304,117 @@ __device__ __forceinline__ void mma16(float *c, const uint32_t *a, uint32_t b0, 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// 2^(x - m) f, and 0 where f is: a row that saw nothing or padding, whatever its x holds.
+__device__ __forceinline__ float join_p(float x, float m, float f) { return f == 0.f ? 0.f : ex2(x - m) * f; }
+
+// The join within a cluster, instead of partial sums in memory and a second launch: the
+// CTAs of one (b, hk) hold its splits.  so: this CTA's [warp][ROWS][SO] (scaled to the
+// warps' common maximum).  Each CTA writes its share of o and adds the weights of its own
+// slots, whose logits it wrote itself.
+template <typename T, int KC, int D, int ROWS, int SO>
+__device__ __forceinline__ void cluster_join(const SplitParams &p, const Span &s, float *so, float (*s_m)[ROWS],
+                                             float (*s_l)[ROWS], const int *s_blk) {
+  cg::cluster_group cl = cg::this_cluster();
+  const int cs = cl.num_blocks(), rank = cl.block_rank(), tid = threadIdx.x;
+  __shared__ float s_f[8][ROWS], s_M[ROWS], s_inv[ROWS];
+  // the CTA's own (m, l) and O: warp 0's place takes the sums
+  const int nr = min(ROWS, p.R);
+  float cm = 0.f, cl_ = 0.f;
+  if (tid < ROWS) {
+    cm = s_m[0][tid];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) cm = fmax_nan(cm, s_m[w][tid]);
+#pragma unroll
+    for (int w = 0; w < NW; ++w) cl_ += s_m[w][tid] == -INFINITY ? 0.f : s_l[w][tid] * ex2(s_m[w][tid] - cm);
+  }
+  for (int i = tid; i < nr * (D / 4); i += blockDim.x) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    float4 o = *reinterpret_cast<const float4 *>(so + r * SO + d);
+#pragma unroll
+    for (int w = 1; w < NW; ++w) {
+      const float4 x = *reinterpret_cast<const float4 *>(so + (w * ROWS + r) * SO + d);
+      o.x += x.x, o.y += x.y, o.z += x.z, o.w += x.w;
+    }
+    *reinterpret_cast<float4 *>(so + r * SO + d) = o;
+  }
+  __syncthreads();
+  if (tid < ROWS) {
+    s_m[0][tid] = cm;
+    s_l[0][tid] = cl_;
+  }
+  if (cs > 1)
+    cl.sync();
+  else
+    __syncthreads();
+  if (tid < ROWS) {
+    float m[8], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < cs) {
+        m[c] = cl.map_shared_rank(&s_m[0][0], c)[tid];
+        M = fmax_nan(M, m[c]);
+      }
+#pragma unroll
+    for (int c = 0; c < 8; ++c)
+      if (c < cs) {
+        const float f = m[c] == -INFINITY ? 0.f : ex2(m[c] - M);
+        s_f[c][tid] = f;
+        if (f != 0.f) L = fmaf(cl.map_shared_rank(&s_l[0][0], c)[tid], f, L);
+      }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    s_M[tid] = M;
+    s_inv[tid] = tid < nr ? inv : 0.f;
+  }
+  __syncthreads();
+  for (int i = rank * blockDim.x + tid; i < nr * (D / 4); i += cs * blockDim.x) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < cs; ++c) {
+      const float f = s_f[c][r];
+      if (f == 0.f) continue;  // nothing seen there
+      const float4 x = *reinterpret_cast<const float4 *>(cl.map_shared_rank(so, c) + r * SO + d);
+      o.x = fmaf(x.x, f, o.x), o.y = fmaf(x.y, f, o.y), o.z = fmaf(x.z, f, o.z), o.w = fmaf(x.w, f, o.w);
+    }
+    const float inv = s_inv[r];
+    int rb, rh, rt;
+    split_row(p, s.b, s.hk, r, rb, rh, rt);
+    T *op = reinterpret_cast<T *>(p.o) + rb * p.o_sb + rh * p.o_sh + rt * p.o_sl + d;
+    const float y[4] = {o.x * inv, o.y * inv, o.z * inv, o.w * inv};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 2)
+        op[e] = Mma<T>::from_f(y[e]);
+      else
+        op[e] = y[e];
+    }
+  }
+  if (p.weight) {
+    float *wp = p.weight + s.b * p.w_sb + s.hk * p.w_sh;
+    const float *lg = p.logits + (long long)s.grpid * p.ncap * p.rpad;
+    const int rpad = p.rpad;  // 8, 16 or 32 here
+    for (int j = s.c_lo * KC + tid; j < s.c_hi * KC; j += blockDim.x) {
+      int key = j;
+      if (p.sel) {
+        const int blk = j / p.bs;
+        key = s_blk[blk] * p.bs + (j - blk * p.bs);
+      }
+      if (key >= s.len) continue;
+      const float4 *x = reinterpret_cast<const float4 *>(lg + (long long)j * rpad);
+      const float w0 = wp[key];
+      float w = 0.f;
+      for (int r = 0; r < rpad; r += 8) {
+        const float4 a = x[r / 4], b = x[r / 4 + 1];
+        w += (join_p(a.x, s_M[r], s_inv[r]) + join_p(a.y, s_M[r + 1], s_inv[r + 1])) +
+             (join_p(a.z, s_M[r + 2], s_inv[r + 2]) + join_p(a.w, s_M[r + 3], s_inv[r + 3]));
+        w += (join_p(b.x, s_M[r + 4], s_inv[r + 4]) + join_p(b.y, s_M[r + 5], s_inv[r + 5])) +
+             (join_p(b.z, s_M[r + 6], s_inv[r + 6]) + join_p(b.w, s_M[r + 7], s_inv[r + 7]));
+      }
+      wp[key] = w0 + w;
+    }
+  }
+  if (cs > 1) cl.sync();  // nobody leaves while its O may be read
+}
+
 __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {  // 8x8 of 16 bits, transposed over the warp
   uint32_t d;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
@@ -306,7 +422,7 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t a) {  // 8x8 of 16 bits, 
 }
 
 // ------------------------------------------------------------------ bf16 / f16
-template <typename T, int D, int NR>
+template <typename T, int D, int NR, bool CL>
 __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     split_mma_kernel(const SplitParams p, int rtiles, int min_chunks) {
   using C = SplitCfg<T, D>;
@@ -325,7 +441,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
   const int g = lane >> 2, tq = lane & 3;
   pdl_trigger();  // the join may take its place on the SMs; it waits for this grid
   Span sp;
-  if (!split_span<KC, ROWS>(p, rtiles, min_chunks, sp, s_blk, s_gate, s_blk + 2 * kMaxLive, &s_n)) {
+  if (!split_span<KC, ROWS, CL>(p, rtiles, min_chunks, sp, s_blk, s_gate, s_blk + 2 * kMaxLive, &s_n)) {
     if (last) pdl_wait();
     return;
   }
@@ -335,11 +451,20 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
   uint8_t *wring = ring + warp * NST * C::STAGE;
   const uint32_t wr0 = smem_u32(wring);
   const uint64_t policy = evict_first_policy();
+  const T *k2_ = nullptr, *v2_ = nullptr;  // the shared keys
+  if constexpr (CL) {
+    k2_ = reinterpret_cast<const T *>(p.k2) + sp.hk * p.k2_sh;
+    v2_ = reinterpret_cast<const T *>(p.v2) + sp.hk * p.v2_sh;
+  }
   auto load = [&](int c, int st) {
     if (c < sp.c_hi) {
-      float gt;
-      const int key0 = split_key<KC>(p, s_blk, s_gate, c, gt);
-      split_load<T, D>(kb_, vb_, p.k_sl, p.v_sl, key0, len, wr0 + st * C::STAGE, policy);
+      if (CL && c < sp.nch2) {
+        split_load<T, D>(k2_, v2_, p.k2_sl, p.v2_sl, c * KC, p.n2, wr0 + st * C::STAGE, policy);
+      } else {
+        float gt;
+        const int key0 = split_key<KC>(p, s_blk, s_gate, c - sp.nch2, gt);
+        split_load<T, D>(kb_, vb_, p.k_sl, p.v_sl, key0, len, wr0 + st * C::STAGE, policy);
+      }
     }
     cp_commit();
   };
@@ -390,8 +515,9 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
       load(c + (NST - 1) * NW, nst);
     }
     const uint32_t ka = wr0 + st * C::STAGE, va = ka + KC * D * 2;
-    float gate;
-    const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
+    const bool pre = CL && c < sp.nch2;  // shared keys: every row sees them
+    float gate = 0.f;
+    const int key0 = pre ? c * KC : split_key<KC>(p, s_blk, s_gate, c - sp.nch2, gate);
     // ---- S^T = K Q^T
     float s[KT][NR][4];  // keys g, g + 8 of tile kt; rows 2t, 2t + 1
     constexpr int PS = KT * NR >= 4 ? 1 : 2;  // partial sums over the dims: independent chains
@@ -420,8 +546,8 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[kt][n][e] = PS == 2 ? s2[0][kt][n][e] + s2[PS - 1][kt][n][e] : s2[0][kt][n][e];
     // ---- online softmax (log2 domain); masked and missing keys are -inf
-    const bool masked = key0 + KC - 1 > all_see;
-    const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
+    const bool masked = key0 + KC - 1 > (pre ? p.n2 - 1 : all_see);
+    const bool mixed = !pre && masked && all_see < len - 1;  // some row misses a key that another sees
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       float mx[2] = {-INFINITY, -INFINITY};
@@ -430,7 +556,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = fmaf(s[kt][n][e], p.scale2, gate);
-          if (masked && key0 + kt * 16 + g + 8 * (e >> 1) > qlast[n][e & 1]) x = -INFINITY;
+          if (masked && key0 + kt * 16 + g + 8 * (e >> 1) > (pre ? p.n2 - 1 : qlast[n][e & 1])) x = -INFINITY;
           s[kt][n][e] = x;
           mx[e & 1] = fmax_nan(mx[e & 1], x);
         }
@@ -565,12 +691,16 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
       }
     }
   __syncthreads();
-  split_write<D, ROWS, SO>(p, sp, so, s_m, s_l);
-  if (last) pdl_wait();
+  if constexpr (CL) {
+    cluster_join<T, KC, D, ROWS, SO>(p, sp, so, s_m, s_l, s_blk);
+  } else {
+    split_write<D, ROWS, SO>(p, sp, so, s_m, s_l);
+    if (last) pdl_wait();
+  }
 }
 
 // ------------------------------------------------------------------ fp32
-template <int D, int NR>
+template <int D, int NR, bool CL>
 __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
     split_f32_kernel(const SplitParams p, int rtiles, int min_chunks) {
   using C = SplitCfg<float, D>;
@@ -588,7 +718,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   const int g = lane >> 2, tq = lane & 3;
   pdl_trigger();
   Span sp;
-  if (!split_span<KC, ROWS>(p, rtiles, min_chunks, sp, s_blk, s_gate, s_blk + 2 * kMaxLive, &s_n)) {
+  if (!split_span<KC, ROWS, CL>(p, rtiles, min_chunks, sp, s_blk, s_gate, s_blk + 2 * kMaxLive, &s_n)) {
     if (last) pdl_wait();
     return;
   }
@@ -598,11 +728,20 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   uint8_t *wring = ring + warp * NST * C::STAGE;
   const uint32_t wr0 = smem_u32(wring);
   const uint64_t policy = evict_first_policy();
+  const float *k2_ = nullptr, *v2_ = nullptr;  // the shared keys
+  if constexpr (CL) {
+    k2_ = reinterpret_cast<const float *>(p.k2) + sp.hk * p.k2_sh;
+    v2_ = reinterpret_cast<const float *>(p.v2) + sp.hk * p.v2_sh;
+  }
   auto load = [&](int c, int st) {
     if (c < sp.c_hi) {
-      float gt;
-      const int key0 = split_key<KC>(p, s_blk, s_gate, c, gt);
-      split_load<float, D>(kb_, vb_, p.k_sl, p.v_sl, key0, len, wr0 + st * C::STAGE, policy);
+      if (CL && c < sp.nch2) {
+        split_load<float, D>(k2_, v2_, p.k2_sl, p.v2_sl, c * KC, p.n2, wr0 + st * C::STAGE, policy);
+      } else {
+        float gt;
+        const int key0 = split_key<KC>(p, s_blk, s_gate, c - sp.nch2, gt);
+        split_load<float, D>(kb_, vb_, p.k_sl, p.v_sl, key0, len, wr0 + st * C::STAGE, policy);
+      }
     }
     cp_commit();
   };
@@ -673,8 +812,9 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
       load(c + (NST - 1) * NW, nst);
     }
     const uint8_t *sk = wring + st * C::STAGE, *sv = sk + KC * D * 4;
-    float gate;
-    const int key0 = split_key<KC>(p, s_blk, s_gate, c, gate);
+    const bool pre = CL && c < sp.nch2;  // shared keys: every row sees them
+    float gate = 0.f;
+    const int key0 = pre ? c * KC : split_key<KC>(p, s_blk, s_gate, c - sp.nch2, gate);
     // ---- S^T = K Q^T
     float s[NR][4], sr[NR][4];  // keys g, g + 8; rows 2t, 2t + 1: the leading products, the others
 #pragma unroll
@@ -711,15 +851,15 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
       }
     }
     // ---- online softmax (log2 domain); masked and missing keys are -inf
-    const bool masked = key0 + KC - 1 > all_see;
-    const bool mixed = masked && all_see < len - 1;  // some row misses a key that another sees
+    const bool masked = key0 + KC - 1 > (pre ? p.n2 - 1 : all_see);
+    const bool mixed = !pre && masked && all_see < len - 1;  // some row misses a key that another sees
 #pragma unroll
     for (int n = 0; n < NR; ++n) {
       float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           float x = fmaf(s[n][e] + sr[n][e], p.scale2, gate);
-          if (masked && key0 + g + 8 * (e >> 1) > qlast[n][e & 1]) x = -INFINITY;
+          if (masked && key0 + g + 8 * (e >> 1) > (pre ? p.n2 - 1 : qlast[n][e & 1])) x = -INFINITY;
           s[n][e] = x;
           mx[e & 1] = fmax_nan(mx[e & 1], x);
         }
@@ -868,8 +1008,12 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
       }
     }
   __syncthreads();
-  split_write<D, ROWS, SO>(p, sp, so, s_m, s_l);
-  if (last) pdl_wait();
+  if constexpr (CL) {
+    cluster_join<float, KC, D, ROWS, SO>(p, sp, so, s_m, s_l, s_blk);
+  } else {
+    split_write<D, ROWS, SO>(p, sp, so, s_m, s_l);
+    if (last) pdl_wait();
+  }
 }
 
 // ------------------------------------------------------------------ join
@@ -897,9 +1041,6 @@ constexpr int kJoinThreads = 256;
 // kpb slots of one (b, hk): lse of its R rows from the splits' (m, l), then the sum over
 // the rows of 2^(x - m) / l, eight rows to a lane and LPK lanes to a slot, so that a
 // warp reads whole lines of the logits.
-// 2^(x - m) f, and 0 where f is: a row that saw nothing or padding, whatever its x holds.
-__device__ __forceinline__ float join_p(float x, float m, float f) { return f == 0.f ? 0.f : ex2(x - m) * f; }
-
 template <int LPK, bool SEL>
 __device__ __forceinline__ void join_weights(const JoinParams &p, int bh, int b, int hk, int tile, const float *sj) {
   constexpr int KPW = 32 / LPK, STEP = KPW * (kJoinThreads / 32);  // slots of a warp, of the CTA per step
@@ -1127,7 +1268,7 @@ int split_count(int dtype, int D, long long groups, int R, long long n) {
   }
 }
 
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool CL>
 static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream_t st) {
   using C = SplitCfg<T, D>;
   const int rtiles = (p.R + ROWS - 1) / ROWS;
@@ -1136,44 +1277,75 @@ static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream
   static_assert(C::KC * D * C::ES >= ROWS * C::KC * 4, "a chunk's K buffer holds its P");
   void (*kern)(const SplitParams, int, int);
   if constexpr (C::ES == 2)
-    kern = split_mma_kernel<T, D, ROWS / 8>;
+    kern = split_mma_kernel<T, D, ROWS / 8, CL>;
   else
-    kern = split_f32_kernel<D, ROWS / 8>;
+    kern = split_f32_kernel<D, ROWS / 8, CL>;
   static std::atomic<uint64_t> done{0};
   allow_smem(reinterpret_cast<const void *>(kern), most, done);
   const dim3 grid((unsigned)(groups * rtiles), p.nsplit);
   const int smem = p.sel ? most : base;
-  if (p.after)
+  if constexpr (CL) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(NW * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 1, at.val.clusterDim.y = p.nsplit, at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kern, p, rtiles, NW);
+  } else if (p.after) {
     launch_after(kern, grid, NW * 32, smem, st, p, rtiles, NW);
-  else
+  } else {
     kern<<<grid, NW * 32, smem, st>>>(p, rtiles, NW);
+  }
   return check_launch("split");
 }
 
-template <typename T, int D>
+template <typename T, int D, bool CL>
 static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStream_t st) {
   const int rows = split_rows<T, D>(p.R);
-  if (rows == 8) return launch_rows<T, D, 8>(p, groups, st);
+  if (rows == 8) return launch_rows<T, D, 8, CL>(p, groups, st);
   if constexpr (SplitCfg<T, D>::MAXROWS == 32)
-    if (rows == 32) return launch_rows<T, D, 32>(p, groups, st);
-  return launch_rows<T, D, 16>(p, groups, st);
+    if (rows == 32) return launch_rows<T, D, 32, CL>(p, groups, st);
+  return launch_rows<T, D, 16, CL>(p, groups, st);
 }
 
-template <int D>
+template <int D, bool CL>
 static bsa_status launch_split_d(int dtype, const SplitParams &p, long long groups, cudaStream_t st) {
-  if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D>(p, groups, st);
-  if (dtype == BSA_F16) return launch_mma_d<__half, D>(p, groups, st);
-  return launch_mma_d<float, D>(p, groups, st);
+  if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D, CL>(p, groups, st);
+  if (dtype == BSA_F16) return launch_mma_d<__half, D, CL>(p, groups, st);
+  return launch_mma_d<float, D, CL>(p, groups, st);
 }
 
-bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStream_t st) {
+template <bool CL>
+static bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStream_t st) {
   const long long groups = p.fold ? p.Hkv : (long long)p.B * p.Hkv;
   switch (D) {
-    case 32: return launch_split_d<32>(dtype, p, groups, st);
-    case 64: return launch_split_d<64>(dtype, p, groups, st);
-    case 128: return launch_split_d<128>(dtype, p, groups, st);
-    default: return launch_split_d<256>(dtype, p, groups, st);
+    case 32: return launch_split_d<32, CL>(dtype, p, groups, st);
+    case 64: return launch_split_d<64, CL>(dtype, p, groups, st);
+    case 128: return launch_split_d<128, CL>(dtype, p, groups, st);
+    default: return launch_split_d<256, CL>(dtype, p, groups, st);
   }
+}
+
+// CTAs of the cluster that does a (b, hk) of R rows and n keys in one launch, or 0 where
+// splits and a join are the better way: more rows than a tile, or more than 32 rounds of
+// a CTA's warps in all (four per CTA of a full cluster), unless one CTA per head is what
+// the splits come to.  One launch saves 3 us of the host's time and the partial sums'
+// way through memory; with few heads and many keys eight CTAs per head draw too little
+// of HBM.
+static int cluster_size(int dtype, int D, long long groups, int R, long long n) {
+  const int es = (int)elem_size(dtype), kc = es == 2 && D <= 64 ? 32 : 16;
+  const int most = D == 256 || (es == 2 && D == 32) ? 16 : 32;
+  const long long steps = (n + kc * NW - 1) / (kc * NW);
+  if (R > most) return 0;
+  if (steps > 32) return split_count(dtype, D, groups, R, n) == 1 ? 1 : 0;
+  int cs = 1;
+  while (cs < 8 && cs * 2 <= steps && groups * cs * 2 <= 2 * 148) cs *= 2;
+  return cs;
 }
 
 template <typename T>
@@ -1228,7 +1400,7 @@ static bsa_status check_kv(const bsa_view &v, int dtype, const char *who, const 
 namespace {
 constexpr int kMaxWeightRows = 4096;
 struct WeightedPlan {
-  int nsplit;
+  int cl, nsplit;  // cl: CTAs of a cluster per head (one launch), or 0
   int rpad;
   long long ncap, rows;
   size_t o_po, o_ml, o_lg, o_lv, bytes;
@@ -1237,13 +1409,15 @@ WeightedPlan weighted_plan(const bsa_decode_weighted_args *a) {
   WeightedPlan w;
   const int R = (a->Hq / a->Hkv) * a->T;
   const long long n = a->sel ? (long long)a->kk * a->bs : a->L;
-  w.nsplit = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, n);
+  w.cl = cluster_size(a->dtype, a->D, (long long)a->B * a->Hkv, R, n);
+  w.nsplit = w.cl ? w.cl : split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, n);
   w.ncap = (n + 31) / 32 * 32;
   w.rpad = (R + 7) / 8 * 8;
   w.rows = (long long)a->B * a->Hq * a->T;
+  const size_t parts = w.cl ? 0 : (size_t)w.nsplit * w.rows;
   w.o_po = 0;
-  w.o_ml = align_up((size_t)w.nsplit * w.rows * a->D * 4, 256);
-  w.o_lg = align_up(w.o_ml + (size_t)w.nsplit * w.rows * 8, 256);
+  w.o_ml = align_up(parts * a->D * 4, 256);
+  w.o_lg = align_up(w.o_ml + parts * 8, 256);
   w.o_lv = align_up(w.o_lg + (size_t)a->B * a->Hkv * w.rpad * w.ncap * 4, 256);
   w.bytes = align_up(w.o_lv + (a->sel ? (size_t)a->B * a->Hkv * (1 + a->kk) * 4 : 0), 256);
   return w;
@@ -1299,7 +1473,13 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
   p.rpad = w.rpad;
   p.live = a->sel ? reinterpret_cast<int *>(base + w.o_lv) : nullptr;
   p.status = a->status;
-  if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
+  if (w.cl) {
+    p.live = nullptr;
+    p.o = a->o.ptr, p.o_sb = a->o.sb, p.o_sh = a->o.sh, p.o_sl = a->o.sl;
+    p.weight = a->weight, p.w_sb = a->weight_sb, p.w_sh = a->weight_sh;
+    return launch_split<true>(a->dtype, a->D, p, st);
+  }
+  if (bsa_status s = launch_split<false>(a->dtype, a->D, p, st)) return s;
   JoinParams j{};
   j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
   j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;
@@ -1320,7 +1500,11 @@ int prefix_sm100_splits(const bsa_decode_prefix_args *a);
 bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParams &p, cudaStream_t st);
 
 namespace {
+// Bytes of the prefix read by all sequences together, up to which each reads it for
+// itself: 5 us of L2.
+constexpr long long kAgainBytes = 32 << 20;
 struct PrefixPlan {
+  int cl;      // CTAs of a cluster per (b, hk) (one launch), or 0
   bool tc;     // the prefix on the tensor-memory kernel
   int np, ns;  // splits of the prefix and of the own slots
   long long rows;
@@ -1329,12 +1513,16 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(const bsa_decode_prefix_args *a) {
   PrefixPlan w;
   const int R = (a->Hq / a->Hkv) * a->T;
-  w.tc = prefix_sm100_applicable(a);
+  // a small step: every sequence reads the prefix for itself (from L2 but once), in one launch
+  const long long groups = (long long)a->B * a->Hkv, again = groups * a->P * a->D * 2 * (long long)elem_size(a->dtype);
+  w.cl = again <= kAgainBytes ? cluster_size(a->dtype, a->D, groups, R, (long long)a->P + a->S) : 0;
+  w.tc = !w.cl && prefix_sm100_applicable(a);
   w.np = w.tc ? prefix_sm100_splits(a) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P) : 0;
   w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S);
   w.rows = (long long)a->B * a->Hq * a->T;
-  w.o_ml = align_up((size_t)(w.np + w.ns) * w.rows * a->D * 4, 256);
-  w.bytes = align_up(w.o_ml + (size_t)(w.np + w.ns) * w.rows * 8, 256);
+  const size_t parts = w.cl ? 0 : (size_t)(w.np + w.ns) * w.rows;
+  w.o_ml = align_up(parts * a->D * 4, 256);
+  w.bytes = align_up(w.o_ml + parts * 8 + 256, 256);
   return w;
 }
 }  // namespace
@@ -1369,14 +1557,20 @@ bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes
   p.po = reinterpret_cast<float *>(base);
   p.pml = reinterpret_cast<float2 *>(base + w.o_ml);
   p.status = a->status;
-  if (a->P > 0) {
+  if (w.cl) {
+    p.k2 = a->pk.ptr, p.k2_sh = a->pk.sh, p.k2_sl = a->pk.sl;
+    p.v2 = a->pv.ptr, p.v2_sh = a->pv.sh, p.v2_sl = a->pv.sl;
+    p.n2 = a->P;
+    p.o = a->o.ptr, p.o_sb = a->o.sb, p.o_sh = a->o.sh, p.o_sl = a->o.sl;
+  } else if (a->P > 0) {
     p.k = a->pk.ptr, p.k_sb = 0, p.k_sh = a->pk.sh, p.k_sl = a->pk.sl;
     p.v = a->pv.ptr, p.v_sb = 0, p.v_sh = a->pv.sh, p.v_sl = a->pv.sl;
     p.fold = 1;
     p.R = a->B * p.grp * a->T;
     p.nkeys = a->P;
     p.split0 = 0, p.nsplit = w.np;
-    if (bsa_status s = w.tc ? launch_prefix_sm100(a, p, st) : launch_split(a->dtype, a->D, p, st)) return s;
+    if (bsa_status s = w.tc ? launch_prefix_sm100(a, p, st) : launch_split<false>(a->dtype, a->D, p, st))
+      return s;
   }
   p.k = a->k.ptr, p.k_sb = a->k.sb, p.k_sh = a->k.sh, p.k_sl = a->k.sl;
   p.v = a->v.ptr, p.v_sb = a->v.sb, p.v_sh = a->v.sh, p.v_sl = a->v.sl;
@@ -1385,9 +1579,13 @@ bsa_status run_prefix(const bsa_decode_prefix_args *a, void *ws, size_t ws_bytes
   p.nkeys = a->S;
   p.lens = a->lens;
   p.causal = 1;
+  if (w.cl) {
+    p.nsplit = w.cl;
+    return launch_split<true>(a->dtype, a->D, p, st);
+  }
   p.split0 = w.np, p.nsplit = w.ns;
   p.after = a->P > 0;
-  if (bsa_status s = launch_split(a->dtype, a->D, p, st)) return s;
+  if (bsa_status s = launch_split<false>(a->dtype, a->D, p, st)) return s;
   JoinParams j{};
   j.o = a->o.ptr, j.o_sb = a->o.sb, j.o_sh = a->o.sh, j.o_sl = a->o.sl;
   j.B = a->B, j.Hq = a->Hq, j.Hkv = a->Hkv, j.grp = p.grp, j.T = a->T, j.D = a->D;

@@ -37,6 +37,15 @@ struct SplitParams {
   long long ncap;
   int rpad;             // rows padded to a multiple of 8
   int *live;            // with sel and logits: [b*Hkv + hk][1 + kk] count and live block ids
+  // One launch (a cluster per (b, hk) joins its own splits): keys before the own ones,
+  // shared by the batch and seen by every row, the output, and the running sums.
+  const void *k2, *v2;
+  int64_t k2_sh, k2_sl, v2_sh, v2_sl;
+  int n2;
+  void *o;
+  int64_t o_sb, o_sh, o_sl;
+  float *weight;        // optional, with logits
+  int64_t w_sb, w_sh;
   int after;            // launched beside the kernel before it, whose end it waits for at its own
   int32_t *status;
 };

@@ -128,6 +128,10 @@ def _check_weighted(q, k, v, w, sel, gate, bs, L, scale=None):
     ("bf16", 128, 1, 8, 1, 20, 20), ("f32", 64, 1, 8, 2, 16, 16), ("bf16", 256, 1, 8, 2, 300, 7),
     ("f16", 64, 1, 2, 2, 17, 2), ("f32", 128, 1, 64, 1, 40, 3), ("bf16", 64, 1, 4, 4, 32, 32),
     ("f16", 128, 1, 8, 8, 9001, 1), ("f32", 256, 1, 1, 1, 1, 1),
+    # beyond one cluster: splits and their join
+    ("bf16", 64, 1, 40, 2, 5000, 1), ("f32", 128, 1, 24, 2, 2500, 3), ("f32", 32, 1, 40, 1, 3000, 1),
+    ("bf16", 256, 1, 24, 1, 2100, 2), ("f16", 32, 2, 6, 2, 4200, 3), ("f32", 256, 1, 2, 1, 2100, 1),
+    ("f32", 64, 1, 80, 1, 2200, 1), ("bf16", 128, 40, 8, 8, 2100, 1),
 ])
 def test_weighted_every_slot(cuda, dtype, D, B, Hq, Hkv, L, T):
     q, k, v, w, _, _ = _weighted_case(cuda, dtype, D, B, Hq, Hkv, L, T, seed=D + L)
@@ -139,6 +143,8 @@ def test_weighted_every_slot(cuda, dtype, D, B, Hq, Hkv, L, T):
     ("f32", 64, 2, 4, 2, 777, 2, 32, 9, True, False), ("bf16", 256, 1, 16, 2, 2000, 3, 96, 6, True, True),
     ("f16", 32, 2, 4, 1, 500, 1, 32, 40, True, False), ("bf16", 128, 1, 4, 2, 31, 1, 64, 3, False, True),
     ("f32", 256, 1, 2, 1, 300, 1, 64, 4, True, True), ("f32", 32, 1, 24, 1, 999, 4, 160, 5, False, True),
+    ("f16", 128, 1, 8, 2, 9000, 2, 128, 30, True, True), ("f32", 64, 1, 4, 2, 5000, 1, 64, 40, True, False),
+    ("bf16", 64, 2, 12, 1, 20000, 3, 96, 60, False, True),
 ])
 def test_weighted_selected_blocks(cuda, dtype, D, B, Hq, Hkv, L, T, bs, kk, gate, per_head):
     q, k, v, w, sel, gt = _weighted_case(cuda, dtype, D, B, Hq, Hkv, L, T, bs, kk, gate, per_head, seed=L)
@@ -378,6 +384,10 @@ def _prefix_case(cuda, dtype, D, B, Hq, Hkv, P, S, T, seed=0):
     ("bf16", 128, 1, 64, 1, 640, 64, 3), ("bf16", 64, 150, 2, 2, 130, 12, 1), ("f16", 128, 2, 2, 2, 8192, 1, 1),
     ("f16", 32, 70, 4, 2, 1111, 30, 1), ("bf16", 256, 66, 8, 4, 1500, 9, 1), ("bf16", 64, 1, 4, 4, 0, 50, 2),
     ("f32", 64, 2, 4, 2, 0, 3, 1), ("f16", 128, 64, 4, 1, 127, 600, 4), ("bf16", 128, 3, 384, 3, 256, 6, 1),
+    # more than one launch: two row tiles, one, and the split kernels
+    ("bf16", 64, 40, 8, 1, 6000, 5, 1), ("f16", 32, 70, 4, 2, 9000, 30, 1), ("bf16", 64, 150, 2, 2, 5000, 12, 1),
+    ("f16", 64, 12, 2, 1, 5001, 9, 3), ("f32", 128, 20, 8, 2, 2600, 3, 1), ("f32", 64, 3, 4, 1, 4000, 600, 2),
+    ("bf16", 32, 5, 2, 2, 6000, 70, 1), ("f16", 128, 30, 8, 2, 3000, 700, 2), ("bf16", 256, 3, 8, 2, 4500, 30, 1),
 ])
 def test_prefix(cuda, dtype, D, B, Hq, Hkv, P, S, T):
     _check_prefix(*_prefix_case(cuda, dtype, D, B, Hq, Hkv, P, S, T, seed=P + S))
