@@ -1,7 +1,8 @@
 // Split-key attention of few query rows (decode steps) in bf16 / f16 / fp32, the
 // join of the splits, and the running sum of every slot's attention weight.
 //
-//   split_mma_kernel, split_f32_kernel   partial softmax and O of one split
+//   split_mma_kernel, split_f32_kernel, split_f32_rows_kernel   partial softmax and O of
+//                       one split
 //   split_join_kernel   joins the splits of every row; with weights, also adds the sum
 //                       over the rows of p = 2^(x - lse) to each slot's sum
 // The kernels are bound by reading K and V once (HBM).
@@ -33,6 +34,11 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live, u
   asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2, %3;" ::"r"(dst), "l"(src), "r"(n),
                "l"(policy)
                : "memory");
+}
+
+// Without the policy: rows that other CTAs read too.
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
 // fp32 products on the tensor cores: x = x1 + x2 + x3, each the bf16 rounding of what is
@@ -197,13 +203,17 @@ __device__ __forceinline__ bool split_span(const SplitParams &p, int rtiles, int
   s.c_lo = min(nch, (int)blockIdx.y * cps);
   s.c_hi = min(nch, s.c_lo + cps);
   s.split = p.split0 + blockIdx.y;
-  if (CL || s.c_lo < s.c_hi) return true;
-  for (int r = tid; r < ROWS && s.r0 + r < p.R; r += blockDim.x) {
-    int rb, rh, rtt;
-    const long long gr = split_row(p, s.b, s.hk, s.r0 + r, rb, rh, rtt);
-    p.pml[(long long)s.split * p.rows + gr] = make_float2(-INFINITY, 0.f);
+  if constexpr (!CL) {
+    if (s.c_lo >= s.c_hi) {
+      for (int r = tid; r < ROWS && s.r0 + r < p.R; r += blockDim.x) {
+        int rb, rh, rtt;
+        const long long gr = split_row(p, s.b, s.hk, s.r0 + r, rb, rh, rtt);
+        p.pml[(long long)s.split * p.rows + gr] = make_float2(-INFINITY, 0.f);
+      }
+      return false;
+    }
   }
-  return false;
+  return true;
 }
 
 // First key of chunk c, and its gate.
@@ -1016,6 +1026,259 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   }
 }
 
+// fp32, a shared prefix for many rows: the warps take different rows (16 each) and the
+// same keys.  The chunk's K and V are turned into operands (three bf16 terms, in the order
+// of the products' registers) once for the CTA, where the kernel above does it for every
+// 16 or 32 rows: with many rows that was two thirds of its instructions.  Bound by the
+// products (mma.sync): 1200 rows x 20000 keys, D 256, 8 heads, in 5.24 ms, 225 TFLOP/s of
+// bf16 products (of 300 measured); 7.94 ms by the kernel above.  Which rows take it:
+// rows_over_warps.
+template <int D>
+struct RowsCfg {
+  static constexpr int W = D == 256 ? 4 : 8, NR = 2, ROWS = 8 * NR * W, KC = 16;
+  static constexpr int STAGE = KC * D * 8, FRAGS = KC * D * 6;
+  static constexpr int SMEM = 3 * ROWS * D * 2 + 2 * STAGE + 2 * FRAGS;
+};
+
+template <int D>
+__global__ void __launch_bounds__(RowsCfg<D>::W * 32, 1)
+    split_f32_rows_kernel(const SplitParams p, int rtiles) {
+  using C = RowsCfg<D>;
+  constexpr int KC = C::KC, NR = C::NR, KS = D / 16, ROWS = C::ROWS;
+  constexpr int VW = D >= 64 ? 4 : 2, VG = D / (16 * VW);
+  extern __shared__ __align__(128) uint8_t sm[];
+  uint8_t *sQ = sm;                              // three bf16 terms [ROWS][D]
+  uint8_t *raw = sm + 3 * ROWS * D * 2;          // [stage]: K and V as they are
+  uint4 *fk = reinterpret_cast<uint4 *>(raw + 2 * C::STAGE);  // [k-step][term][lane]
+  uint4 *fv = fk + KS * 3 * 32;                  // [tile of O^T][term][lane]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, tq = lane & 3;
+  pdl_trigger();
+  const int hk = blockIdx.x / rtiles, row0 = (blockIdx.x % rtiles) * ROWS, r0 = row0 + warp * 8 * NR;
+  const int len = p.nkeys, nch = (len + KC - 1) / KC, cps = (nch + p.nsplit - 1) / p.nsplit;
+  const int c_lo = min(nch, (int)blockIdx.y * cps), c_hi = min(nch, c_lo + cps), split = p.split0 + blockIdx.y;
+  int rb, rh, rtt;
+  if (c_lo >= c_hi) {
+    for (int r = row0 + tid; r < min(p.R, row0 + ROWS); r += C::W * 32)
+      p.pml[(long long)split * p.rows + split_row(p, 0, hk, r, rb, rh, rtt)] = make_float2(-INFINITY, 0.f);
+    return;
+  }
+  const float *kb_ = reinterpret_cast<const float *>(p.k) + hk * p.k_sh;
+  const float *vb_ = reinterpret_cast<const float *>(p.v) + hk * p.v_sh;
+  const uint32_t raw0 = smem_u32(raw);
+  auto load = [&](int c) {
+    if (c < c_hi) {
+      const uint32_t dk = raw0 + (c & 1) * C::STAGE, dv = dk + KC * D * 4;
+#pragma unroll
+      for (int it = 0; it < KC * D / 4 / (C::W * 32); ++it) {
+        const int i = it * C::W * 32 + tid, row = i / (D / 4), ch = i % (D / 4);
+        const bool ok = c * KC + row < len;
+        const int64_t key = ok ? c * KC + row : 0;
+        const uint32_t off = sw_off<4, D>(row, ch);
+        cp16(dk + off, kb_ + key * p.k_sl + ch * 4, ok);
+        cp16(dv + off, vb_ + key * p.v_sl + ch * 4, ok);
+      }
+    }
+    cp_commit();
+  };
+  load(c_lo);
+  for (int i = tid; i < ROWS * (D / 4); i += blockDim.x) {
+    const int r = i / (D / 4), d = (i % (D / 4)) * 4;
+    float x[4] = {0.f, 0.f, 0.f, 0.f};
+    if (row0 + r < p.R) {
+      split_row(p, 0, hk, row0 + r, rb, rh, rtt);
+      const float *qp = reinterpret_cast<const float *>(p.q) + rb * p.q_sb + rh * p.q_sh + rtt * p.q_sl + d;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = qp[e];
+    }
+    uint32_t u[3], w[3];
+    split3(x[0], x[1], u);
+    split3(x[2], x[3], w);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+      *reinterpret_cast<uint2 *>(sQ + k * ROWS * D * 2 + sw_off<2, D>(r, d / 8) + (d & 4) * 2) = make_uint2(u[k], w[k]);
+  }
+
+  float acc[NR][KS][4], m[NR][2], l[NR][2];
+#pragma unroll
+  for (int n = 0; n < NR; ++n) {
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[n][ks][e] = 0.f;
+    m[n][0] = m[n][1] = -INFINITY;
+    l[n][0] = l[n][1] = 0.f;
+  }
+  for (int c = c_lo; c < c_hi; ++c) {
+    cp_wait<0>();
+    __syncthreads();  // the chunk is here, and nobody reads the last one's operands
+    load(c + 1);
+    const uint8_t *sk = raw + (c & 1) * C::STAGE, *sv = sk + KC * D * 4;
+    for (int i = tid; i < KS * 32; i += C::W * 32) {  // K: (k-step, lane)
+      const int ks = i >> 5, gg = (i & 31) >> 2, tt = i & 3;
+      uint4 f[3];
+      uint32_t u[3];
+      const float4 x = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(gg, ks * 4 + tt));
+      const float4 y = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(gg + 8, ks * 4 + tt));
+      split3(x.x, x.y, u);
+      f[0].x = u[0], f[1].x = u[1], f[2].x = u[2];
+      split3(y.x, y.y, u);
+      f[0].y = u[0], f[1].y = u[1], f[2].y = u[2];
+      split3(x.z, x.w, u);
+      f[0].z = u[0], f[1].z = u[1], f[2].z = u[2];
+      split3(y.z, y.w, u);
+      f[0].w = u[0], f[1].w = u[1], f[2].w = u[2];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) fk[(ks * 3 + k) * 32 + (i & 31)] = f[k];
+    }
+    for (int i = tid; i < VG * 32; i += C::W * 32) {  // V: (column group, lane), VW tiles each
+      const int v = i >> 5, gg = (i & 31) >> 2, tt = i & 3;
+      float x[4][2][VW];
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int key = 2 * tt + (q & 1) + (q >> 1) * 8, col = (v * 2 + h) * 8 * VW + VW * gg;
+          const uint8_t *at = sv + sw_off<4, D>(key, col >> 2) + (col & 3) * 4;
+          if constexpr (VW == 4)
+            *reinterpret_cast<float4 *>(x[q][h]) = *reinterpret_cast<const float4 *>(at);
+          else
+            *reinterpret_cast<float2 *>(x[q][h]) = *reinterpret_cast<const float2 *>(at);
+        }
+#pragma unroll
+      for (int e = 0; e < VW; ++e) {
+        uint4 f[3];
+        uint32_t u[3];
+        split3(x[0][0][e], x[1][0][e], u);
+        f[0].x = u[0], f[1].x = u[1], f[2].x = u[2];
+        split3(x[0][1][e], x[1][1][e], u);
+        f[0].y = u[0], f[1].y = u[1], f[2].y = u[2];
+        split3(x[2][0][e], x[3][0][e], u);
+        f[0].z = u[0], f[1].z = u[1], f[2].z = u[2];
+        split3(x[2][1][e], x[3][1][e], u);
+        f[0].w = u[0], f[1].w = u[1], f[2].w = u[2];
+#pragma unroll
+        for (int k = 0; k < 3; ++k) fv[((v * VW + e) * 3 + k) * 32 + (i & 31)] = f[k];
+      }
+    }
+    __syncthreads();
+    // ---- S^T = K Q^T
+    float s[NR][4], sr[NR][4];
+#pragma unroll
+    for (int n = 0; n < NR; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = sr[n][e] = 0.f;
+#pragma unroll 4
+    for (int ks = 0; ks < KS; ++ks) {
+      uint4 a[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) a[k] = fk[(ks * 3 + k) * 32 + lane];
+      const uint32_t a0[4] = {a[0].x, a[0].y, a[0].z, a[0].w}, a1[4] = {a[1].x, a[1].y, a[1].z, a[1].w};
+      const uint32_t a2[4] = {a[2].x, a[2].y, a[2].z, a[2].w};
+      uint2 q[NR][3];
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+          q[n][k] = *reinterpret_cast<const uint2 *>(
+              sQ + k * ROWS * D * 2 + sw_off<2, D>(warp * 8 * NR + n * 8 + g, ks * 2 + (tq >> 1)) + (tq & 1) * 8);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(s[n], a0, q[n][0].x, q[n][0].y);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(sr[n], a2, q[n][0].x, q[n][0].y);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(sr[n], a0, q[n][2].x, q[n][2].y);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(sr[n], a1, q[n][1].x, q[n][1].y);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(sr[n], a1, q[n][0].x, q[n][0].y);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(sr[n], a0, q[n][1].x, q[n][1].y);
+    }
+    // ---- online softmax (log2 domain); missing keys are -inf
+    uint32_t pb[NR][2][3];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float x = (s[n][e] + sr[n][e]) * p.scale2;
+        if (c * KC + g + 8 * (e >> 1) >= len) x = -INFINITY;
+        s[n][e] = x;
+        mx[e & 1] = fmax_nan(mx[e & 1], x);
+      }
+      float al[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
+        const float mn = fmax_nan(m[n][h], mx[h]);
+        al[h] = mn == -INFINITY ? 1.f : ex2(m[n][h] - mn);
+        m[n][h] = mn;
+      }
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+        l[n][0] *= al[0];
+        l[n][1] *= al[1];
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[n][ks][e] *= al[e & 1];
+      }
+      const float off[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[n][e] = ex2(s[n][e] - off[e & 1]);
+        l[n][e & 1] += s[n][e];
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        split3(s[n][2 * h], s[n][2 * h + 1], pb[n][h]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) pb[n][h][k] = movmatrix(pb[n][h][k]);
+      }
+    }
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      uint4 a[3];
+#pragma unroll
+      for (int k = 0; k < 3; ++k) a[k] = fv[(ks * 3 + k) * 32 + lane];
+      const uint32_t a0[4] = {a[0].x, a[0].y, a[0].z, a[0].w}, a1[4] = {a[1].x, a[1].y, a[1].z, a[1].w};
+      const uint32_t a2[4] = {a[2].x, a[2].y, a[2].z, a[2].w};
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a2, pb[n][0][0], pb[n][1][0]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a0, pb[n][0][2], pb[n][1][2]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a1, pb[n][0][1], pb[n][1][1]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a1, pb[n][0][0], pb[n][1][0]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a0, pb[n][0][1], pb[n][1][1]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a0, pb[n][0][0], pb[n][1][0]);
+    }
+  }
+  // ---- this warp's rows
+#pragma unroll
+  for (int n = 0; n < NR; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], o);
+      const int r = r0 + n * 8 + 2 * tq + h;
+      if (r >= p.R) continue;
+      const long long at = (long long)split * p.rows + split_row(p, 0, hk, r, rb, rh, rtt);
+      if (g == 0) p.pml[at] = make_float2(m[n][h], l[n][h]);
+      float *op = p.po + at * D + VW * g;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        op[(ks / VW) * 16 * VW + ks % VW] = acc[n][ks][h];
+        op[(ks / VW) * 16 * VW + 8 * VW + ks % VW] = acc[n][ks][2 + h];
+      }
+    }
+}
+
 // ------------------------------------------------------------------ join
 struct JoinParams {
   void *o;
@@ -1257,9 +1520,22 @@ static int split_count_t(long long groups, int R, long long n) {
   return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, 148 * C::MINB, 4, kMaxSplit);
 }
 
+// Whether the rows of a shared prefix go over the warps (split_f32_rows_kernel).  Times of
+// it against split_f32_kernel, 20000 keys, 8 heads, us: D 256, 36 rows 278 : 373, 1200 rows
+// 5240 : 7940; D 128, 64 rows 254 : 197, 96 rows 245 : 287, 1200 rows 2347 : 3124; D 64,
+// 96 rows 153 : 97, 1200 rows 1069 : 1143, with 2 heads 362 : 295 (its barriers and the
+// one CTA per SM show where a chunk has few products).
+static bool rows_over_warps(int dtype, int D, bool fold, int R) {
+  return dtype == BSA_F32 && fold && (D == 256 ? R > 32 : D == 128 && R > 64);
+}
+
 // Splits of the partial kernel for n keys, `groups` K/V head groups and R rows each.
-int split_count(int dtype, int D, long long groups, int R, long long n) {
+int split_count(int dtype, int D, long long groups, int R, long long n, bool fold = false) {
   const bool f = dtype == BSA_F32;
+  if (rows_over_warps(dtype, D, fold, R)) {
+    const int rows = D == 256 ? RowsCfg<256>::ROWS : RowsCfg<128>::ROWS;
+    return choose_split(groups * ((R + rows - 1) / rows), (n + 15) / 16, 148, 6, kMaxSplit);
+  }
   switch (D) {
     case 32: return f ? split_count_t<float, 32>(groups, R, n) : split_count_t<__half, 32>(groups, R, n);
     case 64: return f ? split_count_t<float, 64>(groups, R, n) : split_count_t<__half, 64>(groups, R, n);
@@ -1313,8 +1589,22 @@ static bsa_status launch_mma_d(const SplitParams &p, long long groups, cudaStrea
   return launch_rows<T, D, 16, CL>(p, groups, st);
 }
 
+template <int D>
+static bsa_status launch_f32_rows(const SplitParams &p, long long groups, cudaStream_t st) {
+  using C = RowsCfg<D>;
+  static_assert(C::SMEM <= 232448, "shared memory of one CTA");
+  const int rtiles = (p.R + C::ROWS - 1) / C::ROWS;
+  static std::atomic<uint64_t> done{0};
+  allow_smem(reinterpret_cast<const void *>(split_f32_rows_kernel<D>), C::SMEM, done);
+  split_f32_rows_kernel<D>
+      <<<dim3((unsigned)(groups * rtiles), p.nsplit), C::W * 32, C::SMEM, st>>>(p, rtiles);
+  return check_launch("split_f32_rows");
+}
+
 template <int D, bool CL>
 static bsa_status launch_split_d(int dtype, const SplitParams &p, long long groups, cudaStream_t st) {
+  if constexpr (!CL && D >= 128)
+    if (rows_over_warps(dtype, D, p.fold, p.R)) return launch_f32_rows<D>(p, groups, st);
   if (dtype == BSA_BF16) return launch_mma_d<__nv_bfloat16, D, CL>(p, groups, st);
   if (dtype == BSA_F16) return launch_mma_d<__half, D, CL>(p, groups, st);
   return launch_mma_d<float, D, CL>(p, groups, st);
@@ -1336,7 +1626,8 @@ static bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStrea
 // a CTA's warps in all (four per CTA of a full cluster), unless one CTA per head is what
 // the splits come to.  One launch saves 3 us of the host's time and the partial sums'
 // way through memory; with few heads and many keys eight CTAs per head draw too little
-// of HBM.
+// of HBM (fp32, D 64, two sequences of 4097 slots, two heads: 9.4 us by splits, 19 by
+// clusters).
 static int cluster_size(int dtype, int D, long long groups, int R, long long n) {
   const int es = (int)elem_size(dtype), kc = es == 2 && D <= 64 ? 32 : 16;
   const int most = D == 256 || (es == 2 && D == 32) ? 16 : 32;
@@ -1501,7 +1792,8 @@ bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParam
 
 namespace {
 // Bytes of the prefix read by all sequences together, up to which each reads it for
-// itself: 5 us of L2.
+// itself: 5 us of L2 (18 groups that share 2311 keys, 43 MB, fp32: 19 us by splits, 33 by
+// clusters).
 constexpr long long kAgainBytes = 32 << 20;
 struct PrefixPlan {
   int cl;      // CTAs of a cluster per (b, hk) (one launch), or 0
@@ -1517,7 +1809,7 @@ PrefixPlan prefix_plan(const bsa_decode_prefix_args *a) {
   const long long groups = (long long)a->B * a->Hkv, again = groups * a->P * a->D * 2 * (long long)elem_size(a->dtype);
   w.cl = again <= kAgainBytes ? cluster_size(a->dtype, a->D, groups, R, (long long)a->P + a->S) : 0;
   w.tc = !w.cl && prefix_sm100_applicable(a);
-  w.np = w.tc ? prefix_sm100_splits(a) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P) : 0;
+  w.np = w.tc ? prefix_sm100_splits(a) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P, true) : 0;
   w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S);
   w.rows = (long long)a->B * a->Hq * a->T;
   const size_t parts = w.cl ? 0 : (size_t)(w.np + w.ns) * w.rows;
