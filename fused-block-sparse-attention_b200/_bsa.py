@@ -652,7 +652,7 @@ def _launch(name, packed, like):
     nbytes = fn[1](packed)
     if nbytes == 0:   # validation failed: the call reports why
         _check(fn[0](packed, None, 0, None))
-    ws = like.new_empty(nbytes >> 1)    # at least nbytes: no element is smaller than two
+    ws = like.new_empty(nbytes // like.element_size())   # whole: nbytes is a multiple of 256
     st = fn[0](packed, ws.data_ptr(), nbytes, _raw_stream(dev))
     if st:
         _check(st)

@@ -398,6 +398,28 @@ __global__ void __launch_bounds__(256, 6) evict_move_kernel(const bsa_evict_args
 }
 
 // ------------------------------------------------------------------ host
+// Whether rows of an output (budget words each, x) meet rows of its source (L words, y)
+// without being the same view.  Exact for equal strides, else by the spans.
+static bool rows_meet(const void *x, int64_t xb, int64_t xh, const void *y, int64_t yb, int64_t yh,
+                      const bsa_evict_args *a) {
+  const int64_t B = a->B, H = a->Hkv, d = ((const char *)x - (const char *)y) / 4;
+  const bool like = (xb == yb || B == 1) && (xh == yh || H == 1);
+  if (like && d == 0) return false;
+  if (d >= yb * (B - 1) + yh * (H - 1) + a->L || -d >= xb * (B - 1) + xh * (H - 1) + a->budget) return false;
+  if (!like) return true;
+  for (int64_t j = 1 - B; j < B; ++j) {  // row offsets d + j sb + i sh in (-budget, L), |i| < H
+    const int64_t e = d + (B > 1 ? j * yb : 0);
+    if (H == 1 || yh == 0) {
+      if (e > -(int64_t)a->budget && e < a->L) return true;
+      continue;
+    }
+    int64_t i = -e / yh;  // the three around the nearest row
+    for (int64_t k = i - 1; k <= i + 1; ++k)
+      if (k > -H && k < H && e + k * yh > -(int64_t)a->budget && e + k * yh < a->L) return true;
+  }
+  return false;
+}
+
 static bsa_status evict_check(const bsa_evict_args *a) {
   if (a->dtype != BSA_BF16 && a->dtype != BSA_F16 && a->dtype != BSA_F32)
     return fail(BSA_ERR_DTYPE, "evict: dtype must be bf16, f16 or f32");
@@ -419,7 +441,17 @@ static bsa_status evict_check(const bsa_evict_args *a) {
   for (const bsa_view *v : {&a->k, &a->v})
     if (reinterpret_cast<uintptr_t>(v->ptr) % 16 || (v->sb * es) % 16 || (v->sh * es) % 16 || (v->sl * es) % 16)
       return fail(BSA_ERR_STRIDE, "evict: k and v need 16-byte aligned bases and strides");
+  for (const bsa_view *v : {&a->k, &a->v})
+    if (!lies_apart(a->B, v->sb, a->Hkv, v->sh, a->L, v->sl, a->D))
+      return fail(BSA_ERR_STRIDE, "evict: rows of k or v share memory");
   const long long nblk = (a->budget + a->bs - 1) / a->bs;
+  if (!lies_apart(a->B, a->wo_sb, a->Hkv, a->wo_sh, 1, 0, a->budget) ||
+      !lies_apart(a->B, a->po_sb, a->Hkv, a->po_sh, 1, 0, a->budget) ||
+      (a->kmin && !lies_apart(a->B, a->km_sb, a->Hkv, a->km_sh, nblk, a->km_sn, a->D)))
+    return fail(BSA_ERR_STRIDE, "evict: rows of an output share memory");
+  if (rows_meet(a->weight_out, a->wo_sb, a->wo_sh, a->weight, a->w_sb, a->w_sh, a) ||
+      rows_meet(a->pos_out, a->po_sb, a->po_sh, a->pos, a->p_sb, a->p_sh, a))
+    return fail(BSA_ERR_STRIDE, "evict: weight_out / pos_out must be weight / pos or lie apart from them");
   if (nblk * a->B * a->Hkv >= (1LL << 31)) return fail(BSA_ERR_SHAPE, "evict: too many blocks");
   return BSA_OK;
 }

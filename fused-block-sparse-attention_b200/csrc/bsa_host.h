@@ -49,6 +49,10 @@ inline void allow_smem(const void *kern, int bytes, std::atomic<uint64_t> &done)
 
 inline size_t elem_size(int dtype) { return dtype == BSA_F32 ? 4 : 2; }
 
+// Whether the elements of an operand that a kernel writes, (B, H, L) rows of D, lie apart:
+// each stride steps over what the shorter ones span (an expanded axis does not).
+bool lies_apart(int64_t B, int64_t sb, int64_t H, int64_t sh, int64_t L, int64_t sl, int64_t D);
+
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 // Encodes a 4-D tiled tensor map over a (B, H, L, D) view of 16-bit elements

@@ -11,6 +11,7 @@
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "bsa_host.h"
 #include "bsa_split.cuh"
@@ -1688,6 +1689,26 @@ static bsa_status check_kv(const bsa_view &v, int dtype, const char *who, const 
 }
 
 // ------------------------------------------------------------------ decode_weighted
+bool lies_apart(int64_t B, int64_t sb, int64_t H, int64_t sh, int64_t L, int64_t sl, int64_t D) {
+  std::pair<int64_t, int64_t> ax[3] = {{sb, B}, {sh, H}, {sl, L}};
+  std::sort(ax, ax + 3);
+  int64_t span = D;
+  for (const auto &[stride, n] : ax) {
+    if (n <= 1) continue;
+    if (stride < span) return false;
+    span += stride * (n - 1);
+  }
+  return true;
+}
+
+// The output of a decode step.
+static bsa_status check_out(const char *who, const bsa_view &o, int B, int Hq, int T, int D) {
+  if (!o.ptr) return fail(BSA_ERR_ARG, std::string(who) + ": o is NULL");
+  if (!lies_apart(B, o.sb, Hq, o.sh, T, o.sl, D))
+    return fail(BSA_ERR_STRIDE, std::string(who) + ": rows of o share memory");
+  return BSA_OK;
+}
+
 namespace {
 constexpr int kMaxWeightRows = 4096;
 struct WeightedPlan {
@@ -1729,7 +1750,10 @@ static bsa_status weighted_check(const bsa_decode_weighted_args *a) {
     return fail(BSA_ERR_ARG, "decode_weighted: a gate needs a selection");
   }
   if (a->L >= (1 << 30)) return fail(BSA_ERR_SHAPE, "decode_weighted: L too large");
-  if (!a->q.ptr || !a->o.ptr || !a->weight) return fail(BSA_ERR_ARG, "decode_weighted: NULL tensor");
+  if (!a->q.ptr || !a->weight) return fail(BSA_ERR_ARG, "decode_weighted: NULL tensor");
+  if (bsa_status s = check_out("decode_weighted", a->o, a->B, a->Hq, a->T, a->D)) return s;
+  if (!lies_apart(a->B, a->weight_sb, a->Hkv, a->weight_sh, 1, 0, a->L))
+    return fail(BSA_ERR_STRIDE, "decode_weighted: rows of weight share memory");
   if (bsa_status s = check_kv(a->k, a->dtype, "decode_weighted", "k", true)) return s;
   return check_kv(a->v, a->dtype, "decode_weighted", "v", true);
 }
@@ -1823,7 +1847,8 @@ static bsa_status prefix_check(const bsa_decode_prefix_args *a) {
   if (bsa_status s = check_rows("decode_prefix", a->dtype, a->B, a->Hq, a->Hkv, a->D, a->T, a->scale)) return s;
   if (a->P < 0 || a->S <= 0) return fail(BSA_ERR_SHAPE, "decode_prefix: needs P >= 0 and S >= 1");
   if (a->P >= (1 << 30) || a->S >= (1 << 30)) return fail(BSA_ERR_SHAPE, "decode_prefix: P or S too large");
-  if (!a->q.ptr || !a->o.ptr || !a->lens) return fail(BSA_ERR_ARG, "decode_prefix: NULL tensor");
+  if (!a->q.ptr || !a->lens) return fail(BSA_ERR_ARG, "decode_prefix: NULL tensor");
+  if (bsa_status s = check_out("decode_prefix", a->o, a->B, a->Hq, a->T, a->D)) return s;
   if (a->P > 0) {
     if (bsa_status s = check_kv(a->pk, a->dtype, "decode_prefix", "pk", false)) return s;
     if (bsa_status s = check_kv(a->pv, a->dtype, "decode_prefix", "pv", false)) return s;

@@ -293,7 +293,8 @@ bsa_status bsa_decode_weighted(const bsa_decode_weighted_args *a, void *workspac
  * slots < budget stay; the others fill the freed slots, both in ascending order:
  * the fewest rows move, and slots >= budget keep their contents.  k, v: (B, Hkv,
  * >= L, D), changed in place.  weight_out, pos_out: (B, Hkv, >= budget), the
- * survivors' sums and positions; they may be weight and pos themselves.  kmin, kmax
+ * survivors' sums and positions: weight and pos themselves, or memory apart from
+ * them; what is written must not share memory with itself (an expanded axis is refused).  kmin, kmax
  * (optional, both or none): fp32 per-block min / max of the keys (block stride
  * km_sn, unit D stride) as bsa_pool computes them; blocks whose rows changed are
  * pooled anew, and a last block that ends at the budget counts zeros past it.

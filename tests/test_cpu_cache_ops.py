@@ -37,7 +37,7 @@ P = 4096
 
 def _view(D=64):
     import _bsa
-    return _bsa.View(P, 64 * D, 64 * D, D)
+    return _bsa.View(P, 4 * 64 * D, 64 * D, D)
 
 
 def _weighted():
@@ -45,6 +45,7 @@ def _weighted():
     a = _bsa.DecodeWeightedArgs(_bsa.BF16, 1, 4, 2, 60, 64, 32, 1, 3, 0.125)
     a.q = a.k = a.v = a.o = _view()
     a.weight = a.sel = P
+    a.weight_sb, a.weight_sh = 2 * 64, 64
     return a
 
 
@@ -53,6 +54,8 @@ def _evict():
     a = _bsa.EvictArgs(_bsa.BF16, 1, 2, 60, 64, 32, 30, 5, 1, 60)
     a.k = a.v = _view()
     a.weight = a.pos = a.weight_out = a.pos_out = P
+    a.w_sb = a.p_sb = a.wo_sb = a.po_sb = 2 * 64
+    a.w_sh = a.p_sh = a.wo_sh = a.po_sh = 64
     return a
 
 
@@ -109,6 +112,52 @@ def test_unaligned_cache_is_refused(op, view, field, value, code):
     a = {"weighted": _weighted, "evict": _evict, "prefix": _prefix}[op]()
     setattr(getattr(a, view), field, value)
     assert getattr(_bsa.lib(), name)(ctypes.byref(a), P, 1 << 40, None) == getattr(_bsa, "ERR_" + code)
+
+
+# Written operands whose rows share memory: two CTAs would write one place.
+SHARED = [
+    ("weighted", dict(weight_sh=0)), ("weighted", dict(weight_sh=59)), ("weighted", dict(B=2, weight_sb=64)),
+    ("weighted", {"o.sh": 0}), ("weighted", {"o.sh": 63}), ("weighted", dict(T=2) | {"o.sl": 0}),
+    ("prefix", {"o.sb": 0}), ("prefix", {"o.sh": 32}),
+    ("evict", {"k.sl": 0}), ("evict", {"v.sh": 0}), ("evict", {"k.sh": 59 * 64}), ("evict", {"v.sl": 32}),
+    ("evict", dict(wo_sh=29, weight_out=P + 65536)), ("evict", dict(po_sh=0, pos_out=P + 65536)),
+    ("evict", dict(kmin=P, kmax=P, km_sh=0, km_sn=64)), ("evict", dict(kmin=P, kmax=P, km_sh=64, km_sn=0, budget=60)),
+    # an output that meets its source without being it
+    ("evict", dict(weight_out=P + 4)), ("evict", dict(weight_out=P - 4)), ("evict", dict(pos_out=P + 59 * 4)),
+    ("evict", dict(pos_out=P + 64 * 4)), ("evict", dict(weight_out=P - 29 * 4)), ("evict", dict(wo_sh=128)),
+    ("evict", dict(weight_out=P + 63 * 4)),
+]
+APART = [
+    ("weighted", dict(weight_sh=60)), ("weighted", dict(B=2, weight_sb=60, weight_sh=120)), ("weighted", {"o.sh": 64}),
+    ("weighted", dict(Hq=2, Hkv=1, weight_sh=0)), ("evict", {"k.sl": 128, "k.sh": 64}),
+    ("evict", dict(weight_out=P + 128 * 4)), ("evict", dict(weight_out=P - 30 * 4, w_sh=90, wo_sh=90)),
+    ("evict", dict(pos_out=P + 60 * 4, p_sh=90, po_sh=90)), ("evict", dict(Hkv=1, weight_out=P + 60 * 4, wo_sh=0)),
+]
+
+
+def _set(a, change):
+    for k, v in change.items():
+        view, _, field = k.partition(".")
+        setattr(getattr(a, view), field, v) if field else setattr(a, k, v)
+
+
+@pytest.mark.parametrize("op,change", SHARED, ids=lambda x: str(x)[:40])
+def test_shared_rows_are_refused(op, change):
+    import _bsa
+    a = {"weighted": _weighted, "evict": _evict, "prefix": _prefix}[op]()
+    name = {"weighted": "bsa_decode_weighted", "evict": "bsa_evict", "prefix": "bsa_decode_prefix"}[op]
+    _set(a, change)
+    assert getattr(_bsa.lib(), name)(ctypes.byref(a), P, 1 << 40, None) == _bsa.ERR_STRIDE
+    assert b"memory" in _bsa.lib().bsa_last_error() or b"apart" in _bsa.lib().bsa_last_error()
+
+
+@pytest.mark.parametrize("op,change", APART, ids=lambda x: str(x)[:40])
+def test_interleaved_rows_are_accepted(op, change):
+    import _bsa
+    a = {"weighted": _weighted, "evict": _evict, "prefix": _prefix}[op]()
+    name = {"weighted": "bsa_decode_weighted", "evict": "bsa_evict", "prefix": "bsa_decode_prefix"}[op]
+    _set(a, change)
+    assert getattr(_bsa.lib(), name + "_workspace")(ctypes.byref(a)) > 0
 
 
 def test_null_args():

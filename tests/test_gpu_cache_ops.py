@@ -564,3 +564,108 @@ def test_deterministic(cuda, dtype):
     assert torch.equal(_bsa.decode_weighted(q, k, v, w1, L=3001), _bsa.decode_weighted(q, k, v, w2, L=3001))
     assert torch.equal(w1, w2)
     assert torch.equal(_bsa.decode_prefix(*pf), _bsa.decode_prefix(*pf))
+
+
+# ------------------------------------------------------------------ calls off the usual path
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("L", [50, 5000])
+def test_weighted_expanded_and_aliased_operands(cuda, dtype, L):
+    """K/V read by several batch rows or heads (expanded), V the same tensor as K, a query
+    on an odd offset whose rows the output replaces."""
+    import _bsa
+    B, Hq, Hkv, T, D = 3, 8, 2, 2, 64
+    q, k, v, w, _, _ = _weighted_case(cuda, dtype, D, 1, Hq, 1, L, T)
+    k, v = k.expand(B, Hkv, -1, -1), v.expand(B, Hkv, -1, -1)
+    w = torch.rand(B, Hkv, L, generator=torch.Generator().manual_seed(1)).to(cuda)
+    buf = _rand(torch.Generator().manual_seed(2), B, T, Hq, D + 1, dt=DT[dtype], dev=cuda)
+    q = buf[..., 1:].transpose(1, 2)
+    ref, add = _ref_weighted(q, k, k, w, None, None, 64, L, D ** -0.5)
+    e, w0 = _rel(q, k[:, :, :L], D ** -0.5), w.double()
+    edge = buf[..., 0].clone()
+    o = _bsa.decode_weighted(q, k, k, w, L=L, out=q)
+    assert o.data_ptr() == q.data_ptr() and torch.equal(buf[..., 0], edge)
+    _close_o(o, ref, e, float(k[:, :, :L].abs().max()), "o")
+    assert bool(((w.double() - w0 - add).abs() <= e * add + 2 ** -23 * (w0 + add)).all())
+
+
+def test_weighted_many_sequences(cuda):
+    """More (batch, head) pairs than a grid's second axis holds."""
+    import _bsa
+    B, L, D = 66000, 9, 32
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (_rand(g, B, 1, n, D, dt=torch.bfloat16, dev=cuda) for n in (1, L, L))
+    w = torch.zeros(B, 1, L, device=cuda)
+    o = _bsa.decode_weighted(q, k, v, w)
+    p = torch.softmax(q.double() @ k.double().transpose(2, 3) * D ** -0.5, -1)
+    e = _rel(q, k, D ** -0.5)
+    _close_o(o, p @ v.double(), e, float(v.abs().max()), "o")
+    assert bool(((w.double() - p[:, :, 0]).abs() <= e * p[:, :, 0] + 2 ** -23).all())
+
+
+@pytest.mark.parametrize("dtype,D,B,H,L,budget,recent,sink,bs,kind,out", [
+    # slots that do not fit a cluster's registers, ties over several CTAs, one slot left, blocks of one slot
+    ("bf16", 32, 1, 2, 300001, 150000, 1000, 4, 128, "plain", False), ("f16", 32, 2, 1, 140000, 139999, 0, 0, 64, "ties", True),
+    ("f32", 32, 1, 1, 200000, 77777, 5, 0, 1024, "equal", False), ("bf16", 64, 1, 2, 5000, 1, 1, 0, 64, "plain", False),
+    ("bf16", 64, 2, 2, 300, 200, 3, 2, 1, "special", False),
+])
+def test_evict_long_and_small(cuda, dtype, D, B, H, L, budget, recent, sink, bs, kind, out):
+    _check_evict(cuda, dtype, D, B, H, L, budget, recent, sink, bs, kind, L + budget, out)
+
+
+def test_evict_interleaved_outputs(cuda):
+    """Sums and their outputs in one buffer, rows side by side; K and V in one, head by head."""
+    import _bsa
+    B, H, L, D, n = 2, 3, 700, 64, 300
+    g = torch.Generator().manual_seed(5)
+    kv = _rand(g, B, L, H, 2, D, dt=torch.bfloat16, dev=cuda)
+    k, v = kv[:, :, :, 0].transpose(1, 2), kv[:, :, :, 1].transpose(1, 2)
+    wbuf = torch.rand(B, H, 2, L, generator=g).to(cuda)
+    pbuf = torch.arange(L, dtype=torch.int32, device=cuda).repeat(B, H, 2, 1)
+    src = _ref_evict(wbuf[:, :, 0].cpu(), pbuf[:, :, 0].cpu(), L, n, L, 20, 3).to(cuda)
+    b, h = torch.arange(B, device=cuda).view(-1, 1, 1), torch.arange(H, device=cuda).view(1, -1, 1)
+    want = [t[b, h, src] for t in (k, v, wbuf[:, :, 0], pbuf[:, :, 0])]
+    w0 = wbuf[:, :, 0].clone()
+    _bsa.evict(k, v, wbuf[:, :, 0], pbuf[:, :, 0], budget=n, recent=20, sink=3, weight_out=wbuf[:, :, 1],
+               pos_out=pbuf[:, :, 1])
+    for x, y in zip((k, v, wbuf[:, :, 1], pbuf[:, :, 1]), want):
+        assert torch.equal(x[:, :, :n], y)
+    assert torch.equal(wbuf[:, :, 0], w0)
+
+
+@pytest.mark.parametrize("dtype,D,B,Hq,Hkv,P,S,T", [
+    # fp32 rows over the warps: several row tiles, a last one of one row, chunks that end inside
+    ("f32", 256, 33, 4, 1, 1500, 9, 1), ("f32", 256, 9, 4, 1, 33, 70, 1), ("f32", 128, 43, 6, 2, 2001, 5, 1),
+    ("f32", 128, 65, 1, 1, 15, 300, 3), ("f32", 128, 129, 2, 2, 700, 4, 1), ("f32", 64, 300, 4, 1, 1000, 8, 1),
+])
+def test_prefix_many_rows_fp32(cuda, dtype, D, B, Hq, Hkv, P, S, T):
+    _check_prefix(*_prefix_case(cuda, dtype, D, B, Hq, Hkv, P, S, T, seed=P))
+
+
+@pytest.mark.parametrize("dtype,B", [("bf16", 2), ("bf16", 40), ("f32", 40)])
+def test_prefix_expanded_and_aliased_operands(cuda, dtype, B):
+    """A prefix shared by the heads too (expanded), own slots shared by the batch, the
+    output in the query's place."""
+    import _bsa
+    Hq, Hkv, P, S, T, D = 4, 2, 500, 20, 1, 64
+    q, pk, pv, k, v, lens = _prefix_case(cuda, dtype, D, B, Hq, Hkv, P, S, T, seed=B)
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0, 0.0, 0.0)
+    pk, pv = pk[:1].expand(Hkv, -1, -1), pv[:1].expand(Hkv, -1, -1)
+    k, v = k[:1].expand(B, -1, -1, -1), v[:1].expand(B, -1, -1, -1)
+    want = _check_prefix(q, pk, pv, k, v, lens)
+    out = _bsa.decode_prefix(q, pk, pv, k, v, lens, out=q)
+    assert out.data_ptr() == q.data_ptr() and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_prefix_nan_query_stays_in_its_row(cuda, dtype):
+    """A NaN in one head's query stays in its row."""
+    import _bsa
+    q, pk, pv, k, v, lens = _prefix_case(cuda, dtype, 128, 20, 8, 1, 400, 6, 1)
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0, 0.0, 0.0)
+    want = _bsa.decode_prefix(q, pk, pv, k, v, lens)
+    q2 = q.clone()
+    q2[3, 5] = float("nan")
+    o = _bsa.decode_prefix(q2, pk, pv, k, v, lens)
+    assert bool(o[3, 5].isnan().all())
+    o[3, 5] = want[3, 5]
+    assert torch.equal(o, want)
