@@ -1514,11 +1514,11 @@ static int choose_split(long long groups, long long steps, int slots, int fixed,
 constexpr int kMaxSplit = 296;
 
 template <typename T, int D>
-static int split_count_t(long long groups, int R, long long n) {
+static int split_count_t(long long groups, int R, long long n, int sms) {
   using C = SplitCfg<T, D>;
   const int rows = split_rows<T, D>(R);
   const long long step = C::KC * NW;
-  return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, 148 * C::MINB, 4, kMaxSplit);
+  return choose_split(groups * ((R + rows - 1) / rows), (n + step - 1) / step, sms * C::MINB, 4, kMaxSplit);
 }
 
 // Whether the rows of a shared prefix go over the warps (split_f32_rows_kernel).  Times of
@@ -1530,18 +1530,19 @@ static bool rows_over_warps(int dtype, int D, bool fold, int R) {
   return dtype == BSA_F32 && fold && (D == 256 ? R > 32 : D == 128 && R > 64);
 }
 
-// Splits of the partial kernel for n keys, `groups` K/V head groups and R rows each.
-int split_count(int dtype, int D, long long groups, int R, long long n, bool fold = false) {
+// Splits of the partial kernel for n keys, `groups` K/V head groups and R rows each, on
+// `sms` SMs.
+int split_count(int dtype, int D, long long groups, int R, long long n, bool fold = false, int sms = 148) {
   const bool f = dtype == BSA_F32;
   if (rows_over_warps(dtype, D, fold, R)) {
     const int rows = D == 256 ? RowsCfg<256>::ROWS : RowsCfg<128>::ROWS;
     return choose_split(groups * ((R + rows - 1) / rows), (n + 15) / 16, 148, 6, kMaxSplit);
   }
   switch (D) {
-    case 32: return f ? split_count_t<float, 32>(groups, R, n) : split_count_t<__half, 32>(groups, R, n);
-    case 64: return f ? split_count_t<float, 64>(groups, R, n) : split_count_t<__half, 64>(groups, R, n);
-    case 128: return f ? split_count_t<float, 128>(groups, R, n) : split_count_t<__half, 128>(groups, R, n);
-    default: return f ? split_count_t<float, 256>(groups, R, n) : split_count_t<__half, 256>(groups, R, n);
+    case 32: return f ? split_count_t<float, 32>(groups, R, n, sms) : split_count_t<__half, 32>(groups, R, n, sms);
+    case 64: return f ? split_count_t<float, 64>(groups, R, n, sms) : split_count_t<__half, 64>(groups, R, n, sms);
+    case 128: return f ? split_count_t<float, 128>(groups, R, n, sms) : split_count_t<__half, 128>(groups, R, n, sms);
+    default: return f ? split_count_t<float, 256>(groups, R, n, sms) : split_count_t<__half, 256>(groups, R, n, sms);
   }
 }
 
@@ -1811,7 +1812,7 @@ bsa_status run_weighted(const bsa_decode_weighted_args *a, void *ws, size_t ws_b
 
 // ------------------------------------------------------------------ decode_prefix
 bool prefix_sm100_applicable(const bsa_decode_prefix_args *a);
-int prefix_sm100_splits(const bsa_decode_prefix_args *a);
+int prefix_sm100_splits(const bsa_decode_prefix_args *a, int &left);
 bsa_status launch_prefix_sm100(const bsa_decode_prefix_args *a, const SplitParams &p, cudaStream_t st);
 
 namespace {
@@ -1833,8 +1834,9 @@ PrefixPlan prefix_plan(const bsa_decode_prefix_args *a) {
   const long long groups = (long long)a->B * a->Hkv, again = groups * a->P * a->D * 2 * (long long)elem_size(a->dtype);
   w.cl = again <= kAgainBytes ? cluster_size(a->dtype, a->D, groups, R, (long long)a->P + a->S) : 0;
   w.tc = !w.cl && prefix_sm100_applicable(a);
-  w.np = w.tc ? prefix_sm100_splits(a) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P, true) : 0;
-  w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S);
+  int left = 148;  // SMs that the prefix leaves to the own slots
+  w.np = w.tc ? prefix_sm100_splits(a, left) : a->P > 0 ? split_count(a->dtype, a->D, a->Hkv, a->B * R, a->P, true) : 0;
+  w.ns = split_count(a->dtype, a->D, (long long)a->B * a->Hkv, R, a->S, false, left);
   w.rows = (long long)a->B * a->Hq * a->T;
   const size_t parts = w.cl ? 0 : (size_t)(w.np + w.ns) * w.rows;
   w.o_ml = align_up(parts * a->D * 4, 256);

@@ -107,6 +107,75 @@ __device__ __forceinline__ void commit_if(uint32_t on, uint64_t *bar) {
       : "memory");
 }
 
+// ---- CTA pairs (cta_group::2, a cluster of two): one product over both CTAs' rows.  A and
+// the accumulator are each CTA's own 128 rows (M = 256); B's N rows lie half in each CTA's
+// shared memory, at the same offset.  The CTA of rank 0 issues; both allocate and free.
+__device__ __forceinline__ void pair_alloc(uint32_t *dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(dst_smem)),
+               "r"(ncols)
+               : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_dealloc(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
+}
+__device__ __forceinline__ void pair_mma_if(uint32_t on, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                            uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+__device__ __forceinline__ void pair_mma_ts_if(uint32_t on, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                               uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(on)
+      : "memory");
+}
+// Arrives once on `bar` of both CTAs.
+__device__ __forceinline__ void pair_commit_if(uint32_t on, uint64_t *bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %2;\n\t}\n" ::"r"(
+          smem_u32(bar)),
+      "r"(on), "h"((uint16_t)3)
+      : "memory");
+}
+// The address of `bar` in the CTA of rank 0, and an arrival there.  What it tells of are
+// completed TMEM reads and writes (wait::ld, wait::st) and shared-memory writes behind a
+// proxy fence; a release at cluster scope would wait for the memory system besides, 1500
+// cycles at each arrival.
+__device__ __forceinline__ uint32_t pair_first(uint64_t *bar) {
+  uint32_t a;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(a) : "r"(smem_u32(bar)));
+  return a;
+}
+__device__ __forceinline__ void pair_arrive(uint32_t first_bar) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(first_bar) : "memory");
+}
+// Barrier over the threads of both CTAs.
+__device__ __forceinline__ void pair_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// A box of this CTA's own memory and shared memory (no multicast), counted on a barrier of
+// either CTA of the pair.
+__device__ __forceinline__ void pair_tma_load_4d(void *dst, const CUtensorMap *map, uint32_t bar, int c0, int c1,
+                                                 int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+      " [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
+}
+
 // Shared-memory matrix descriptor, 128-byte swizzle, sm_100 version field.
 //  K-major tiles (rows of 128 B holding 64 16-bit K elements): lbo unused,
 //  sbo = 1024 (8-row group stride).  MN-major tiles (rows = K, 128 B = 64 MN

@@ -641,6 +641,17 @@ def test_prefix_many_rows_fp32(cuda, dtype, D, B, Hq, Hkv, P, S, T):
     _check_prefix(*_prefix_case(cuda, dtype, D, B, Hq, Hkv, P, S, T, seed=P))
 
 
+@pytest.mark.parametrize("dtype,D,B,Hq,Hkv,P,S,T", [
+    # D 256 and more than 128 rows: pairs of CTAs; one key tile, a ragged last one, a second CTA
+    # with few rows or none, several row tiles, as many steps as the ring is long and more
+    ("bf16", 256, 17, 8, 1, 128, 5, 1), ("f16", 256, 129, 2, 2, 300, 5, 1), ("bf16", 256, 33, 8, 2, 1000, 9, 1),
+    ("f16", 256, 70, 8, 2, 20001, 33, 1), ("bf16", 256, 40, 8, 1, 33000, 20, 2), ("f16", 256, 65, 16, 1, 129, 40, 3),
+    ("bf16", 256, 64, 4, 2, 70000, 5, 1), ("bf16", 256, 300, 2, 2, 191, 3, 1),
+])
+def test_prefix_pairs(cuda, dtype, D, B, Hq, Hkv, P, S, T):
+    _check_prefix(*_prefix_case(cuda, dtype, D, B, Hq, Hkv, P, S, T, seed=P))
+
+
 @pytest.mark.parametrize("dtype,B", [("bf16", 2), ("bf16", 40), ("f32", 40)])
 def test_prefix_expanded_and_aliased_operands(cuda, dtype, B):
     """A prefix shared by the heads too (expanded), own slots shared by the batch, the
