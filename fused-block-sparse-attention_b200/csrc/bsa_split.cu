@@ -126,7 +126,10 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 // fp32, split_f32_kernel: the same on three bf16 terms of every operand (above).  A
 // contraction may take its index in any order and O's rows any place, so a thread's
 // 16-byte piece of a K row is its two pairs of a k-step (dims 4t .. 4t+3), and 16-byte
-// pieces of V rows feed four tiles of O (tile e holds columns 4j + e of a group).
+// pieces of V rows feed four tiles of O (tile e holds columns 4j + e of a group).  The
+// products truncate their sums, always towards zero, so a chunk's part of O starts at zero
+// and is added by a rounding addition (20000 keys, D 256: 4.7e-7 of the output's norm;
+// summed on in the products 1.2e-5, and plain fp32 arithmetic 2.9e-7).
 template <typename T, int D>
 struct SplitCfg {
   static constexpr int ES = sizeof(T), E16 = 16 / ES;
@@ -942,13 +945,15 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
           }
 #pragma unroll
           for (int n = 0; n < NR; ++n) {
-            float *o = acc[n][v * VW + e];
+            float o[4] = {0.f, 0.f, 0.f, 0.f};  // this chunk's part (above)
             mma16<__nv_bfloat16>(o, a[2], pb[n][0][0], pb[n][1][0]);
             mma16<__nv_bfloat16>(o, a[0], pb[n][0][2], pb[n][1][2]);
             mma16<__nv_bfloat16>(o, a[1], pb[n][0][1], pb[n][1][1]);
             mma16<__nv_bfloat16>(o, a[1], pb[n][0][0], pb[n][1][0]);
             mma16<__nv_bfloat16>(o, a[0], pb[n][0][1], pb[n][1][1]);
             mma16<__nv_bfloat16>(o, a[0], pb[n][0][0], pb[n][1][0]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) acc[n][v * VW + e][x] += o[x];
           }
         }
       }
@@ -1031,8 +1036,8 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
 // same keys.  The chunk's K and V are turned into operands (three bf16 terms, in the order
 // of the products' registers) once for the CTA, where the kernel above does it for every
 // 16 or 32 rows: with many rows that was two thirds of its instructions.  Bound by the
-// products (mma.sync): 1200 rows x 20000 keys, D 256, 8 heads, in 5.24 ms, 225 TFLOP/s of
-// bf16 products (of 300 measured); 7.94 ms by the kernel above.  Which rows take it:
+// products (mma.sync): 1200 rows x 20000 keys, D 256, 8 heads, in 5.46 ms, 216 TFLOP/s of
+// bf16 products (of 300 measured); 8.46 ms by the kernel above.  Which rows take it:
 // rows_over_warps.
 template <int D>
 struct RowsCfg {
@@ -1246,18 +1251,25 @@ __global__ void __launch_bounds__(RowsCfg<D>::W * 32, 1)
       for (int k = 0; k < 3; ++k) a[k] = fv[(ks * 3 + k) * 32 + lane];
       const uint32_t a0[4] = {a[0].x, a[0].y, a[0].z, a[0].w}, a1[4] = {a[1].x, a[1].y, a[1].z, a[1].w};
       const uint32_t a2[4] = {a[2].x, a[2].y, a[2].z, a[2].w};
+      float o[NR][4];
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a2, pb[n][0][0], pb[n][1][0]);
+      for (int n = 0; n < NR; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a0, pb[n][0][2], pb[n][1][2]);
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(o[n], a2, pb[n][0][0], pb[n][1][0]);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a1, pb[n][0][1], pb[n][1][1]);
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(o[n], a0, pb[n][0][2], pb[n][1][2]);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a1, pb[n][0][0], pb[n][1][0]);
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(o[n], a1, pb[n][0][1], pb[n][1][1]);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a0, pb[n][0][1], pb[n][1][1]);
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(o[n], a1, pb[n][0][0], pb[n][1][0]);
 #pragma unroll
-      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(acc[n][ks], a0, pb[n][0][0], pb[n][1][0]);
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(o[n], a0, pb[n][0][1], pb[n][1][1]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n) mma16<__nv_bfloat16>(o[n], a0, pb[n][0][0], pb[n][1][0]);
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[n][ks][e] += o[n][e];
     }
   }
   // ---- this warp's rows
@@ -1522,10 +1534,10 @@ static int split_count_t(long long groups, int R, long long n, int sms) {
 }
 
 // Whether the rows of a shared prefix go over the warps (split_f32_rows_kernel).  Times of
-// it against split_f32_kernel, 20000 keys, 8 heads, us: D 256, 36 rows 278 : 373, 1200 rows
-// 5240 : 7940; D 128, 64 rows 254 : 197, 96 rows 245 : 287, 1200 rows 2347 : 3124; D 64,
-// 96 rows 153 : 97, 1200 rows 1069 : 1143, with 2 heads 362 : 295 (its barriers and the
-// one CTA per SM show where a chunk has few products).
+// it against split_f32_kernel, 20000 keys, 8 heads, us: D 256, 36 rows 290 : 382, 1200 rows
+// 5461 : 8456; D 128, 64 rows 245 : 209, 96 rows 247 : 305, 1200 rows 2359 : 3396; D 64,
+// 96 rows 150 : 115, 1200 rows 1404 : 1290 (its barriers and the one CTA per SM show where
+// a chunk has few products).
 static bool rows_over_warps(int dtype, int D, bool fold, int R) {
   return dtype == BSA_F32 && fold && (D == 256 ? R > 32 : D == 128 && R > 64);
 }
