@@ -446,7 +446,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
   uint8_t *sQ = sm;                                   // [ROWS][D] swizzled
   uint8_t *ring = sm + ROWS * D * 2;
-  int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
+  int *s_blk = reinterpret_cast<int *>(ring + p.ring);  // with a selection: 3 * kMaxLive words
   float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
   // Launched to start beside the prefix kernel: its last CTA ends no earlier than that
   // kernel, so that waiting for this grid is waiting for both.
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
   const int len = sp.len, r0 = sp.r0;
   const T *kb_ = reinterpret_cast<const T *>(p.k) + (p.fold ? 0 : sp.b * p.k_sb) + sp.hk * p.k_sh;
   const T *vb_ = reinterpret_cast<const T *>(p.v) + (p.fold ? 0 : sp.b * p.v_sb) + sp.hk * p.v_sh;
-  uint8_t *wring = ring + warp * NST * C::STAGE;
+  uint8_t *wring = ring + warp * p.stages * C::STAGE;
   const uint32_t wr0 = smem_u32(wring);
   const uint64_t policy = evict_first_policy();
   const T *k2_ = nullptr, *v2_ = nullptr;  // the shared keys
@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
   uint8_t *sQ = sm;                                   // fp32 rows first, then three bf16 terms [ROWS][D]
   uint8_t *ring = sm + 3 * ROWS * D * 2;
-  int *s_blk = reinterpret_cast<int *>(ring + C::RING);  // with a selection: 3 * kMaxLive words
+  int *s_blk = reinterpret_cast<int *>(ring + p.ring);  // with a selection: 3 * kMaxLive words
   float *s_gate = reinterpret_cast<float *>(s_blk + kMaxLive);
   const bool last = p.after && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
   const int len = sp.len, r0 = sp.r0;
   const float *kb_ = reinterpret_cast<const float *>(p.k) + (p.fold ? 0 : sp.b * p.k_sb) + sp.hk * p.k_sh;
   const float *vb_ = reinterpret_cast<const float *>(p.v) + (p.fold ? 0 : sp.b * p.v_sb) + sp.hk * p.v_sh;
-  uint8_t *wring = ring + warp * NST * C::STAGE;
+  uint8_t *wring = ring + warp * p.stages * C::STAGE;
   const uint32_t wr0 = smem_u32(wring);
   const uint64_t policy = evict_first_policy();
   const float *k2_ = nullptr, *v2_ = nullptr;  // the shared keys
@@ -1559,11 +1559,12 @@ int split_count(int dtype, int D, long long groups, int R, long long n, bool fol
 }
 
 template <typename T, int D, int ROWS, bool CL>
-static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream_t st) {
+static bsa_status launch_rows(SplitParams p, long long groups, cudaStream_t st) {
   using C = SplitCfg<T, D>;
   const int rtiles = (p.R + ROWS - 1) / ROWS;
-  const int base = ROWS * D * (C::ES == 4 ? 6 : 2) + C::RING, most = base + 3 * kMaxLive * 4;
-  static_assert(C::RING >= NW * ROWS * (D + 4) * 4, "the ring holds the warps' O for the join");
+  constexpr int rows = ROWS * D * (C::ES == 4 ? 6 : 2), join = NW * ROWS * (D + 4) * 4;
+  constexpr int most = rows + C::RING + 3 * kMaxLive * 4;
+  static_assert(C::RING >= join, "the ring holds the warps' O for the join");
   static_assert(C::KC * D * C::ES >= ROWS * C::KC * 4, "a chunk's K buffer holds its P");
   void (*kern)(const SplitParams, int, int);
   if constexpr (C::ES == 2)
@@ -1572,8 +1573,15 @@ static bsa_status launch_rows(const SplitParams &p, long long groups, cudaStream
     kern = split_f32_kernel<D, ROWS / 8, CL>;
   static std::atomic<uint64_t> done{0};
   allow_smem(reinterpret_cast<const void *>(kern), most, done);
+  // The ring: no more warps and stages than a CTA has chunks, so that short caches get more
+  // CTAs per SM (D 256, 1256 heads of 21 slots, us: fp32 79 -> 47, bf16 45 -> 27).
+  const long long n = p.sel ? (long long)p.kk * p.bs : p.nkeys;
+  const long long nch = (CL ? (p.n2 + C::KC - 1) / C::KC : 0) + (n + C::KC - 1) / C::KC;
+  const long long cps = std::max<long long>(NW, (nch + p.nsplit - 1) / p.nsplit);
+  p.stages = (int)std::min<long long>(C::NST, (cps + NW - 1) / NW);
+  p.ring = std::max(join, (int)std::min<long long>(NW, nch) * p.stages * C::STAGE);
   const dim3 grid((unsigned)(groups * rtiles), p.nsplit);
-  const int smem = p.sel ? most : base;
+  const int smem = rows + p.ring + (p.sel ? 3 * kMaxLive * 4 : 0);
   if constexpr (CL) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;

@@ -47,6 +47,7 @@ struct SplitParams {
   float *weight;        // optional, with logits
   int64_t w_sb, w_sh;
   int after;            // launched beside the kernel before it, whose end it waits for at its own
+  int stages, ring;     // ring stages per warp and bytes of the ring (split_mma, split_f32)
   int32_t *status;
 };
 
