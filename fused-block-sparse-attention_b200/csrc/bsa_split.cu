@@ -1644,20 +1644,23 @@ static bsa_status launch_split(int dtype, int D, const SplitParams &p, cudaStrea
 }
 
 // CTAs of the cluster that does a (b, hk) of R rows and n keys in one launch, or 0 where
-// splits and a join are the better way: more rows than a tile, or more than 32 rounds of
-// a CTA's warps in all (four per CTA of a full cluster), unless one CTA per head is what
-// the splits come to.  One launch saves 3 us of the host's time and the partial sums'
-// way through memory; with few heads and many keys eight CTAs per head draw too little
-// of HBM (fp32, D 64, two sequences of 4097 slots, two heads: 9.4 us by splits, 19 by
-// clusters).
+// splits and a join are the better way: more rows than a tile, or more than 16 rounds of a
+// CTA's warps in all (fp32: 4, its rounds are three times as long), unless one CTA per head
+// is what the splits come to.  One launch saves 3 us of the host's time and the partial
+// sums' way through memory; with few heads and many keys eight CTAs per head draw too little
+// of HBM.  Device time, clusters : splits, us: bf16, D 256, one sequence, 1000 slots, 2 heads
+// 10.4 : 8.9, 2000 slots, 8 heads 12.2 : 9.6; fp32, D 128, 500 slots, 32 heads 11.2 : 12.1,
+// 1000 slots, 16 heads 22.3 : 12.6.  All CTAs of a launch have to run at once (bf16, D 256,
+// 148 heads of 300 slots: 20.4 in pairs, one CTA per SM, 12.3 alone).
 static int cluster_size(int dtype, int D, long long groups, int R, long long n) {
   const int es = (int)elem_size(dtype), kc = es == 2 && D <= 64 ? 32 : 16;
   const int most = D == 256 || (es == 2 && D == 32) ? 16 : 32;
   const long long steps = (n + kc * NW - 1) / (kc * NW);
   if (R > most) return 0;
-  if (steps > 32) return split_count(dtype, D, groups, R, n) == 1 ? 1 : 0;
+  if (steps > (es == 4 ? 4 : 16)) return split_count(dtype, D, groups, R, n) == 1 ? 1 : 0;
+  const int slots = kc * D * es * 2 >= 16384 ? 148 : 2 * 148;  // SplitCfg's CTAs per SM
   int cs = 1;
-  while (cs < 8 && cs * 2 <= steps && groups * cs * 2 <= 2 * 148) cs *= 2;
+  while (cs < 8 && cs * 2 <= steps && groups * cs * 2 <= slots) cs *= 2;
   return cs;
 }
 
