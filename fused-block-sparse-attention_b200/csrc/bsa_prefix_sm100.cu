@@ -3,16 +3,21 @@
 //
 //   S = Q K^T, P = 2^(S * scale * log2e - m), O += P V   per 128 prefix keys,
 // with K, V through shared memory by TMA, S, P and O in TMEM, and (m, l, O) of the
-// split left in fp32 for split_join_kernel.  Unlike the sequence forward, a row tile
-// gathers its rows from different sequences, every key is visible to every row, and
-// the keys are split so that all SMs work on few rows.
+// split left in fp32 for split_join_kernel.  P goes in as two 16-bit terms (split2), as in
+// the split kernels, so that its rounding does not add to the output's and a sequence's
+// precision does not hang on how many others are served beside it: in one term the error
+// against 64 bits was 1.4 times that of the output's rounding alone (bf16, 65536 keys
+// 2.33e-3 -> 1.65e-3; f16, 32768 keys 2.92e-4 -> 2.08e-4).  The second product with V took
+// these from 46 to 51.5 us and from 108 to 123.  Unlike the sequence forward, a row tile gathers its rows
+// from different sequences, every key is visible to every row, and the keys are split so
+// that all SMs work on few rows.
 //
 // NT = 2 (D 64, 128; more than 128 rows): one CTA owns two row tiles that share every
 // K/V tile: half the shared-memory fill per product.  NT = 1: up to 128 rows.  PAIR (D 256,
 // more than 128 rows; O fills TMEM, so a CTA holds one row tile): two CTAs' row tiles in
 // one product (M = 256), each with half of every K and V tile in its shared memory; alone,
 // each read all of K and V, and their way from L2 bounded both (39 bytes per cycle and SM;
-// 65536 keys, 256 rows of 2 heads: 58.9 us then, 44.5 now, a step at HBM's pace).  The first
+// 65536 keys, 256 rows of 2 heads, P in one term: 58.9 us alone, 44.5 in pairs).  The first
 // CTA issues for both and its barriers take both CTAs' loads and softmax warps; commits go
 // to both.  A tile's step is a chain S -> softmax -> PV, so what counts is
 // that the next S is there when a softmax ends:
@@ -20,9 +25,9 @@
 //     under the exponentials of this one.  Eight softmax warps, half a row per thread;
 //     the halves exchange their maxima through shared memory.
 //   NT = 2 ("half steps"): TMEM holds O and 128 columns per tile besides; steps of 64
-//     keys use them as two S buffers, each overlaid by its own P, so S runs one step
-//     ahead.  (One buffer of 128 keys left S waiting for PV: 6600 cycles per 128 keys
-//     and pair of tiles, tensor pipe 33% busy.)  Four warps per tile, a row per thread.
+//     keys use them as two S buffers, each overlaid by both terms of its own P, so S runs
+//     one step ahead.  (One buffer of 128 keys left S waiting for PV: 6600 cycles per 128
+//     keys and pair of tiles, tensor pipe 33% busy.)  Four warps per tile, a row per thread.
 //
 // K and V move as units of min(D, 128) columns x one step's keys in one ring, so that PV is
 // issued with N = 128: a 128x64x16 product costs as much tensor time as three quarters
@@ -69,7 +74,8 @@ struct PX {
   // TMEM columns of tile t (step parity b)
   static constexpr int S(int t, int b) { return 128 * t + (HALF ? 64 * b : 0); }
   static constexpr int P(int t, int b) { return HALF ? S(t, b) : 128 * NT + 64 * t; }
-  static constexpr int O(int t) { return (HALF ? 256 : 192 * NT) + DP * t; }
+  static constexpr int PLO = HALF ? 32 : 64;       // from P's first term to its second
+  static constexpr int O(int t) { return 256 + DP * t; }
   static constexpr uint32_t COLS = O(NT - 1) + DP <= 256 ? 256 : 512;
   static_assert(O(NT - 1) + DP <= 512 && SMEM <= 232448 && (2 * U + 7 * NT + 2) * 8 + 4 <= 512, "fits the SM");
 };
@@ -275,13 +281,15 @@ __global__ void __launch_bounds__(PX<DP, NT, PAIR>::THREADS, 1)
         wait(&r_full[sl], ((n0 + u) / U) & 1);
         const uint64_t dv = tc05::sdesc(sR0 + sl * X::UNIT, X::CHUNK, 1024);
 #pragma unroll
-        for (int ks = 0; ks < X::UROWS / 16; ++ks)
-          if constexpr (PAIR)  // units are halves of the keys, N all columns
-            tc05::pair_mma_ts_if(on, tc05::taddr(tmem, 0, X::O(t)), ap + 32 * u + 8 * ks, dv + 128 * ks, IDESC_PV,
-                                 (j > 0 || u > 0 || ks > 0) ? 1u : 0u);
-          else
-            tc05::mma_f16_ts_if(on, tc05::taddr(tmem, 0, X::O(t) + 64 * UC * u), ap + 8 * ks, dv + 128 * ks, IDESC_PV,
-                                (j > 0 || ks > 0) ? 1u : 0u);
+        for (int term = 0; term < 2; ++term)
+#pragma unroll
+          for (int ks = 0; ks < X::UROWS / 16; ++ks)
+            if constexpr (PAIR)  // units are halves of the keys, N all columns
+              tc05::pair_mma_ts_if(on, tc05::taddr(tmem, 0, X::O(t)), ap + X::PLO * term + 32 * u + 8 * ks,
+                                   dv + 128 * ks, IDESC_PV, (j > 0 || u > 0 || term > 0 || ks > 0) ? 1u : 0u);
+            else
+              tc05::mma_f16_ts_if(on, tc05::taddr(tmem, 0, X::O(t) + 64 * UC * u), ap + X::PLO * term + 8 * ks,
+                                  dv + 128 * ks, IDESC_PV, (j > 0 || term > 0 || ks > 0) ? 1u : 0u);
         commit(&r_empty[sl]);
       }
       commit(&o_done[2 * t + b]);
@@ -393,14 +401,14 @@ __global__ void __launch_bounds__(PX<DP, NT, PAIR>::THREADS, 1)
       }
       const float off = m_used == -INFINITY ? 0.f : px_shift<T>() - m_used;
       const float2 sc2 = make_float2(p.scale2, p.scale2), of2 = make_float2(off, off);
-      uint32_t w[32];
+      uint32_t w[32], w2[32];  // the two terms of P
       float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
       for (int c = 0; c < 64; c += 2) {
         const float2 x = fma2(make_float2(s[c], s[c + 1]), sc2, of2);
         const float2 e = make_float2(ex2(x.x), ex2(x.y));
         sum[(c >> 1) & 1] = add2(sum[(c >> 1) & 1], e);
-        w[c >> 1] = Mma<T>::pack(e.x, e.y);
+        split2<T>(e.x, e.y, w[c >> 1], w2[c >> 1]);
       }
       const float2 st = add2(sum[0], sum[1]);
       l += st.x + st.y;
@@ -421,6 +429,7 @@ __global__ void __launch_bounds__(PX<DP, NT, PAIR>::THREADS, 1)
         tc05::wait_st();
       }
       tc05::st32(tp, reinterpret_cast<const float *>(w));
+      tc05::st32(tp + X::PLO, reinterpret_cast<const float *>(w2));
       tc05::wait_st();
       tc05::fence_before();
       __syncwarp();
@@ -489,14 +498,15 @@ namespace {
 // Row tiles of 128 or 256, and the splits of the prefix (an SM each, or two for a pair).
 // The kernel that reads the sequences' own slots starts on the SMs that this one leaves
 // free, so fewer splits than fill the SMs can be the faster whole.  The split is the one of
-// the least estimate, from measured times: a CTA's key tiles (1.46 us with a pair, 1.83 with
-// two row tiles of D 128) and its start and end; own slots at 24 GB/s per CTA beside this
-// kernel, two per SM up to D 128; what does not fit beside it comes after, never in less
+// the least estimate, from measured times: a CTA's key tile (all 148 SMs busy, us, bf16 and
+// f16: one row tile D 32 1.2, D 64 1.3, D 128 1.3, D 256 2.6; two row tiles D 32 2.0, D 64
+// 2.1, D 128 2.4; a pair 2.1) and its start and end; own slots at 19.5 GB/s per CTA beside
+// this kernel, two per SM up to D 128; what does not fit beside it comes after, never in less
 // than most of a CTA's time; the join reads and writes 8 bytes per row, column and split.
-// Lengths are not known here: half of the capacity is assumed.  Measured, us: 32768 keys,
-// 512 rows of 8 heads, D 128, 128 sequences of up to 1024 slots: 5, 6, 7, 8 splits 110, 107,
-// 108, 112; 65536 keys, 256 rows of 2 heads, D 256, 32 of up to 512: 26, 28, 31, 32, 37
-// splits 45, 44, 44, 55, 53.
+// Lengths are not known here: half of the capacity is assumed.  Only speed hangs on any of
+// it.  Measured at two shapes, us: 32768 keys, 512 rows of 8 heads, D 128, 128 sequences of
+// up to 1024 slots: 4, 5, 6, 7, 8 splits 163, 140, 126, 129, 133; 65536 keys, 256 rows of 2
+// heads, D 256, 32 of up to 512: 26, 28, 31, 32, 37 splits 57, 56, 53, 54, 62.
 void prefix_shape(const bsa_decode_prefix_args *a, int &nt, bool &pair, int &rtiles, int &cps, int &nsplit) {
   const int R = a->B * (a->Hq / a->Hkv) * a->T;
   nt = a->D <= 128 && R > 128 ? 2 : 1;
@@ -504,8 +514,9 @@ void prefix_shape(const bsa_decode_prefix_args *a, int &nt, bool &pair, int &rti
   const int sms = pair ? 2 : 1;  // of one CTA or pair
   rtiles = (R + 128 * nt * sms - 1) / (128 * nt * sms);
   const long long items = (long long)a->Hkv * rtiles, nkt = (a->P + PX_KEYS - 1) / PX_KEYS;
-  const double tile = pair ? 1.46 : nt == 2 ? 1.83 : 1.5, ends = pair ? 9 : 5;  // us
-  const double cta = (double)a->S * a->D * 2 / 24e3;                            // of one sequence and head
+  const double tile = pair ? 2.1 : nt == 2 ? (a->D == 128 ? 2.4 : 2.1) : a->D == 256 ? 2.6 : 1.3;  // us
+  const double ends = pair ? 9 : 5;
+  const double cta = (double)a->S * a->D * 2 / 19.5e3;                          // of one sequence and head
   const double own = (double)a->B * a->Hkv * cta / (a->D == 256 ? 1 : 2);       // SM time
   const double join = (double)a->Hkv * R * a->D * 8 / 5e6;                      // per split
   double best = -1;

@@ -8,6 +8,8 @@
 // so splits of one cache and splits of two different K/V (a shared prefix and a
 // sequence's own slots) are joined alike.
 #pragma once
+#include <type_traits>
+
 #include "bsa_common.cuh"
 
 namespace bsa {
@@ -50,6 +52,27 @@ struct SplitParams {
   int stages, ring;     // ring stages per warp and bytes of the ring (split_mma, split_f32)
   int32_t *status;
 };
+
+// p, q >= 0 as two 16-bit terms each, p = hi + lo up to 2^-16 p (bf16) or 2^-22 p + 2^-25
+// (f16), packed.  hi is cut off below p, never rounded to it, so that both terms of a
+// positive p are positive and an infinity times them stays what it is (a term that is zero
+// or negative makes infinity - infinity of it); p = 0 gives 0 and 0.  f16 has no terms below
+// 2^-24: there hi is left 2^-24 further below p, and p < 2^-23 may lose a term.
+template <typename T>
+__device__ __forceinline__ void split2(float p, float q, uint32_t &hi, uint32_t &lo) {
+  constexpr float kBelow = 1.f - 0x1p-24f;  // the next float below
+  if constexpr (std::is_same<T, __half>::value) {
+    asm("cvt.rz.relu.f16x2.f32 %0, %1, %2;"
+        : "=r"(hi)
+        : "f"(fmaf(q, kBelow, -0x1p-24f)), "f"(fmaf(p, kBelow, -0x1p-24f)));
+    const float2 h = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+    lo = Mma<T>::pack(p - h.x, q - h.y);
+  } else {
+    const uint32_t a = __float_as_uint(p * kBelow), b = __float_as_uint(q * kBelow);
+    hi = __byte_perm(a, b, 0x7632);
+    lo = Mma<T>::pack(p - __uint_as_float(a & 0xffff0000u), q - __uint_as_float(b & 0xffff0000u));
+  }
+}
 
 // Global row (b*Hq + h)*T + t of local row r of K/V head hk.
 __device__ __forceinline__ long long split_row(const SplitParams &p, int b, int hk, int r, int &rb,
