@@ -121,7 +121,10 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 // O's registers was padding; 480 instructions per 16 keys at D 128 kept the warps from
 // drawing their share of HBM.  P^T reaches its operand layout by movmatrix, in two 16-bit
 // terms (p = hi + lo, hi = round(p), lo = round(p - hi)), so its rounding does not add to
-// the output's; the extra products are free under HBM's time.
+// the output's; the extra products are free under HBM's time.  f16 has nothing below 2^-24, so
+// there P, l and O are 2^15 larger and m is kept 15 lower: with p = 1 for the largest, many keys
+// 2^-20 and less below it (behind an attention sink) lost bits or came to nothing in O
+// while l counted them.
 //
 // fp32, split_f32_kernel: the same on three bf16 terms of every operand (above).  A
 // contraction may take its index in any order and O's rows any place, so a thread's
@@ -441,6 +444,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
     split_mma_kernel(const SplitParams p, int rtiles, int min_chunks) {
   using C = SplitCfg<T, D>;
   constexpr int KC = C::KC, NST = C::NST, KS = D / 16, KT = KC / 16, ROWS = 8 * NR, SO = D + 4;
+  constexpr float SHIFT = std::is_same<T, __half>::value ? 15.f : 0.f;  // of m below the maximum
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int s_n;
   __shared__ float s_m[NW][ROWS], s_l[NW][ROWS];
@@ -588,7 +592,7 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) mx[h] = fmax_nan(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], o));
-        const float mn = fmax_nan(m[n][h], mx[h]);
+        const float mn = fmax_nan(m[n][h], mx[h] - SHIFT);
         al[h] = mn == -INFINITY ? 1.f : ex2(m[n][h] - mn);
         m[n][h] = mn;
       }

@@ -52,3 +52,71 @@ def test_prefix_rounds_the_output_alone(cuda, dtype, D, B, Hq, Hkv, P, T):
     ref = _ref_prefix(q, pk, pv, k, v, lens)
     err, once = (x.norm() / ref.norm() for x in (o - ref, ref.to(dt).double() - ref))
     assert err <= 1.05 * once, "%.3g against %.3g of one rounding" % (err, once)
+
+
+# A sink: one slot that takes nearly all of the weight and holds V = 0, and n slots `gap` nats
+# below it, alike in weight, V around 1000, so that the output is theirs alone.  One product of
+# a logit is not zero, so it is exact but for fp32 roundings of at most 26 (its size in log2
+# units): three of 2^-24 (the product of the scale and log2 e, that with the logit, the
+# subtraction of the maximum) and, in fp32, 2^-21 of dropped terms, with 2^-22 of ex2 less than
+# 2^-15 together.  A softmax weight goes into the products with two terms: to 2^-16 of itself
+# (bf16), and f16 to 2^-25 absolutely with the largest at 2^15, so to 2^-25 2^(26-15) = 2^-14
+# at 18 nats.  fp32: three terms, 2^-21 with the dropped products.  Then the output's rounding.
+GAPS = (12.1, 14.3, 16.2, 17.9)
+TERM = {"bf16": 2 ** -16, "f16": 2 ** -14, "f32": 2 ** -21}
+
+
+def _sink(dt, D, n, seed, dev):
+    """q (4, 1, D) of one head per gap and k, v (1 + n, D), the sink first."""
+    g = torch.Generator().manual_seed(seed)
+    q = torch.zeros(4, 1, D)
+    q[:, 0, 0] = torch.tensor(GAPS) * D ** 0.5 / 8
+    k = torch.randn(1 + n, D, generator=g)
+    k[:, 0] = 0
+    k[0, 0] = 8
+    v = 1000 + 250 * torch.randn(1 + n, D, generator=g)
+    v[0] = 0
+    return (x.to(dt).to(dev) for x in (q, k, v))
+
+
+def _check_sink(dtype, o, q, k, v, term=None):
+    x = q[:, 0].double() @ k.double().t() * q.shape[-1] ** -0.5
+    p = torch.softmax(x, -1)
+    ref, mean = p @ v.double(), p @ v.double().abs()
+    tol = torch.finfo(o.dtype).eps / 2 + 2 ** -15 + (term or TERM[dtype])
+    err = (o.double() - ref).norm(dim=-1) / mean.norm(dim=-1)
+    assert bool((err <= tol).all()), "%.3g of the norm, %.3g allowed" % (err.max(), tol)
+    return p
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,B,Hkv,n", [
+    # one launch; splits; so many heads that a warp has thousands of slots to itself
+    (64, 1, 1, 1500), (256, 2, 1, 900), (32, 2, 2, 500), (128, 1, 2, 40000), (32, 1, 1, 30000), (64, 40, 8, 20000),
+])
+def test_weighted_behind_a_sink(cuda, dtype, D, B, Hkv, n):
+    import _bsa
+    q, k, v = _sink(DT[dtype], D, n, n, cuda)
+    w = torch.zeros(B, Hkv, 1 + n, device=cuda)
+    o = _bsa.decode_weighted(q.repeat(B, Hkv, 1, 1), k.expand(B, Hkv, -1, -1), v.expand(B, Hkv, -1, -1), w)
+    p = _check_sink(dtype, o.view(B, Hkv, 4, D), q, k, v).sum(0)
+    assert bool(((w.double() - p).abs() <= 2 ** -14 * p).all())
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,B,Hkv,n,S", [
+    # the sink and the others in the prefix: one launch, split kernels; in the own slots
+    (64, 2, 1, 1000, 1), (128, 3, 2, 30000, 1), (32, 4, 1, 20000, 1), (256, 1, 2, 9000, 1), (64, 3, 2, 0, 20000),
+])
+def test_prefix_behind_a_sink(cuda, dtype, D, B, Hkv, n, S):
+    import _bsa
+    q, k, v = _sink(DT[dtype], D, max(n, S), n, cuda)
+    if n:    # no own slots in use
+        pk, pv, lens = k.expand(Hkv, -1, -1), v.expand(Hkv, -1, -1), torch.zeros(B, dtype=torch.int32, device=cuda)
+        ko = vo = torch.zeros(B, Hkv, S, D, dtype=k.dtype, device=cuda)
+    else:
+        pk = pv = torch.zeros(Hkv, 0, D, dtype=k.dtype, device=cuda)
+        ko, vo = k.expand(B, Hkv, -1, -1), v.expand(B, Hkv, -1, -1)
+        lens = torch.full((B,), 1 + S, dtype=torch.int32, device=cuda)
+    o = _bsa.decode_prefix(q.repeat(B, Hkv, 1, 1), pk, pv, ko, vo, lens)
+    _check_sink(dtype, o.view(B, Hkv, 4, D), q, k, v)
