@@ -120,3 +120,22 @@ def test_prefix_behind_a_sink(cuda, dtype, D, B, Hkv, n, S):
         lens = torch.full((B,), 1 + S, dtype=torch.int32, device=cuda)
     o = _bsa.decode_prefix(q.repeat(B, Hkv, 1, 1), pk, pv, ko, vo, lens)
     _check_sink(dtype, o.view(B, Hkv, 4, D), q, k, v)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,B,Hkv,n", [
+    # many rows: the tensor-memory kernel (one row tile, two, pairs), fp32 rows over the warps;
+    # the last three with so many that one split has all of the keys
+    (64, 12, 1, 9000), (128, 8, 2, 9000), (128, 70, 1, 12000), (256, 9, 2, 6000),
+    (64, 4736, 2, 2900), (128, 4736, 2, 2900), (256, 2368, 2, 2900),
+])
+def test_prefix_of_many_rows_behind_a_sink(cuda, dtype, D, B, Hkv, n):
+    """The tensor-memory kernel's maximum may lag by 2 (log2), f16 terms start at 2^13:
+    2^-25 2^(26-13) = 2^-12 of a weight at 18 nats."""
+    import _bsa
+    q, k, v = _sink(DT[dtype], D, n, n, cuda)
+    pk, pv = (x.repeat(Hkv, 1, 1) for x in (k, v))
+    pk[1:], pv[1:] = pk[1:].roll(-1, 1), pv[1:].roll(-1, 1)   # the second head's sink comes last
+    own = torch.zeros(B, Hkv, 1, D, dtype=k.dtype, device=cuda)
+    o = _bsa.decode_prefix(q.repeat(B, Hkv, 1, 1), pk, pv, own, own, torch.zeros(B, dtype=torch.int32, device=cuda))
+    _check_sink(dtype, o.view(B, Hkv, 4, D), q, k, v, 2 ** -12 if dtype == "f16" else None)
