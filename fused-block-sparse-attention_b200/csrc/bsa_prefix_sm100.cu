@@ -8,9 +8,9 @@
 // precision does not hang on how many others are served beside it: in one term the error
 // against 64 bits was 1.4 times that of the output's rounding alone (bf16, 65536 keys
 // 2.33e-3 -> 1.65e-3; f16, 32768 keys 2.92e-4 -> 2.08e-4).  The second product with V took
-// these from 46 to 51.5 us and from 108 to 123.  Unlike the sequence forward, a row tile gathers its rows
-// from different sequences, every key is visible to every row, and the keys are split so
-// that all SMs work on few rows.
+// these from 46 to 51.5 us and from 108 to 123.  Unlike the sequence forward, a row tile
+// gathers its rows from different sequences, every key is visible to every row, and the
+// keys are split so that all SMs work on few rows.
 //
 // NT = 2 (D 64, 128; more than 128 rows): one CTA owns two row tiles that share every
 // K/V tile: half the shared-memory fill per product.  NT = 1: up to 128 rows.  PAIR (D 256,
@@ -52,8 +52,9 @@ constexpr int PX_CHUNK = PX_KEYS * 64 * 2;  // 16 KB: 128 rows x 64 columns
 // so P may be as much larger than 1.  f16 ends at 2^16 and has nothing below 2^-24: there P is
 // 2^13 larger (at most 2^15; m is stored lower by as much), so that keys 18 nats below the
 // largest, many of them behind an attention sink, still count to half a step of f16.  With
-// 2^7 and 8 their sum was off by 0.5% (one split of 2900 keys); 2^13 and 2 cost 5% of the time (32768 keys, 512 rows
-// of 8 heads, D 128: 138.2 us with 8, 138.5 with 4, 142 with 3, 146 with 2, 150 with 1).
+// 2^7 and 8 their sum was off by 0.5% (one split of 2900 keys); 2^13 and 2 cost 5% of the
+// time (32768 keys, 512 rows of 8 heads, D 128, at the power limit: 138.2 us with 8, 138.5
+// with 4, 142 with 3, 146 with 2, 150 with 1).
 template <typename T>
 constexpr float px_shift() {
   return std::is_same<T, __half>::value ? 13.f : 0.f;

@@ -42,18 +42,24 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
 }
 
-// fp32 products on the tensor cores: x = x1 + x2 + x3, each the bf16 rounding of what is
-// left (8 bits each, so all 24), and x y = x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1 up
-// to 2^-23 |x y| (the other three).  Six bf16 products take the time of one and a half
-// tf32 ones (mma.sync, measured 300 against 80 TFLOP/s), of which two-term tf32 splits
-// need three.  The terms of two neighbours, packed; an infinity is its own first term.
+// fp32 products on the tensor cores: x = x1 + x2 + x3, each what is left cut off to bf16 (8
+// bits each, so all 24), and x y = x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1 up to
+// 2^-21 |x y| (the other three; 2^-24.6 on average).  Six bf16 products take the time of one
+// and a half tf32 ones (mma.sync, measured 300 against 80 TFLOP/s), of which two-term tf32
+// splits need three.  The terms of two neighbours, packed.  Each is cut off below what is
+// left, so that all have the sign of x and none is zero: an infinity (its own first term, the
+// others zero) times them stays what it is, where terms of unlike sign make infinity -
+// infinity of it, and cutting off does not take the largest floats to infinity.
 __device__ __forceinline__ void split3(float x, float y, uint32_t *u) {
-  u[0] = Mma<__nv_bfloat16>::pack(x, y);
-  float x1 = __uint_as_float(u[0] << 16), y1 = __uint_as_float(u[0] & 0xffff0000u);
+  constexpr float kBelow = 1.f - 0x1p-24f;  // the next float below
+  uint32_t a = __float_as_uint(x * kBelow), b = __float_as_uint(y * kBelow);
+  u[0] = __byte_perm(a, b, 0x7632);
+  float x1 = __uint_as_float(a & 0xffff0000u), y1 = __uint_as_float(b & 0xffff0000u);
   const float rx = x == x1 ? 0.f : x - x1, ry = y == y1 ? 0.f : y - y1;
-  u[1] = Mma<__nv_bfloat16>::pack(rx, ry);
-  x1 = __uint_as_float(u[1] << 16), y1 = __uint_as_float(u[1] & 0xffff0000u);
-  u[2] = Mma<__nv_bfloat16>::pack(rx - x1, ry - y1);
+  a = __float_as_uint(rx * kBelow), b = __float_as_uint(ry * kBelow);
+  u[1] = __byte_perm(a, b, 0x7632);
+  x1 = __uint_as_float(a & 0xffff0000u), y1 = __uint_as_float(b & 0xffff0000u);
+  u[2] = __byte_perm(__float_as_uint(rx - x1), __float_as_uint(ry - y1), 0x7632);
 }
 // Maximum that keeps a NaN: a row with a NaN logit ends as NaN, not as an empty row.
 __device__ __forceinline__ float fmax_nan(float a, float b) {
@@ -120,11 +126,10 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 // head group, times the new tokens), and with the rows as M half of every product and of
 // O's registers was padding; 480 instructions per 16 keys at D 128 kept the warps from
 // drawing their share of HBM.  P^T reaches its operand layout by movmatrix, in two 16-bit
-// terms (p = hi + lo, hi = round(p), lo = round(p - hi)), so its rounding does not add to
-// the output's; the extra products are free under HBM's time.  f16 has nothing below 2^-24, so
-// there P, l and O are 2^15 larger and m is kept 15 lower: with p = 1 for the largest, many keys
-// 2^-20 and less below it (behind an attention sink) lost bits or came to nothing in O
-// while l counted them.
+// terms (split2), so its rounding does not add to the output's; the extra products are
+// free under HBM's time.  f16 has nothing below 2^-24, so there P, l and O are 2^15 larger
+// and m is kept 15 lower: with p = 1 for the largest, many keys 2^-20 and less below it
+// (behind an attention sink) lost bits or came to nothing in O while l counted them.
 //
 // fp32, split_f32_kernel: the same on three bf16 terms of every operand (above).  A
 // contraction may take its index in any order and O's rows any place, so a thread's
@@ -622,11 +627,9 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<T, D>::MINB)
         for (int n = 0; n < NR; ++n)
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float x = s[kt][n][2 * h], y = s[kt][n][2 * h + 1];
-            const uint32_t u = Mma<T>::pack(x, y);
-            const T *ht = reinterpret_cast<const T *>(&u);
-            hi[n][h] = movmatrix(u);
-            lo[n][h] = movmatrix(Mma<T>::pack(x - Mma<T>::to_f(ht[0]), y - Mma<T>::to_f(ht[1])));
+            split2<T>(s[kt][n][2 * h], s[kt][n][2 * h + 1], hi[n][h], lo[n][h]);
+            hi[n][h] = movmatrix(hi[n][h]);
+            lo[n][h] = movmatrix(lo[n][h]);
           }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {

@@ -139,3 +139,110 @@ def test_prefix_of_many_rows_behind_a_sink(cuda, dtype, D, B, Hkv, n):
     own = torch.zeros(B, Hkv, 1, D, dtype=k.dtype, device=cuda)
     o = _bsa.decode_prefix(q.repeat(B, Hkv, 1, 1), pk, pv, own, own, torch.zeros(B, dtype=torch.int32, device=cuda))
     _check_sink(dtype, o.view(B, Hkv, 4, D), q, k, v, 2 ** -12 if dtype == "f16" else None)
+
+
+# Infinities where a row does look.  A V column that holds one is that infinity in the output
+# of every row that gives it weight (two of unlike sign: NaN) and the other columns are what
+# they are; a K row with -inf (or the type's lowest value) in a column that every query meets
+# with a positive number has logit -inf (or far below) and weight 0.
+def _infinite(k, v, q, at_v, at_k, low):
+    """Puts them into k, v (..., n, D) and returns (columns of v with +inf, -inf, both)."""
+    cols = (1, 2, 5)
+    for i, j in enumerate(at_v):
+        v[..., j, cols[i % 2]] = math.inf if i % 2 == 0 else -math.inf
+        v[..., j, cols[2]] = math.inf if i % 2 == 0 else -math.inf
+    for j in at_k:
+        k[..., j, 7] = low
+    q[..., 7] = q[..., 7].abs() + 0.5
+    return cols
+
+
+def _check_infinite(o, ref, tol, cols):
+    assert bool((o[..., cols[0]] == math.inf).all()) and bool((o[..., cols[1]] == -math.inf).all())
+    assert bool(o[..., cols[2]].isnan().all())
+    rest = [d for d in range(o.shape[-1]) if d not in cols]
+    err = (o.double() - ref).abs()[..., rest]
+    assert bool((err <= tol[..., rest]).all()), "%.3g" % err.max()
+
+
+def _attend(q, k, v, see, dead):
+    """Softmax attention of rows q (R, D) in 64 bits: see (R, n); dead: keys of weight 0."""
+    k, v = k.double().clone(), torch.where(v.isfinite(), v.double(), 0.0)
+    k[dead] = 0
+    x = (q.double() @ k.t() * q.shape[-1] ** -0.5).masked_fill(~see, -math.inf)
+    x[:, dead] = -math.inf
+    p = torch.softmax(x, -1)
+    # the bounds of the other test file: logits, P's terms, the output's rounding
+    D = q.shape[-1]
+    top = float(q.double().norm(dim=-1).max() * k.norm(dim=-1).max()) * D ** -0.5
+    e = 2 * (8 + (3 * D / 8 if q.dtype == torch.float32 else D / 8)) * 2 ** -23 * top + 2 ** -18
+    o = p @ v
+    return o, p, (2 * e + 2 ** -15) * v.abs().max() + torch.finfo(q.dtype).eps * o.abs()
+
+
+@pytest.mark.parametrize("low", [-math.inf, "lowest"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,B,Hq,Hkv,L,T,bs", [
+    # one launch, splits, several new tokens, selected blocks
+    (64, 2, 4, 2, 700, 1, 0), (256, 1, 8, 1, 500, 2, 0), (32, 1, 24, 1, 300, 3, 0), (128, 1, 8, 2, 9000, 1, 0),
+    (64, 1, 40, 2, 8000, 4, 0), (256, 1, 4, 2, 7000, 1, 0), (128, 1, 4, 2, 900, 1, 32),
+])
+def test_weighted_visible_infinities(cuda, dtype, D, B, Hq, Hkv, L, T, bs, low):
+    import _bsa
+    g = torch.Generator().manual_seed(L)
+    dt, grp = DT[dtype], Hq // Hkv
+    low = torch.finfo(dt).min if low == "lowest" else low
+    q = _rand(g, B, Hq, T, D, dt=dt, dev=cuda)
+    k, v = (_rand(g, B, Hkv, L, D, dt=dt, dev=cuda) for _ in range(2))
+    w = torch.rand(B, Hkv, L, generator=g).to(cuda)
+    at_k = [3, 40, L - T - 1]
+    slots, sel, kw = torch.arange(L, device=cuda), None, {}
+    if bs:
+        ids = [0, 1, (L - 1) // bs]
+        slots = torch.cat([torch.arange(i * bs, min(L, (i + 1) * bs), device=cuda) for i in ids])
+        sel, kw = torch.tensor(ids, dtype=torch.int32, device=cuda).expand(B, Hkv, 3), dict(bs=bs)
+    # the slots of a row's largest and least weight, and one between
+    x = q[0, 0, 0].double() @ k[0, 0, slots[:len(slots) - T]].double().t()
+    cols = _infinite(k, v, q, [int(slots[x.argmax()]), 33, int(slots[x.argmin()]), 17], at_k, low)
+    dead = (slots.unsqueeze(1) == torch.tensor(at_k, device=cuda)).any(1)
+    w0 = w.double()
+    o = _bsa.decode_weighted(q, k, v, w, sel, L=L, **kw)
+    add = torch.zeros_like(w0)
+    for b, h, t in itertools.product(range(B), range(Hkv), range(T)):
+        see = (slots <= L - T + t).expand(grp, -1)
+        rows = slice(h * grp, (h + 1) * grp)
+        ref, p, tol = _attend(q[b, rows, t], k[b, h, slots], v[b, h, slots], see, dead)
+        _check_infinite(o[b, rows, t], ref, tol, cols)
+        add[b, h, slots] += p.sum(0)
+    e = 2 ** -9    # of the logits' e above for these sizes (top < 2^6: (8 + 96) 2^-15)
+    assert bool(((w.double() - w0 - add).abs() <= e * add + 2 ** -23 * (w0 + add)).all())
+
+
+@pytest.mark.parametrize("low", [-math.inf, "lowest"])
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D,B,Hq,Hkv,P,S", [
+    # one launch, splits; many rows: one row tile, two, pairs, fp32 rows over the warps
+    (64, 2, 4, 2, 700, 3), (128, 2, 8, 2, 9000, 5), (64, 12, 4, 1, 9000, 3), (32, 40, 8, 1, 6000, 2),
+    (128, 40, 4, 1, 9000, 3), (256, 9, 4, 1, 3000, 3), (256, 40, 4, 1, 5000, 3),
+])
+def test_prefix_visible_infinities(cuda, dtype, D, B, Hq, Hkv, P, S, low):
+    import _bsa
+    g = torch.Generator().manual_seed(P)
+    dt, grp = DT[dtype], Hq // Hkv
+    low = torch.finfo(dt).min if low == "lowest" else low
+    q = _rand(g, B, Hq, 1, D, dt=dt, dev=cuda)
+    pk, pv = (_rand(g, Hkv, P, D, dt=dt, dev=cuda) for _ in range(2))
+    k, v = (_rand(g, B, Hkv, S, D, dt=dt, dev=cuda) for _ in range(2))
+    lens = torch.full((B,), S, dtype=torch.int32, device=cuda)
+    x = q[0, 0, 0].double() @ pk[0].double().t()
+    cols = _infinite(pk, pv, q, [int(x.argmax()), 33, int(x.argmin()), 17], [3, 40, P - 1], low)
+    _infinite(k, v, q, [], [0], low)
+    v[:, :, 1, cols[0]] = math.inf
+    o = _bsa.decode_prefix(q, pk, pv, k, v, lens)
+    dead = torch.zeros(P + S, dtype=torch.bool, device=cuda)
+    dead[[3, 40, P - 1, P]] = True
+    for b, h in itertools.product(range(B), range(Hkv)):
+        rows = slice(h * grp, (h + 1) * grp)
+        kk, vv = torch.cat([pk[h], k[b, h]]), torch.cat([pv[h], v[b, h]])
+        ref, _, tol = _attend(q[b, rows, 0], kk, vv, torch.ones(grp, P + S, dtype=torch.bool, device=cuda), dead)
+        _check_infinite(o[b, rows, 0], ref, tol, cols)
