@@ -145,6 +145,12 @@ class PrefixCache:
     def append(self, k_new, v_new, active=None):
         """Appends T tokens (B, Hkv, T, D) to every sequence, or to those whose entry of
         `active` (B truth values) is true."""
+        B, Hkv, _, D = self.k.shape
+        if k_new.dim() != 4 or v_new.shape != k_new.shape or \
+                (k_new.shape[0], k_new.shape[1], k_new.shape[3]) != (B, Hkv, D):
+            raise ValueError("k_new and v_new must be (%d, %d, T, %d)" % (B, Hkv, D))
+        if active is not None and len(active) != B:
+            raise ValueError("active must hold %d truth values" % B)
         T = k_new.shape[2]
         who = [b for b in range(len(self.used)) if active is None or active[b]]
         if any(self.used[b] + T > self.k.shape[2] for b in who):
