@@ -155,8 +155,6 @@ class PrefixCache:
         who = [b for b in range(len(self.used)) if active is None or active[b]]
         if any(self.used[b] + T > self.k.shape[2] for b in who):
             raise ValueError("cache full")
-        if not who:
-            return
         dev = self.k.device
         b = torch.tensor(who, device=dev, dtype=torch.long)
         at = torch.tensor([self.used[i] for i in who], device=dev, dtype=torch.long).view(-1, 1) + \

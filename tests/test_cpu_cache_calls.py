@@ -24,13 +24,3 @@ def test_append_of_another_shape_is_refused(k, v, active):
     with pytest.raises(ValueError):
         c.append(torch.ones(k), torch.ones(v), active)
     assert c.used == [0, 0, 0] and c.lens.tolist() == [0, 0, 0] and not c.k.any() and not c.v.any()
-
-
-@pytest.mark.parametrize("T,active", [(1, [False] * 3), (2, [0, 0, 0]), (0, None)])
-def test_append_of_nothing(T, active):
-    """No sequence takes part, or no token is new: the cache stays as it is."""
-    c = _prefix_cache()
-    c.append(torch.ones(3, 2, 2, 64), torch.ones(3, 2, 2, 64), [True, False, True])
-    k = c.k.clone()
-    c.append(torch.ones(3, 2, T, 64), torch.ones(3, 2, T, 64), active)
-    assert c.used == c.lens.tolist() == [2, 0, 2] and torch.equal(c.k, k)
