@@ -26,7 +26,8 @@ beside the first `sink` and the last `recent` tokens:
     cache.evict(4096, recent=256, sink=4)
 
 A survivor may move to a freed slot (cache.pos tells its token position), so keys are
-cached with their rotary embedding already applied, as the attention expects them.
+cached with their rotary embedding already applied, as the attention expects them.  Masks
+go by slot: with several new tokens (T > 1) attend before evicting, as above.
 
 A batch behind one prefix.  PrefixCache holds the prefix's K/V once and every
 sequence's own continuation, of any length; prefix_attention reads the prefix once
@@ -58,6 +59,7 @@ class DecodeCache:
         self.kmax = torch.zeros_like(self.kmin)
         self.L = 0          # slots in use
         self.seen = 0       # tokens appended so far
+        self.ordered = 0    # newest tokens that lie in the last slots, in order
         self.weight = self.pos = None
         if track:
             self.weight = torch.zeros(B, Hkv, max_len, dtype=torch.float32, device=device)
@@ -82,6 +84,7 @@ class DecodeCache:
             self.pos[:, :, L0:L1] = torch.arange(self.seen, self.seen + T, dtype=torch.int32,
                                                  device=self.pos.device)
         self.seen += T
+        self.ordered += T
 
     def evict(self, budget, *, recent=0, sink=0):
         """Keeps `budget` slots per (b, hk): the first `sink` and last `recent` tokens,
@@ -94,6 +97,7 @@ class DecodeCache:
         _bsa.evict(self.k, self.v, self.weight, self.pos, budget=budget, L=self.L, seen=self.seen,
                    recent=recent, sink=sink, kmin=self.kmin, kmax=self.kmax, bs=self.bs)
         self.L = budget
+        self.ordered = 0
         return gone
 
     def select_quest(self, q_new, *, topk, sink=True):
@@ -113,8 +117,17 @@ class DecodeCache:
         return sel[:, :, 0]
 
 
+def _check_order(q_new, cache):
+    """Masks go by slot, so rows before the last need the new tokens in the last slots: refused
+    when an eviction since may have moved them (one row sees every slot, in any order)."""
+    if q_new.shape[2] > max(1, cache.ordered) and cache.ordered < cache.seen:
+        raise ValueError("%d rows after an eviction, but only %d tokens appended since: attend "
+                         "before evicting" % (q_new.shape[2], cache.ordered))
+
+
 def decode_attention(q_new, cache, sel, gate=None, *, scale=None, mask_mode=_bsa.MASK_TOKEN):
     """o (B, Hq, T, D) of the T newest tokens attending to their selected cache blocks."""
+    _check_order(q_new, cache)
     return _bsa.decode(q_new, cache.k, cache.v, sel, gate, bs=cache.bs, L=cache.L,
                        mask_mode=mask_mode, scale=scale)
 
@@ -124,6 +137,7 @@ def decode_attention_weighted(q_new, cache, sel=None, gate=None, *, scale=None):
     cache.weight (a cache with track=True).  sel=None attends to every slot."""
     if cache.weight is None:
         raise ValueError("decode_attention_weighted needs a cache with track=True")
+    _check_order(q_new, cache)
     return _bsa.decode_weighted(q_new, cache.k, cache.v, cache.weight, sel, gate, bs=cache.bs,
                                 L=cache.L, scale=scale)
 

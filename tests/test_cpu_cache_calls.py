@@ -24,3 +24,55 @@ def test_append_of_another_shape_is_refused(k, v, active):
     with pytest.raises(ValueError):
         c.append(torch.ones(k), torch.ones(v), active)
     assert c.used == [0, 0, 0] and c.lens.tolist() == [0, 0, 0] and not c.k.any() and not c.v.any()
+
+
+@pytest.mark.parametrize("T,active", [(1, [False] * 3), (2, [0, 0, 0]), (0, None)])
+def test_append_of_nothing(T, active):
+    """No sequence takes part, or no token is new: the cache stays as it is."""
+    c = _prefix_cache()
+    c.append(torch.ones(3, 2, 2, 64), torch.ones(3, 2, 2, 64), [True, False, True])
+    k = c.k.clone()
+    c.append(torch.ones(3, 2, T, 64), torch.ones(3, 2, T, 64), active)
+    assert c.used == c.lens.tolist() == [2, 0, 2] and torch.equal(c.k, k)
+
+
+@pytest.fixture
+def decode_calls(monkeypatch):
+    """decode.py with CPU tensors, its launches recorded."""
+    import _bsa
+    import decode
+    calls = []
+    monkeypatch.setattr(_bsa, "pool", lambda x, bs, **kw: [torch.zeros(x.shape[0], x.shape[1], -(-x.shape[2] // bs), x.shape[3])] * 2)
+    for name in ("decode_weighted", "decode", "evict"):
+        monkeypatch.setattr(_bsa, name, lambda *a, _n=name, **kw: calls.append(_n))
+    return decode, calls
+
+
+def test_rows_of_moved_tokens_are_refused(decode_calls):
+    """A row's mask goes by slot.  An eviction may move the newest tokens to freed slots, where
+    the rows before them would see them; one row sees every slot and needs no order."""
+    decode, calls = decode_calls
+    c = decode.DecodeCache(1, 2, 40, 64, bs=8, device="cpu", track=True)
+    q = lambda T: _t(1, 4, T, 64)  # noqa: E731
+    sel = _t(1, 2, 2, dt=torch.int32)
+    c.append(_t(1, 2, 20, 64), _t(1, 2, 20, 64))
+    decode.decode_attention_weighted(q(20), c)
+    decode.decode_attention(q(3), c, sel)
+    assert c.evict(20) == 0                       # nothing went, nothing moved
+    decode.decode_attention_weighted(q(3), c)
+    assert c.evict(16) == 4
+    n = len(calls)
+    for call in (lambda: decode.decode_attention_weighted(q(2), c), lambda: decode.decode_attention(q(2), c, sel),
+                 lambda: decode.decode_attention_weighted(q(2), c, sel)):
+        with pytest.raises(ValueError):
+            call()
+    assert len(calls) == n
+    decode.decode_attention_weighted(q(1), c)
+    decode.decode_attention(q(1), c, sel)
+    c.append(_t(1, 2, 1, 64), _t(1, 2, 1, 64))
+    with pytest.raises(ValueError):
+        decode.decode_attention_weighted(q(2), c)
+    c.append(_t(1, 2, 2, 64), _t(1, 2, 2, 64))
+    decode.decode_attention_weighted(q(3), c)     # appended since: in order again
+    with pytest.raises(ValueError):
+        decode.decode_attention_weighted(q(4), c)
