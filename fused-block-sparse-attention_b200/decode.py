@@ -117,17 +117,9 @@ class DecodeCache:
         return sel[:, :, 0]
 
 
-def _check_order(q_new, cache):
-    """Masks go by slot, so rows before the last need the new tokens in the last slots: refused
-    when an eviction since may have moved them (one row sees every slot, in any order)."""
-    if q_new.shape[2] > max(1, cache.ordered) and cache.ordered < cache.seen:
-        raise ValueError("%d rows after an eviction, but only %d tokens appended since: attend "
-                         "before evicting" % (q_new.shape[2], cache.ordered))
-
-
 def decode_attention(q_new, cache, sel, gate=None, *, scale=None, mask_mode=_bsa.MASK_TOKEN):
-    """o (B, Hq, T, D) of the T newest tokens attending to their selected cache blocks."""
-    _check_order(q_new, cache)
+    """o (B, Hq, T, D) of the T newest tokens attending to their selected cache blocks; rows
+    before the last count on the new tokens lying in the last slots, in order."""
     return _bsa.decode(q_new, cache.k, cache.v, sel, gate, bs=cache.bs, L=cache.L,
                        mask_mode=mask_mode, scale=scale)
 
@@ -137,7 +129,12 @@ def decode_attention_weighted(q_new, cache, sel=None, gate=None, *, scale=None):
     cache.weight (a cache with track=True).  sel=None attends to every slot."""
     if cache.weight is None:
         raise ValueError("decode_attention_weighted needs a cache with track=True")
-    _check_order(q_new, cache)
+    T = q_new.shape[2]
+    if T > max(1, cache.ordered) and cache.ordered < cache.seen:
+        # masks go by slot, and the eviction may have moved a row's own and later tokens; one
+        # row sees every slot, in any order
+        raise ValueError("%d rows after an eviction, but only %d tokens appended since: attend "
+                         "before evicting" % (T, cache.ordered))
     return _bsa.decode_weighted(q_new, cache.k, cache.v, cache.weight, sel, gate, bs=cache.bs,
                                 L=cache.L, scale=scale)
 
