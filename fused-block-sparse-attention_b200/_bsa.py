@@ -602,6 +602,11 @@ def _row_operand(t, name, B, Hkv, n, dtype):
     raise BsaError(ERR_STRIDE, "%s must have unit stride along the slots" % name)
 
 
+def _int32(t):
+    """Ids or lengths as the kernels read them; 64-bit ones outside 32 bits stay outside."""
+    return (t.clamp(-1, 2 ** 31 - 1) if t.dtype == torch.int64 else t).to(torch.int32).contiguous()
+
+
 def _query_out(q, shape, out):
     """(q with unit stride along D, its strides, o, o's strides) of a decode step."""
     if len(shape) != 4:
@@ -688,7 +693,7 @@ def decode_weighted(q, k, v, weight, sel=None, gate=None, *, bs=None, L=None, sc
         if bs is None or not 0 < bs < 2 ** 30:
             raise BsaShapeError(ERR_ARG, "decode_weighted: a selection needs its block size bs")
         if sel.dtype != torch.int32 or sel.stride(-1) != 1:
-            sel = sel.to(torch.int32).contiguous()
+            sel = _int32(sel)
         ss, sst = sel.shape, sel.stride()
         if not (ss[0] == B and (len(ss) == 2 or (len(ss) == 3 and ss[1] in (1, Hkv)))):
             raise BsaShapeError(ERR_SHAPE, "decode_weighted: sel must be (B, kk) or (B, Hkv, kk)")
@@ -799,7 +804,7 @@ def decode_prefix(q, pk, pv, k, v, lens, *, scale=None, out=None):
     if lens.shape != (B,) or lens.is_floating_point():
         raise BsaShapeError(ERR_SHAPE, "decode_prefix: lens must be (B,) whole numbers")
     if lens.dtype is not torch.int32 or not lens.is_contiguous():
-        lens = lens.to(torch.int32).contiguous()
+        lens = _int32(lens)
     _launch("bsa_decode_prefix", _pack_prefix(
         _dtype(q), B, Hq, Hkv, D, ps[1], S, T, D ** -0.5 if scale is None else scale,
         q.data_ptr(), qst[0], qst[1], qst[2], pk.data_ptr(), 0, pkst[0], pkst[1], pv.data_ptr(), 0, pvst[0], pvst[1],

@@ -75,3 +75,36 @@ def test_rows_of_moved_tokens_are_refused(decode_calls):
     decode.decode_attention_weighted(q(3), c)     # appended since: in order again
     with pytest.raises(ValueError):
         decode.decode_attention_weighted(q(4), c)
+
+
+@pytest.fixture
+def ids_of(monkeypatch):
+    """_bsa with CPU tensors let through; what the launches would read as ids or lengths."""
+    import ctypes
+
+    import _bsa
+    got = []
+    structs = {"bsa_decode_weighted": (_bsa.DecodeWeightedArgs, "sel", 3), "bsa_decode_prefix": (_bsa.DecodePrefixArgs, "lens", 3)}
+
+    def launch(name, a, like):
+        cls, field, n = structs[name]
+        at = getattr(cls.from_buffer_copy(a), field)
+        got.append(list((ctypes.c_int32 * n).from_address(at)))
+    monkeypatch.setattr(_bsa, "_need_cuda", lambda *ts: None)
+    monkeypatch.setattr(_bsa, "status_tensor", lambda device: torch.zeros(1, dtype=torch.int32))
+    monkeypatch.setattr(_bsa, "_launch", launch)
+    return _bsa, got
+
+
+def test_wide_ids_and_lengths_stay_outside(ids_of):
+    """64-bit ids and lengths past 32 bits are outside the cache, not other ids and lengths."""
+    bsa, got = ids_of
+    for dt, x in ((torch.int64, [2 ** 32 + 1, -2 ** 33, 2]), (torch.int64, [2 ** 31, -2 ** 32 + 1, 0]),
+                  (torch.int32, [2 ** 31 - 1, -5, 1]), (torch.int16, [-1, 7, 3])):
+        bsa.decode_weighted(_t(1, 2, 1, 64), _t(1, 2, 256, 64), _t(1, 2, 256, 64), _t(1, 2, 256, dt=torch.float32),
+                            torch.tensor(x, dtype=dt).view(1, 3), bs=32)
+        bsa.decode_prefix(_t(3, 2, 1, 64), _t(2, 8, 64), _t(2, 8, 64), _t(3, 2, 9, 64), _t(3, 2, 9, 64),
+                          torch.tensor(x, dtype=dt))
+        for ids, end in zip(got[-2:], (8, 9)):
+            for a, b in zip(x, ids):
+                assert a == b if 0 <= a <= end else not 0 <= b <= end, (a, b)
