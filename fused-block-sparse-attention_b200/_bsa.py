@@ -193,6 +193,7 @@ SYMBOLS = {
     "bsa_decode_prefix": (ctypes.c_int, [ctypes.POINTER(DecodePrefixArgs), ctypes.c_void_p,
                                          ctypes.c_size_t, ctypes.c_void_p]),
     "bsa_status_decode": (ctypes.c_int, [ctypes.c_int32]),
+    "bsa_status_word": (ctypes.c_int, [ctypes.POINTER(ctypes.c_void_p)]),
     "bsa_last_error": (ctypes.c_char_p, []),
     "bsa_version": (ctypes.c_int32, []),
 }
@@ -265,6 +266,24 @@ def _prep(t):
 _status = {}
 
 
+class _Word:
+    """One int32 of device memory, for torch.as_tensor."""
+
+    def __init__(self, ptr):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (ptr, False), "version": 2}
+
+
+def _new_status(key):
+    """A zeroed status word of device `key`; while a stream is captured, one that is no part
+    of the graph (whose replays would clear it)."""
+    with torch.cuda.device(key):
+        if not torch.cuda.is_current_stream_capturing():
+            return torch.zeros(1, dtype=torch.int32, device="cuda:%d" % key)
+        p = ctypes.c_void_p()
+        _check(lib().bsa_status_word(ctypes.byref(p)))
+        return torch.as_tensor(_Word(p.value), device="cuda:%d" % key)
+
+
 def status_tensor(device):
     """The persistent device status word of `device` (int32, cleared by check_status)."""
     if isinstance(device, int):
@@ -273,7 +292,7 @@ def status_tensor(device):
         dev = torch.device(device)
         key = dev.index if dev.index is not None else torch.cuda.current_device()
     if key not in _status:
-        _status[key] = torch.zeros(1, dtype=torch.int32, device="cuda:%d" % key)
+        _status[key] = _new_status(key)
     return _status[key]
 
 

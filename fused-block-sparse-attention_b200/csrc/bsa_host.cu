@@ -107,4 +107,24 @@ bsa_status make_tmap_f32_rows(CUtensorMap *out, const float *ptr, int G, int row
 
 }  // namespace bsa
 
+extern "C" bsa_status bsa_status_word(int32_t **word) {
+  if (!word) return bsa::fail(BSA_ERR_ARG, "status_word: word is NULL");
+  *word = nullptr;
+  // Relaxed: this thread may allocate and wait on streams of its own while it captures one.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  void *p = nullptr;
+  cudaStream_t st = nullptr;
+  cudaError_t e = cudaMalloc(&p, sizeof(int32_t));
+  if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, sizeof(int32_t), st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (st) cudaStreamDestroy(st);
+  if (e != cudaSuccess && p) cudaFree(p);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e != cudaSuccess) return bsa::fail(BSA_ERR_LAUNCH, std::string("status_word: ") + cudaGetErrorString(e));
+  *word = static_cast<int32_t *>(p);
+  return BSA_OK;
+}
+
 extern "C" const char *bsa_last_error(void) { return bsa::g_last_error.c_str(); }

@@ -438,6 +438,12 @@ bsa_status bsa_rope(const bsa_rope_args *a, bsa_stream_t stream);
 /* Turns a device status word (already copied to the host) into a bsa_status. */
 bsa_status bsa_status_decode(int32_t device_word);
 
+/* A zeroed status word of the current device, never freed: for a caller whose first need of
+ * one comes while its thread captures a stream, where an allocation and a zeroing of its
+ * own would become nodes of the graph and clear the word at every replay.  The allocation
+ * is made at once, outside the capture.  Waits for nothing but its own zeroing. */
+bsa_status bsa_status_word(int32_t **word);
+
 /* Thread-local message of the last failing call ("" if none). */
 const char *bsa_last_error(void);
 
