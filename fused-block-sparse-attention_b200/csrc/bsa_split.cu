@@ -24,7 +24,10 @@ namespace {
 constexpr int NW = 4;          // warps per CTA of the partial kernel
 constexpr int kMaxLive = 512;  // block ids of one selection row
 
-// K and V are read once: they leave L2 first, so that the logits stay there for the join.
+// K and V are read once: they leave L2 first, so that the logits stay there for the join
+// (3 x 32777 slots, 32 heads, 4 rows each, D 128: 88 us, 97 without).  A shared prefix that
+// several clusters or row tiles read comes with the same policy: without it those times are
+// the same within 1%.
 __device__ __forceinline__ uint64_t evict_first_policy() {
   uint64_t p;
   asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
@@ -74,8 +77,8 @@ __device__ __forceinline__ void cp_wait() {
 }
 
 // Live block ids (and gates) of one selection row: the first occurrence of each id
-// that holds slots before L, unless its gate is -inf; in slot order; by one warp.
-// Returns their count.
+// that holds slots before L, unless its gate is -inf; in the selection's order; by one
+// warp, which compares each id with all before it (kk^2 / 64 steps).  Returns their count.
 __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_blk, float *s_gate,
                           int *s_raw) {
   const int lane = threadIdx.x & 31;
@@ -413,7 +416,7 @@ __device__ __forceinline__ void cluster_join(const SplitParams &p, const Span &s
   if (p.weight) {
     float *wp = p.weight + s.b * p.w_sb + s.hk * p.w_sh;
     const float *lg = p.logits + (long long)s.grpid * p.ncap * p.rpad;
-    const int rpad = p.rpad;  // 8, 16 or 32 here
+    const int rpad = p.rpad;  // 8, 16, 24 or 32 here
     for (int j = s.c_lo * KC + tid; j < s.c_hi * KC; j += blockDim.x) {
       int key = j;
       if (p.sel) {
