@@ -47,12 +47,12 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, bool live) {
 
 // fp32 products on the tensor cores: x = x1 + x2 + x3, each what is left cut off to bf16 (8
 // bits each, so all 24), and x y = x1 y1 + x1 y2 + x2 y1 + x2 y2 + x1 y3 + x3 y1 up to
-// 2^-21 |x y| (the other three; 2^-24.6 on average).  Six bf16 products take the time of one
-// and a half tf32 ones (mma.sync, measured 300 against 80 TFLOP/s), of which two-term tf32
-// splits need three.  The terms of two neighbours, packed.  Each is cut off below what is
-// left, so that all have the sign of x and none is zero: an infinity (its own first term, the
-// others zero) times them stays what it is, where terms of unlike sign make infinity -
-// infinity of it, and cutting off does not take the largest floats to infinity.
+// 2^-21 |x y| (the other three).  Six bf16 products take the time of one and a half tf32
+// ones (mma.sync, measured 300 against 80 TFLOP/s), of which two-term tf32 splits need
+// three.  The terms of two neighbours, packed.  Each is cut off below what is left, so that
+// all have the sign of x and none is zero: an infinity (its own first term, the others zero)
+// times them stays what it is, where terms of unlike sign make infinity - infinity of it,
+// and cutting off does not take the largest floats to infinity.
 __device__ __forceinline__ void split3(float x, float y, uint32_t *u) {
   constexpr float kBelow = 1.f - 0x1p-24f;  // the next float below
   uint32_t a = __float_as_uint(x * kBelow), b = __float_as_uint(y * kBelow);
@@ -63,6 +63,17 @@ __device__ __forceinline__ void split3(float x, float y, uint32_t *u) {
   u[1] = __byte_perm(a, b, 0x7632);
   x1 = __uint_as_float(a & 0xffff0000u), y1 = __uint_as_float(b & 0xffff0000u);
   u[2] = __byte_perm(__float_as_uint(rx - x1), __float_as_uint(ry - y1), 0x7632);
+}
+// The same for K and V, whose terms may have any sign, as long as those of q and P have not:
+// the first is x without its low bits (no border to infinity), the others are rounded, so
+// that what the products drop is half as large.
+__device__ __forceinline__ void split3_kv(float x, float y, uint32_t *u) {
+  u[0] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x7632);
+  float x1 = __uint_as_float(__float_as_uint(x) & 0xffff0000u), y1 = __uint_as_float(__float_as_uint(y) & 0xffff0000u);
+  const float rx = x == x1 ? 0.f : x - x1, ry = y == y1 ? 0.f : y - y1;
+  u[1] = Mma<__nv_bfloat16>::pack(rx, ry);
+  x1 = __uint_as_float(u[1] << 16), y1 = __uint_as_float(u[1] & 0xffff0000u);
+  u[2] = Mma<__nv_bfloat16>::pack(rx - x1, ry - y1);
 }
 // Maximum that keeps a NaN: a row with a NaN logit ends as NaN, not as an empty row.
 __device__ __forceinline__ float fmax_nan(float a, float b) {
@@ -851,9 +862,9 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float4 x = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(g + 8 * h, ks * 4 + tq));
-        split3(x.x, x.y, u);
+        split3_kv(x.x, x.y, u);
         a[0][h] = u[0], a[1][h] = u[1], a[2][h] = u[2];
-        split3(x.z, x.w, u);
+        split3_kv(x.z, x.w, u);
         a[0][2 + h] = u[0], a[1][2 + h] = u[1], a[2][2 + h] = u[2];
       }
 #pragma unroll
@@ -948,9 +959,9 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
           uint32_t a[3][4], u[3];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            split3(x[0][h][e], x[1][h][e], u);
+            split3_kv(x[0][h][e], x[1][h][e], u);
             a[0][h] = u[0], a[1][h] = u[1], a[2][h] = u[2];
-            split3(x[2][h][e], x[3][h][e], u);
+            split3_kv(x[2][h][e], x[3][h][e], u);
             a[0][2 + h] = u[0], a[1][2 + h] = u[1], a[2][2 + h] = u[2];
           }
 #pragma unroll
@@ -1136,13 +1147,13 @@ __global__ void __launch_bounds__(RowsCfg<D>::W * 32, 1)
       uint32_t u[3];
       const float4 x = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(gg, ks * 4 + tt));
       const float4 y = *reinterpret_cast<const float4 *>(sk + sw_off<4, D>(gg + 8, ks * 4 + tt));
-      split3(x.x, x.y, u);
+      split3_kv(x.x, x.y, u);
       f[0].x = u[0], f[1].x = u[1], f[2].x = u[2];
-      split3(y.x, y.y, u);
+      split3_kv(y.x, y.y, u);
       f[0].y = u[0], f[1].y = u[1], f[2].y = u[2];
-      split3(x.z, x.w, u);
+      split3_kv(x.z, x.w, u);
       f[0].z = u[0], f[1].z = u[1], f[2].z = u[2];
-      split3(y.z, y.w, u);
+      split3_kv(y.z, y.w, u);
       f[0].w = u[0], f[1].w = u[1], f[2].w = u[2];
 #pragma unroll
       for (int k = 0; k < 3; ++k) fk[(ks * 3 + k) * 32 + (i & 31)] = f[k];
@@ -1165,13 +1176,13 @@ __global__ void __launch_bounds__(RowsCfg<D>::W * 32, 1)
       for (int e = 0; e < VW; ++e) {
         uint4 f[3];
         uint32_t u[3];
-        split3(x[0][0][e], x[1][0][e], u);
+        split3_kv(x[0][0][e], x[1][0][e], u);
         f[0].x = u[0], f[1].x = u[1], f[2].x = u[2];
-        split3(x[0][1][e], x[1][1][e], u);
+        split3_kv(x[0][1][e], x[1][1][e], u);
         f[0].y = u[0], f[1].y = u[1], f[2].y = u[2];
-        split3(x[2][0][e], x[3][0][e], u);
+        split3_kv(x[2][0][e], x[3][0][e], u);
         f[0].z = u[0], f[1].z = u[1], f[2].z = u[2];
-        split3(x[2][1][e], x[3][1][e], u);
+        split3_kv(x[2][1][e], x[3][1][e], u);
         f[0].w = u[0], f[1].w = u[1], f[2].w = u[2];
 #pragma unroll
         for (int k = 0; k < 3; ++k) fv[((v * VW + e) * 3 + k) * 32 + (i & 31)] = f[k];
