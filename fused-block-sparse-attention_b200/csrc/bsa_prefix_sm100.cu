@@ -7,8 +7,8 @@
 // the split kernels, so that its rounding does not add to the output's and a sequence's
 // precision does not hang on how many others are served beside it: in one term the error
 // against 64 bits was 1.4 times that of the output's rounding alone (bf16, 65536 keys
-// 2.33e-3 -> 1.65e-3; f16, 32768 keys 2.92e-4 -> 2.08e-4).  The second product with V took
-// these from 46 to 51.5 us and from 108 to 123.  Unlike the sequence forward, a row tile
+// 2.33e-3 -> 1.65e-3; f16, 32768 keys 2.92e-4 -> 2.08e-4).  The second product with V and
+// its terms took these from 46 to 51.5 us and from 108 to 123.  Unlike the sequence forward, a row tile
 // gathers its rows from different sequences, every key is visible to every row, and the
 // keys are split so that all SMs work on few rows.
 //

@@ -150,8 +150,8 @@ __device__ int build_live(const SplitParams &p, int b, int hk, int len, int *s_b
 // 16-byte piece of a K row is its two pairs of a k-step (dims 4t .. 4t+3), and 16-byte
 // pieces of V rows feed four tiles of O (tile e holds columns 4j + e of a group).  The
 // products truncate their sums, always towards zero, so a chunk's part of O starts at zero
-// and is added by a rounding addition (20000 keys, D 256: 4.7e-7 of the output's norm;
-// summed on in the products 1.2e-5, and plain fp32 arithmetic 2.9e-7).
+// and is added by a rounding addition (20000 keys, D 256: 5.2e-7 of the output's norm, plain fp32
+// arithmetic 8.2e-7; summed on in the products it was 25 times as much).
 template <typename T, int D>
 struct SplitCfg {
   static constexpr int ES = sizeof(T), E16 = 16 / ES;
@@ -1057,8 +1057,8 @@ __global__ void __launch_bounds__(NW * 32, SplitCfg<float, D>::MINB)
 // same keys.  The chunk's K and V are turned into operands (three bf16 terms, in the order
 // of the products' registers) once for the CTA, where the kernel above does it for every
 // 16 or 32 rows: with many rows that was two thirds of its instructions.  Bound by the
-// products (mma.sync): 1200 rows x 20000 keys, D 256, 8 heads, in 5.46 ms, 216 TFLOP/s of
-// bf16 products (of 300 measured); 8.46 ms by the kernel above.  Which rows take it:
+// products (mma.sync): 1200 rows x 20000 keys, D 256, 8 heads, in 5.48 ms, 215 TFLOP/s of
+// bf16 products (of 300 measured); 8.22 ms by the kernel above.  Which rows take it:
 // rows_over_warps.
 template <int D>
 struct RowsCfg {
@@ -1555,9 +1555,9 @@ static int split_count_t(long long groups, int R, long long n, int sms) {
 }
 
 // Whether the rows of a shared prefix go over the warps (split_f32_rows_kernel).  Times of
-// it against split_f32_kernel, 20000 keys, 8 heads, us: D 256, 36 rows 290 : 382, 1200 rows
-// 5461 : 8456; D 128, 64 rows 245 : 209, 96 rows 247 : 305, 1200 rows 2359 : 3396; D 64,
-// 96 rows 150 : 115, 1200 rows 1404 : 1290 (its barriers and the one CTA per SM show where
+// it against split_f32_kernel, 20000 keys, 8 heads, us: D 256, 36 rows 294 : 378, 1200 rows
+// 5484 : 8224; D 128, 64 rows 246 : 212, 96 rows 248 : 310, 1200 rows 2325 : 3424; D 64,
+// 96 rows 154 : 112, 1200 rows 1410 : 1249 (its barriers and the one CTA per SM show where
 // a chunk has few products).
 static bool rows_over_warps(int dtype, int D, bool fold, int R) {
   return dtype == BSA_F32 && fold && (D == 256 ? R > 32 : D == 128 && R > 64);

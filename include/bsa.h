@@ -266,7 +266,9 @@ bsa_status bsa_decode(const bsa_decode_args *a, void *workspace, size_t workspac
  * position <= query position, a repeated id counts once, an id outside the cache is
  * skipped and reported, a block whose gate is -inf is skipped), and the other slots'
  * sums stay as they are.  A row that sees no key gives o = 0 and no weight.  Masked and unused K/V rows
- * may hold anything, infinities and NaN included.  No counterpart in the reference.
+ * may hold anything, infinities and NaN included; an infinity that a row does see acts as
+ * the definition has it (in V: that infinity in the output; a logit of -inf: weight 0).
+ * Weights below 2^-100 of a row's largest (f16: 2^-36) may count as 0 in that.  No counterpart in the reference.
  * Limits: D 32, 64, 128 or 256; (Hq/Hkv) * T <= 4096; bs a multiple of 32 and
  * kk <= 512 with a selection; k, v bases and strides multiples of 16 bytes.  Device
  * workspace: the splits' partial sums and the fp32 logits (4 bytes per query row
@@ -323,7 +325,9 @@ bsa_status bsa_evict(const bsa_evict_args *a, void *workspace, size_t workspace_
  * tokens the last of them; clamped to [0, S], reported when outside).  Row t sees
  * the whole prefix and the own slots j <= lens[b] - T + t; o = softmax over both.
  * A row that sees no key gives 0.  P may be 0.  Unused and masked slots may hold
- * anything.  No counterpart in the reference.  D 32, 64, 128 or 256; k, v, pk, pv
+ * anything, visible infinities as in bsa_decode_weighted.  Every path holds sums and
+ * softmax statistics in fp32 and takes the weights into the products to 2^-16 or better,
+ * so a row's precision does not depend on how many rows share the prefix (its bits do).  No counterpart in the reference.  D 32, 64, 128 or 256; k, v, pk, pv
  * bases and strides multiples of 16 bytes.  Workspace: the splits' partial sums. */
 typedef struct {
   int32_t dtype, B, Hq, Hkv, D, P, S, T;
